@@ -473,6 +473,131 @@ int hipq_dequantize_i32(const int32_t *x_nhwc, float *y_nchw, int N, int C, int 
 /* A plain device-to-device copy kernel of known size; the calibration reference for HBM counters. */
 int hipq_copy_bytes(const void *src, void *dst, size_t count, void *stream);
 
+/* ==== operators of language models ============================================================
+ * No counterpart in the reference, whose quantized operators end at 8-bit weights and activations of convolutional networks:
+ * what stands here is defined by its formula, and checked against that formula in 64 bits.
+ *
+ * Unlike the operators above, activations are rows of 16-bit floats (float16 or bfloat16) as a program has them: row after row, with
+ * strides counted in elements.  Every sum, softmax statistic and norm is held in 32 bits; results are rounded once.  Nothing here
+ * allocates at run time (some calls take the caller's workspace), so all of it may be captured into a HIP graph; a captured
+ * call keeps the pointers that it was given.  Arrays are on the device of the current context unless "host" says otherwise.
+ */
+#define HIPQ_REAL_F32 0
+#define HIPQ_REAL_F16 1
+#define HIPQ_REAL_BF16 2
+
+#define HIPQ_ACT_NONE 0
+#define HIPQ_ACT_SILU 1 /* v / (1 + exp(-v)) */
+#define HIPQ_ACT_GELU 2 /* v / (1 + exp(-2 sqrt(2 / pi) (v + 0.044715 v^3))), the tanh form */
+
+/* ---- products with 4-bit weights (beside the fully-connected layers above, whose weights have 8)
+ *   y[m][n] = sum over groups g of scale[n][g] * sum over k in g of x[m][k] * (q[n][k] - zero[n][g]),  + bias[n]
+ * With an activation the plan holds two projections of N outputs each, the gate's rows first:
+ *   y[m][n] = act(y_gate[m][n]) * y_up[m][n]                         (each with its bias; one launch). */
+typedef struct hipq_w4_desc {
+    int32_t N, K;       /* outputs (of each projection) and inputs; K a multiple of 32 */
+    int32_t group;      /* weights that share a scale: 32, 64 or 128; the last group of a row may be shorter */
+    int32_t type;       /* of x, y, scales and bias: HIPQ_REAL_F16 or HIPQ_REAL_BF16 */
+    int32_t activation; /* HIPQ_ACT_* */
+} hipq_w4_desc;
+
+typedef struct hipq_w4_plan hipq_w4_plan;
+
+/*
+ * Setup: lays the weights out for the kernels, on the device behind the work of `stream`, and waits for it: then the plan serves every
+ * stream, and the arrays are no longer needed.  q: rows of K / 2 bytes, the lower half of a byte first; scales: rows of ceil(K / group); zeros: one byte
+ * (0..15; the upper half of a byte is ignored) in the place of each scale, or NULL: 8 everywhere; bias: a value per row, or NULL.
+ * There are N rows, or 2 N with an activation.
+ */
+int hipq_w4_plan_create(const hipq_w4_desc *desc, const uint8_t *q, const void *scales, const uint8_t *zeros, const void *bias, void *stream,
+                        hipq_w4_plan **plan_out);
+void hipq_w4_plan_destroy(hipq_w4_plan *plan);
+/* Name of the kernel that hipq_w4_run launches for M rows ("" for a number of rows that it refuses).  The string is static. */
+const char *hipq_w4_plan_kernel(const hipq_w4_plan *plan, int M);
+/* x: M rows of K, x_stride elements apart (a multiple of 8, the first row at a multiple of 16 bytes); y: M rows of N, y_stride apart.
+ * M may be 0.  The plan belongs to the device that it was created on.  workspace: hipq_w4_workspace bytes at a multiple of 16 (0: none,
+ * may be NULL), whose content is of no interest before and after; calls that may run at the same time need one each. */
+size_t hipq_w4_workspace(const hipq_w4_plan *plan, int M);
+int hipq_w4_run(const hipq_w4_plan *plan, const void *x, int64_t x_stride, void *y, int64_t y_stride, int M, void *workspace,
+                size_t workspace_bytes, void *stream);
+
+/* ---- a paged cache of keys and values, and the attention that reads it
+ * Keys and values lie in pages: element (page p, head h, token t of the page, i) at ((p * heads + h) * page + t) * dim + i.  In 8 bits
+ * (quantized = 1) the value is code * scale with one float scale for each (p, h, t); codes are int8 in -127..127. */
+typedef struct hipq_kv_cache {
+    void *k, *v;               /* of `type`, or int8 */
+    float *k_scale, *v_scale;  /* quantized only: [pages][heads][page] */
+    int32_t pages, heads, page, dim; /* page: a multiple of 16; dim: 64, 128 or 256 */
+    int32_t type;              /* of the queries, keys and values that come in: HIPQ_REAL_F16 or HIPQ_REAL_BF16 */
+    int32_t quantized;
+} hipq_kv_cache;
+
+/*
+ * New tokens: every query and key head is normed (only where its weights are given: x / sqrt(mean(x^2) + eps) * w), rotated by its
+ * token's position, and rounded; queries go to q_out, keys and - as they are - values into the cache.  In 8 bits the scale is the
+ * largest magnitude of the (rotated, unrounded) head / 127, and codes are value / scale rounded to nearest even; a head with an
+ * infinity or NaN gets what that arithmetic gives for its scale and codes that are not defined.
+ * Rotation: table[pos] holds rot / 2 cosines, then rot / 2 sines; the pairs of the first `rot` elements are (i, i + rot / 2), or
+ * (2 i, 2 i + 1) where interleaved: (a, b) -> (a c - b s, b c + a s).  What lies behind `rot` is not turned.
+ * slots[t]: page * page size + place.  A token whose slot lies outside the cache (-1 marks a padded row) or whose position lies outside
+ * the table is left alone: neither its row of q_out nor the cache is written.  Two tokens of one call must not have the same slot.
+ * q_out may be q itself (same strides).  Strides are in elements, multiples of 8; all pointers at multiples of 16 bytes.
+ */
+typedef struct hipq_kv_append_desc {
+    const void *q, *k, *v; /* [tokens][heads][dim] */
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+    void *q_out;
+    const int32_t *positions, *slots;
+    const float *table;
+    const void *q_norm, *k_norm; /* [dim] of `type`, or NULL */
+    int32_t tokens, q_heads, table_rows, rot, interleaved;
+    float eps;
+} hipq_kv_append_desc;
+int hipq_kv_append(const hipq_kv_cache *cache, const hipq_kv_append_desc *desc, void *stream);
+
+/*
+ * Attention of each sequence's new tokens over its tokens in the cache, its new ones - appended before - among them.
+ * Sequence b: tokens 0..lens[b] - 1 of the pages blocks[b][0], blocks[b][1], ...; its new tokens are rows starts[b]..starts[b + 1] - 1 of
+ * q and the last starts[b + 1] - starts[b] tokens of the cache.  A new token sees all tokens before the new ones, and of the new ones:
+ * without a mask itself and those in front of it (a chain); with one those whose bit is set in its 64-bit word mask[row] (a tree's
+ * ancestors and itself; at most 64 new tokens a sequence).  Query head h reads the cache's head h / (q_heads / heads).
+ *   o = sum_t softmax_t(scale * q . k_t) v_t over the tokens seen; 0 where there is none.
+ * Rows of o that belong to no sequence are left as they are.  Entries of blocks behind a sequence's end are not read; a block outside
+ * the cache holds no tokens (they are not seen).  Lengths beyond `longest`, and more new tokens than `most_new`, are cut off there: the
+ * caller's bounds, from which the host divides the work.
+ * workspace: hipq_kv_attend_workspace bytes at a multiple of 16 (0: none, may be NULL), whose content is of no interest before and after;
+ * calls that may run at the same time need one each.
+ */
+typedef struct hipq_kv_attend_desc {
+    const void *q;
+    void *o;
+    int64_t q_token, q_head, o_token, o_head;
+    const int32_t *starts, *lens, *blocks; /* [sequences + 1], [sequences], [sequences][blocks_stride] */
+    const uint64_t *mask;                  /* [rows of q], or NULL */
+    int64_t blocks_stride;
+    int32_t sequences, tokens, q_heads; /* tokens: rows of q and o */
+    int32_t blocks_per_sequence, most_new, longest;
+    float scale;
+} hipq_kv_attend_desc;
+size_t hipq_kv_attend_workspace(const hipq_kv_cache *cache, const hipq_kv_attend_desc *desc);
+int hipq_kv_attend(const hipq_kv_cache *cache, const hipq_kv_attend_desc *desc, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * A token of every row of scores (beside hipq_softmax_u8, which makes them probabilities).  With w_i = exp((x_i - max x) / temperature), and the
+ * row's tokens ordered by score, equal ones by index, those are kept that
+ *   are among the first top_k (top_k <= 0: all),
+ *   and have less than top_p of the weight of those in front of them (the first always; top_p >= 1: all),
+ *   and have w_i >= min_p (the first always).
+ * The token is the first one, by index, at which the running sum of the kept weights exceeds uniform * their sum (uniform in [0, 1)).
+ * A temperature that is not above 0 takes the highest score, the lowest index among equal ones.  Scores of -infinity and NaN are never
+ * taken: a row of nothing else gives -1; of +infinities each has the same weight, and nothing else has any.
+ * Weights are summed in 64-bit fixed point, so that no order of summation shows in a result.
+ * temperature, top_k, top_p, min_p: a value per row, or NULL (1, all, all, all).  logits: rows of `vocab` of `type` (HIPQ_REAL_*), `stride`
+ * elements apart, at any address that the type allows.
+ */
+int hipq_sample(const void *logits, int type, int rows, int vocab, int64_t stride, const float *uniform, const float *temperature,
+                const int32_t *top_k, const float *top_p, const float *min_p, int64_t *tokens, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

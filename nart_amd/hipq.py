@@ -26,6 +26,31 @@ class ConvDesc(C.Structure):  # hipq_conv2d_desc
 
 
 DTYPE_U8, DTYPE_I8 = 0, 1
+REAL_F32, REAL_F16, REAL_BF16 = 0, 1, 2
+
+
+class W4Desc(C.Structure):  # hipq_w4_desc
+    _fields_ = [(n, C.c_int32) for n in ("N", "K", "group", "type", "activation")]
+
+
+class KvCacheStruct(C.Structure):  # hipq_kv_cache
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] \
+        + [(n, C.c_int32) for n in ("pages", "heads", "page", "dim", "type", "quantized")]
+
+
+class KvAppendDesc(C.Structure):  # hipq_kv_append_desc
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v")] \
+        + [(n, C.c_int64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "out_token", "out_head")] \
+        + [(n, C.c_void_p) for n in ("q_out", "positions", "slots", "table", "q_norm", "k_norm")] \
+        + [(n, C.c_int32) for n in ("tokens", "q_heads", "table_rows", "rot", "interleaved")] + [("eps", C.c_float)]
+
+
+class KvAttendDesc(C.Structure):  # hipq_kv_attend_desc
+    _fields_ = [(n, C.c_void_p) for n in ("q", "o")] + [(n, C.c_int64) for n in ("q_token", "q_head", "o_token", "o_head")] \
+        + [(n, C.c_void_p) for n in ("starts", "lens", "blocks", "mask")] + [("blocks_stride", C.c_int64)] \
+        + [(n, C.c_int32) for n in ("sequences", "tokens", "q_heads", "blocks_per_sequence", "most_new", "longest")] + [("scale", C.c_float)]
+
+
 TILE_INDEX = {"128x128": 0, "256x64": 1, "128x64": 2, "64x128": 3, "64x64": 4}  # hipq_conv2d_plan_select
 
 
@@ -108,6 +133,15 @@ _SIGS = {
     "hipq_dequantize_i8": (C.c_int, [C.c_void_p, C.c_void_p] + [C.c_int] * 5 + [C.c_float, C.c_void_p]),
     "hipq_dequantize_i32": (C.c_int, [C.c_void_p, C.c_void_p] + [C.c_int] * 5 + [C.c_float, C.c_void_p]),
     "hipq_copy_bytes": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "hipq_w4_plan_create": (C.c_int, [C.POINTER(W4Desc), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(C.c_void_p)]),
+    "hipq_w4_plan_destroy": (None, [C.c_void_p]),
+    "hipq_w4_plan_kernel": (C.c_char_p, [C.c_void_p, C.c_int]),
+    "hipq_w4_workspace": (C.c_size_t, [C.c_void_p, C.c_int]),
+    "hipq_w4_run": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "hipq_kv_append": (C.c_int, [C.POINTER(KvCacheStruct), C.POINTER(KvAppendDesc), C.c_void_p]),
+    "hipq_kv_attend_workspace": (C.c_size_t, [C.POINTER(KvCacheStruct), C.POINTER(KvAttendDesc)]),
+    "hipq_kv_attend": (C.c_int, [C.POINTER(KvCacheStruct), C.POINTER(KvAttendDesc), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "hipq_sample": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int64] + [C.c_void_p] * 7),
 }
 EXPORTS = tuple(_SIGS)
 
@@ -170,6 +204,7 @@ def _calls():
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
         mod.init(torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
+        mod.types(torch.float32, torch.float16, torch.bfloat16, torch.int32, torch.int64, torch.uint8, torch.int8)
         _CALLS = mod
     return _CALLS
 
@@ -554,3 +589,146 @@ def dequantize_u8(x, y_nchw, ialpha, izp):
     if rc:
         check(rc)
     return y_nchw
+
+
+# ---- operators of language models (include/hipq.h: the section of that name) ------------------------
+_ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}
+
+
+class LinearW4:
+    """Products with 4-bit weights and group scales; with an activation the gated pair act(x Wg^T) * (x Wu^T) in one launch.
+
+    q: uint8 [N, K / 2], the lower half of a byte first; scales: [N, ceil(K / group)] in float16 or bfloat16, which x and y then are
+    as well; zeros: uint8 like scales (None: 8 everywhere); bias: [N] like scales, or None.  With an activation ("silu", "gelu") the
+    rows are those of the gate, then those of the other projection.  All on the current device; the plan keeps a copy of its own."""
+
+    def __init__(self, q, scales, group=128, zeros=None, bias=None, activation=None):
+        import torch
+        self.handle = None
+        types = {torch.float16: REAL_F16, torch.bfloat16: REAL_BF16}
+        if activation not in _ACTIVATIONS:
+            raise ValueError("activation: None, 'silu' or 'gelu' is expected")
+        if q.dim() != 2 or q.dtype != torch.uint8:
+            raise ValueError("q: uint8 with two dimensions is expected")
+        if scales.dtype not in types:
+            raise ValueError("scales: float16 or bfloat16 is expected")
+        rows, k = q.shape[0], 2 * q.shape[1]
+        if group not in (32, 64, 128):
+            raise ValueError("group: 32, 64 or 128 is expected")
+        gated = activation is not None
+        if rows == 0 or (gated and rows % 2):
+            raise ValueError("q: %s" % ("an even number of rows is expected" if rows else "it has no rows"))
+        for t, name, shape, dtype in ((scales, "scales", (rows, -(-k // group)), scales.dtype), (zeros, "zeros", (rows, -(-k // group)), torch.uint8),
+                                      (bias, "bias", (rows,), scales.dtype)):
+            if t is not None and (tuple(t.shape) != shape or t.dtype != dtype):
+                raise ValueError("%s: %s of shape %s is expected" % (name, dtype, shape))
+        current = torch.cuda.current_device()
+        for t, name in ((q, "q"), (scales, "scales"), (zeros, "zeros"), (bias, "bias")):
+            if t is not None and t.get_device() != current:
+                raise ValueError("%s is not on the current device" % name)
+        q, scales, zeros, bias = (None if t is None else t.contiguous() for t in (q, scales, zeros, bias))
+        self.N, self.K, self.type, self.dtype = rows // 2 if gated else rows, k, types[scales.dtype], scales.dtype
+        d = W4Desc(N=self.N, K=k, group=group, type=self.type, activation=_ACTIVATIONS[activation])
+        h = C.c_void_p()
+        check(lib().hipq_w4_plan_create(C.byref(d), _ptr(q), _ptr(scales), _ptr(zeros), _ptr(bias), _stream(), C.byref(h)))
+        self.handle, self._address = h, h.value
+
+    def kernel(self, m):
+        """Name of the kernel that m rows run on."""
+        return lib().hipq_w4_plan_kernel(self.handle, int(m)).decode()
+
+    def __call__(self, x, y=None):
+        """y = x W^T + bias: x [M, K] (or with more dimensions in front), y [M, N]; rows may have gaps between them."""
+        if not self._address:
+            raise ValueError("the plan is closed")
+        if x.dim() != 2:
+            front = x.shape[:-1]
+            if y is not None:
+                raise ValueError("y: only with an x of two dimensions")
+            return self(x.reshape(-1, x.shape[-1])).view(*front, self.N)
+        calls = _CALLS or _calls()
+        m = x.shape[0]
+        if y is None:
+            y = x.new_empty((m, self.N))
+        need = calls.w4_workspace(self._address, m)
+        rc = calls.w4_run(self._address, self.type, self.N, self.K, x, y, _bytes_like(x, need) if need else None)
+        if rc:
+            check(rc)
+        return y
+
+    def close(self):
+        if self.handle:
+            lib().hipq_w4_plan_destroy(self.handle)
+            self.handle, self._address = None, 0
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _bytes_like(t, count):
+    import torch
+    return torch.empty(count, dtype=torch.uint8, device=t.device)
+
+
+class KvCache:
+    """A paged cache of keys and values over the caller's tensors: k, v [pages, heads, page, dim] in float16, bfloat16 or int8; in int8 with
+    k_scale, v_scale float32 [pages, heads, page].  They stay the caller's (who allocates, copies and keeps pages), and are kept alive
+    here."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._struct = _calls().kv_cache(k, v, k_scale, v_scale)
+        self._device = k.get_device()
+        self._scale = k.shape[-1] ** -0.5
+
+    def append(self, q, k, v, positions, slots, table, out=None, q_norm=None, k_norm=None, eps=1e-6, interleaved=False):
+        """New tokens: q [tokens, q heads, dim] normed, rotated and written to out (may be q); k and v [tokens, heads, dim] - k normed and
+        rotated - to the cache's `slots` (page * page size + place; -1: a padded row, left alone).  positions, slots: int32; table:
+        float32 [positions, rot], cosines then sines (None: nothing is rotated); q_norm, k_norm: weights of a norm per head, or None."""
+        calls = _CALLS or _calls()
+        if out is None:
+            out = q.new_empty(q.shape)
+        rc = calls.kv_append(self._struct, self._device, q, k, v, positions, slots, table, out, q_norm, k_norm, eps, int(interleaved))
+        if rc:
+            check(rc)
+        return out
+
+    def attend(self, q, starts, lens, blocks, most_new, mask=None, scale=None, out=None, longest=None):
+        """Attention of the new tokens q [tokens, q heads, dim] over the cache: sequence b has rows starts[b] .. starts[b + 1] - 1 of q (at
+        most `most_new`), lens[b] tokens of the pages blocks[b] - the new ones, appended before, the last of them.  A new token sees
+        what is in front of it and itself; with mask (int64 [tokens]) of the new ones those whose bit is set.  starts, lens, blocks:
+        int32; scale: dim ** -0.5 by default; longest: a bound of lens, by default what blocks holds.  Rows of no sequence stay as
+        they are in `out`."""
+        calls = _CALLS or _calls()
+        if out is None:
+            out = q.new_empty(q.shape)
+        rc = calls.kv_attend(self._struct, self._device, q, out, starts, lens, blocks, mask, most_new, longest, self._scale if scale is None else scale,
+                             lambda count: _bytes_like(q, count))
+        if rc:
+            check(rc)
+        return out
+
+
+def rotation_table(positions, rot, base=10000.0):
+    """float32 [positions, rot] for KvCache.append on the current device: cosines, then sines, of position * base ** (-2 i / rot).  The angles
+    are formed in 64 bits: in 32 those of far positions have lost their place in the circle."""
+    import torch
+    angle = torch.arange(positions, dtype=torch.float64, device="cuda")[:, None] * float(base) ** -(
+        torch.arange(0, rot, 2, dtype=torch.float64, device="cuda") / rot)
+    return torch.cat((angle.cos(), angle.sin()), 1).float()
+
+
+def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
+    """A token of every row of logits [rows, vocab] (float32, float16 or bfloat16) from given numbers `uniform` in [0, 1) (include/hipq.h:
+    hipq_sample).  temperature, top_p, min_p: float32 [rows], top_k: int32 [rows], or None.  int64 [rows]; -1 where a row has nothing."""
+    calls = _CALLS or _calls()
+    if out is None:
+        import torch
+        out = torch.empty(logits.shape[0], dtype=torch.int64, device=logits.device)
+    rc = calls.sample(logits, uniform, temperature, top_k, top_p, min_p, out)
+    if rc:
+        check(rc)
+    return out
