@@ -5,7 +5,7 @@
 // scores are divided into 2048 intervals below the maximum, the interval is found in which the running sum reaches `need`, what lies in it is
 // collected and divided again by the bits of the scores, until an interval is a single score.
 // Weights are 64-bit fixed point, 2^-43 of the largest: sums do not depend on their order, so that neither atomics nor the number of
-// threads show in a result, and they come from a polynomial in 64 bits (2^-43 of their value off at most): a running sum in 32 bits goes wrong
+// threads show in a result, and they come from a polynomial in 64 bits (2^-37 of their value off at most): a running sum in 32 bits goes wrong
 // where two tokens' borders lie closer than its rounding, at 10^5 tokens once in some hundred rows.
 //
 // One work-group has a row, and reads it some times: the first from memory, the others from the caches.
@@ -19,6 +19,18 @@ namespace hipq {
 constexpr int THREADS = 1024, WAVES = THREADS / 64, BINS = 2048, LIST = 4096, FRACTION = 43;
 constexpr int MOST_VOCAB = 1 << 20; // sums of weights fit 64 bits
 
+// 2^(i / 32) and 2^(i / 1024)
+__constant__ const double POWERS[2][32] = {
+    {1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+     1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332, 1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+     1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+     1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002},
+    {1.0, 1.0006771306930664, 1.0013547198921082, 1.002032767907594, 1.0027112750502025, 1.0033902416308227, 1.004069667960554, 1.0047495543507072,
+     1.0054299011128027, 1.006110708558573, 1.0067919769999607, 1.0074737067491204, 1.0081558981184175, 1.0088385514204294, 1.0095216669679448, 1.0102052450739643,
+     1.0108892860517005, 1.011573790214578, 1.0122587578762337, 1.0129441893505169, 1.0136300849514894, 1.0143164449934257, 1.0150032697908125, 1.0156905596583505,
+     1.016378314910953, 1.0170665358637463, 1.0177552228320703, 1.0184443761314785, 1.019133996077738, 1.0198240829868295, 1.0205146371749483, 1.0212056589585028},
+};
+
 struct SampleArgs {
     const void *logits;
     int64_t stride;
@@ -31,7 +43,7 @@ struct SampleArgs {
 struct SampleShared {
     uint64_t bins[BINS];
     uint32_t list[LIST];
-    double powers[256]; // 2^(i / 256)
+    double powers[1024]; // 2^(i / 1024)
     uint64_t wave[WAVES];
     uint64_t sum, before;
     uint32_t bin, listed, low, high;
@@ -45,12 +57,11 @@ struct Scores {
     struct __attribute__((packed, aligned(TYPE == HIPQ_REAL_F32 ? 4 : 2))) Vec {
         u32x4 v;
     };
-    __device__ static __forceinline__ float clean(float x) { return x == x ? x : -__builtin_inff(); } // NaN: never taken
     __device__ static __forceinline__ float one(const void *row, int i)
     {
         if (TYPE == HIPQ_REAL_F32)
-            return clean(((const float *)row)[i]);
-        return clean(Real16<TYPE == HIPQ_REAL_F32 ? HIPQ_REAL_F16 : TYPE>::low(((const uint16_t *)row)[i]));
+            return ((const float *)row)[i];
+        return Real16<TYPE == HIPQ_REAL_F32 ? HIPQ_REAL_F16 : TYPE>::low(((const uint16_t *)row)[i]);
     }
     // elements i .. i + E - 1, those behind the end as -infinity
     __device__ static __forceinline__ void some(const void *row, int i, int end, float (&x)[E])
@@ -60,12 +71,21 @@ struct Scores {
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 using R = Real16<TYPE == HIPQ_REAL_F32 ? HIPQ_REAL_F16 : TYPE>;
-                x[e] = clean(TYPE == HIPQ_REAL_F32 ? __builtin_bit_cast(float, (uint32_t)v[e % 4]) : e & 1 ? R::high(v[e / 2]) : R::low(v[e / 2]));
+                x[e] = TYPE == HIPQ_REAL_F32 ? __builtin_bit_cast(float, (uint32_t)v[e % 4]) : e & 1 ? R::high(v[e / 2]) : R::low(v[e / 2]);
             }
         } else {
 #pragma unroll
             for (int e = 0; e < E; e++)
-                x[e] = i + e < end ? one(row, i + e) : -__builtin_inff();
+                x[e] = -__builtin_inff();
+            if (i < end) { // all at once: one after the other, eight loads took 3 us
+                float y[E];
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    y[e] = one(row, min(i + e, end - 1));
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    x[e] = i + e < end ? y[e] : x[e];
+            }
         }
     }
 };
@@ -89,9 +109,10 @@ struct Row {
     const void *row;
     int tid, lane, wave;
     float top, per_bin; // intervals of a unit of score
+    bool infinite = false;
     double rate;        // log2(e) / temperature
-    // the border: scores above key are kept, and of those equal to it the first `ties` (up to index `last`)
-    uint32_t key = 0, ties = 0xffffffffu;
+    // the border: scores above that of key are kept, and of those equal to it the first `ties` (up to index `last`)
+    uint32_t key = 0x007fffffu /* -infinity's */, ties = 0xffffffffu;
     int last = 0x7fffffff;
     uint64_t least = 0; // smallest weight that min-p keeps
 
@@ -101,52 +122,54 @@ struct Row {
         row = (const uint8_t *)a.logits + (int64_t)blockIdx.x * a.stride * (TYPE == HIPQ_REAL_F32 ? 4 : 2);
     }
 
-    template <class F>
-    __device__ __forceinline__ void each(F f)
+    // where there are infinities they are all that counts, one like the other
+    __device__ __forceinline__ void settle(float (&x)[E]) const
     {
-        constexpr int U = E / 2, STEP = THREADS * E;
-        for (int base = tid * E; base < a.vocab; base += U * STEP) {
-            float x[U][E];
+        if (infinite)
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                Scores<TYPE>::some(row, base + u * STEP, a.vocab, x[u]);
-#pragma unroll
-            for (int u = 0; u < U; u++)
-#pragma unroll
-                for (int e = 0; e < E; e++)
-                    f(x[u][e], base + u * STEP + e);
-        }
+            for (int e = 0; e < E; e++)
+                x[e] = x[e] == __builtin_inff() ? 0.0f : -__builtin_inff();
     }
 
-    // 2^(rate (x - top)) in units of 2^-43: 2^(n / 256) from the table times 2^r, |r| <= 1 / 512, to the fourth term (the fifth is under 2^-48)
-    __device__ __forceinline__ uint64_t weight(float x) const
+    // f(scores, index of the first) of the row's part [from, to), 16 bytes at a time, `lanes` threads side by side, the next 16 bytes on
+    // their way.  The loop is short on purpose: what runs once is bound by the fetch of its instructions
+    template <class F>
+    __device__ __forceinline__ void each(int from, int to, int id, int lanes, F f)
     {
-        if (x == top)
-            return (uint64_t)1 << FRACTION;
-        const double y = ((double)x - (double)top) * rate; // below 0
-        if (!(y > -44.5))
-            return 0;
-        const double big = 6755399441055744.0 / 256; // 1.5 * 2^52 / 256: what is added keeps eight bits behind the point
+        float x[E], ahead[E];
+        Scores<TYPE>::some(row, from + id * E, to, x);
+#pragma unroll 1
+        for (int base = from; base < to; base += lanes * E) {
+            const int i = base + id * E;
+            Scores<TYPE>::some(row, i + lanes * E, to, ahead);
+            settle(x);
+            f(x, i);
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                x[e] = ahead[e];
+        }
+    }
+    template <class F>
+    __device__ __forceinline__ void each(F f) { each(0, a.vocab, tid, THREADS, f); }
+
+    // 2^(rate (x - top)) in units of 2^-43: 2^(n / 1024) from the table times 2^r, |r| <= 1 / 2048, to the second power (the third is under
+    // 2^-37 of the whole).  No branch, and no instruction to spare: a pass takes 64 / 4 of a wave's clocks for each.  The result is RAW more.
+    static constexpr uint64_t RAW = 0x4330000000000000ull; // 2^52: a sum's lower bits are the rounded number
+    __device__ __forceinline__ uint64_t raw_weight(float x) const
+    {
+        const double y = fmax(((double)x - (double)top) * rate, -60.0); // at most 0; NaN and all below count as 2^-60, which rounds to 0
+        const double big = 6755399441055744.0 / 1024;                   // 1.5 * 2^52 / 1024: what is added keeps ten bits behind the point
         const double t = y + big, r = y - (t - big);
         const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
-        double p = __builtin_fma(r, 0.0096181291076284772, 0.055504108664821580);
-        p = __builtin_fma(p, r, 0.24022650695910071);
-        p = __builtin_fma(p, r, 0.69314718055994531);
-        p = __builtin_fma(p, r, 1.0);
-        const double one = 4503599627370496.0; // 2^52: the sum's lower bits are the rounded number
-        return __builtin_bit_cast(uint64_t, __builtin_ldexp(p * s.powers[n & 255], (n >> 8) + FRACTION) + one) - __builtin_bit_cast(uint64_t, one);
+        const double p = __builtin_fma(__builtin_fma(r, 0.24022650695910071, 0.69314718055994531), r, 1.0);
+        return __builtin_bit_cast(uint64_t, __builtin_ldexp(p * s.powers[n & 1023], (n >> 10) + FRACTION) + 4503599627370496.0);
     }
+    __device__ __forceinline__ uint64_t weight(float x) const { return raw_weight(x) - RAW; }
     __device__ __forceinline__ int bin_of(float x) const
     {
         const float v = (top - x) * per_bin;
         return v < BINS - 1 ? (int)v : BINS - 1;
     }
-    __device__ __forceinline__ bool kept(float x, int i) const
-    {
-        const uint32_t k = key_of(x);
-        return k > key || (k == key && i <= last);
-    }
-
     __device__ __forceinline__ void clear_bins()
     {
         for (int i = tid; i < BINS; i += THREADS)
@@ -192,10 +215,9 @@ struct Row {
         return reached;
     }
 
-    // moves the border to where `need` is reached; the bins hold the first division.  MASS: of weight, otherwise of tokens.  The tokens
+    // moves the border to where `need` is reached; the bins hold the first division.  mass: of weight, otherwise of tokens.  The tokens
     // counted are those above the present border, and `ties` at it.
-    template <bool MASS>
-    __device__ __forceinline__ void cut(uint64_t need)
+    __device__ __forceinline__ void cut(bool mass, uint64_t need)
     {
         if (!find(need))
             return;
@@ -205,56 +227,57 @@ struct Row {
             s.listed = 0, s.low = 0xffffffffu, s.high = 0;
         __syncthreads();
         const uint32_t old = key, old_ties = ties;
-        uint32_t low = 0xffffffffu, high = 0;
-        each([&](float x, int i) INLINE {
-            if (bin_of(x) == bin && x > -__builtin_inff() && i < a.vocab) {
-                const uint32_t k = key_of(x);
-                if (k > old || (k == old && old_ties == 0xffffffffu)) {
-                    low = min(low, k), high = max(high, k);
-                    const uint32_t at = atomicAdd(&s.listed, 1u);
-                    if (at < LIST)
-                        s.list[at] = k;
-                }
-            }
-        });
-        const bool tied = old_ties != 0xffffffffu && bin_of(score_of(old)) == bin; // the border's own ties count as many as are kept
-        if (tied)
-            low = min(low, old), high = max(high, old);
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2)
-            low = min(low, (uint32_t)__shfl_xor((int)low, o)), high = max(high, (uint32_t)__shfl_xor((int)high, o));
-        if (lane == 0)
-            atomicMin(&s.low, low), atomicMax(&s.high, high);
-        __syncthreads();
-        low = s.low, high = s.high;
-        const uint32_t listed = s.listed;
-        for (int level = 0; level < 4; level++) { // 11 bits of the interval [low, high] at a time: at most three times
+        // the border's own ties count as many as are kept
+        const bool tied = old_ties != 0xffffffffu && bin_of(score_of(old)) == bin;
+        uint32_t low = tied ? old : 0xffffffffu, high = tied ? old : 0, listed = 0;
+#pragma unroll 1
+        for (int level = 0; level < 5; level++) { // 0: what lies in the bin is listed; then 11 bits of the interval [low, high] at a time: at most three times
             const int bits = high == low ? 0 : 32 - __clz((int)(high - low)), shift = bits > 11 ? bits - 11 : 0;
-            clear_bins();
-            __syncthreads();
-            auto add = [&](uint32_t k) INLINE {
+            auto add = [&](uint32_t k, uint64_t times) INLINE {
                 if (k >= low && k <= high)
-                    atomicAdd((unsigned long long *)&s.bins[(high - k) >> shift], (unsigned long long)(MASS ? weight(score_of(k)) : 1));
+                    atomicAdd((unsigned long long *)&s.bins[(high - k) >> shift], (unsigned long long)(mass ? weight(score_of(k)) * times : times));
             };
-            if (listed <= LIST) {
-                for (uint32_t i = tid; i < listed; i += THREADS)
-                    add(s.list[i]);
-            } else
-                each([&](float x, int i) INLINE {
-                    if (bin_of(x) == bin && x > -__builtin_inff() && i < a.vocab) {
-                        const uint32_t k = key_of(x);
-                        if (k > old || (k == old && old_ties == 0xffffffffu))
-                            add(k);
+            if (level > 0) {
+                clear_bins();
+                __syncthreads();
+            }
+            if (level == 0 || listed > LIST)
+                each([&](const float(&x)[E], int) INLINE {
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        const uint32_t k = key_of(x[e]);
+                        if (bin_of(x[e]) == bin && x[e] > -__builtin_inff() && (k > old || (k == old && old_ties == 0xffffffffu))) {
+                            if (level == 0) {
+                                low = min(low, k), high = max(high, k);
+                                const uint32_t at = atomicAdd(&s.listed, 1u);
+                                if (at < LIST)
+                                    s.list[at] = k;
+                            } else
+                                add(k, 1);
+                        }
                     }
                 });
-            if (tied && tid == 0 && old >= low && old <= high)
-                atomicAdd((unsigned long long *)&s.bins[(high - old) >> shift], (unsigned long long)(MASS ? weight(score_of(old)) * old_ties : old_ties));
+            else
+                for (uint32_t i = tid; i < listed; i += THREADS)
+                    add(s.list[i], 1);
+            if (level == 0) {
+#pragma unroll
+                for (int o = 1; o < 64; o *= 2)
+                    low = min(low, (uint32_t)__shfl_xor((int)low, o)), high = max(high, (uint32_t)__shfl_xor((int)high, o));
+                if (lane == 0)
+                    atomicMin(&s.low, low), atomicMax(&s.high, high);
+                __syncthreads();
+                low = s.low, high = s.high, listed = s.listed;
+                continue;
+            }
+            if (tied && tid == 0)
+                add(old, old_ties);
             __syncthreads();
             find(need);
             need -= s.before;
             const uint32_t at = s.bin, to = high - (at << shift);
             if (shift == 0) {
-                const uint64_t each_one = MASS ? weight(score_of(to)) : 1, there = s.bins[at] / each_one, wanted = (need + each_one - 1) / each_one;
+                const uint64_t each_one = mass ? weight(score_of(to)) : 1, there = s.bins[at] / each_one, wanted = (need + each_one - 1) / each_one;
                 key = to;
                 // all of them: those of the row, or as many as an earlier border left
                 ties = wanted < there ? (uint32_t)wanted : tied && to == old ? old_ties : 0xffffffffu;
@@ -268,24 +291,13 @@ struct Row {
         }
     }
 
-    // The first index, in order, at which the running sum of f exceeds `target(sum)`; f: 64-bit whole numbers, their sum above 0.
+    // The first index, in order, at which the running sum exceeds `target(sum)`; f: the sum of some scores' numbers, and each, if asked for.
     template <class F, class T>
     __device__ __forceinline__ int locate(F f, T target)
     {
-        const int part = (a.vocab + WAVES * E - 1) / (WAVES * E) * E, from = wave * part, to = min(a.vocab, from + part);
+        const int part = (a.vocab + WAVES * E - 1) / (WAVES * E) * E, from = min(a.vocab, wave * part), to = min(a.vocab, from + part);
         uint64_t v = 0;
-        constexpr int U = E / 2, STEP = 64 * E;
-        for (int base = from + lane * E; base < to; base += U * STEP) {
-            float x[U][E];
-#pragma unroll
-            for (int u = 0; u < U; u++)
-                Scores<TYPE>::some(row, base + u * STEP, to, x[u]);
-#pragma unroll
-            for (int u = 0; u < U; u++)
-#pragma unroll
-                for (int e = 0; e < E; e++)
-                    v += f(x[u][e], base + u * STEP + e);
-        }
+        each(from, to, lane, 64, [&](const float(&x)[E], int i) INLINE { v += f(x, i, nullptr); });
 #pragma unroll
         for (int o = 1; o < 64; o *= 2)
             v += __shfl_xor(v, o);
@@ -303,23 +315,23 @@ struct Row {
         const int begin = w * part, end = min(a.vocab, begin + part);
         if (tid == 0)
             s.index = -1;
+#pragma unroll 1
         for (int base = begin; base < end; base += THREADS * E) {
             float x[E];
             const int i = base + tid * E;
             Scores<TYPE>::some(row, i, end, x);
-            uint64_t own = 0;
-#pragma unroll
-            for (int e = 0; e < E; e++)
-                own += f(x[e], i + e);
+            settle(x);
+            uint64_t own, each_one[E];
+            own = f(x, i, each_one);
             uint64_t run = front + scan(own);
             if (run <= goal && goal < run + own) {
-                int e = 0;
-                for (; e < E - 1; e++) {
-                    run += f(x[e], i + e);
-                    if (run > goal)
-                        break;
+                int at = i;
+#pragma unroll
+                for (int e = 0; e < E - 1; e++) {
+                    run += each_one[e];
+                    at += run <= goal;
                 }
-                s.index = i + e;
+                s.index = at;
             }
             __syncthreads();
             front += s.sum;
@@ -338,10 +350,13 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
     const int tid = threadIdx.x;
     const float none = -__builtin_inff();
 
-    if (tid < 256)
-        s.powers[tid] = exp2((double)tid / 256);
+    s.powers[tid] = POWERS[0][tid >> 5] * POWERS[1][tid & 31];
     float top = none;
-    r.each([&](float x, int) INLINE { top = fmaxf(top, x); });
+    r.each([&](const float(&x)[Row<TYPE>::E], int) INLINE {
+#pragma unroll
+        for (int e = 0; e < Row<TYPE>::E; e++)
+            top = fmaxf(top, x[e]);
+    });
 #pragma unroll
     for (int o = 1; o < 64; o *= 2)
         top = fmaxf(top, __shfl_xor(top, o));
@@ -351,19 +366,25 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
     for (int w = 0; w < WAVES; w++)
         top = fmaxf(top, __builtin_bit_cast(float, s.list[w]));
     __syncthreads();
-    r.top = top;
+    r.infinite = top == __builtin_inff();
+    r.top = r.infinite ? 0.0f : top;
     const float t = a.temperature ? a.temperature[blockIdx.x] : 1.0f;
     if (top == none) {
         if (tid == 0)
             a.tokens[blockIdx.x] = -1;
         return;
     }
+    top = r.top;
     if (!(t > 0)) {
         if (tid == 0)
             s.index = 0x7fffffff;
         __syncthreads();
         int first = 0x7fffffff;
-        r.each([&](float x, int i) INLINE { first = x == top ? min(first, i) : first; });
+        r.each([&](const float(&x)[Row<TYPE>::E], int i) INLINE {
+#pragma unroll
+            for (int e = 0; e < Row<TYPE>::E; e++)
+                first = x[e] == top ? min(first, i + e) : first;
+        });
 #pragma unroll
         for (int o = 1; o < 64; o *= 2)
             first = min(first, __shfl_xor(first, o));
@@ -385,57 +406,89 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
     const int k = a.top_k ? a.top_k[blockIdx.x] : 0;
     const float p = a.top_p ? a.top_p[blockIdx.x] : 1.0f;
     const bool by_count = k > 0 && k < a.vocab, by_mass = p < 1;
-    if (by_count) {
-        r.clear_bins();
-        __syncthreads();
-        r.each([&](float x, int i) INLINE {
-            if (x > none)
-                atomicAdd((unsigned long long *)&s.bins[r.bin_of(x)], 1ull);
-        });
-        __syncthreads();
-        // a border among scores without weight changes nothing
-        r.template cut<false>((uint64_t)k);
-    }
-    if (by_mass) {
+#pragma unroll 1
+    for (int filter = 0; filter < 2; filter++) { // top-k, then top-p among what it keeps
+        const bool mass = filter == 1;
+        if (!(mass ? by_mass : by_count))
+            continue;
         r.clear_bins();
         __syncthreads();
         const uint32_t key = r.key, ties = r.ties;
-        r.each([&](float x, int i) INLINE {
-            const uint32_t own = key_of(x);
-            if (x > none && (own > key || (own == key && ties == 0xffffffffu))) {
-                const uint64_t w = r.weight(x);
-                if (w)
-                    atomicAdd((unsigned long long *)&s.bins[r.bin_of(x)], (unsigned long long)w);
+        const float border = score_of(key);
+        r.each([&](const float(&x)[Row<TYPE>::E], int) INLINE {
+            bool in[Row<TYPE>::E], any = false;
+#pragma unroll
+            for (int e = 0; e < Row<TYPE>::E; e++) {
+                any |= in[e] = x[e] > border || (x[e] == border && ties == 0xffffffffu && border > none);
+            }
+            if (any) {
+                uint64_t w[Row<TYPE>::E];
+                if (mass)
+#pragma unroll
+                    for (int e = 0; e < Row<TYPE>::E; e++)
+                        w[e] = r.weight(x[e]);
+#pragma unroll
+                for (int e = 0; e < Row<TYPE>::E; e++)
+                    if (in[e])
+                        atomicAdd((unsigned long long *)&s.bins[r.bin_of(x[e])], mass ? (unsigned long long)w[e] : 1ull);
             }
         });
         if (tid == 0 && ties != 0xffffffffu)
-            atomicAdd((unsigned long long *)&s.bins[r.bin_of(score_of(key))], (unsigned long long)(r.weight(score_of(key)) * ties));
+            atomicAdd((unsigned long long *)&s.bins[r.bin_of(score_of(key))], (unsigned long long)(mass ? r.weight(score_of(key)) * ties : ties));
         __syncthreads();
-        r.scan(s.bins[2 * tid] + s.bins[2 * tid + 1]);
-        __syncthreads();
-        const double goal = p > 0 ? ceil((double)p * (double)s.sum) : 1;
-        r.template cut<true>(goal > 1 ? (uint64_t)goal : 1);
-    }
-    if (r.ties != 0xffffffffu) {
-        const uint32_t key = r.key;
-        const uint64_t before = r.ties - 1;
-        r.last = r.locate([&](float x, int) INLINE { return (uint64_t)(key_of(x) == key); }, [&](uint64_t) INLINE { return before; });
-        __syncthreads();
+        uint64_t need = (uint64_t)k; // a border among scores without weight changes nothing
+        if (mass) {
+            r.scan(s.bins[2 * tid] + s.bins[2 * tid + 1]);
+            __syncthreads();
+            const double goal = p > 0 ? ceil((double)p * (double)s.sum) : 1;
+            need = goal > 1 ? (uint64_t)goal : 1;
+        }
+        r.cut(mass, need);
     }
     const double u = (double)a.uniform[blockIdx.x];
-    const int index = r.locate(
-        [&](float x, int i) INLINE -> uint64_t {
-            if (!r.kept(x, i))
-                return 0;
-            const uint64_t w = r.weight(x);
-            return w >= r.least ? w : 0;
-        },
-        [&](uint64_t all) INLINE {
-            const double at = u > 0 ? u * (double)all : 0;
-            return at < (double)all ? (uint64_t)at : all - 1;
-        });
-    if (tid == 0)
-        a.tokens[blockIdx.x] = index;
+    constexpr uint64_t RAW = Row<TYPE>::RAW;
+    const uint64_t least = RAW + r.least;
+    const float border = score_of(r.key);
+#pragma unroll 1
+    for (int last = r.ties == 0xffffffffu; last < 2; last++) { // the last of the ties that are kept, then the token
+        const int index = r.locate(
+            [&](const float(&x)[Row<TYPE>::E], int i, uint64_t *each_one) INLINE -> uint64_t {
+                bool in[Row<TYPE>::E], any = false;
+#pragma unroll
+                for (int e = 0; e < Row<TYPE>::E; e++)
+                    any |= in[e] = last == 0 ? x[e] == border : x[e] > border || (x[e] == border && i + e <= r.last);
+                uint64_t sum = 0;
+                if (any) {
+                    uint64_t w[Row<TYPE>::E];
+#pragma unroll
+                    for (int e = 0; e < Row<TYPE>::E; e++)
+                        w[e] = last == 0 ? RAW + 1 : r.raw_weight(x[e]);
+#pragma unroll
+                    for (int e = 0; e < Row<TYPE>::E; e++) {
+                        w[e] = in[e] && (last == 0 || w[e] >= least) ? w[e] : RAW;
+                        sum += w[e];
+                        if (each_one)
+                            each_one[e] = w[e] - RAW;
+                    }
+                    sum -= RAW * Row<TYPE>::E;
+                } else if (each_one)
+#pragma unroll
+                    for (int e = 0; e < Row<TYPE>::E; e++)
+                        each_one[e] = 0;
+                return sum;
+            },
+            [&](uint64_t all) INLINE -> uint64_t {
+                if (last == 0)
+                    return r.ties - 1;
+                const double at = u > 0 ? u * (double)all : 0;
+                return at < (double)all ? (uint64_t)at : all - 1;
+            });
+        if (last == 0)
+            r.last = index;
+        else if (tid == 0)
+            a.tokens[blockIdx.x] = index;
+        __syncthreads();
+    }
 }
 
 } // namespace hipq
