@@ -55,8 +55,19 @@ def test_linear_shapes(m, n, k, group):
     check_linear(randn(g, dtype, m, k), weights(g, dtype, n, k, group, zeros=n != 17, bias=n != 31), group)
 
 
+@pytest.mark.parametrize("dtype, group, zeros", [(BF16, 128, False), (F16, 128, True), (BF16, 64, True), (F16, 64, False), (BF16, 32, True), (F16, 32, False)])
+@pytest.mark.parametrize("m, n, k, kernel", [(3, 20500, 1056, "w4_tile_16x128"), (9, 16500, 2144, "w4_tile_16x128"), (24, 9000, 2080, "w4_tile_32x128"), (33, 300, 2112, "w4_tile_32x128"),
+                                             (60, 16400, 96, "w4_tile_64x128"), (100, 400, 2112, "w4_tile_64x128"), (90, 16400, 160, "w4_tile_128x128"),
+                                             (200, 300, 2112, "w4_tile_128x128"), (150, 8200, 160, "w4_tile_128x256"), (140, 8200, 1056, "w4_tile_128x256")])
+def test_linear_kernels(m, n, k, kernel, dtype, group, zeros):
+    """Every kernel, with and without work-groups that share the reduction, and reductions that end inside a block."""
+    g = gen(m + group)
+    plan, _ = check_linear(randn(g, dtype, m, k), weights(g, dtype, n, k, group, zeros=zeros), group)
+    assert plan.kernel(m) == kernel
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu"])
-@pytest.mark.parametrize("m, n, k, group", [(1, 100, 256, 128), (16, 33, 160, 32), (20, 100, 512, 64), (70, 16, 128, 128), (210, 200, 384, 64)])
+@pytest.mark.parametrize("m, n, k, group", [(1, 100, 256, 128), (16, 33, 160, 32), (20, 100, 512, 64), (70, 16, 128, 128), (210, 200, 384, 64), (7, 10300, 1056, 128), (140, 4200, 160, 32), (50, 9000, 96, 64)])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_linear_gated(dtype, m, n, k, group, act):
     g = gen(m)
