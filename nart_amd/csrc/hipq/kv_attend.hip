@@ -13,8 +13,10 @@
 //   * Keys are read in operand order: lane c of 16 has token c, 16 bytes of it.  Values are read row by row as well, lane c the elements
 //     c DIM / 16 ..., and turned in registers: half an instruction for each value takes the halves of two tokens into one register.
 //     Nothing goes through LDS and no wave waits for another until the end.
-//   * Four waves of a work-group take tiles of 32 tokens in turn, each one tile ahead in registers; the tokens of a sequence are split over
+//   * Four waves of a work-group take tiles of 32 tokens in turn, each a tile ahead in its loads; the tokens of a sequence are split over
 //     work-groups until the chip is full, and a second kernel joins the parts.
+#include <type_traits>
+
 #include "real16.h"
 
 namespace hipq {
@@ -32,18 +34,31 @@ struct AttendArgs {
     float *part_o, *part_ml; // [sequence][head][split][row][dim], [...][row][2]
 };
 
+// an address that is the same in all lanes, kept in scalar registers: a lane's part of it is then 32 bits that stay
+typedef const uint8_t __attribute__((address_space(1))) *gbytes_t;
+__device__ static __forceinline__ gbytes_t uniform(const void *p)
+{
+    gbytes_t g = (gbytes_t)p;
+    asm("" : "+s"(g));
+    return g;
+}
+template <class T>
+__device__ static __forceinline__ T at(gbytes_t p, uint32_t offset)
+{
+    return *(const __attribute__((address_space(1))) T *)(p + offset);
+}
+
 constexpr float NONE = -__builtin_inff();
 
-// DIM values of one row in 16-bit floats or codes: what a lane reads of a key or value
+// codes 0..7 of two dwords, as 16-bit floats
 template <int TYPE>
-__device__ static __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi) // eight codes + 128 (exact in either type)
+__device__ static __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi)
 {
     u32x4 o;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const uint32_t w = i < 2 ? lo : hi;
-        const float a = (float)((w >> (16 * (i & 1))) & 255), b = (float)((w >> (16 * (i & 1) + 8)) & 255);
-        o[i] = Real16<TYPE>::pack(a, b);
+        o[i] = Real16<TYPE>::pack_exact((float)(int8_t)(w >> (16 * (i & 1))), (float)(int8_t)(w >> (16 * (i & 1) + 8)));
     }
     return o;
 }
@@ -63,16 +78,21 @@ struct Sequence {
 };
 
 template <int TYPE, int DIM, bool QUANT, int RT>
-__global__ __launch_bounds__(256) void kv_attend_kernel(const AttendArgs a)
+__global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 && DIM == 128 && RT == 2) ? 1 : 2) void kv_attend_kernel(const AttendArgs a)
 {
     using R = Real16<TYPE>;
     constexpr int KS = DIM / 32, VD = DIM / 16;       // products of a score; values of a lane
     constexpr int KW = QUANT ? DIM / 64 : DIM / 32;   // 16-byte loads of a key
     constexpr int VW = QUANT ? VD / 4 : VD / 2;       // dwords of a lane's part of a value
+    constexpr int WIDTH = QUANT ? DIM : 2 * DIM;      // bytes of a row of the cache
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, j = lane >> 4;
-    const int split = blockIdx.x % a.splits, rest = blockIdx.x / a.splits;
-    const int rb = rest % a.row_blocks, h = rest / a.row_blocks % a.cache.heads, b = rest / a.row_blocks / a.cache.heads;
+    // work-groups go to the 8 XCDs in turn: XCD x takes the x-th contiguous eighth, the row blocks that read the same tokens side by side
+    const int eighth = gridDim.x / 8, item = (int)(blockIdx.x % 8) * eighth + (int)(blockIdx.x / 8);
+    const int rb = item % a.row_blocks, split = item / a.row_blocks % a.splits, rest = item / a.row_blocks / a.splits;
+    const int h = rest % a.cache.heads, b = rest / a.cache.heads;
+    if (b >= a.d.sequences)
+        return;
     const Sequence seq(a, b);
     const int rows = seq.count * a.group, r0 = rb * 16 * RT;
     if (r0 >= rows)
@@ -82,110 +102,124 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const AttendArgs a)
     const int most = a.d.mask ? seq.len : min(seq.len, seq.old + min(rows - 1, r0 + 16 * RT - 1) / a.group + 1);
     const int t1 = min(t0 + share, most);
 
-    // queries, and what a row sees
-    u32x4 q[RT][KS];
-    f32x4 init[RT]; // codes are stored as code + 128 in the product: less 128 times the sum of q
-    int own[RT];
-    uint64_t mask[RT];
-    bool there[RT];
+    // queries
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    // in LDS where they would take the registers of a second work-group, in operand order: [rt][ks][lane], behind what the end needs
+    constexpr bool Q_LDS = RT > 1;
+    float *const lm = (float *)lds, *const ll = lm + 4 * RT * 16; // [wave][row]
+    f32x4 *const lo = (f32x4 *)(ll + 4 * RT * 16);                // [2][RT * VD][64]
+    u32x4 *const lq = (u32x4 *)(lo + 2 * RT * VD * 64);
+    u32x4 q[Q_LDS ? 1 : RT][Q_LDS ? 1 : KS];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        const int row = r0 + 16 * rt + c;
-        there[rt] = row < rows;
-        own[rt] = there[rt] ? row / a.group : 0;
-        const uint16_t *x = (const uint16_t *)a.d.q + (int64_t)(seq.row0 + own[rt]) * a.d.q_token + (int64_t)(h * a.group + (there[rt] ? row % a.group : 0)) * a.d.q_head;
-        mask[rt] = a.d.mask ? a.d.mask[seq.row0 + own[rt]] : 0;
-        float sum = 0;
+        const int row = min(r0 + 16 * rt + c, rows - 1);
+        const uint16_t *x = (const uint16_t *)a.d.q + (int64_t)(seq.row0 + row / a.group) * a.d.q_token + (int64_t)(h * a.group + row % a.group) * a.d.q_head;
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
-            q[rt][ks] = *(const u32x4 *)(x + (QUANT ? ks / 2 * 64 + j * 16 + ks % 2 * 8 : ks * 32 + j * 8));
-            if (QUANT)
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    sum += R::low(q[rt][ks][e]) + R::high(q[rt][ks][e]);
+            const u32x4 *from = (const u32x4 *)(x + (QUANT ? ks / 2 * 64 + j * 16 + ks % 2 * 8 : ks * 32 + j * 8));
+            if (!Q_LDS)
+                q[Q_LDS ? 0 : rt][Q_LDS ? 0 : ks] = *from;
+            else if ((rt * KS + ks) % 4 == wave)
+                lq[(rt * KS + ks) * 64 + lane] = *from;
         }
-        if (QUANT) {
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-        }
-        const float s = QUANT ? -128.0f * sum : 0.0f;
-        init[rt] = f32x4{s, s, s, s};
     }
+    if (Q_LDS)
+        __syncthreads();
 
-    float m[RT], l[RT], lv[RT]; // lv: the sum of what multiplies the codes
-    float unit = 0;             // float16 codes: p is multiplied by value scale / unit, unit the largest scale so far or more, to stay in range
+    float m[RT], l[RT];
+    f32x4 lsum[RT]; // 16 bits: the sums of p, by a multiply by ones
+    float unit = 0; // float16 codes: p is multiplied by value scale / unit, unit the largest scale so far or more, to stay in range
     f32x4 o[RT][VD];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        m[rt] = NONE, l[rt] = lv[rt] = 0;
+        m[rt] = NONE, l[rt] = 0;
+        lsum[rt] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < VD; i++)
             o[rt][i] = f32x4{0, 0, 0, 0};
     }
 
     // a tile: two halves of 16 tokens, each in one page
+    struct Pages {
+        int page[2]; // -1: not there
+        int place[2];
+    };
     u32x4 kx[2][KW];
     uint32_t vx[2][4][VW];
     f32x4 ksc[2], vsc[2];
-    bool half_there[2];
     const int32_t *blocks = a.d.blocks + (int64_t)b * a.d.blocks_stride;
     const int halves = (seq.len + 15) / 16, page16 = a.cache.page / 16;
-    auto load = [&](int t) {
+    auto pages_of = [&](int t) {
+        Pages p;
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             const int t16 = t / 16 + s;
-            int at = a.page_magic ? (int)(((uint64_t)(uint32_t)t16 * a.page_magic) >> 32) >> a.page_shift : t16;
-            const int in = t16 - at * page16;
-            int page = t16 < halves ? blocks[at] : -1;
-            half_there[s] = page >= 0 && page < a.cache.pages;
-            page = half_there[s] ? page : 0;
-            const int64_t row = ((int64_t)page * a.cache.heads + h) * a.cache.page + in * 16;
-            const uint8_t *k = (const uint8_t *)a.cache.k + row * (QUANT ? DIM : 2 * DIM), *v = (const uint8_t *)a.cache.v + row * (QUANT ? DIM : 2 * DIM);
+            const int at = a.page_magic ? (int)(((uint64_t)(uint32_t)t16 * a.page_magic) >> 32) >> a.page_shift : t16;
+            const int page = __builtin_amdgcn_readfirstlane(t16 < halves ? blocks[at] : -1);
+            p.page[s] = page >= 0 && page < a.cache.pages ? page : -1;
+            p.place[s] = (t16 - at * page16) * 16;
+        }
+        return p;
+    };
+    auto row_of = [&](const Pages &p, int s) { return ((int64_t)max(p.page[s], 0) * a.cache.heads + h) * a.cache.page + p.place[s]; };
+    auto load_k = [&](const Pages &p) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const int64_t row = row_of(p, s);
+            const gbytes_t k = uniform((const uint8_t *)a.cache.k + row * WIDTH);
 #pragma unroll
             for (int i = 0; i < KW; i++)
-                kx[s][i] = *(const u32x4 *)(k + c * (QUANT ? DIM : 2 * DIM) + i * 64 + j * 16);
+                kx[s][i] = at<u32x4>(k, c * WIDTH + j * 16 + i * 64);
+            if (QUANT)
+                ksc[s] = at<f32x4>(uniform(a.cache.k_scale + row), j * 16);
+        }
+    };
+    auto load_v = [&](const Pages &p) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const int64_t row = row_of(p, s);
+            const gbytes_t v = uniform((const uint8_t *)a.cache.v + row * WIDTH);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const uint8_t *from = v + (j * 4 + r) * (QUANT ? DIM : 2 * DIM) + c * (4 * VW);
+                const uint32_t from = (j * 4 + r) * WIDTH + c * (4 * VW);
                 if (VW == 1)
-                    vx[s][r][0] = *(const uint32_t *)from;
+                    vx[s][r][0] = at<uint32_t>(v, from);
                 else if (VW == 2) {
-                    const u32x2 w = *(const u32x2 *)from;
+                    const u32x2 w = at<u32x2>(v, from);
                     vx[s][r][0] = w[0], vx[s][r][VW - 1] = w[1];
                 } else
 #pragma unroll
                     for (int i = 0; i < VW; i += 4) {
-                        const u32x4 w = *(const u32x4 *)(from + 4 * i);
+                        const u32x4 w = at<u32x4>(v, from + 4 * i);
 #pragma unroll
                         for (int e = 0; e < 4 && i + e < VW; e++)
                             vx[s][r][i + e] = w[e];
                     }
             }
-            if (QUANT) {
-                ksc[s] = *(const f32x4 *)(a.cache.k_scale + row + j * 4);
-                vsc[s] = *(const f32x4 *)(a.cache.v_scale + row + j * 4);
-            }
+            if (QUANT)
+                vsc[s] = at<f32x4>(uniform(a.cache.v_scale + row), j * 16);
         }
     };
 
-    auto tile = [&](int t) {
-        // scores
-        f32x4 s[RT][2];
+    // The next tile's keys are asked for when this one's are multiplied, its values when this one's are: each has the other's work to
+    // arrive in, and no second set of registers.  (Behind the last tile something is loaded once more, for nothing: a branch around it
+    // would make every wait one for all loads.)  MASKED: not all rows see the whole tile.
+    auto tile = [&](int t, const Pages &now, const Pages &next, auto MASKED) __attribute__((always_inline)) {
+        constexpr bool masked = decltype(MASKED)::value;
+        u32x4 k[2][KS];
 #pragma unroll
         for (int half = 0; half < 2; half++)
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                u32x4 k;
-                if (QUANT)
-                    k = widen<TYPE>(kx[half][ks / 2][ks % 2 * 2] ^ 0x80808080u, kx[half][ks / 2][ks % 2 * 2 + 1] ^ 0x80808080u);
-                else
-                    k = kx[half][ks];
+            for (int ks = 0; ks < KS; ks++)
+                k[half][ks] = QUANT ? widen<TYPE>(kx[half][ks / (QUANT ? 2 : 1)][ks % 2 * 2], kx[half][ks / (QUANT ? 2 : 1)][ks % 2 * 2 + 1]) : kx[half][ks / (QUANT ? 2 : 1)];
+        float kscale[2][4];
+        if (QUANT)
 #pragma unroll
-                for (int rt = 0; rt < RT; rt++)
-                    s[rt][half] = R::mfma(k, q[rt][ks], ks ? s[rt][half] : init[rt]);
-            }
-        // all rows see the whole tile unless it holds a new token, the end, or a page that is not there
-        const bool masked = t + 32 > min(seq.old, seq.len) || !half_there[0] || !half_there[1];
+            for (int e = 0; e < 8; e++)
+                kscale[e / 4][e % 4] = ksc[e / 4][e % 4] * a.scale2;
+        __builtin_amdgcn_sched_barrier(0); // what is done earlier than it is written does not fit the registers
+        load_k(next);
+        __builtin_amdgcn_sched_barrier(0);
         bool strange = false;
         if (masked) {
             // tokens that are not there may hold anything: their values are taken as 0, so that 0 times them is 0
@@ -193,7 +227,7 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const AttendArgs a)
             for (int half = 0; half < 2; half++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const bool in = half_there[half] && t + half * 16 + j * 4 + r < seq.len;
+                    const bool in = now.page[half] >= 0 && t + half * 16 + j * 4 + r < seq.len;
                     if (QUANT)
                         vsc[half][r] = in ? vsc[half][r] : 0.0f;
 #pragma unroll
@@ -217,12 +251,10 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const AttendArgs a)
                 const float f = unit / top; // 0 at the first, where nothing is there to be scaled
                 unit = top;
 #pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    lv[rt] *= f;
+                for (int rt = 0; rt < RT; rt++)
 #pragma unroll
                     for (int i = 0; i < VD; i++)
                         o[rt][i] *= f;
-                }
             }
             const float f = unit > 0 ? 1.0f / unit : 0.0f;
             vsc[0] *= f, vsc[1] *= f;
@@ -231,55 +263,69 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const AttendArgs a)
         u32x4 seen[RT]; // where values are infinite or NaN: ones at the tokens that a row sees
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
+            f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int half = 0; half < 2; half++)
+                    s[half] = R::mfma(k[half][ks], Q_LDS ? lq[(rt * KS + ks) * 64 + lane] : q[Q_LDS ? 0 : rt][Q_LDS ? 0 : ks], s[half]);
             float x[8], top = NONE;
             uint32_t sees = 0;
+            // what a row sees is looked up again for every such tile: there are few, and it would be in the way in all others
+            const int row = r0 + 16 * rt + c, own = row / a.group;
+            const uint64_t mask = masked && a.d.mask && row < rows ? a.d.mask[seq.row0 + own] : 0;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const int half = e / 4, r = e % 4, token = t + half * 16 + j * 4 + r;
-                x[e] = s[rt][half][r] * a.scale2;
-                if (QUANT)
-                    x[e] *= ksc[half][r];
+                x[e] = QUANT ? s[half][r] * kscale[half][r] : s[half][r];
                 if (masked) {
                     const int fresh = token - seq.old;
-                    const bool see = half_there[half] && token < seq.len && there[rt] &&
-                                     (fresh < 0 || (a.d.mask ? fresh < 64 && ((mask[rt] >> (fresh & 63)) & 1) : fresh <= own[rt]));
+                    const bool see = now.page[half] >= 0 && token < seq.len && row < rows &&
+                                     (fresh < 0 || (a.d.mask ? fresh < 64 && ((mask >> (fresh & 63)) & 1) : fresh <= own));
                     sees |= (uint32_t)see << e;
                     x[e] = see ? x[e] : NONE;
                 }
                 top = fmaxf(top, x[e]);
             }
+            if (!QUANT)
+                top *= a.scale2;
+            // outputs are scaled by 1 where the reference stays: scaled only where it moves, they were copied around that branch
+            float f = 1.0f;
             if (__any(top > m[rt] + 8.0f)) {
                 top = fmaxf(top, m[rt]);
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
-                const float f = top == NONE ? 1.0f : exp2_fast(m[rt] - top);
+                f = top == NONE ? 1.0f : exp2_fast(m[rt] - top);
                 m[rt] = top;
-                l[rt] *= f, lv[rt] *= f;
-#pragma unroll
-                for (int i = 0; i < VD; i++)
-                    o[rt][i] *= f;
             }
+            asm("" : "+v"(f)); // or the products go into the branch all the same
+            l[rt] *= f;
+            lsum[rt] *= f;
+#pragma unroll
+            for (int i = 0; i < VD; i++)
+                o[rt][i] *= f;
             const float ref = m[rt] == NONE ? 0.0f : m[rt];
             float y[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                y[e] = exp2_fast(x[e] - ref);
-                l[rt] += y[e];
+                y[e] = exp2_fast(QUANT ? x[e] - ref : __builtin_fmaf(x[e], a.scale2, -ref));
                 if (QUANT) {
+                    l[rt] += y[e];
                     y[e] *= vsc[e / 4][e % 4];
                     if (masked)
                         y[e] = (sees >> e) & 1 ? y[e] : 0.0f;
                 }
             }
+            const uint32_t one = R::pack(1.0f, 0.0f);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 p[rt][e] = R::pack(y[2 * e], y[2 * e + 1]);
-                if (QUANT)
-                    lv[rt] += R::low(p[rt][e]) + R::high(p[rt][e]);
-                const uint32_t one = R::pack(1.0f, 0.0f);
                 seen[rt][e] = ((sees >> (2 * e)) & 1 ? one : 0) | ((sees >> (2 * e + 1)) & 1 ? one << 16 : 0);
             }
+            if (!QUANT)
+                lsum[rt] = R::mfma(u32x4{one * 0x10001u, one * 0x10001u, one * 0x10001u, one * 0x10001u}, p[rt], lsum[rt]);
         }
+        __builtin_amdgcn_sched_barrier(0);
         // output
         const bool any_strange = masked && __any(strange);
 #pragma unroll
@@ -288,20 +334,18 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const AttendArgs a)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int half = e / 2, r = e % 2 * 2;
-                if (QUANT) {
-                    const float x0 = (float)(((vx[half][r][i / 4] ^ 0x80808080u) >> (8 * (i % 4))) & 255),
-                                x1 = (float)(((vx[half][r + 1][i / 4] ^ 0x80808080u) >> (8 * (i % 4))) & 255);
-                    v[e] = R::pack(x0, x1);
-                } else
+                if (QUANT)
+                    v[e] = R::pack_exact((float)(int8_t)(vx[half][r][i / 4] >> (8 * (i % 4))), (float)(int8_t)(vx[half][r + 1][i / 4] >> (8 * (i % 4))));
+                else
                     v[e] = __builtin_amdgcn_perm(vx[half][r + 1][i / 2], vx[half][r][i / 2], i % 2 ? 0x07060302u : 0x05040100u);
             }
             if (!QUANT && any_strange) {
                 // an infinity or NaN among the values near the end reaches the rows that see it, as NaN, and no other
                 u32x4 bad = {0, 0, 0, 0};
+                const uint32_t one = R::pack(1.0f, 0.0f);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const bool lo = !(fabsf(R::low(v[e])) < __builtin_inff()), hi = !(fabsf(R::high(v[e])) < __builtin_inff());
-                    const uint32_t one = R::pack(1.0f, 0.0f);
                     bad[e] = (lo ? one : 0) | (hi ? one << 16 : 0);
                     v[e] &= (lo ? 0 : 0xffffu) | (hi ? 0 : 0xffff0000u);
                 }
@@ -317,34 +361,42 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const AttendArgs a)
             for (int rt = 0; rt < RT; rt++)
                 o[rt][i] = R::mfma(v, p[rt], o[rt][i]);
         }
+        load_v(next);
     };
 
-    for (int t = t0 + wave * 32; t < t1; t += 128) {
-        load(t);
-        tile(t);
+    int t = t0 + wave * 32;
+    if (t < t1) {
+        Pages now = pages_of(t), next = pages_of(t + 128);
+        load_k(now);
+        load_v(now);
+        // all rows see a whole tile unless it holds a new token, the end, or a page that is not there; from the first such tile on each is
+        // looked at token by token
+        const int clear = min(min(seq.old, seq.len), t1);
+        while (t + 32 <= clear && now.page[0] >= 0 && now.page[1] >= 0) {
+            const Pages after = pages_of(t + 256);
+            tile(t, now, next, std::false_type{});
+            now = next, next = after, t += 128;
+        }
+        for (; t < t1; t += 128) {
+            const Pages after = pages_of(t + 256);
+            tile(t, now, next, std::true_type{});
+            now = next, next = after;
+        }
     }
 
     // the four waves' parts: a row's reference and sums over its lanes, then over the waves, then the outputs in two steps
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    float *lm = (float *)lds, *ll = lm + 4 * RT * 16; // [wave][row]
-    f32x4 *lo = (f32x4 *)(ll + 4 * RT * 16);          // [2][RT * VD][64]
     float f[RT], sum[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        l[rt] += __shfl_xor(l[rt], 16);
-        l[rt] += __shfl_xor(l[rt], 32);
         if (QUANT) {
-            lv[rt] += __shfl_xor(lv[rt], 16);
-            lv[rt] += __shfl_xor(lv[rt], 32);
-            const float less = -128.0f * lv[rt];
-#pragma unroll
-            for (int i = 0; i < VD; i++)
-                o[rt][i] += less;
+            l[rt] += __shfl_xor(l[rt], 16);
+            l[rt] += __shfl_xor(l[rt], 32);
             if (TYPE == HIPQ_REAL_F16)
 #pragma unroll
                 for (int i = 0; i < VD; i++)
                     o[rt][i] *= unit;
-        }
+        } else
+            l[rt] = lsum[rt][0];
         if (j == 0)
             lm[wave * RT * 16 + rt * 16 + c] = m[rt], ll[wave * RT * 16 + rt * 16 + c] = l[rt];
     }
@@ -387,12 +439,12 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const AttendArgs a)
         return;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        if (!there[rt])
-            continue;
         const int row = r0 + 16 * rt + c;
+        if (row >= rows)
+            continue;
         if (a.splits == 1) {
             const float inv = sum[rt] > 0 ? 1.0f / sum[rt] : sum[rt] == 0 ? 0.0f : sum[rt];
-            uint16_t *y = (uint16_t *)a.d.o + (int64_t)(seq.row0 + own[rt]) * a.d.o_token + (int64_t)(h * a.group + row % a.group) * a.d.o_head;
+            uint16_t *y = (uint16_t *)a.d.o + (int64_t)(seq.row0 + row / a.group) * a.d.o_token + (int64_t)(h * a.group + row % a.group) * a.d.o_head;
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
@@ -413,33 +465,47 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(const AttendArgs a)
     }
 }
 
-// Joins the parts of a row: DIM / 4 neighbouring lanes have a row.
-template <int TYPE, int DIM>
+// Joins the parts of a row: DIM / 4 lanes side by side have its elements, SIDE such groups of a work-group its parts in turn.
+template <int TYPE, int DIM, int SIDE>
 __global__ __launch_bounds__(256) void kv_attend_join_kernel(const AttendArgs a)
 {
     using R = Real16<TYPE>;
-    constexpr int LANES = DIM / 4;
-    const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
-    const int i0 = threadIdx.x % LANES * 4, bh = (int)(id / a.rows), row = (int)(id % a.rows);
-    if (bh >= a.d.sequences * a.cache.heads)
-        return;
-    const int b = bh / a.cache.heads, h = bh % a.cache.heads;
-    const Sequence seq(a, b);
-    if (row >= seq.count * a.group)
-        return;
+    constexpr int LANES = DIM / 4, ROWS = 256 / LANES / SIDE;
+    __shared__ f32x4 lo[SIDE > 1 ? 256 : 1];
+    __shared__ float ll[SIDE > 1 ? 256 / LANES : 1];
+    const int tid = threadIdx.x, i0 = tid % LANES * 4, side = tid / LANES % SIDE;
+    const int64_t id = (int64_t)blockIdx.x * ROWS + tid / LANES / SIDE;
+    const int bh = (int)(id / a.rows), row = (int)(id % a.rows), b = bh / a.cache.heads, h = bh % a.cache.heads;
+    const bool in = bh < a.d.sequences * a.cache.heads;
+    const Sequence seq(a, in ? b : 0);
+    const bool there = in && row < seq.count * a.group;
     const int64_t at = (int64_t)bh * a.splits * a.rows + row;
-    float top = NONE;
-    for (int s = 0; s < a.splits; s++)
-        top = fmaxf(top, a.part_ml[2 * (at + (int64_t)s * a.rows)]);
-    const float ref = top == NONE ? 0.0f : top;
-    float l = 0;
+    float top = NONE, l = 0;
     f32x4 o = {0, 0, 0, 0};
-    for (int s = 0; s < a.splits; s++) {
-        const int64_t p = at + (int64_t)s * a.rows;
-        const float f = exp2_fast(a.part_ml[2 * p] - ref);
-        l += f * a.part_ml[2 * p + 1];
-        o += f * *(const f32x4 *)(a.part_o + p * DIM + i0);
+    if (there) {
+        for (int s = 0; s < a.splits; s++)
+            top = fmaxf(top, a.part_ml[2 * (at + (int64_t)s * a.rows)]);
+        const float ref = top == NONE ? 0.0f : top;
+        for (int s = side; s < a.splits; s += SIDE) {
+            const int64_t p = at + (int64_t)s * a.rows;
+            const float f = exp2_fast(a.part_ml[2 * p] - ref);
+            l += f * a.part_ml[2 * p + 1];
+            o += f * *(const f32x4 *)(a.part_o + p * DIM + i0);
+        }
     }
+    if (SIDE > 1) {
+        lo[SIDE > 1 ? tid : 0] = o;
+        if (i0 == 0)
+            ll[SIDE > 1 ? tid / LANES : 0] = l;
+        __syncthreads();
+        if (side > 0)
+            return;
+#pragma unroll
+        for (int u = 1; u < SIDE; u++)
+            o += lo[SIDE > 1 ? u * LANES + tid : 0], l += ll[SIDE > 1 ? tid / LANES + u : 0];
+    }
+    if (!there)
+        return;
     const float inv = l > 0 ? 1.0f / l : l == 0 ? 0.0f : l;
     uint16_t *y = (uint16_t *)a.d.o + (int64_t)(seq.row0 + row / a.group) * a.d.o_token + (int64_t)(h * a.group + row % a.group) * a.d.o_head;
     const u32x2 w = {R::pack(o[0] * inv, o[1] * inv), R::pack(o[2] * inv, o[3] * inv)};
@@ -465,7 +531,7 @@ static int check_attend(const hipq_kv_cache *c, const hipq_kv_attend_desc *d)
     HIPQ_REQUIRE(d->blocks_per_sequence >= 0 && (int64_t)d->blocks_per_sequence * c->page < ((int64_t)1 << 31), "attend: %d blocks of a sequence", d->blocks_per_sequence);
     HIPQ_REQUIRE(d->blocks_stride >= d->blocks_per_sequence || d->sequences <= 1, "attend: rows of blocks overlap");
     HIPQ_REQUIRE(d->longest >= 0, "attend: the longest sequence has %d tokens", d->longest);
-    HIPQ_REQUIRE(d->scale == d->scale && d->scale < 1e30f && d->scale > -1e30f, "attend: scale %g", (double)d->scale);
+    HIPQ_REQUIRE(d->scale > 0 && d->scale < 1e30f, "attend: scale %g", (double)d->scale);
     const int64_t rows = (int64_t)d->most_new * (d->q_heads / c->heads);
     HIPQ_REQUIRE(rows < (1 << 24), "attend: %lld rows of a sequence", (long long)rows);
     return 0;
@@ -476,11 +542,13 @@ static AttendShape shape_of(const hipq_kv_cache *c, const hipq_kv_attend_desc *d
     AttendShape s = {};
     const int group = d->q_heads / c->heads;
     s.rows = d->most_new * group;
-    s.rt = s.rows <= 16 ? 1 : s.rows <= 32 || c->dim == 256 ? 2 : 4;
+    s.rt = s.rows <= 16 || c->dim == 256 ? 1 : 2; // two blocks of 256-wide outputs are all of a wave's registers
     s.row_blocks = (s.rows + 16 * s.rt - 1) / (16 * s.rt);
     const int64_t longest = d->longest < (int64_t)d->blocks_per_sequence * c->page ? d->longest : (int64_t)d->blocks_per_sequence * c->page;
     const int64_t items = (int64_t)d->sequences * c->heads * s.row_blocks;
-    const int64_t want = items ? (512 + items - 1) / items : 1, most = (longest + 255) / 256;
+    // A work-group a CU is enough, and two where that leaves some with a longer sequence than others: us with 256, 512 and 1024 work-groups of
+    // 8 trees of 16 tokens on 4096: 38, 42, 54; one token on 2 x 131072: 186, 197, 201; of 32 sequences up to 4096 in 8 bits: 62, 52, 55
+    const int64_t target = items < 256 ? 256 : 512, want = items ? (target + items - 1) / items : 1, most = (longest + 255) / 256;
     s.splits = (int)(want < most ? want : most);
     s.splits = s.splits < 1 ? 1 : s.splits > 64 ? 64 : s.splits;
     if (s.splits > 1)
@@ -491,7 +559,7 @@ static AttendShape shape_of(const hipq_kv_cache *c, const hipq_kv_attend_desc *d
 template <int TYPE, int DIM, bool QUANT, int RT>
 static int launch_attend(const AttendArgs &a, int64_t items, hipStream_t st)
 {
-    const size_t lds = (2 * 4 * RT * 16) * 4 + (size_t)2 * RT * (DIM / 16) * 64 * 16;
+    const size_t lds = (2 * 4 * RT * 16) * 4 + (size_t)2 * RT * (DIM / 16) * 64 * 16 + (RT > 1 ? (size_t)RT * (DIM / 32) * 1024 : 0);
     static thread_local bool allowed[64] = {};
     int device = 0;
     HIPQ_CHECK_HIP(hipGetDevice(&device));
@@ -500,18 +568,14 @@ static int launch_attend(const AttendArgs &a, int64_t items, hipStream_t st)
         if (device < 64)
             allowed[device] = true;
     }
-    kv_attend_kernel<TYPE, DIM, QUANT, RT><<<dim3((unsigned)(items * a.splits)), dim3(256), lds, st>>>(a);
+    kv_attend_kernel<TYPE, DIM, QUANT, RT><<<dim3((unsigned)((items * a.splits + 7) / 8 * 8)), dim3(256), lds, st>>>(a);
     return launch_status("kv_attend_kernel");
 }
 
 template <int TYPE, int DIM, bool QUANT>
 static int launch_attend(const AttendArgs &a, int rt, int64_t items, hipStream_t st)
 {
-    if (rt == 1)
-        return launch_attend<TYPE, DIM, QUANT, 1>(a, items, st);
-    if (rt == 2 || DIM == 256)
-        return launch_attend<TYPE, DIM, QUANT, 2>(a, items, st);
-    return launch_attend<TYPE, DIM, QUANT, DIM == 256 ? 2 : 4>(a, items, st);
+    return rt == 1 ? launch_attend<TYPE, DIM, QUANT, 1>(a, items, st) : launch_attend<TYPE, DIM, QUANT, DIM == 256 ? 1 : 2>(a, items, st);
 }
 
 template <int TYPE, int DIM>
@@ -521,8 +585,13 @@ static int launch_attend(const AttendArgs &a, int rt, int64_t items, hipStream_t
         return 1;
     if (a.splits == 1)
         return 0;
-    const int64_t threads = (int64_t)a.d.sequences * a.cache.heads * a.rows * (DIM / 4);
-    kv_attend_join_kernel<TYPE, DIM><<<dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st>>>(a);
+    // few rows of many parts: the parts side by side, all groups of a work-group at one row
+    const int64_t rows = (int64_t)a.d.sequences * a.cache.heads * a.rows;
+    constexpr int GROUPS = 1024 / DIM;
+    if (rows <= 4096 && a.splits >= 8)
+        kv_attend_join_kernel<TYPE, DIM, GROUPS><<<dim3((unsigned)rows), dim3(256), 0, st>>>(a);
+    else
+        kv_attend_join_kernel<TYPE, DIM, 1><<<dim3((unsigned)((rows + GROUPS - 1) / GROUPS)), dim3(256), 0, st>>>(a);
     return launch_status("kv_attend_join_kernel");
 }
 
@@ -555,7 +624,7 @@ extern "C" int hipq_kv_attend(const hipq_kv_cache *cache, const hipq_kv_attend_d
     HIPQ_REQUIRE(((uintptr_t)d->q | (uintptr_t)d->o) % 16 == 0 && (d->q_token | d->q_head | d->o_token | d->o_head) % 8 == 0,
                  "attend: heads have to start at multiples of 16 bytes");
     HIPQ_REQUIRE(s.workspace == 0 || (workspace && workspace_bytes >= s.workspace && (uintptr_t)workspace % 16 == 0), "attend: a workspace of %zu bytes is needed", s.workspace);
-    HIPQ_REQUIRE(items * s.splits < ((int64_t)1 << 31), "attend: %lld work-groups", (long long)items * s.splits);
+    HIPQ_REQUIRE(items * s.splits * 16 * s.rt < ((int64_t)1 << 31), "attend: %lld work-groups", (long long)items * s.splits);
     AttendArgs a = {};
     a.cache = *cache, a.d = *d;
     if (cache->pages == 0)

@@ -27,6 +27,8 @@ struct Real16<HIPQ_REAL_BF16> {
         const bf16x2 v = {(__bf16)a, (__bf16)b};
         return __builtin_bit_cast(uint32_t, v);
     }
+    // of numbers that the type holds
+    __device__ static __forceinline__ uint32_t pack_exact(float a, float b) { return pack(a, b); }
     // 16 x 16 products over k = 32: a lane holds row (a) or column (b) lane % 16, k = 8 (lane / 16) + 0..7; of the result column
     // lane % 16, rows 4 (lane / 16) + 0..3
     __device__ static __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c)
@@ -44,6 +46,8 @@ struct Real16<HIPQ_REAL_F16> {
         const f16x2 v = {(_Float16)a, (_Float16)b};
         return __builtin_bit_cast(uint32_t, v);
     }
+    // one instruction, which rounds to zero, instead of three
+    __device__ static __forceinline__ uint32_t pack_exact(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)); }
     __device__ static __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
