@@ -16,7 +16,7 @@
 
 namespace hipq {
 
-constexpr int THREADS = 1024, WAVES = THREADS / 64, BINS = 2048, LIST = 4096, FRACTION = 43;
+constexpr int THREADS = 1024, WAVES = THREADS / 64, BINS = 2048, LIST = 4096, FEW = THREADS, FRACTION = 43;
 constexpr int MOST_VOCAB = 1 << 20; // sums of weights fit 64 bits
 
 // 2^(i / 32) and 2^(i / 1024)
@@ -42,10 +42,13 @@ struct SampleArgs {
 
 struct SampleShared {
     uint64_t bins[BINS];
-    uint32_t list[LIST];
+    union {
+        uint32_t list[LIST];
+        uint64_t few[FEW];
+    };
     double powers[1024]; // 2^(i / 1024)
-    uint64_t wave[WAVES];
-    uint64_t sum, before;
+    uint64_t wave[WAVES], region[WAVES];
+    uint64_t before;
     uint32_t bin, listed, low, high;
     float top;
     int index;
@@ -53,40 +56,46 @@ struct SampleShared {
 
 template <int TYPE>
 struct Scores {
-    static constexpr int E = TYPE == HIPQ_REAL_F32 ? 4 : 8; // of a 16-byte load
-    struct __attribute__((packed, aligned(TYPE == HIPQ_REAL_F32 ? 4 : 2))) Vec {
-        u32x4 v;
+    static constexpr int SIZE = TYPE == HIPQ_REAL_F32 ? 4 : 2, WORD = 4 / SIZE, LOAD = 4 * WORD; // scores of a word and of a 16-byte load
+    static constexpr uint32_t NONE = TYPE == HIPQ_REAL_F32 ? 0xff800000u : TYPE == HIPQ_REAL_F16 ? 0xfc00fc00u : 0xff80ff80u; // -infinity
+    template <int N>
+    struct __attribute__((packed, aligned(SIZE))) Words {
+        uint32_t v __attribute__((ext_vector_type(N)));
     };
-    __device__ static __forceinline__ float one(const void *row, int i)
+    // N words from score i on, those behind the end as -infinity
+    template <int N>
+    __device__ static __forceinline__ void load(const void *row, int i, int end, uint32_t (&v)[N])
     {
-        if (TYPE == HIPQ_REAL_F32)
-            return ((const float *)row)[i];
-        return Real16<TYPE == HIPQ_REAL_F32 ? HIPQ_REAL_F16 : TYPE>::low(((const uint16_t *)row)[i]);
-    }
-    // elements i .. i + E - 1, those behind the end as -infinity
-    __device__ static __forceinline__ void some(const void *row, int i, int end, float (&x)[E])
-    {
-        if (i + E <= end) {
-            const u32x4 v = ((const Vec *)((const uint8_t *)row + (int64_t)i * (16 / E)))->v;
+        if (i + N * WORD <= end) {
+            const auto w = ((const Words<N> *)((const uint8_t *)row + (int64_t)i * SIZE))->v;
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                using R = Real16<TYPE == HIPQ_REAL_F32 ? HIPQ_REAL_F16 : TYPE>;
-                x[e] = TYPE == HIPQ_REAL_F32 ? __builtin_bit_cast(float, (uint32_t)v[e % 4]) : e & 1 ? R::high(v[e / 2]) : R::low(v[e / 2]);
-            }
+            for (int n = 0; n < N; n++)
+                v[n] = w[n];
         } else {
 #pragma unroll
-            for (int e = 0; e < E; e++)
-                x[e] = -__builtin_inff();
+            for (int n = 0; n < N; n++)
+                v[n] = NONE;
             if (i < end) { // all at once: one after the other, eight loads took 3 us
-                float y[E];
+                uint32_t y[N * WORD];
 #pragma unroll
-                for (int e = 0; e < E; e++)
-                    y[e] = one(row, min(i + e, end - 1));
+                for (int e = 0; e < N * WORD; e++) {
+                    const int at = min(i + e, end - 1);
+                    y[e] = SIZE == 4 ? ((const uint32_t *)row)[at] : ((const uint16_t *)row)[at];
+                }
 #pragma unroll
-                for (int e = 0; e < E; e++)
-                    x[e] = i + e < end ? y[e] : x[e];
+                for (int e = 0; e < N * WORD; e++) {
+                    const uint32_t one = i + e < end ? y[e] : SIZE == 4 ? NONE : NONE & 0xffffu;
+                    v[e / WORD] = SIZE == 4 ? one : e % WORD ? v[e / WORD] | one << 16 : one;
+                }
             }
         }
+    }
+    __device__ static __forceinline__ void four(const uint32_t *v, float (&x)[4])
+    {
+        using R = Real16<TYPE == HIPQ_REAL_F32 ? HIPQ_REAL_F16 : TYPE>;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            x[e] = SIZE == 4 ? __builtin_bit_cast(float, v[e]) : e & 1 ? R::high(v[e / 2]) : R::low(v[e / 2]);
     }
 };
 
@@ -101,9 +110,34 @@ __device__ static __forceinline__ float score_of(uint32_t key)
     return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
+__device__ static __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ static __forceinline__ uint64_t uniform(uint64_t v) { return (uint64_t)uniform((uint32_t)(v >> 32)) << 32 | uniform((uint32_t)v); }
+__device__ static __forceinline__ float uniform(float v) { return __builtin_bit_cast(float, uniform(__builtin_bit_cast(uint32_t, v))); }
+__device__ static __forceinline__ uint64_t of_lane(uint64_t v, int lane)
+{
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+// v plus that of the lane which HOW names, in the rows of 16 lanes that ROWS has a bit for; 0 where there is none
+template <int HOW, int ROWS = 15>
+__device__ static __forceinline__ uint64_t plus(uint64_t v)
+{
+    return v + ((uint64_t)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), HOW, ROWS, 15, false) << 32 |
+                (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, HOW, ROWS, 15, false));
+}
+// sums up to each lane: of its 16 lanes, and of all 64
+__device__ static __forceinline__ uint64_t sums16(uint64_t v)
+{
+    return plus<0x118>(plus<0x114>(plus<0x112>(plus<0x111>(v)))); // lanes 1, 2, 4, 8 in front
+}
+__device__ static __forceinline__ uint64_t sums64(uint64_t v)
+{
+    return plus<0x143, 12>(plus<0x142, 10>(sums16(v))); // the last lane of the row in front, that of the first two rows
+}
+
 template <int TYPE>
 struct Row {
-    static constexpr int E = Scores<TYPE>::E;
+    using S = Scores<TYPE>;
+    static constexpr int E = 4; // scores that a pass works on at a time
     const SampleArgs &a;
     SampleShared &s;
     const void *row;
@@ -115,6 +149,7 @@ struct Row {
     uint32_t key = 0x007fffffu /* -infinity's */, ties = 0xffffffffu;
     int last = 0x7fffffff;
     uint64_t least = 0; // smallest weight that min-p keeps
+    uint64_t sum = 0;   // of the last scan
 
     __device__ Row(const SampleArgs &a_, SampleShared &s_) : a(a_), s(s_)
     {
@@ -131,22 +166,28 @@ struct Row {
                 x[e] = x[e] == __builtin_inff() ? 0.0f : -__builtin_inff();
     }
 
-    // f(scores, index of the first) of the row's part [from, to), 16 bytes at a time, `lanes` threads side by side, the next 16 bytes on
-    // their way.  The loop is short on purpose: what runs once is bound by the fetch of its instructions
+    // f(four scores, index of the first) of the row's part [from, to), 16 bytes at a time, `lanes` threads side by side, the next 16 bytes
+    // on their way.  The loops are short on purpose: what runs once is bound by the fetch of its instructions
     template <class F>
     __device__ __forceinline__ void each(int from, int to, int id, int lanes, F f)
     {
-        float x[E], ahead[E];
-        Scores<TYPE>::some(row, from + id * E, to, x);
+        uint32_t v[4], ahead[4];
+        S::load(row, from + id * S::LOAD, to, v);
 #pragma unroll 1
-        for (int base = from; base < to; base += lanes * E) {
-            const int i = base + id * E;
-            Scores<TYPE>::some(row, i + lanes * E, to, ahead);
-            settle(x);
-            f(x, i);
+        for (int base = from; base < to; base += lanes * S::LOAD) {
+            const int i = base + id * S::LOAD;
+            S::load(row, i + lanes * S::LOAD, to, ahead);
+#pragma unroll 1
+            for (int part = 0; part < S::LOAD; part += E) {
+                float x[E];
+                S::four(v, x);
+                settle(x);
+                f(x, i + part);
+                v[0] = v[2], v[1] = v[3]; // of 16-bit scores the second four
+            }
 #pragma unroll
-            for (int e = 0; e < E; e++)
-                x[e] = ahead[e];
+            for (int e = 0; e < 4; e++)
+                v[e] = ahead[e];
         }
     }
     template <class F>
@@ -176,28 +217,17 @@ struct Row {
             s.bins[i] = 0;
     }
 
-    // sum over the threads in front, and s.sum over all; every thread calls it
+    // sum over the threads in front, and `sum` over all; every thread calls it
     __device__ __forceinline__ uint64_t scan(uint64_t v)
     {
-        uint64_t in = v;
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const uint64_t up = __shfl_up(in, o);
-            in += lane >= o ? up : 0;
-        }
+        const uint64_t in = sums64(v);
         __syncthreads(); // s.wave may still be read
         if (lane == 63)
             s.wave[wave] = in;
         __syncthreads();
-        uint64_t front = 0, all = 0;
-        for (int w = 0; w < WAVES; w++) {
-            const uint64_t t = s.wave[w];
-            front += w < wave ? t : 0;
-            all += t;
-        }
-        if (tid == 0)
-            s.sum = all;
-        return front + in - v;
+        const uint64_t waves = sums16(s.wave[lane & 15]);
+        sum = of_lane(waves, 15);
+        return (uniform((uint32_t)wave) ? of_lane(waves, (int)uniform((uint32_t)wave) - 1) : 0) + in - v;
     }
 
     // the first bin in which the running sum reaches need: s.bin, and s.before what lies in front of it.  false: the sum stays below
@@ -205,8 +235,7 @@ struct Row {
     {
         const uint64_t b0 = s.bins[2 * tid], b1 = s.bins[2 * tid + 1];
         const uint64_t front = scan(b0 + b1);
-        __syncthreads();
-        const bool reached = s.sum >= need;
+        const bool reached = sum >= need;
         if (front < need && need <= front + b0)
             s.bin = 2 * tid, s.before = front;
         else if (front + b0 < need && need <= front + b0 + b1)
@@ -221,8 +250,8 @@ struct Row {
     {
         if (!find(need))
             return;
-        const int bin = (int)s.bin;
-        need -= s.before;
+        const int bin = (int)uniform(s.bin);
+        need -= uniform(s.before);
         if (tid == 0)
             s.listed = 0, s.low = 0xffffffffu, s.high = 0;
         __syncthreads();
@@ -267,17 +296,17 @@ struct Row {
                 if (lane == 0)
                     atomicMin(&s.low, low), atomicMax(&s.high, high);
                 __syncthreads();
-                low = s.low, high = s.high, listed = s.listed;
+                low = uniform(s.low), high = uniform(s.high), listed = uniform(s.listed);
                 continue;
             }
             if (tied && tid == 0)
                 add(old, old_ties);
             __syncthreads();
             find(need);
-            need -= s.before;
-            const uint32_t at = s.bin, to = high - (at << shift);
+            need -= uniform(s.before);
+            const uint32_t at = uniform(s.bin), to = high - (at << shift);
             if (shift == 0) {
-                const uint64_t each_one = mass ? weight(score_of(to)) : 1, there = s.bins[at] / each_one, wanted = (need + each_one - 1) / each_one;
+                const uint64_t each_one = mass ? uniform(weight(score_of(to))) : 1, there = uniform(s.bins[at]) / each_one, wanted = (need + each_one - 1) / each_one;
                 key = to;
                 // all of them: those of the row, or as many as an earlier border left
                 ties = wanted < there ? (uint32_t)wanted : tied && to == old ? old_ties : 0xffffffffu;
@@ -291,27 +320,55 @@ struct Row {
         }
     }
 
-    // The first index, in order, at which the running sum exceeds `target(sum)`; f: the sum of some scores' numbers, and each, if asked for.
-    template <class F, class T>
-    __device__ __forceinline__ int locate(F f, T target)
+    // The row in WAVES parts, one for each wave: where that of wave w begins and ends
+    __device__ __forceinline__ int part() const { return (a.vocab + WAVES * S::LOAD - 1) / (WAVES * S::LOAD) * S::LOAD; }
+    __device__ __forceinline__ int from() const { return min(a.vocab, wave * part()); }
+    __device__ __forceinline__ int to() const { return min(a.vocab, from() + part()); }
+    // the parts' sums: v is a thread's
+    __device__ __forceinline__ void set_regions(uint64_t v)
     {
-        const int part = (a.vocab + WAVES * E - 1) / (WAVES * E) * E, from = min(a.vocab, wave * part), to = min(a.vocab, from + part);
-        uint64_t v = 0;
-        each(from, to, lane, 64, [&](const float(&x)[E], int i) INLINE { v += f(x, i, nullptr); });
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2)
-            v += __shfl_xor(v, o);
+        v = sums64(v);
+        if (lane == 63)
+            s.region[wave] = v;
         __syncthreads();
-        if (lane == 0)
-            s.wave[wave] = v;
-        __syncthreads();
-        uint64_t all = 0, front = 0;
-        for (int i = 0; i < WAVES; i++)
-            all += s.wave[i];
-        const uint64_t goal = target(all);
-        int w = 0;
-        for (; w < WAVES - 1 && front + s.wave[w] <= goal; w++)
-            front += s.wave[w];
+    }
+
+    // The threads' numbers, the first n of them, from the largest to the smallest (those behind are 0): exchanges over distances that
+    // halve, in the wave's registers where both ends are in it: 28 steps of 140 ns at 100 numbers
+    __device__ __forceinline__ uint64_t sort(uint64_t v, int n)
+    {
+        const bool some = wave * 64 < 2 * n; // waves that can hold some on their way
+#pragma unroll 1
+        for (int size = 2; size < 2 * n; size *= 2)
+#pragma unroll 1
+            for (int apart = size / 2; apart > 0; apart /= 2) {
+                if (apart >= 64) {
+                    __syncthreads();
+                    s.few[tid] = v;
+                    __syncthreads();
+                }
+                if (some) {
+                    const uint64_t other = apart < 64 ? __shfl_xor(v, apart) : s.few[tid ^ apart];
+                    v = (v > other) == (((tid & size) == 0) == ((tid & apart) == 0)) ? v : other;
+                }
+            }
+        return v;
+    }
+
+    // The first index, in order, at which the running sum exceeds `target(sum)`; f: the sum of some scores' numbers, and each, if asked for.
+    // known: the regions hold their sums.
+    template <class F, class T>
+    __device__ __forceinline__ int locate(bool known, F f, T target)
+    {
+        if (!known) {
+            uint64_t v = 0;
+            each(from(), to(), lane, 64, [&](const float(&x)[E], int i) INLINE { v += f(x, i, nullptr); });
+            set_regions(v);
+        }
+        const int part = this->part();
+        const uint64_t regions = sums16(s.region[lane & 15]), goal = target(of_lane(regions, 15));
+        const int w = min(WAVES - 1, (int)__popcll(__ballot(lane < WAVES && regions <= goal)));
+        uint64_t front = w ? of_lane(regions, w - 1) : 0;
         const int begin = w * part, end = min(a.vocab, begin + part);
         if (tid == 0)
             s.index = -1;
@@ -319,7 +376,9 @@ struct Row {
         for (int base = begin; base < end; base += THREADS * E) {
             float x[E];
             const int i = base + tid * E;
-            Scores<TYPE>::some(row, i, end, x);
+            uint32_t v[E / S::WORD];
+            S::load(row, i, end, v);
+            S::four(v, x);
             settle(x);
             uint64_t own, each_one[E];
             own = f(x, i, each_one);
@@ -334,11 +393,11 @@ struct Row {
                 s.index = at;
             }
             __syncthreads();
-            front += s.sum;
-            if (s.index >= 0)
+            front += sum;
+            if ((int)uniform((uint32_t)s.index) >= 0)
                 break;
         }
-        return s.index;
+        return (int)uniform((uint32_t)s.index);
     }
 };
 
@@ -347,14 +406,15 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
 {
     __shared__ SampleShared s;
     Row<TYPE> r(a, s);
+    constexpr int E = Row<TYPE>::E;
     const int tid = threadIdx.x;
     const float none = -__builtin_inff();
 
     s.powers[tid] = POWERS[0][tid >> 5] * POWERS[1][tid & 31];
     float top = none;
-    r.each([&](const float(&x)[Row<TYPE>::E], int) INLINE {
+    r.each([&](const float(&x)[E], int) INLINE {
 #pragma unroll
-        for (int e = 0; e < Row<TYPE>::E; e++)
+        for (int e = 0; e < E; e++)
             top = fmaxf(top, x[e]);
     });
 #pragma unroll
@@ -363,8 +423,11 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
     if (r.lane == 0)
         s.list[r.wave] = __builtin_bit_cast(uint32_t, top);
     __syncthreads();
-    for (int w = 0; w < WAVES; w++)
-        top = fmaxf(top, __builtin_bit_cast(float, s.list[w]));
+    top = __builtin_bit_cast(float, s.list[r.lane & (WAVES - 1)]);
+#pragma unroll
+    for (int o = 1; o < WAVES; o *= 2)
+        top = fmaxf(top, __shfl_xor(top, o));
+    top = uniform(top);
     __syncthreads();
     r.infinite = top == __builtin_inff();
     r.top = r.infinite ? 0.0f : top;
@@ -380,9 +443,9 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
             s.index = 0x7fffffff;
         __syncthreads();
         int first = 0x7fffffff;
-        r.each([&](const float(&x)[Row<TYPE>::E], int i) INLINE {
+        r.each([&](const float(&x)[E], int i) INLINE {
 #pragma unroll
-            for (int e = 0; e < Row<TYPE>::E; e++)
+            for (int e = 0; e < E; e++)
                 first = x[e] == top ? min(first, i + e) : first;
         });
 #pragma unroll
@@ -406,6 +469,17 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
     const int k = a.top_k ? a.top_k[blockIdx.x] : 0;
     const float p = a.top_p ? a.top_p[blockIdx.x] : 1.0f;
     const bool by_count = k > 0 && k < a.vocab, by_mass = p < 1;
+    bool known = false;
+    const double u = (double)a.uniform[blockIdx.x];
+    auto goal_of = [&](uint64_t all) INLINE -> uint64_t {
+        const double at = u > 0 ? u * (double)all : 0;
+        return at < (double)all ? (uint64_t)at : all - 1;
+    };
+    auto need_of = [&](uint64_t all) INLINE -> uint64_t {
+        const double goal = p > 0 ? ceil((double)p * (double)all) : 1;
+        return goal > 1 ? (uint64_t)goal : 1;
+    };
+    constexpr uint64_t RAW = Row<TYPE>::RAW;
 #pragma unroll 1
     for (int filter = 0; filter < 2; filter++) { // top-k, then top-p among what it keeps
         const bool mass = filter == 1;
@@ -415,20 +489,19 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
         __syncthreads();
         const uint32_t key = r.key, ties = r.ties;
         const float border = score_of(key);
-        r.each([&](const float(&x)[Row<TYPE>::E], int) INLINE {
-            bool in[Row<TYPE>::E], any = false;
+        r.each([&](const float(&x)[E], int) INLINE {
+            bool in[E], any = false;
 #pragma unroll
-            for (int e = 0; e < Row<TYPE>::E; e++) {
+            for (int e = 0; e < E; e++)
                 any |= in[e] = x[e] > border || (x[e] == border && ties == 0xffffffffu && border > none);
-            }
             if (any) {
-                uint64_t w[Row<TYPE>::E];
+                uint64_t w[E];
                 if (mass)
 #pragma unroll
-                    for (int e = 0; e < Row<TYPE>::E; e++)
+                    for (int e = 0; e < E; e++)
                         w[e] = r.weight(x[e]);
 #pragma unroll
-                for (int e = 0; e < Row<TYPE>::E; e++)
+                for (int e = 0; e < E; e++)
                     if (in[e])
                         atomicAdd((unsigned long long *)&s.bins[r.bin_of(x[e])], mass ? (unsigned long long)w[e] : 1ull);
             }
@@ -439,50 +512,104 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
         uint64_t need = (uint64_t)k; // a border among scores without weight changes nothing
         if (mass) {
             r.scan(s.bins[2 * tid] + s.bins[2 * tid + 1]);
+            need = need_of(r.sum);
+        }
+        // The quick way, where the scores around the border are few: top-k's are all that can be taken, with it everything is decided among
+        // them; top-p's border is decided among those of its interval, while the weight of all above is summed in the same pass.
+        if (mass ? key == 0x007fffffu : k <= FEW / 2) {
+            const bool found = r.find(need);
+            const int bin = (int)uniform(s.bin);
+            const uint64_t before = uniform(s.before);
+            if (!found || bin == BINS - 1)
+                continue; // nothing with a weight is cut
+            if (tid == 0)
+                s.listed = 0, s.low = 0xffffffffu, s.index = -1;
             __syncthreads();
-            const double goal = p > 0 ? ceil((double)p * (double)s.sum) : 1;
-            need = goal > 1 ? (uint64_t)goal : 1;
+            uint64_t above = 0;
+            r.each(r.from(), r.to(), r.lane, 64, [&](const float(&x)[E], int i) INLINE {
+                int b[E], least_b = BINS;
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    b[e] = x[e] > none ? r.bin_of(x[e]) : BINS;
+                    least_b = min(least_b, b[e]);
+                    if (b[e] == bin || (!mass && b[e] < bin)) {
+                        const uint32_t at = atomicAdd(&s.listed, 1u);
+                        if (at < FEW)
+                            s.few[at] = (uint64_t)key_of(x[e]) << 32 | ~(uint32_t)(i + e); // a larger one comes first
+                    }
+                }
+                if (mass && least_b < bin)
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        const uint64_t w = r.weight(x[e]);
+                        above += b[e] < bin && w >= r.least ? w : 0;
+                    }
+            });
+            r.set_regions(above);
+            const int n = (int)uniform(s.listed);
+            if (n <= FEW) {
+                const uint64_t entry = r.sort(tid < n ? s.few[tid] : 0, n);
+                const int index = (int)~(uint32_t)entry;
+                uint64_t w = tid < (mass ? n : min(n, k)) ? r.weight(score_of((uint32_t)(entry >> 32))) : 0;
+                const uint64_t front = r.scan(w);
+                if (mass) {
+                    if (tid < n && before + front < need) {
+                        if (w >= r.least)
+                            atomicAdd((unsigned long long *)&s.region[(uint32_t)index / (uint32_t)r.part()], (unsigned long long)w);
+                        if (before + front + w >= need)
+                            s.low = (uint32_t)(entry >> 32), s.index = index;
+                    }
+                    __syncthreads();
+                    r.key = uniform(s.low), r.last = (int)uniform((uint32_t)s.index);
+                    known = true;
+                    continue;
+                }
+                const uint64_t most = by_mass ? need_of(r.sum) : ~0ull;
+                w = front < most && w >= r.least ? w : 0;
+                // in the order of their indices
+                const uint64_t at = r.sort(w ? (uint64_t)(MOST_VOCAB - 1 - index) << (FRACTION + 1) | w : 0, min(n, k));
+                w = at & ((2ull << FRACTION) - 1);
+                const uint64_t run = r.scan(w);
+                const uint64_t goal = goal_of(r.sum);
+                if (run <= goal && goal < run + w)
+                    a.tokens[blockIdx.x] = MOST_VOCAB - 1 - (int)(at >> (FRACTION + 1));
+                return;
+            }
         }
         r.cut(mass, need);
     }
-    const double u = (double)a.uniform[blockIdx.x];
-    constexpr uint64_t RAW = Row<TYPE>::RAW;
     const uint64_t least = RAW + r.least;
     const float border = score_of(r.key);
 #pragma unroll 1
     for (int last = r.ties == 0xffffffffu; last < 2; last++) { // the last of the ties that are kept, then the token
         const int index = r.locate(
-            [&](const float(&x)[Row<TYPE>::E], int i, uint64_t *each_one) INLINE -> uint64_t {
-                bool in[Row<TYPE>::E], any = false;
+            known,
+            [&](const float(&x)[E], int i, uint64_t *each_one) INLINE -> uint64_t {
+                bool in[E], any = false;
 #pragma unroll
-                for (int e = 0; e < Row<TYPE>::E; e++)
+                for (int e = 0; e < E; e++)
                     any |= in[e] = last == 0 ? x[e] == border : x[e] > border || (x[e] == border && i + e <= r.last);
                 uint64_t sum = 0;
                 if (any) {
-                    uint64_t w[Row<TYPE>::E];
+                    uint64_t w[E];
 #pragma unroll
-                    for (int e = 0; e < Row<TYPE>::E; e++)
+                    for (int e = 0; e < E; e++)
                         w[e] = last == 0 ? RAW + 1 : r.raw_weight(x[e]);
 #pragma unroll
-                    for (int e = 0; e < Row<TYPE>::E; e++) {
+                    for (int e = 0; e < E; e++) {
                         w[e] = in[e] && (last == 0 || w[e] >= least) ? w[e] : RAW;
                         sum += w[e];
                         if (each_one)
                             each_one[e] = w[e] - RAW;
                     }
-                    sum -= RAW * Row<TYPE>::E;
+                    sum -= RAW * E;
                 } else if (each_one)
 #pragma unroll
-                    for (int e = 0; e < Row<TYPE>::E; e++)
+                    for (int e = 0; e < E; e++)
                         each_one[e] = 0;
                 return sum;
             },
-            [&](uint64_t all) INLINE -> uint64_t {
-                if (last == 0)
-                    return r.ties - 1;
-                const double at = u > 0 ? u * (double)all : 0;
-                return at < (double)all ? (uint64_t)at : all - 1;
-            });
+            [&](uint64_t all) INLINE -> uint64_t { return last == 0 ? r.ties - 1 : goal_of(all); });
         if (last == 0)
             r.last = index;
         else if (tid == 0)
