@@ -3,7 +3,10 @@
 // A pass over memory: every head is read once and written once, all arithmetic in float32, rounded once.  DIM / 8 neighbouring lanes have a
 // head, 16 bytes each.  A lane reads its partners of the rotation (rot / 2 elements away) itself, from lines that its neighbours
 // read in the same instruction, instead of asking them for eight values through LDS.  The cosines and sines of a token are as many bytes
-// as four of its heads: lanes take HEADS heads of one token in turn and keep them.
+// as four of its heads: lanes take up to 8 heads of one token in turn and keep them, the norm's weights multiplied in, the next head on
+// its way.  With a division for each 8-bit code and weights read anew for each head its arithmetic took longer than its bytes: 5000 tokens of
+// 40 + 8 + 8 heads of 128, fp16 into int8, 50 us; now 35.5 (133 MB at 3.7 TB/s; 2, 4 or 28 heads a lane: 44.5, 36.7, 40.2).
+// 32 tokens of 32 + 8 + 8 heads: 3.5 us.
 #include "real16.h"
 
 namespace hipq {
@@ -11,10 +14,37 @@ namespace hipq {
 struct AppendArgs {
     hipq_kv_cache cache;
     hipq_kv_append_desc d;
-    int chunks, per_chunk; // work items of a token, and their heads
+    int blocks, per_chunk; // work-groups that all tokens take for the same heads, and how many heads those are
     uint32_t page_magic;
     int page_shift;
 };
+
+// codes of a lane's eight values: v / scale, rounded to nearest even
+__device__ static __forceinline__ u32x2 codes_of(const float (&v)[8], float scale)
+{
+    u32x2 w = {0, 0};
+    if (scale > 0x1p-100f && scale < __builtin_inff()) {
+        // the quotient from one division a head: v r, and once what that leaves.  With r rounded correctly so is the quotient.  Adding
+        // 1.5 * 2^23 rounds it, and leaves the code in the low byte.  (A division an element was a third of all instructions.)
+        const float r = 1.0f / scale;
+        uint32_t c[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float q = v[e] * r;
+            c[e] = __builtin_bit_cast(uint32_t, __builtin_fmaf(__builtin_fmaf(-q, scale, v[e]), r, q) + 12582912.0f);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e += 4)
+            w[e / 4] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[e + 3], c[e + 2], 0x0c0c0400), __builtin_amdgcn_perm(c[e + 1], c[e], 0x0c0c0400), 0x05040100);
+    } else
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            // a subnormal scale that was rounded down makes more than 127 of the largest
+            const float code = scale > 0 ? fminf(fmaxf(rintf(v[e] / scale), -127.0f), 127.0f) : 0.0f;
+            w[e / 4] |= ((uint32_t)(int)code & 255) << (8 * (e % 4));
+        }
+    return w;
+}
 
 // QUANT: into an int8 cache
 template <int TYPE, int DIM, bool QUANT>
@@ -23,14 +53,13 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a)
     using R = Real16<TYPE>;
     constexpr int LANES = DIM / 8;
     const hipq_kv_append_desc &d = a.d;
-    const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
+    const int chunk = blockIdx.x / a.blocks, token = (int)((blockIdx.x - chunk * a.blocks) * 256 + threadIdx.x) / LANES;
     const int i0 = (threadIdx.x % LANES) * 8;
-    if (id >= (int64_t)a.chunks * d.tokens)
+    if (token >= d.tokens)
         return;
-    const int chunk = (int)(id / d.tokens), token = (int)(id - (int64_t)chunk * d.tokens);
-    const int heads = a.cache.heads, all = d.q_heads + 2 * heads;
+    const int heads = a.cache.heads;
     const int slot = d.slots[token], pos = d.positions[token];
-    const int from = chunk * a.per_chunk, to = min(all, from + a.per_chunk);
+    const int from = chunk * a.per_chunk, to = min(d.q_heads + 2 * heads, from + a.per_chunk);
 
     // partners of the lane's elements, and the sign of the sine: side by side the lane has both; otherwise rot / 2 in front or behind
     const int half = d.rot / 2;
@@ -59,81 +88,107 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a)
             }
         }
     }
-    const int page = a.page_magic ? (int)(((uint64_t)(uint32_t)slot * a.page_magic) >> 32) >> a.page_shift : slot;
+    const int page = (int)(((uint64_t)(uint32_t)slot * a.page_magic) >> 32) >> a.page_shift;
     const int place = slot - page * a.cache.page;
-
-    for (int head = from; head < to; head++) {
-        const bool query = head < d.q_heads, key = !query && head < d.q_heads + heads;
-        const int h = query ? head : key ? head - d.q_heads : head - d.q_heads - heads;
-        const uint16_t *x = query ? (const uint16_t *)d.q + token * d.q_token + h * d.q_head
-                            : key ? (const uint16_t *)d.k + token * d.k_token + h * d.k_head
-                                  : (const uint16_t *)d.v + token * d.v_token + h * d.v_head;
-        const u32x4 own = *(const u32x4 *)(x + i0);
-        float v[8];
+    auto widen = [](const u32x4 &w, float (&v)[8]) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < 8; e++)
-            v[e] = e & 1 ? R::high(own[e / 2]) : R::low(own[e / 2]);
-        if (query || key) {
-            const u32x4 other = *(const u32x4 *)(x + partner);
-            float o[8];
+            v[e] = e & 1 ? R::high(w[e / 2]) : R::low(w[e / 2]);
+    };
+
+#pragma unroll 1
+    for (int what = 0; what < 3; what++) { // queries, keys, values: those of this work item
+        const int before = what == 0 ? 0 : what == 1 ? d.q_heads : d.q_heads + heads;
+        const int begin = max(from - before, 0), end = min(to - before, what == 0 ? d.q_heads : heads);
+        if (begin >= end)
+            continue;
+        const uint16_t *x = what == 0 ? (const uint16_t *)d.q + token * d.q_token
+                            : what == 1 ? (const uint16_t *)d.k + token * d.k_token
+                                        : (const uint16_t *)d.v + token * d.v_token;
+        const int64_t step = what == 0 ? d.q_head : what == 1 ? d.k_head : d.v_head;
+        x += begin * step;
+        u32x4 own = *(const u32x4 *)(x + i0), other = own;
+        const bool apart = what < 2 && d.rot && !d.interleaved;
+        if (apart)
+            other = *(const u32x4 *)(x + partner);
+        // the head's weights go into the cosines and sines
+        const uint16_t *norm = (const uint16_t *)(what == 0 ? d.q_norm : what == 1 ? d.k_norm : nullptr);
+        float c[8], s[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            c[e] = cs[e], s[e] = sn[e];
+        if (norm) {
+            float w[8], wo[8];
+            widen(*(const u32x4 *)(norm + i0), w);
+            widen(*(const u32x4 *)(norm + partner), wo);
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                o[e] = e & 1 ? R::high(other[e / 2]) : R::low(other[e / 2]);
-            const uint16_t *norm = (const uint16_t *)(query ? d.q_norm : d.k_norm);
-            if (norm) {
-                float sum = 0;
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    sum = __builtin_fmaf(v[e], v[e], sum);
-#pragma unroll
-                for (int s = 1; s < LANES; s *= 2)
-                    sum += __shfl_xor(sum, s);
-                const float r = 1.0f / sqrtf(sum * (1.0f / DIM) + d.eps);
-                const u32x4 w = *(const u32x4 *)(norm + i0), wo = *(const u32x4 *)(norm + partner);
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    v[e] = v[e] * r * (e & 1 ? R::high(w[e / 2]) : R::low(w[e / 2]));
-                    o[e] = o[e] * r * (e & 1 ? R::high(wo[e / 2]) : R::low(wo[e / 2]));
-                }
-            }
-            if (turned) {
-                float t[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    t[e] = v[e] * cs[e] + (d.interleaved ? v[e ^ 1] : o[e]) * sn[e];
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    v[e] = t[e];
-            }
+                c[e] *= w[e], s[e] *= d.interleaved ? w[e ^ 1] : wo[e];
         }
-        if (query || !QUANT) {
-            u32x4 w;
+#pragma unroll 1
+        for (int h = begin; h < end; h++) {
+            float v[8];
+            widen(own, v);
+            if (what < 2) {
+                float o[8];
+                if (apart)
+                    widen(other, o);
+                else
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                w[e] = R::pack(v[2 * e], v[2 * e + 1]);
-            uint16_t *y = query ? (uint16_t *)d.q_out + token * d.out_token + h * d.out_head
-                                : (uint16_t *)(key ? a.cache.k : a.cache.v) + (((int64_t)page * heads + h) * a.cache.page + place) * DIM;
-            *(u32x4 *)(y + i0) = w;
-        } else {
-            float most = 0;
+                    for (int e = 0; e < 8; e++)
+                        o[e] = v[e ^ 1];
+                x += step;
+                if (h + 1 < end) { // the next head on its way
+                    own = *(const u32x4 *)(x + i0);
+                    if (apart)
+                        other = *(const u32x4 *)(x + partner);
+                }
+                if (norm) {
+                    float sum = 0;
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                most = fmaxf(most, fabsf(v[e]));
+                    for (int e = 0; e < 8; e++)
+                        sum = __builtin_fmaf(v[e], v[e], sum);
 #pragma unroll
-            for (int s = 1; s < LANES; s *= 2)
-                most = fmaxf(most, __shfl_xor(most, s));
-            const float scale = most / 127.0f;
-            u32x2 w = {0, 0};
+                    for (int l = 1; l < LANES; l *= 2)
+                        sum += __shfl_xor(sum, l);
+                    const float r = 1.0f / sqrtf(sum * (1.0f / DIM) + d.eps);
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                // a scale rounded down (a subnormal one by much) makes more than 127 of the largest
-                const float code = scale > 0 ? fminf(fmaxf(rintf(v[e] / scale), -127.0f), 127.0f) : 0.0f;
-                w[e / 4] |= ((uint32_t)(int)code & 255) << (8 * (e % 4));
+                    for (int e = 0; e < 8; e++)
+                        v[e] *= r, o[e] *= r;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    v[e] *= c[e];
+                if (turned)
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        v[e] = __builtin_fmaf(o[e], s[e], v[e]);
+            } else {
+                x += step;
+                if (h + 1 < end)
+                    own = *(const u32x4 *)(x + i0);
             }
             const int64_t row = ((int64_t)page * heads + h) * a.cache.page + place;
-            *(u32x2 *)((uint8_t *)(key ? a.cache.k : a.cache.v) + row * DIM + i0) = w;
-            if (i0 == 0)
-                (key ? a.cache.k_scale : a.cache.v_scale)[row] = scale;
+            if (what == 0 || !QUANT) {
+                u32x4 w;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    w[e] = R::pack(v[2 * e], v[2 * e + 1]);
+                uint16_t *y = what == 0 ? (uint16_t *)d.q_out + token * d.out_token + h * d.out_head : (uint16_t *)(what == 1 ? a.cache.k : a.cache.v) + row * DIM;
+                *(u32x4 *)(y + i0) = w;
+            } else {
+                float most = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    most = fmaxf(most, fabsf(v[e]));
+#pragma unroll
+                for (int l = 1; l < LANES; l *= 2)
+                    most = fmaxf(most, __shfl_xor(most, l));
+                const float scale = most / 127.0f;
+                *(u32x2 *)((uint8_t *)(what == 1 ? a.cache.k : a.cache.v) + row * DIM + i0) = codes_of(v, scale);
+                if (i0 == 0)
+                    (what == 1 ? a.cache.k_scale : a.cache.v_scale)[row] = scale;
+            }
         }
     }
 }
@@ -155,8 +210,10 @@ int check_cache(const hipq_kv_cache *c)
 template <int TYPE, int DIM>
 static int launch_append(AppendArgs &a, hipStream_t st)
 {
-    const int64_t threads = (int64_t)a.chunks * a.d.tokens * (DIM / 8);
-    const dim3 grid((unsigned)((threads + 255) / 256));
+    const int all = a.d.q_heads + 2 * a.cache.heads, chunks = (all + a.per_chunk - 1) / a.per_chunk;
+    a.blocks = (int)(((int64_t)a.d.tokens * (DIM / 8) + 255) / 256);
+    HIPQ_REQUIRE((int64_t)a.blocks * chunks < ((int64_t)1 << 31), "append: %d tokens of %d heads", a.d.tokens, all);
+    const dim3 grid((unsigned)(a.blocks * chunks));
     if (a.cache.quantized)
         kv_append_kernel<TYPE, DIM, true><<<grid, dim3(256), 0, st>>>(a);
     else
@@ -202,6 +259,5 @@ extern "C" int hipq_kv_append(const hipq_kv_cache *cache, const hipq_kv_append_d
     const int all = d->q_heads + 2 * cache->heads;
     const int64_t work = (int64_t)all * d->tokens;
     a.per_chunk = work >= 65536 ? 8 : work >= 16384 ? 2 : 1;
-    a.chunks = (all + a.per_chunk - 1) / a.per_chunk;
     return cache->type == HIPQ_REAL_BF16 ? launch_append<HIPQ_REAL_BF16>(a, (hipStream_t)stream) : launch_append<HIPQ_REAL_F16>(a, (hipStream_t)stream);
 }
