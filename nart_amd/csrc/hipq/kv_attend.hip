@@ -49,6 +49,7 @@ __device__ static __forceinline__ T at(gbytes_t p, uint32_t offset)
 }
 
 constexpr float NONE = -__builtin_inff();
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 // codes 0..7 of two dwords, as 16-bit floats
 template <int TYPE>
@@ -110,10 +111,12 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
     f32x4 *const lo = (f32x4 *)(ll + 4 * RT * 16);                // [2][RT * VD][64]
     u32x4 *const lq = (u32x4 *)(lo + 2 * RT * VD * 64);
     u32x4 q[Q_LDS ? 1 : RT][Q_LDS ? 1 : KS];
+    int own[RT], qh[RT]; // the lane's rows (the last one again behind it): new token and query head
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         const int row = min(r0 + 16 * rt + c, rows - 1);
-        const uint16_t *x = (const uint16_t *)a.d.q + (int64_t)(seq.row0 + row / a.group) * a.d.q_token + (int64_t)(h * a.group + row % a.group) * a.d.q_head;
+        own[rt] = row / a.group, qh[rt] = h * a.group + row - own[rt] * a.group;
+        const uint16_t *x = (const uint16_t *)a.d.q + (int64_t)(seq.row0 + own[rt]) * a.d.q_token + (int64_t)qh[rt] * a.d.q_head;
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
             const u32x4 *from = (const u32x4 *)(x + (QUANT ? ks / 2 * 64 + j * 16 + ks % 2 * 8 : ks * 32 + j * 8));
@@ -128,7 +131,7 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
 
     float m[RT], l[RT];
     f32x4 lsum[RT]; // 16 bits: the sums of p, by a multiply by ones
-    float unit = 0; // float16 codes: p is multiplied by value scale / unit, unit the largest scale so far or more, to stay in range
+    float unit = 0, per_unit = 0; // float16 codes: p is multiplied by value scale / unit, unit the largest scale so far or more, to stay in range
     f32x4 o[RT][VD];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
@@ -220,23 +223,31 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
         __builtin_amdgcn_sched_barrier(0); // what is done earlier than it is written does not fit the registers
         load_k(next);
         __builtin_amdgcn_sched_barrier(0);
-        bool strange = false;
+        bool any_strange = false; // infinities or NaN among values that not all rows see
         if (masked) {
             // tokens that are not there may hold anything: their values are taken as 0, so that 0 times them is 0
 #pragma unroll
-            for (int half = 0; half < 2; half++)
+            for (int half = 0; half < 2; half++) {
+                const int there = now.page[half] >= 0 ? seq.len - t - half * 16 - j * 4 : 0;
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const bool in = now.page[half] >= 0 && t + half * 16 + j * 4 + r < seq.len;
                     if (QUANT)
-                        vsc[half][r] = in ? vsc[half][r] : 0.0f;
+                        vsc[half][r] = r < there ? vsc[half][r] : 0.0f;
 #pragma unroll
-                    for (int i = 0; i < VW; i++) {
-                        vx[half][r][i] = in ? vx[half][r][i] : 0;
-                        if (!QUANT)
-                            strange |= !(fabsf(R::low(vx[half][r][i])) < __builtin_inff()) || !(fabsf(R::high(vx[half][r][i])) < __builtin_inff());
-                    }
+                    for (int i = 0; i < VW; i++)
+                        vx[half][r][i] = r < there ? vx[half][r][i] : 0;
                 }
+            }
+            if (!QUANT && (a.d.mask || seq.count > 1)) {
+                u16x2 largest = {0, 0};
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+#pragma unroll
+                    for (int i = 0; i < VW; i++)
+                        largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2, vx[e / 4][e % 4][i] & 0x7fff7fffu));
+                constexpr uint16_t inf = TYPE == HIPQ_REAL_BF16 ? 0x7f80 : 0x7c00;
+                any_strange = __any(largest[0] >= inf || largest[1] >= inf);
+            }
         }
         if (QUANT && TYPE == HIPQ_REAL_F16) {
             float top = 0;
@@ -247,20 +258,19 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
 #pragma unroll
                 for (int s = 1; s < 64; s *= 2)
                     top = fmaxf(top, __shfl_xor(top, s));
-                top = fminf(top, 3e38f);
+                top = fminf(fmaxf(top, 1e-30f), 3e38f);
                 const float f = unit / top; // 0 at the first, where nothing is there to be scaled
-                unit = top;
+                unit = top, per_unit = 1.0f / top;
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++)
 #pragma unroll
                     for (int i = 0; i < VD; i++)
                         o[rt][i] *= f;
             }
-            const float f = unit > 0 ? 1.0f / unit : 0.0f;
-            vsc[0] *= f, vsc[1] *= f;
+            vsc[0] *= per_unit, vsc[1] *= per_unit;
         }
         u32x4 p[RT];
-        u32x4 seen[RT]; // where values are infinite or NaN: ones at the tokens that a row sees
+        uint32_t sees[RT]; // a bit for each of the lane's 8 tokens: seen by the row
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
@@ -270,40 +280,41 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
                 for (int half = 0; half < 2; half++)
                     s[half] = R::mfma(k[half][ks], Q_LDS ? lq[(rt * KS + ks) * 64 + lane] : q[Q_LDS ? 0 : rt][Q_LDS ? 0 : ks], s[half]);
             float x[8], top = NONE;
-            uint32_t sees = 0;
-            // what a row sees is looked up again for every such tile: there are few, and it would be in the way in all others
-            const int row = r0 + 16 * rt + c, own = row / a.group;
-            const uint64_t mask = masked && a.d.mask && row < rows ? a.d.mask[seq.row0 + own] : 0;
+            if (masked) {
+                const uint64_t mask = a.d.mask ? a.d.mask[seq.row0 + own[rt]] : 0;
+                sees[rt] = 0;
+#pragma unroll
+                for (int half = 0; half < 2; half++) { // four tokens from `first` on
+                    const int first = t + half * 16 + j * 4, fresh = first - seq.old;
+                    const int there = now.page[half] >= 0 ? min(max(seq.len - first, 0), 4) : 0;
+                    uint32_t bits = (1u << min(max(own[rt] + 1 - fresh, 0), 4)) - 1;
+                    if (a.d.mask)
+                        bits = fresh >= 0 ? (uint32_t)(mask >> min(fresh, 63)) & (fresh < 64 ? 15u : 0u)
+                                          : (uint32_t)mask << min(-fresh, 4) | ((1u << min(-fresh, 4)) - 1);
+                    sees[rt] |= (bits & ((1u << there) - 1)) << (4 * half);
+                }
+            }
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const int half = e / 4, r = e % 4, token = t + half * 16 + j * 4 + r;
-                x[e] = QUANT ? s[half][r] * kscale[half][r] : s[half][r];
-                if (masked) {
-                    const int fresh = token - seq.old;
-                    const bool see = now.page[half] >= 0 && token < seq.len && row < rows &&
-                                     (fresh < 0 || (a.d.mask ? fresh < 64 && ((mask >> (fresh & 63)) & 1) : fresh <= own));
-                    sees |= (uint32_t)see << e;
-                    x[e] = see ? x[e] : NONE;
-                }
+                x[e] = QUANT ? s[e / 4][e % 4] * kscale[e / 4][e % 4] : s[e / 4][e % 4];
+                if (masked)
+                    x[e] = (sees[rt] >> e) & 1 ? x[e] : NONE;
                 top = fmaxf(top, x[e]);
             }
             if (!QUANT)
                 top *= a.scale2;
-            // outputs are scaled by 1 where the reference stays: scaled only where it moves, they were copied around that branch
-            float f = 1.0f;
             if (__any(top > m[rt] + 8.0f)) {
                 top = fmaxf(top, m[rt]);
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
-                f = top == NONE ? 1.0f : exp2_fast(m[rt] - top);
+                const float f = top == NONE ? 1.0f : exp2_fast(m[rt] - top);
                 m[rt] = top;
-            }
-            asm("" : "+v"(f)); // or the products go into the branch all the same
-            l[rt] *= f;
-            lsum[rt] *= f;
+                l[rt] *= f;
+                lsum[rt] *= f;
 #pragma unroll
-            for (int i = 0; i < VD; i++)
-                o[rt][i] *= f;
+                for (int i = 0; i < VD; i++)
+                    o[rt][i] *= f;
+            }
             const float ref = m[rt] == NONE ? 0.0f : m[rt];
             float y[8];
 #pragma unroll
@@ -313,21 +324,18 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
                     l[rt] += y[e];
                     y[e] *= vsc[e / 4][e % 4];
                     if (masked)
-                        y[e] = (sees >> e) & 1 ? y[e] : 0.0f;
+                        y[e] = (sees[rt] >> e) & 1 ? y[e] : 0.0f;
                 }
             }
             const uint32_t one = R::pack(1.0f, 0.0f);
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
+            for (int e = 0; e < 4; e++)
                 p[rt][e] = R::pack(y[2 * e], y[2 * e + 1]);
-                seen[rt][e] = ((sees >> (2 * e)) & 1 ? one : 0) | ((sees >> (2 * e + 1)) & 1 ? one << 16 : 0);
-            }
             if (!QUANT)
                 lsum[rt] = R::mfma(u32x4{one * 0x10001u, one * 0x10001u, one * 0x10001u, one * 0x10001u}, p[rt], lsum[rt]);
         }
         __builtin_amdgcn_sched_barrier(0);
         // output
-        const bool any_strange = masked && __any(strange);
 #pragma unroll
         for (int i = 0; i < VD; i++) {
             u32x4 v;
@@ -339,7 +347,7 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
                 else
                     v[e] = __builtin_amdgcn_perm(vx[half][r + 1][i / 2], vx[half][r][i / 2], i % 2 ? 0x07060302u : 0x05040100u);
             }
-            if (!QUANT && any_strange) {
+            if (masked && !QUANT && any_strange) {
                 // an infinity or NaN among the values near the end reaches the rows that see it, as NaN, and no other
                 u32x4 bad = {0, 0, 0, 0};
                 const uint32_t one = R::pack(1.0f, 0.0f);
@@ -351,7 +359,11 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
                 }
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
-                    const f32x4 n = R::mfma(bad, seen[rt], f32x4{0, 0, 0, 0});
+                    u32x4 seen; // ones at the tokens that a row sees
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        seen[e] = ((sees[rt] >> (2 * e)) & 1 ? one : 0) | ((sees[rt] >> (2 * e + 1)) & 1 ? one << 16 : 0);
+                    const f32x4 n = R::mfma(bad, seen, f32x4{0, 0, 0, 0});
 #pragma unroll
                     for (int r = 0; r < 4; r++)
                         o[rt][i][r] = n[r] > 0 ? __builtin_nanf("") : o[rt][i][r];
@@ -364,20 +376,30 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
         load_v(next);
     };
 
+    // all rows see a whole tile unless it holds a new token, the end, or a page that is not there; from the first such tile on each is
+    // looked at token by token.  Which that is, is found beforehand: a loop that ends on what it reads kept two sets of all its registers
+    int clear = min(min(seq.old, seq.len), t1);
+    for (int at = t0 / a.cache.page + lane; (int64_t)at * a.cache.page < clear; at += 64)
+        if (blocks[at] < 0 || blocks[at] >= a.cache.pages)
+            clear = min(clear, at * a.cache.page);
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2)
+        clear = min(clear, __shfl_xor(clear, s));
+    clear = __builtin_amdgcn_readfirstlane(clear);
     int t = t0 + wave * 32;
     if (t < t1) {
         Pages now = pages_of(t), next = pages_of(t + 128);
         load_k(now);
         load_v(now);
-        // all rows see a whole tile unless it holds a new token, the end, or a page that is not there; from the first such tile on each is
-        // looked at token by token
-        const int clear = min(min(seq.old, seq.len), t1);
-        while (t + 32 <= clear && now.page[0] >= 0 && now.page[1] >= 0) {
+        const int whole = clear - t >= 32 ? (clear - t - 32) / 128 + 1 : 0, last = (t1 - t + 127) / 128;
+#pragma unroll 1
+        for (int i = 0; i < whole; i++, t += 128) {
             const Pages after = pages_of(t + 256);
             tile(t, now, next, std::false_type{});
-            now = next, next = after, t += 128;
+            now = next, next = after;
         }
-        for (; t < t1; t += 128) {
+#pragma unroll 1
+        for (int i = whole; i < last; i++, t += 128) {
             const Pages after = pages_of(t + 256);
             tile(t, now, next, std::true_type{});
             now = next, next = after;
@@ -444,7 +466,7 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
             continue;
         if (a.splits == 1) {
             const float inv = sum[rt] > 0 ? 1.0f / sum[rt] : sum[rt] == 0 ? 0.0f : sum[rt];
-            uint16_t *y = (uint16_t *)a.d.o + (int64_t)(seq.row0 + row / a.group) * a.d.o_token + (int64_t)(h * a.group + row % a.group) * a.d.o_head;
+            uint16_t *y = (uint16_t *)a.d.o + (int64_t)(seq.row0 + own[rt]) * a.d.o_token + (int64_t)qh[rt] * a.d.o_head;
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
@@ -560,14 +582,7 @@ template <int TYPE, int DIM, bool QUANT, int RT>
 static int launch_attend(const AttendArgs &a, int64_t items, hipStream_t st)
 {
     const size_t lds = (2 * 4 * RT * 16) * 4 + (size_t)2 * RT * (DIM / 16) * 64 * 16 + (RT > 1 ? (size_t)RT * (DIM / 32) * 1024 : 0);
-    static thread_local bool allowed[64] = {};
-    int device = 0;
-    HIPQ_CHECK_HIP(hipGetDevice(&device));
-    if (lds > 65536 && (device >= 64 || !allowed[device])) {
-        HIPQ_CHECK_HIP(hipFuncSetAttribute((const void *)kv_attend_kernel<TYPE, DIM, QUANT, RT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        if (device < 64)
-            allowed[device] = true;
-    }
+    static_assert((2 * 4 * RT * 16) * 4 + 2 * RT * (DIM / 16) * 64 * 16 + RT * (DIM / 32) * 1024 <= 65536, "more LDS than a launch has without asking");
     kv_attend_kernel<TYPE, DIM, QUANT, RT><<<dim3((unsigned)((items * a.splits + 7) / 8 * 8)), dim3(256), lds, st>>>(a);
     return launch_status("kv_attend_kernel");
 }
