@@ -24,14 +24,17 @@ __device__ static __forceinline__ u32x2 codes_of(const float (&v)[8], float scal
 {
     u32x2 w = {0, 0};
     if (scale > 0x1p-100f && scale < __builtin_inff()) {
-        // the quotient from one division a head: v r, and once what that leaves.  With r rounded correctly so is the quotient.  Adding
-        // 1.5 * 2^23 rounds it, and leaves the code in the low byte.  (A division an element was a third of all instructions.)
+        // the quotient from one division a head: v r is 1.5 units in the last place off at most, after one correction by what it leaves
+        // less than one, and from there a second one rounds correctly (Markstein), as r is rounded.  Adding 1.5 * 2^23 rounds it, and
+        // leaves the code in the low byte.  (A division an element was a third of all instructions.)
         const float r = 1.0f / scale;
         uint32_t c[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const float q = v[e] * r;
-            c[e] = __builtin_bit_cast(uint32_t, __builtin_fmaf(__builtin_fmaf(-q, scale, v[e]), r, q) + 12582912.0f);
+            float q = v[e] * r;
+            q = __builtin_fmaf(__builtin_fmaf(-q, scale, v[e]), r, q);
+            q = __builtin_fmaf(__builtin_fmaf(-q, scale, v[e]), r, q);
+            c[e] = __builtin_bit_cast(uint32_t, q + 12582912.0f);
         }
 #pragma unroll
         for (int e = 0; e < 8; e += 4)

@@ -403,6 +403,10 @@ static int current_device(int *out)
 /* A tensor of the calling thread's device with `dims` dimensions, one of the dtypes in the set `allowed`, its last dimension without gaps. */
 static int tensor(PyObject *t, const char *name, int dims, unsigned allowed, int device, view_t *v)
 {
+    if (t == Py_None) {
+        PyErr_Format(PyExc_ValueError, "%s: a tensor is expected", name);
+        return 0;
+    }
     PyObject *o = PyObject_GetAttr(t, s_dtype);
     if (o == NULL)
         return 0;
@@ -627,8 +631,12 @@ static PyObject *py_kv_attend(ARGS)
     if (!expect(n, 12) || !current_device(&device) || !cache_device(a[1], device) || !tensor(a[2], "q", 3, HALVES, device, &q) || !cache_for(a[0], &q, &c)
         || !tensor(a[3], "out", 3, 1u << q.dtype, device, &o) || !whole_tensor(a[4], "starts", 1, 1u << I32, device, 0, &starts)
         || !whole_tensor(a[5], "lens", 1, 1u << I32, device, 0, &lens) || !tensor(a[6], "blocks", 2, 1u << I32, device, &blocks)
-        || !whole_tensor(a[7], "mask", 1, 1u << I64, device, 1, &mask) || !whole(a[8], &d.most_new) || !number(a[10], &d.scale))
+        || !whole_tensor(a[7], "mask", 1, 1u << I64, device, 1, &mask) || !number(a[10], &d.scale))
         return NULL;
+    const long most_new = PyLong_AsLong(a[8]);
+    if (most_new == -1 && PyErr_Occurred())
+        return NULL;
+    d.most_new = most_new < -1 ? -1 : most_new > 0x7fffffff ? 0x7fffffff : (int)most_new;
     const int64_t b = lens.shape[0], t = q.shape[0];
     if (!shaped(&q, "q", 3, t, q.shape[1], c.dim) || !shaped(&o, "out", 3, t, q.shape[1], c.dim) || !shaped(&starts, "starts", 1, b + 1, 0, 0)
         || !shaped(&blocks, "blocks", 2, b, blocks.shape[1], 0) || !shaped(&mask, "mask", 1, t, 0, 0))

@@ -218,6 +218,26 @@ def test_append_int8_zero_and_tiny_heads():
     assert (scales[2].double() * 127 - 60000.0).abs() < 60000 * 2 ** -23
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_append_int8_codes_are_the_rounded_quotients(dtype, dim):
+    """Bit by bit: code = value / scale in float32, rounded to nearest even, for heads of all magnitudes (in float16 some of 2^14 times a
+    normal number hold infinities: their codes are not defined)."""
+    g = gen(dim)
+    n = 3000
+    size = torch.exp2(torch.randint(-20, 15, (n, 1, 1), device="cuda", generator=g).double())
+    k, v = ((torch.randn((n, 1, dim), device="cuda", generator=g, dtype=torch.float64) * size).to(dtype) for _ in range(2))
+    k[5], k[6, 0, 1:] = 0, 0
+    cache = new_cache(dtype, -(-n // 16), 1, 16, dim, True)
+    index = torch.arange(n, dtype=torch.int32, device="cuda")
+    cache.append(k.new_empty((n, 0, dim)), k, v, index, index, None)
+    for x, codes, scales in ((k, cache.k, cache.k_scale), (v, cache.v, cache.v_scale)):
+        x, s = x.float().cpu()[:, 0], scales.flatten()[:n].cpu()[:, None]
+        assert torch.equal(s, x.abs().amax(-1, keepdim=True) / 127)
+        want, finite = torch.where(s > 0, torch.round(x / s), 0.0), torch.isfinite(s[:, 0])
+        assert torch.equal(codes.reshape(-1, dim)[:n].cpu().float()[finite], want[finite]) and finite.sum() > 0.9 * n
+
+
 def fill_cache(g, dtype, b, heads, page, dim, longest, int8, spare=3):
     """A cache whose pages are in a random order, and its blocks."""
     per = -(-longest // page)
@@ -375,6 +395,47 @@ def test_attend_pages_that_are_not_there():
     a = cache.attend(q, index([0, 1]), index([96]), holes, 1)
     b = cache.attend(q, index([0, 1]), index([64]), packed.contiguous(), 1)
     assert (a.double() - b.double()).abs().max() <= 2 ** -7 * b.abs().max()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_pages_beyond_32_bits(int8):
+    """A cache of more than 2^32 bytes and 2^31 elements: tokens go to its last pages and are read there."""
+    g = gen(70)
+    pages = 36000 if not int8 else 70000
+    cache = hipq.KvCache(*(torch.empty((pages, 8, 64, 128), dtype=torch.int8 if int8 else BF16, device="cuda") for _ in range(2)),
+                         *(torch.empty((pages, 8, 64), device="cuda") if int8 else None for _ in range(2)))
+    assert cache.k.numel() > (1 << 31) and cache.k.numel() * cache.k.element_size() > (1 << 32)
+    blocks = torch.tensor([[pages - 1, 1, pages // 2]], dtype=torch.int32, device="cuda")
+    n = 150
+    at = torch.arange(n, device="cuda")
+    slots = (blocks[0, at // 64] * 64 + at % 64).to(torch.int32)
+    k, v = randn(g, BF16, n, 8, 128), randn(g, BF16, n, 8, 128)
+    cache.append(k, k, v, slots, slots, None)
+    if not int8:
+        assert torch.equal(tokens_of(cache.v, blocks[0], n), v.transpose(0, 1))
+    check_attend(g, cache, blocks, [3], [n], 16, BF16)
+
+
+def test_attend_over_its_queries():
+    """The outputs may lie where the queries lay."""
+    g = gen(71)
+    for longest in (100, 3000):
+        cache, blocks = fill_cache(g, BF16, 2, 2, 16, 128, longest, False)
+        q = randn(g, BF16, 20, 8, 128)
+        index = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+        a = (index([0, 9, 20]), index([longest, longest - 30]), blocks, 11)
+        want = cache.attend(q, *a)
+        assert torch.equal(cache.attend(q, *a, out=q), want)
+
+
+def test_attend_subnormal_value_scales():
+    """Value scales down to the smallest float32: finite outputs, zeros where float16 has none so small."""
+    g = gen(72)
+    cache, blocks = fill_cache(g, F16, 1, 2, 16, 64, 200, True)
+    cache.v_scale.fill_(1e-42)
+    q = randn(g, F16, 1, 4, 64)
+    index = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    assert (cache.attend(q, index([0, 1]), index([200]), blocks, 1) == 0).all()
 
 
 @pytest.mark.parametrize("int8", [False, True])
