@@ -376,21 +376,25 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
         load_v(next);
     };
 
-    // all rows see a whole tile unless it holds a new token, the end, or a page that is not there; from the first such tile on each is
-    // looked at token by token.  Which that is, is found beforehand: a loop that ends on what it reads kept two sets of all its registers
-    int clear = min(min(seq.old, seq.len), t1);
-    for (int at = t0 / a.cache.page + lane; (int64_t)at * a.cache.page < clear; at += 64)
-        if (blocks[at] < 0 || blocks[at] >= a.cache.pages)
-            clear = min(clear, at * a.cache.page);
-#pragma unroll
-    for (int s = 1; s < 64; s *= 2)
-        clear = min(clear, __shfl_xor(clear, s));
-    clear = __builtin_amdgcn_readfirstlane(clear);
     int t = t0 + wave * 32;
     if (t < t1) {
+        // All rows see a whole tile unless it holds a new token, the end, or a page that is not there; from the first such tile on each is
+        // looked at token by token.  Which that is, is found beforehand: a loop that ends on what it reads kept two sets of all its registers
+        int clear = min(min(seq.old, seq.len), t1), page_at = t0 / a.cache.page + lane;
+        int there = (int64_t)page_at * a.cache.page < clear ? blocks[page_at] : 0;
         Pages now = pages_of(t), next = pages_of(t + 128);
         load_k(now);
         load_v(now);
+        do {
+            if (there < 0 || there >= a.cache.pages)
+                clear = min(clear, page_at * a.cache.page);
+            page_at += 64;
+            there = (int64_t)page_at * a.cache.page < clear ? blocks[page_at] : 0;
+        } while (__any((int64_t)page_at * a.cache.page < clear));
+#pragma unroll
+        for (int s = 1; s < 64; s *= 2)
+            clear = min(clear, __shfl_xor(clear, s));
+        clear = __builtin_amdgcn_readfirstlane(clear);
         const int whole = clear - t >= 32 ? (clear - t - 32) / 128 + 1 : 0, last = (t1 - t + 127) / 128;
 #pragma unroll 1
         for (int i = 0; i < whole; i++, t += 128) {
@@ -505,9 +509,11 @@ __global__ __launch_bounds__(256) void kv_attend_join_kernel(const AttendArgs a)
     float top = NONE, l = 0;
     f32x4 o = {0, 0, 0, 0};
     if (there) {
+#pragma unroll 4
         for (int s = 0; s < a.splits; s++)
             top = fmaxf(top, a.part_ml[2 * (at + (int64_t)s * a.rows)]);
         const float ref = top == NONE ? 0.0f : top;
+#pragma unroll 4
         for (int s = side; s < a.splits; s += SIDE) {
             const int64_t p = at + (int64_t)s * a.rows;
             const float f = exp2_fast(a.part_ml[2 * p] - ref);
