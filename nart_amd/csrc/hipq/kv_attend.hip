@@ -15,6 +15,12 @@
 //     Nothing goes through LDS and no wave waits for another until the end.
 //   * Four waves of a work-group take tiles of 32 tokens in turn, each a tile ahead in its loads; the tokens of a sequence are split over
 //     work-groups until the chip is full, and a second kernel joins the parts.
+//   * More than 64 rows of heads of 128 have a kernel of their own (kv_attend_wide_kernel), whose four waves share what they bring from the
+//     cache.
+// What bounds it, measured (32 query heads on 8 of 128 unless said otherwise): one token of 8 sequences of up to 2000 in 16 bits, 14 us and
+// 3.8 for the join: latency, about 3.4 TB/s; one token of 2 x 131072 with 64 heads, 170 to 180 us and 5: 4.6 TB/s, a large copy's rate being
+// 5.2; 16 trees of 32 tokens on up to 8000 in 8 bits, 111 us with the join: vector instructions (300 a tile and wave, a tenth of them for widening
+// codes; the kernel without shared tiles takes 121, a third of its 360 for that).
 #include <type_traits>
 
 #include "real16.h"
@@ -77,6 +83,157 @@ struct Sequence {
     // the tokens of a part: an equal share in whole rounds of the four waves
     __device__ __forceinline__ int share(int splits) const { return ((len + splits - 1) / splits + 127) / 128 * 128; }
 };
+
+// a tile: two halves of 16 tokens, each in one page
+struct Pages {
+    int page[2]; // -1: not there
+    int place[2];
+};
+// where the tokens of a sequence lie
+struct Paging {
+    const int32_t *blocks;
+    int halves, page16, page, pages, heads, shift;
+    uint32_t magic;
+    __device__ __forceinline__ Paging(const AttendArgs &a, const int32_t *blocks_, int len)
+        : blocks(blocks_), halves((len + 15) / 16), page16(a.cache.page / 16), page(a.cache.page), pages(a.cache.pages), heads(a.cache.heads), shift(a.page_shift), magic(a.page_magic)
+    {
+    }
+    __device__ __forceinline__ Pages of(int t) const
+    {
+        Pages p;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const int t16 = t / 16 + s;
+            const int at = magic ? (int)(((uint64_t)(uint32_t)t16 * magic) >> 32) >> shift : t16;
+            // through the scalar cache: behind a barrier the compiler would take a vector load, and wait for all those before it
+            const int number = __builtin_amdgcn_readfirstlane(t16 < halves ? ((const int32_t __attribute__((address_space(4))) *)(uintptr_t)blocks)[at] : -1);
+            p.page[s] = number >= 0 && number < pages ? number : -1;
+            p.place[s] = (t16 - at * page16) * 16;
+        }
+        return p;
+    }
+    // of a half's first token in the cache; some page's where there is none
+    __device__ __forceinline__ int64_t row(const Pages &p, int s, int h) const { return ((int64_t)max(p.page[s], 0) * heads + h) * page + p.place[s]; }
+    // All rows see a whole tile unless it holds a new token, the end, or a page that is not there; from the first such tile on each is looked
+    // at token by token.  Which that is, is found beforehand: a loop that ends on what it reads kept two sets of all its registers.
+    // The first token from t0 on that is not in a page, at most clear.
+    __device__ __forceinline__ int clear_until(int clear, int t0, int lane) const
+    {
+        for (int at = t0 / page + lane; (int64_t)at * page < clear; at += 64)
+            if (blocks[at] < 0 || blocks[at] >= pages)
+                clear = min(clear, at * page);
+#pragma unroll
+        for (int s = 1; s < 64; s *= 2)
+            clear = min(clear, __shfl_xor(clear, s));
+        return __builtin_amdgcn_readfirstlane(clear);
+    }
+};
+
+// a bit for each of a lane's 8 tokens of the tile at t: seen by new token `own` of the sequence
+__device__ static __forceinline__ uint32_t seen_by(const AttendArgs &a, const Sequence &seq, int own, int t, int j, const Pages &now)
+{
+    const uint64_t mask = a.d.mask ? a.d.mask[seq.row0 + own] : 0;
+    uint32_t sees = 0;
+#pragma unroll
+    for (int half = 0; half < 2; half++) { // four tokens from `first` on
+        const int first = t + half * 16 + j * 4, fresh = first - seq.old;
+        const int there = now.page[half] >= 0 ? min(max(seq.len - first, 0), 4) : 0;
+        uint32_t bits = (1u << min(max(own + 1 - fresh, 0), 4)) - 1;
+        if (a.d.mask)
+            bits = fresh >= 0 ? (uint32_t)(mask >> min(fresh, 63)) & (fresh < 64 ? 15u : 0u)
+                              : (uint32_t)mask << min(-fresh, 4) | ((1u << min(-fresh, 4)) - 1);
+        sees |= (bits & ((1u << there) - 1)) << (4 * half);
+    }
+    return sees;
+}
+
+// infinities or NaN among an operand's 16-bit values
+template <int TYPE>
+__device__ static __forceinline__ bool strange(const u32x4 &v)
+{
+    u16x2 largest = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2, v[e] & 0x7fff7fffu));
+    constexpr uint16_t inf = TYPE == HIPQ_REAL_BF16 ? 0x7f80 : 0x7c00;
+    return largest[0] >= inf || largest[1] >= inf;
+}
+// Where values are infinite or NaN they reach the rows that see them, as NaN, and no other: ones in their places, multiplied by ones at the
+// tokens that a row sees.  What is left of the values is finite.
+template <int TYPE, int RT, int VD>
+__device__ static __forceinline__ void not_finite(u32x4 &v, const uint32_t (&sees)[RT], f32x4 (&o)[RT][VD], int i)
+{
+    using R = Real16<TYPE>;
+    u32x4 bad = {0, 0, 0, 0};
+    const uint32_t one = R::pack(1.0f, 0.0f);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const bool lo = !(fabsf(R::low(v[e])) < __builtin_inff()), hi = !(fabsf(R::high(v[e])) < __builtin_inff());
+        bad[e] = (lo ? one : 0) | (hi ? one << 16 : 0);
+        v[e] &= (lo ? 0 : 0xffffu) | (hi ? 0 : 0xffff0000u);
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        u32x4 seen;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            seen[e] = ((sees[rt] >> (2 * e)) & 1 ? one : 0) | ((sees[rt] >> (2 * e + 1)) & 1 ? one << 16 : 0);
+        const f32x4 n = R::mfma(bad, seen, f32x4{0, 0, 0, 0});
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            o[rt][i][r] = n[r] > 0 ? __builtin_nanf("") : o[rt][i][r];
+    }
+}
+
+// A row's weights p of 8 tokens a lane from its scores s: the reference m moves where a score passes it by more than 8, and with it the sums (l
+// of codes, lsum of 16-bit values) and outputs are scaled.
+template <int TYPE, bool QUANT, bool MASKED, int VD>
+__device__ static __forceinline__ void softmax_step(float scale2, const f32x4 (&s)[2], const f32x4 (&kscale)[2], const f32x4 (&vsc)[2], uint32_t sees, float &m, float &l,
+                                                    f32x4 &lsum, f32x4 (&o)[VD], u32x4 &p)
+{
+    using R = Real16<TYPE>;
+    float x[8], top = NONE;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        x[e] = QUANT ? s[e / 4][e % 4] * kscale[e / 4][e % 4] : s[e / 4][e % 4];
+        if (MASKED)
+            x[e] = (sees >> e) & 1 ? x[e] : NONE;
+        top = fmaxf(top, x[e]);
+    }
+    if (!QUANT)
+        top *= scale2;
+    if (__any(top > m + 8.0f)) {
+        top = fmaxf(top, m);
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float f = top == NONE ? 1.0f : exp2_fast(m - top);
+        m = top;
+        l *= f;
+        lsum *= f;
+#pragma unroll
+        for (int i = 0; i < VD; i++)
+            o[i] *= f;
+    }
+    const float ref = m == NONE ? 0.0f : m;
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        y[e] = exp2_fast(QUANT ? x[e] - ref : __builtin_fmaf(x[e], scale2, -ref));
+        if (QUANT) {
+            l += y[e];
+            y[e] *= vsc[e / 4][e % 4];
+            if (MASKED)
+                y[e] = (sees >> e) & 1 ? y[e] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        p[e] = R::pack(y[2 * e], y[2 * e + 1]);
+    if (!QUANT) {
+        const uint32_t one = R::pack(1.0f, 1.0f);
+        lsum = R::mfma(u32x4{one, one, one, one}, p, lsum);
+    }
+}
 
 template <int TYPE, int DIM, bool QUANT, int RT>
 __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 && DIM == 128 && RT == 2) ? 1 : 2) void kv_attend_kernel(const AttendArgs a)
@@ -142,33 +299,15 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
             o[rt][i] = f32x4{0, 0, 0, 0};
     }
 
-    // a tile: two halves of 16 tokens, each in one page
-    struct Pages {
-        int page[2]; // -1: not there
-        int place[2];
-    };
     u32x4 kx[2][KW];
     uint32_t vx[2][4][VW];
     f32x4 ksc[2], vsc[2];
     const int32_t *blocks = a.d.blocks + (int64_t)b * a.d.blocks_stride;
-    const int halves = (seq.len + 15) / 16, page16 = a.cache.page / 16;
-    auto pages_of = [&](int t) {
-        Pages p;
-#pragma unroll
-        for (int s = 0; s < 2; s++) {
-            const int t16 = t / 16 + s;
-            const int at = a.page_magic ? (int)(((uint64_t)(uint32_t)t16 * a.page_magic) >> 32) >> a.page_shift : t16;
-            const int page = __builtin_amdgcn_readfirstlane(t16 < halves ? blocks[at] : -1);
-            p.page[s] = page >= 0 && page < a.cache.pages ? page : -1;
-            p.place[s] = (t16 - at * page16) * 16;
-        }
-        return p;
-    };
-    auto row_of = [&](const Pages &p, int s) { return ((int64_t)max(p.page[s], 0) * a.cache.heads + h) * a.cache.page + p.place[s]; };
+    const Paging paging(a, blocks, seq.len);
     auto load_k = [&](const Pages &p) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            const int64_t row = row_of(p, s);
+            const int64_t row = paging.row(p, s, h);
             const gbytes_t k = uniform((const uint8_t *)a.cache.k + row * WIDTH);
 #pragma unroll
             for (int i = 0; i < KW; i++)
@@ -180,7 +319,7 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
     auto load_v = [&](const Pages &p) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            const int64_t row = row_of(p, s);
+            const int64_t row = paging.row(p, s, h);
             const gbytes_t v = uniform((const uint8_t *)a.cache.v + row * WIDTH);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
@@ -215,15 +354,12 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
                 k[half][ks] = QUANT ? widen<TYPE>(kx[half][ks / (QUANT ? 2 : 1)][ks % 2 * 2], kx[half][ks / (QUANT ? 2 : 1)][ks % 2 * 2 + 1]) : kx[half][ks / (QUANT ? 2 : 1)];
-        float kscale[2][4];
+        f32x4 kscale[2];
         if (QUANT)
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                kscale[e / 4][e % 4] = ksc[e / 4][e % 4] * a.scale2;
+            kscale[0] = ksc[0] * a.scale2, kscale[1] = ksc[1] * a.scale2;
         __builtin_amdgcn_sched_barrier(0); // what is done earlier than it is written does not fit the registers
         load_k(next);
         __builtin_amdgcn_sched_barrier(0);
-        bool any_strange = false; // infinities or NaN among values that not all rows see
         if (masked) {
             // tokens that are not there may hold anything: their values are taken as 0, so that 0 times them is 0
 #pragma unroll
@@ -237,16 +373,6 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
                     for (int i = 0; i < VW; i++)
                         vx[half][r][i] = r < there ? vx[half][r][i] : 0;
                 }
-            }
-            if (!QUANT && (a.d.mask || seq.count > 1)) {
-                u16x2 largest = {0, 0};
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-#pragma unroll
-                    for (int i = 0; i < VW; i++)
-                        largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2, vx[e / 4][e % 4][i] & 0x7fff7fffu));
-                constexpr uint16_t inf = TYPE == HIPQ_REAL_BF16 ? 0x7f80 : 0x7c00;
-                any_strange = __any(largest[0] >= inf || largest[1] >= inf);
             }
         }
         if (QUANT && TYPE == HIPQ_REAL_F16) {
@@ -279,60 +405,9 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
 #pragma unroll
                 for (int half = 0; half < 2; half++)
                     s[half] = R::mfma(k[half][ks], Q_LDS ? lq[(rt * KS + ks) * 64 + lane] : q[Q_LDS ? 0 : rt][Q_LDS ? 0 : ks], s[half]);
-            float x[8], top = NONE;
-            if (masked) {
-                const uint64_t mask = a.d.mask ? a.d.mask[seq.row0 + own[rt]] : 0;
-                sees[rt] = 0;
-#pragma unroll
-                for (int half = 0; half < 2; half++) { // four tokens from `first` on
-                    const int first = t + half * 16 + j * 4, fresh = first - seq.old;
-                    const int there = now.page[half] >= 0 ? min(max(seq.len - first, 0), 4) : 0;
-                    uint32_t bits = (1u << min(max(own[rt] + 1 - fresh, 0), 4)) - 1;
-                    if (a.d.mask)
-                        bits = fresh >= 0 ? (uint32_t)(mask >> min(fresh, 63)) & (fresh < 64 ? 15u : 0u)
-                                          : (uint32_t)mask << min(-fresh, 4) | ((1u << min(-fresh, 4)) - 1);
-                    sees[rt] |= (bits & ((1u << there) - 1)) << (4 * half);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                x[e] = QUANT ? s[e / 4][e % 4] * kscale[e / 4][e % 4] : s[e / 4][e % 4];
-                if (masked)
-                    x[e] = (sees[rt] >> e) & 1 ? x[e] : NONE;
-                top = fmaxf(top, x[e]);
-            }
-            if (!QUANT)
-                top *= a.scale2;
-            if (__any(top > m[rt] + 8.0f)) {
-                top = fmaxf(top, m[rt]);
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float f = top == NONE ? 1.0f : exp2_fast(m[rt] - top);
-                m[rt] = top;
-                l[rt] *= f;
-                lsum[rt] *= f;
-#pragma unroll
-                for (int i = 0; i < VD; i++)
-                    o[rt][i] *= f;
-            }
-            const float ref = m[rt] == NONE ? 0.0f : m[rt];
-            float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                y[e] = exp2_fast(QUANT ? x[e] - ref : __builtin_fmaf(x[e], a.scale2, -ref));
-                if (QUANT) {
-                    l[rt] += y[e];
-                    y[e] *= vsc[e / 4][e % 4];
-                    if (masked)
-                        y[e] = (sees[rt] >> e) & 1 ? y[e] : 0.0f;
-                }
-            }
-            const uint32_t one = R::pack(1.0f, 0.0f);
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                p[rt][e] = R::pack(y[2 * e], y[2 * e + 1]);
-            if (!QUANT)
-                lsum[rt] = R::mfma(u32x4{one * 0x10001u, one * 0x10001u, one * 0x10001u, one * 0x10001u}, p[rt], lsum[rt]);
+            if (masked)
+                sees[rt] = seen_by(a, seq, own[rt], t, j, now);
+            softmax_step<TYPE, QUANT, masked, VD>(a.scale2, s, kscale, vsc, masked ? sees[rt] : 0, m[rt], l[rt], lsum[rt], o[rt], p[rt]);
         }
         __builtin_amdgcn_sched_barrier(0);
         // output
@@ -347,28 +422,8 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
                 else
                     v[e] = __builtin_amdgcn_perm(vx[half][r + 1][i / 2], vx[half][r][i / 2], i % 2 ? 0x07060302u : 0x05040100u);
             }
-            if (masked && !QUANT && any_strange) {
-                // an infinity or NaN among the values near the end reaches the rows that see it, as NaN, and no other
-                u32x4 bad = {0, 0, 0, 0};
-                const uint32_t one = R::pack(1.0f, 0.0f);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const bool lo = !(fabsf(R::low(v[e])) < __builtin_inff()), hi = !(fabsf(R::high(v[e])) < __builtin_inff());
-                    bad[e] = (lo ? one : 0) | (hi ? one << 16 : 0);
-                    v[e] &= (lo ? 0 : 0xffffu) | (hi ? 0 : 0xffff0000u);
-                }
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    u32x4 seen; // ones at the tokens that a row sees
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        seen[e] = ((sees[rt] >> (2 * e)) & 1 ? one : 0) | ((sees[rt] >> (2 * e + 1)) & 1 ? one << 16 : 0);
-                    const f32x4 n = R::mfma(bad, seen, f32x4{0, 0, 0, 0});
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        o[rt][i][r] = n[r] > 0 ? __builtin_nanf("") : o[rt][i][r];
-                }
-            }
+            if (masked && !QUANT && (a.d.mask || seq.count > 1) && __any(strange<TYPE>(v)))
+                not_finite<TYPE>(v, sees, o, i);
 #pragma unroll
             for (int rt = 0; rt < RT; rt++)
                 o[rt][i] = R::mfma(v, p[rt], o[rt][i]);
@@ -378,33 +433,20 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
 
     int t = t0 + wave * 32;
     if (t < t1) {
-        // All rows see a whole tile unless it holds a new token, the end, or a page that is not there; from the first such tile on each is
-        // looked at token by token.  Which that is, is found beforehand: a loop that ends on what it reads kept two sets of all its registers
-        int clear = min(min(seq.old, seq.len), t1), page_at = t0 / a.cache.page + lane;
-        int there = (int64_t)page_at * a.cache.page < clear ? blocks[page_at] : 0;
-        Pages now = pages_of(t), next = pages_of(t + 128);
+        Pages now = paging.of(t), next = paging.of(t + 128);
         load_k(now);
         load_v(now);
-        do {
-            if (there < 0 || there >= a.cache.pages)
-                clear = min(clear, page_at * a.cache.page);
-            page_at += 64;
-            there = (int64_t)page_at * a.cache.page < clear ? blocks[page_at] : 0;
-        } while (__any((int64_t)page_at * a.cache.page < clear));
-#pragma unroll
-        for (int s = 1; s < 64; s *= 2)
-            clear = min(clear, __shfl_xor(clear, s));
-        clear = __builtin_amdgcn_readfirstlane(clear);
+        const int clear = paging.clear_until(min(min(seq.old, seq.len), t1), t0, lane);
         const int whole = clear - t >= 32 ? (clear - t - 32) / 128 + 1 : 0, last = (t1 - t + 127) / 128;
 #pragma unroll 1
         for (int i = 0; i < whole; i++, t += 128) {
-            const Pages after = pages_of(t + 256);
+            const Pages after = paging.of(t + 256);
             tile(t, now, next, std::false_type{});
             now = next, next = after;
         }
 #pragma unroll 1
         for (int i = whole; i < last; i++, t += 128) {
-            const Pages after = pages_of(t + 256);
+            const Pages after = paging.of(t + 256);
             tile(t, now, next, std::true_type{});
             now = next, next = after;
         }
@@ -491,6 +533,253 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
     }
 }
 
+// For more than 64 rows: 128 of a work-group, 32 of each of its four waves, all at the same tile of 32 tokens.  Each wave brings a quarter of
+// the tile - some 16 x 32 operands of keys, turned ones of values - into LDS in operand order, widened from 8 bits once for all 128 rows,
+// a tile ahead of the multiplies that read it; one barrier a tile.  Nothing is joined at the end, as a wave sees all tokens of its rows.
+template <int TYPE, int DIM, bool QUANT>
+__global__ __launch_bounds__(256, 2) void kv_attend_wide_kernel(const AttendArgs a)
+{
+    using R = Real16<TYPE>;
+    constexpr int RT = 2, ROWS = 64 * RT;
+    constexpr int KS = DIM / 32, VD = DIM / 16, KF = KS / 2, VF = VD / 4; // operands of a tile's half, of its values; a wave's share of both
+    constexpr int WIDTH = QUANT ? DIM : 2 * DIM;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, j = lane >> 4;
+    const int eighth = gridDim.x / 8, item = (int)(blockIdx.x % 8) * eighth + (int)(blockIdx.x / 8);
+    const int rb = item % a.row_blocks, split = item / a.row_blocks % a.splits, rest = item / a.row_blocks / a.splits;
+    const int h = rest % a.cache.heads, b = rest / a.cache.heads;
+    if (b >= a.d.sequences)
+        return;
+    const Sequence seq(a, b);
+    const int rows = seq.count * a.group, r0 = rb * ROWS + wave * 16 * RT;
+    if (rb * ROWS >= rows)
+        return;
+    const int share = seq.share(a.splits), t0 = split * share;
+    const int most = a.d.mask ? seq.len : min(seq.len, seq.old + min(rows - 1, rb * ROWS + ROWS - 1) / a.group + 1);
+    const int t1 = min(t0 + share, most);
+
+    __shared__ u32x4 lkv[2][2 * KS + VD][64]; // keys: [half][ks], then values
+    __shared__ f32x4 lsc[2][QUANT ? 16 : 1];  // scales of keys, then of values
+    u32x4 q[RT][KS];
+    int own[RT], qh[RT]; // the lane's rows (the last one again behind it): new token and query head
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const int row = min(r0 + 16 * rt + c, rows - 1);
+        own[rt] = row / a.group, qh[rt] = h * a.group + row - own[rt] * a.group;
+        const uint16_t *x = (const uint16_t *)a.d.q + (int64_t)(seq.row0 + own[rt]) * a.d.q_token + (int64_t)qh[rt] * a.d.q_head;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+            q[rt][ks] = *(const u32x4 *)(x + ks * 32 + j * 8);
+    }
+    float m[RT], l[RT], unit = 0, per_unit = 0;
+    f32x4 lsum[RT], o[RT][VD];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        m[rt] = NONE, l[rt] = 0;
+        lsum[rt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < VD; i++)
+            o[rt][i] = f32x4{0, 0, 0, 0};
+    }
+
+    const int32_t *blocks = a.d.blocks + (int64_t)b * a.d.blocks_stride;
+    const Paging paging(a, blocks, seq.len);
+    // the wave's part of a tile: operands wave KF .. of keys; of values elements (16 VF) wave + VF c ..
+    u32x4 kxs[2][KF];
+    uint32_t vxs[2][2][4];
+    float sxs[2] = {0, 0};
+    auto load = [&](auto SET, const Pages &p) __attribute__((always_inline)) {
+        auto &kx = kxs[decltype(SET)::value];
+        auto &vx = vxs[decltype(SET)::value];
+        auto &sx = sxs[decltype(SET)::value];
+        const int64_t row0 = paging.row(p, 0, h), row1 = paging.row(p, 1, h);
+        const gbytes_t k = uniform((const uint8_t *)a.cache.k + (wave * KF >= KS ? row1 : row0) * WIDTH);
+#pragma unroll
+        for (int n = 0; n < KF; n++) {
+            const uint32_t from = c * WIDTH + ((wave * KF + n) % KS * 32 + j * 8) * (QUANT ? 1 : 2);
+            if (QUANT) {
+                const u32x2 w = at<u32x2>(k, from);
+                kx[n][0] = w[0], kx[n][1] = w[1];
+            } else
+                kx[n] = at<u32x4>(k, from);
+        }
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const gbytes_t v = uniform((const uint8_t *)a.cache.v + (s ? row1 : row0) * WIDTH);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const uint32_t from = (j * 4 + r) * WIDTH + (16 * wave + c) * (QUANT ? VF : 2 * VF);
+                vx[s][r] = (QUANT ? VF : 2 * VF) == 1 ? at<uint8_t>(v, from) : (QUANT ? VF : 2 * VF) == 2 ? at<uint16_t>(v, from) : at<uint32_t>(v, from);
+            }
+        }
+        if (QUANT) // 32 tokens' scales of keys, then of values: every wave has them, or a wait after the branch would be one for all loads
+            sx = *((lane < 32 ? a.cache.k_scale : a.cache.v_scale) + (lane & 16 ? row1 : row0) + (lane & 15));
+    };
+    auto store = [&](auto SET, int t, const Pages &p) __attribute__((always_inline)) {
+        constexpr int to = decltype(SET)::value;
+        auto &kx = kxs[to];
+        auto &vx = vxs[to];
+        auto &sx = sxs[to];
+        if (QUANT) {
+#pragma unroll
+            for (int n = 0; n < KF; n++)
+                asm volatile("" : "+v"(kx[n][0]), "+v"(kx[n][1]));
+#pragma unroll
+            for (int n = 0; n < 8; n++)
+                asm volatile("" : "+v"(vx[n / 4][n % 4]));
+        }
+        if (t + 32 > seq.len || p.page[0] < 0 || p.page[1] < 0) {
+            // tokens that are not there may hold anything: their values are taken as 0, so that 0 times them is 0
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const int there = p.page[s] >= 0 ? seq.len - t - s * 16 - j * 4 : 0;
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    vx[s][r] = r < there ? vx[s][r] : 0;
+            }
+            if (QUANT && lane >= 32)
+                sx = (lane & 16 ? p.page[1] : p.page[0]) >= 0 && t + (lane & 31) < seq.len ? sx : 0.0f;
+        }
+#pragma unroll
+        for (int n = 0; n < KF; n++)
+            lkv[to][wave * KF + n][lane] = QUANT ? widen<TYPE>(kx[n][0], kx[n][1]) : kx[n];
+#pragma unroll
+        for (int n = 0; n < VF; n++) {
+            u32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t v0 = vx[e / 2][e % 2 * 2], v1 = vx[e / 2][e % 2 * 2 + 1];
+                v[e] = QUANT ? R::pack_exact((float)(int8_t)(v0 >> (8 * n)), (float)(int8_t)(v1 >> (8 * n)))
+                             : __builtin_amdgcn_perm(v1, v0, n ? 0x07060302u : 0x05040100u);
+            }
+            lkv[to][2 * KS + wave * VF + n][lane] = v;
+        }
+        if (QUANT && wave == 0)
+            ((float *)lsc[to])[lane] = lane < 32 ? sx * a.scale2 : sx;
+    };
+
+    auto tile = [&](int t, int from, const Pages &now, auto MASKED) __attribute__((always_inline)) {
+        constexpr bool masked = decltype(MASKED)::value;
+        f32x4 kscale[2], vsc[2];
+        if (QUANT)
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+                kscale[s] = lsc[from][s * 4 + j], vsc[s] = lsc[from][8 + s * 4 + j];
+        if (QUANT && TYPE == HIPQ_REAL_F16) {
+            float top = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                top = fmaxf(top, vsc[e / 4][e % 4]);
+            if (__any(top > unit)) {
+#pragma unroll
+                for (int s = 1; s < 64; s *= 2)
+                    top = fmaxf(top, __shfl_xor(top, s));
+                top = fminf(fmaxf(top, 1e-30f), 3e38f);
+                const float f = unit / top;
+                unit = top, per_unit = 1.0f / top;
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int i = 0; i < VD; i++)
+                        o[rt][i] *= f;
+            }
+            vsc[0] *= per_unit, vsc[1] *= per_unit;
+        }
+        f32x4 s[RT][2];
+#pragma unroll
+        for (int half = 0; half < 2; half++)
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const u32x4 k = lkv[from][half * KS + ks][lane];
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+                    s[rt][half] = R::mfma(k, q[rt][ks], ks ? s[rt][half] : f32x4{0, 0, 0, 0});
+            }
+        u32x4 p[RT];
+        uint32_t sees[RT]; // a bit for each of the lane's 8 tokens: seen by the row
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            if (masked)
+                sees[rt] = seen_by(a, seq, own[rt], t, j, now);
+            softmax_step<TYPE, QUANT, masked, VD>(a.scale2, s[rt], kscale, vsc, masked ? sees[rt] : 0, m[rt], l[rt], lsum[rt], o[rt], p[rt]);
+        }
+#pragma unroll
+        for (int i = 0; i < VD; i++) {
+            u32x4 v = lkv[from][2 * KS + i][lane];
+            if (masked && !QUANT && (a.d.mask || seq.count > 1) && __any(strange<TYPE>(v)))
+                not_finite<TYPE>(v, sees, o, i);
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+                o[rt][i] = R::mfma(v, p[rt], o[rt][i]);
+        }
+    };
+    if (t0 < t1) {
+        const std::integral_constant<int, 0> EVEN;
+        const std::integral_constant<int, 1> ODD;
+        Pages now = paging.of(t0), next = paging.of(t0 + 32), then = paging.of(t0 + 64);
+        load(EVEN, now);
+        load(ODD, next);
+        const int clear = paging.clear_until(min(min(seq.old, seq.len), t1), t0, lane);
+        const int whole = clear > t0 ? (clear - t0) / 64 * 2 : 0, last = (t1 - t0 + 31) / 32; // two tiles at a time, each with its set of registers
+        store(EVEN, t0, now);
+        load(EVEN, then);
+        __syncthreads();
+        int t = t0;
+        auto turn = [&](auto SET, auto OTHER, auto MASKED) __attribute__((always_inline)) {
+            const Pages after = paging.of(t + 96);
+            tile(t, decltype(SET)::value, now, MASKED);
+            __builtin_amdgcn_sched_barrier(0); // what is done earlier than it is written does not fit the registers
+            store(OTHER, t + 32, next);
+            load(OTHER, after);
+            __builtin_amdgcn_sched_barrier(0);
+            __syncthreads();
+            __builtin_amdgcn_sched_barrier(0);
+            now = next, next = then, then = after, t += 32;
+        };
+#pragma unroll 1
+        for (int i = 0; i < whole; i += 2) {
+            turn(EVEN, ODD, std::false_type{});
+            turn(ODD, EVEN, std::false_type{});
+        }
+#pragma unroll 1
+        for (int i = whole; i < last; i += 2) {
+            turn(EVEN, ODD, std::true_type{});
+            if (i + 1 < last)
+                turn(ODD, EVEN, std::true_type{});
+        }
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        if (QUANT) {
+            l[rt] += __shfl_xor(l[rt], 16);
+            l[rt] += __shfl_xor(l[rt], 32);
+        } else
+            l[rt] = lsum[rt][0];
+        const int row = r0 + 16 * rt + c;
+        if (row >= rows)
+            continue;
+        const float f = (QUANT && TYPE == HIPQ_REAL_F16 ? unit : 1.0f) * (a.splits > 1 ? 1.0f : l[rt] > 0 ? 1.0f / l[rt] : l[rt] == 0 ? 0.0f : l[rt]);
+        const int64_t at = (((int64_t)b * a.cache.heads + h) * a.splits + split) * a.rows + row;
+        if (a.splits > 1 && j == 0)
+            a.part_ml[2 * at] = m[rt], a.part_ml[2 * at + 1] = l[rt];
+        uint16_t *y = (uint16_t *)a.d.o + (int64_t)(seq.row0 + own[rt]) * a.d.o_token + (int64_t)qh[rt] * a.d.o_head;
+#pragma unroll
+        for (int w = 0; w < 4; w++) { // elements 16 VF w + VF (4 j + r) + n
+            float v[4 * VF];
+#pragma unroll
+            for (int e = 0; e < 4 * VF; e++)
+                v[e] = o[rt][w * VF + e % VF][e / VF] * f;
+            const int i0 = (16 * w + 4 * j) * VF;
+#pragma unroll
+            for (int e = 0; e < 4 * VF; e += 4)
+                if (a.splits > 1)
+                    *(f32x4 *)(a.part_o + at * DIM + i0 + e) = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+                else
+                    *(u32x2 *)(y + i0 + e) = u32x2{R::pack(v[e], v[e + 1]), R::pack(v[e + 2], v[e + 3])};
+        }
+    }
+}
+
 // Joins the parts of a row: DIM / 4 lanes side by side have its elements, SIDE such groups of a work-group its parts in turn.
 template <int TYPE, int DIM, int SIDE>
 __global__ __launch_bounds__(256) void kv_attend_join_kernel(const AttendArgs a)
@@ -542,7 +831,7 @@ __global__ __launch_bounds__(256) void kv_attend_join_kernel(const AttendArgs a)
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------
 struct AttendShape {
-    int rt, row_blocks, rows, splits;
+    int rt, row_blocks, rows, splits; // rt: 16-row blocks of a wave; 8: the wide kernel's work-group
     size_t workspace;
 };
 
@@ -571,12 +860,19 @@ static AttendShape shape_of(const hipq_kv_cache *c, const hipq_kv_attend_desc *d
     const int group = d->q_heads / c->heads;
     s.rows = d->most_new * group;
     s.rt = s.rows <= 16 || c->dim == 256 ? 1 : 2; // two blocks of 256-wide outputs are all of a wave's registers
-    s.row_blocks = (s.rows + 16 * s.rt - 1) / (16 * s.rt);
     const int64_t longest = d->longest < (int64_t)d->blocks_per_sequence * c->page ? d->longest : (int64_t)d->blocks_per_sequence * c->page;
+    // The wide kernel, where it has work for the whole chip, two work-groups a CU with the longest sequences: us against the other
+    // kernel's, 16 trees of 32 tokens on up to 8000 in 8 bits 111 against 121, of 17 tokens 105 against 103; in 16 bits 8 x 32 on up to 4096 44
+    // against 55, 2 x 64 on up to 16000 65 against 89, 41 chains of 34 on up to 825 43 against 53; with less, 64 on 500 of 4 heads, 22 against
+    // 14, and with heads of 64, 24 on up to 4000, 25 against 21.5.  (256 work-groups: 168, 48 and 81 of the first, third and fourth.)
+    const int64_t wide = (int64_t)d->sequences * c->heads * ((s.rows + 127) / 128);
+    if (c->dim == 128 && s.rows > 64 && wide * ((longest + 255) / 256) >= 256)
+        s.rt = 8;
+    s.row_blocks = (s.rows + 16 * s.rt - 1) / (16 * s.rt);
     const int64_t items = (int64_t)d->sequences * c->heads * s.row_blocks;
     // A work-group a CU is enough, and two where that leaves some with a longer sequence than others: us with 256, 512 and 1024 work-groups of
     // 8 trees of 16 tokens on 4096: 38, 42, 54; one token on 2 x 131072: 186, 197, 201; of 32 sequences up to 4096 in 8 bits: 62, 52, 55
-    const int64_t target = items < 256 ? 256 : 512, want = items ? (target + items - 1) / items : 1, most = (longest + 255) / 256;
+    const int64_t target = items < 256 ? 256 : 512, want = s.rt == 8 ? 512 / (items > 512 ? 512 : items) : items ? (target + items - 1) / items : 1, most = (longest + 255) / 256;
     s.splits = (int)(want < most ? want : most);
     s.splits = s.splits < 1 ? 1 : s.splits > 64 ? 64 : s.splits;
     if (s.splits > 1)
@@ -596,6 +892,11 @@ static int launch_attend(const AttendArgs &a, int64_t items, hipStream_t st)
 template <int TYPE, int DIM, bool QUANT>
 static int launch_attend(const AttendArgs &a, int rt, int64_t items, hipStream_t st)
 {
+    if (rt == 8) {
+        if constexpr (DIM == 128)
+            kv_attend_wide_kernel<TYPE, DIM, QUANT><<<dim3((unsigned)((items * a.splits + 7) / 8 * 8)), dim3(256), 0, st>>>(a);
+        return launch_status("kv_attend_wide_kernel");
+    }
     return rt == 1 ? launch_attend<TYPE, DIM, QUANT, 1>(a, items, st) : launch_attend<TYPE, DIM, QUANT, DIM == 256 ? 1 : 2>(a, items, st);
 }
 

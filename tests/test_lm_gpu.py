@@ -397,6 +397,94 @@ def test_attend_pages_that_are_not_there():
     assert (a.double() - b.double()).abs().max() <= 2 ** -7 * b.abs().max()
 
 
+# many rows of heads of 128 over sequences that may be long: 128 rows of a work-group
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("tree", [False, True])
+def test_attend_many_rows(dtype, int8, tree):
+    g, rng = gen(50), np.random.default_rng(50)
+    counts, lens = [34, 0, 1, 20, 64, 33, 17, 5], [1000, 50, 1, 20, 600, 33, 97, 1024]
+    cache, blocks = fill_cache(g, dtype, 8, 8, 48, 128, 1024, int8)
+    check_attend(g, cache, blocks, counts, lens, 32, dtype, mask=trees(rng, counts) if tree else None)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("counts, lens, hq", [([300, 129], [300, 1500], 16), ([128, 1], [2047, 2048], 8), ([65, 97], [96, 1000], 8), ([33, 34], [33, 66], 24)])
+def test_attend_prompts_of_long_sequences(counts, lens, hq, dtype, int8):
+    g = gen(51)
+    cache, blocks = fill_cache(g, dtype, 2, 8, 16, 128, 4096, int8)
+    check_attend(g, cache, blocks, counts, lens, hq, dtype)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_attend_many_rows_that_see_nothing(int8):
+    g = gen(52)
+    counts, lens = [4, 2, 64, 0, 64], [4, 60, 64, 0, 700]
+    mask = torch.zeros(134, dtype=torch.int64, device="cuda")
+    mask[1], mask[3] = 2, 5
+    mask[6 + 63] = -(1 << 63)  # the last bit
+    cache, blocks = fill_cache(g, BF16, 5, 8, 16, 128, 2048, int8)
+    q, got = check_attend(g, cache, blocks, counts, lens, 16, BF16, mask=mask)
+    assert (got[0] == 0).all() and (got[2] == 0).all() and (got[6:6 + 63] == 0).all() and got[6 + 63].abs().max() > 0
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("mask", [False, True])
+def test_attend_many_rows_nothing_from_behind_the_end(int8, mask):
+    g, rng = gen(53), np.random.default_rng(53)
+    counts, lens = [40, 33, 64], [137, 48, 900]
+    cache, blocks = fill_cache(g, F16, 3, 8, 16, 128, 4096, int8)
+    words = trees(rng, counts) if mask else None
+    q, want = check_attend(g, cache, blocks, counts, lens, 32, F16, mask=words)
+    bad = [math.nan, math.inf, -math.inf]
+    for b, n in enumerate(lens):
+        page = int(blocks[b, n // 16])
+        if int8:
+            cache.k_scale[page, :, n % 16:], cache.v_scale[page, :, n % 16:] = bad[b], math.nan
+        else:
+            cache.k[page, :, n % 16:], cache.v[page, :, n % 16:] = bad[b], bad[2 - b]
+        blocks[b, n // 16 + 1:] = [-1, 1 << 30, -(1 << 31)][b]
+    index = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    words = None if words is None else torch.cat((words, words[:2]))
+    got = cache.attend(q, index([0, 40, 73, 137]), index(lens), blocks, 64, mask=words)
+    assert torch.equal(got[:137], want[:137])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_attend_many_rows_values_that_are_not_finite(dtype):
+    """An infinity in a drafted token's value, and a NaN in another's, reach the rows that see them and no others."""
+    g, rng = gen(54), np.random.default_rng(54)
+    cache, blocks = fill_cache(g, dtype, 1, 8, 16, 128, 8192, False)
+    mask = trees(rng, [50])
+    index = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    q = randn(g, dtype, 50, 32, 128)
+    args = (q, index([0, 50]), index([1050]), blocks, 50)
+    want = cache.attend(*args, mask=mask)
+    for new, head, i, value in ((7, 2, 9, math.inf), (30, 5, 126, math.nan)):
+        at = 1000 + new
+        cache.v[blocks[0, at // 16].long(), head, at % 16, i] = value
+        got = cache.attend(*args, mask=mask)
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[((mask >> new) & 1).bool(), 4 * head:4 * head + 4, i] = True
+        assert 0 < hit.sum() < 200 and not torch.isfinite(got[hit]).any() and torch.equal(got[~hit], want[~hit])
+        cache.v[blocks[0, at // 16].long(), head, at % 16, i] = 0
+        want = cache.attend(*args, mask=mask)
+
+
+def test_attend_many_rows_pages_that_are_not_there():
+    g = gen(55)
+    cache, blocks = fill_cache(g, BF16, 2, 8, 16, 128, 4096, False)
+    index = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    q = randn(g, BF16, 80, 16, 128)
+    holes = blocks.clone()
+    holes[:, 2], holes[:, 4] = -1, cache.k.shape[0]
+    packed = torch.cat((blocks[:, [0, 1, 3]], blocks[:, 5:], blocks[:, [2, 4]]), 1).contiguous()
+    a = cache.attend(q, index([0, 40, 80]), index([400, 370]), holes, 40)
+    b = cache.attend(q, index([0, 40, 80]), index([368, 338]), packed, 40)
+    assert (a.double() - b.double()).abs().max() <= 2 ** -7 * b.abs().max()
+
+
 @pytest.mark.parametrize("int8", [False, True])
 def test_pages_beyond_32_bits(int8):
     """A cache of more than 2^32 bytes and 2^31 elements: tokens go to its last pages and are read there."""
