@@ -514,7 +514,7 @@ int hipq_w4_plan_create(const hipq_w4_desc *desc, const uint8_t *q, const void *
 void hipq_w4_plan_destroy(hipq_w4_plan *plan);
 /* Name of the kernel that hipq_w4_run launches for M rows ("" for a number of rows that it refuses).  The string is static. */
 const char *hipq_w4_plan_kernel(const hipq_w4_plan *plan, int M);
-/* x: M rows of K, x_stride elements apart (a multiple of 8, the first row at a multiple of 16 bytes); y: M rows of N, y_stride apart.
+/* x: M rows of K, x_stride elements apart (a multiple of 8 below 2^23, the first row at a multiple of 16 bytes); y: M rows of N, y_stride apart.
  * M may be 0.  The plan belongs to the device that it was created on.  workspace: hipq_w4_workspace bytes at a multiple of 16 (0: none,
  * may be NULL), whose content is of no interest before and after; calls that may run at the same time need one each. */
 size_t hipq_w4_workspace(const hipq_w4_plan *plan, int M);
@@ -563,8 +563,10 @@ int hipq_kv_append(const hipq_kv_cache *cache, const hipq_kv_append_desc *desc, 
  * ancestors and itself; at most 64 new tokens a sequence).  Query head h reads the cache's head h / (q_heads / heads).
  *   o = sum_t softmax_t(scale * q . k_t) v_t over the tokens seen; 0 where there is none.
  * Rows of o that belong to no sequence are left as they are.  Entries of blocks behind a sequence's end are not read; a block outside
- * the cache holds no tokens (they are not seen).  Lengths beyond `longest`, and more new tokens than `most_new`, are cut off there: the
- * caller's bounds, from which the host divides the work.
+ * the cache holds no tokens (they are not seen).  `longest` and `most_new` are the caller's bounds, from which the host divides the work:
+ * of a sequence that is longer, or has more new tokens, nothing outside is read or written, and its rows mean nothing.
+ * The scale is above 0.  o may be q itself (same strides).  Weights are rounded to 16 bits for the product with the values.  A value that is
+ * infinite or NaN reaches the rows that see its token, as NaN or as an infinity.
  * workspace: hipq_kv_attend_workspace bytes at a multiple of 16 (0: none, may be NULL), whose content is of no interest before and after;
  * calls that may run at the same time need one each.
  */
@@ -593,7 +595,7 @@ int hipq_kv_attend(const hipq_kv_cache *cache, const hipq_kv_attend_desc *desc, 
  * taken: a row of nothing else gives -1; of +infinities each has the same weight, and nothing else has any.
  * Weights are summed in 64-bit fixed point, so that no order of summation shows in a result.
  * temperature, top_k, top_p, min_p: a value per row, or NULL (1, all, all, all).  logits: rows of `vocab` of `type` (HIPQ_REAL_*), `stride`
- * elements apart, at any address that the type allows.
+ * elements apart, at any address that the type allows; vocab: up to 2^20.
  */
 int hipq_sample(const void *logits, int type, int rows, int vocab, int64_t stride, const float *uniform, const float *temperature,
                 const int32_t *top_k, const float *top_p, const float *min_p, int64_t *tokens, void *stream);

@@ -46,7 +46,7 @@ struct SampleShared {
         uint32_t list[LIST];
         uint64_t few[FEW];
     };
-    double powers[1024]; // 2^(i / 1024)
+    double powers[1024]; // 2^(43 + i / 1024)
     uint64_t wave[WAVES], region[WAVES];
     uint64_t before;
     uint32_t bin, listed, low, high;
@@ -113,6 +113,7 @@ __device__ static __forceinline__ float score_of(uint32_t key)
 __device__ static __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 __device__ static __forceinline__ uint64_t uniform(uint64_t v) { return (uint64_t)uniform((uint32_t)(v >> 32)) << 32 | uniform((uint32_t)v); }
 __device__ static __forceinline__ float uniform(float v) { return __builtin_bit_cast(float, uniform(__builtin_bit_cast(uint32_t, v))); }
+__device__ static __forceinline__ double uniform(double v) { return __builtin_bit_cast(double, uniform(__builtin_bit_cast(uint64_t, v))); }
 __device__ static __forceinline__ uint64_t of_lane(uint64_t v, int lane)
 {
     return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
@@ -144,7 +145,7 @@ struct Row {
     int tid, lane, wave;
     float top, per_bin; // intervals of a unit of score
     bool infinite = false;
-    double rate;        // log2(e) / temperature
+    double rate, lowest; // log2(e) / temperature; the difference to the top from which on nothing has a weight
     // the border: scores above that of key are kept, and of those equal to it the first `ties` (up to index `last`)
     uint32_t key = 0x007fffffu /* -infinity's */, ties = 0xffffffffu;
     int last = 0x7fffffff;
@@ -171,6 +172,7 @@ struct Row {
     template <class F>
     __device__ __forceinline__ void each(int from, int to, int id, int lanes, F f)
     {
+        asm volatile("" : "+v"(id)); // or every pass's addresses are made at the beginning, and kept
         uint32_t v[4], ahead[4];
         S::load(row, from + id * S::LOAD, to, v);
 #pragma unroll 1
@@ -194,16 +196,18 @@ struct Row {
     __device__ __forceinline__ void each(F f) { each(0, a.vocab, tid, THREADS, f); }
 
     // 2^(rate (x - top)) in units of 2^-43: 2^(n / 1024) from the table times 2^r, |r| <= 1 / 2048, to the second power (the third is under
-    // 2^-37 of the whole).  No branch, and no instruction to spare: a pass takes 64 / 4 of a wave's clocks for each.  The result is RAW more.
+    // 2^-37 of the whole).  No branch, and no instruction to spare: a pass takes 64 / 16 of a wave's clocks for each.  The power of two
+    // goes into the table's number by its exponent, and the sum that rounds is the last product's.  The result is RAW more.
     static constexpr uint64_t RAW = 0x4330000000000000ull; // 2^52: a sum's lower bits are the rounded number
     __device__ __forceinline__ uint64_t raw_weight(float x) const
     {
-        const double y = fmax(((double)x - (double)top) * rate, -60.0); // at most 0; NaN and all below count as 2^-60, which rounds to 0
-        const double big = 6755399441055744.0 / 1024;                   // 1.5 * 2^52 / 1024: what is added keeps ten bits behind the point
-        const double t = y + big, r = y - (t - big);
-        const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
+        const double d = fmax((double)x - (double)top, lowest); // NaN and all below the lowest weigh 2^-17 units, which rounds to 0
+        const double big = 6755399441055744.0 / 1024;            // 1.5 * 2^52 / 1024: what is added keeps ten bits behind the point
+        const double t = __builtin_fma(d, rate, big), r = __builtin_fma(d, rate, big - t);
+        const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, t);
         const double p = __builtin_fma(__builtin_fma(r, 0.24022650695910071, 0.69314718055994531), r, 1.0);
-        return __builtin_bit_cast(uint64_t, __builtin_ldexp(p * s.powers[n & 1023], (n >> 10) + FRACTION) + 4503599627370496.0);
+        const uint64_t power = __builtin_bit_cast(uint64_t, s.powers[n & 1023]) + ((uint64_t)((n & ~1023u) << 10) << 32);
+        return __builtin_bit_cast(uint64_t, __builtin_fma(p, __builtin_bit_cast(double, power), 4503599627370496.0));
     }
     __device__ __forceinline__ uint64_t weight(float x) const { return raw_weight(x) - RAW; }
     __device__ __forceinline__ int bin_of(float x) const
@@ -410,7 +414,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
     const int tid = threadIdx.x;
     const float none = -__builtin_inff();
 
-    s.powers[tid] = POWERS[0][tid >> 5] * POWERS[1][tid & 31];
+    s.powers[tid] = POWERS[0][tid >> 5] * POWERS[1][tid & 31] * (double)((uint64_t)1 << FRACTION);
     float top = none;
     r.each([&](const float(&x)[E], int) INLINE {
 #pragma unroll
@@ -458,19 +462,20 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
             a.tokens[blockIdx.x] = s.index;
         return;
     }
-    r.rate = 1.4426950408889634 / (double)t;
+    r.rate = uniform(1.4426950408889634 / (double)t);
+    r.lowest = uniform(-fmin(60.0 / r.rate, 1e300));
     // 2047 intervals down to where weights are 0, the last one for all below
     r.per_bin = (float)((BINS - 1) * r.rate / 44.5);
-    r.per_bin = r.per_bin < 1e30f ? r.per_bin : 1e30f;
+    r.per_bin = uniform(r.per_bin < 1e30f ? r.per_bin : 1e30f);
     if (a.min_p) {
         const double p = (double)a.min_p[blockIdx.x] * (double)((uint64_t)1 << FRACTION);
-        r.least = p > 0 ? p < (double)((uint64_t)1 << FRACTION) ? (uint64_t)ceil(p) : (uint64_t)1 << FRACTION : 0;
+        r.least = uniform(p > 0 ? p < (double)((uint64_t)1 << FRACTION) ? (uint64_t)ceil(p) : (uint64_t)1 << FRACTION : (uint64_t)0);
     }
-    const int k = a.top_k ? a.top_k[blockIdx.x] : 0;
-    const float p = a.top_p ? a.top_p[blockIdx.x] : 1.0f;
+    const int k = a.top_k ? (int)uniform((uint32_t)a.top_k[blockIdx.x]) : 0;
+    const float p = a.top_p ? uniform(a.top_p[blockIdx.x]) : 1.0f;
     const bool by_count = k > 0 && k < a.vocab, by_mass = p < 1;
     bool known = false;
-    const double u = (double)a.uniform[blockIdx.x];
+    const double u = uniform((double)a.uniform[blockIdx.x]);
     auto goal_of = [&](uint64_t all) INLINE -> uint64_t {
         const double at = u > 0 ? u * (double)all : 0;
         return at < (double)all ? (uint64_t)at : all - 1;
@@ -489,11 +494,12 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
         __syncthreads();
         const uint32_t key = r.key, ties = r.ties;
         const float border = score_of(key);
+        const bool all_ties = ties == 0xffffffffu && border > none;
         r.each([&](const float(&x)[E], int) INLINE {
             bool in[E], any = false;
 #pragma unroll
             for (int e = 0; e < E; e++)
-                any |= in[e] = x[e] > border || (x[e] == border && ties == 0xffffffffu && border > none);
+                any |= in[e] = (x[e] > border) | ((x[e] == border) & all_ties); // no branches: a loop of them took twice the instructions
             if (any) {
                 uint64_t w[E];
                 if (mass)
@@ -528,21 +534,27 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
             uint64_t above = 0;
             r.each(r.from(), r.to(), r.lane, 64, [&](const float(&x)[E], int i) INLINE {
                 int b[E], least_b = BINS;
+                bool here = false;
+                const int from = mass ? bin : 0; // the intervals that are listed
 #pragma unroll
                 for (int e = 0; e < E; e++) {
                     b[e] = x[e] > none ? r.bin_of(x[e]) : BINS;
                     least_b = min(least_b, b[e]);
-                    if (b[e] == bin || (!mass && b[e] < bin)) {
-                        const uint32_t at = atomicAdd(&s.listed, 1u);
-                        if (at < FEW)
-                            s.few[at] = (uint64_t)key_of(x[e]) << 32 | ~(uint32_t)(i + e); // a larger one comes first
-                    }
+                    here |= (b[e] >= from) & (b[e] <= bin);
                 }
+                if (here)
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+                        if ((b[e] >= from) & (b[e] <= bin)) {
+                            const uint32_t at = atomicAdd(&s.listed, 1u);
+                            if (at < FEW)
+                                s.few[at] = (uint64_t)key_of(x[e]) << 32 | ~(uint32_t)(i + e); // a larger one comes first
+                        }
                 if (mass && least_b < bin)
 #pragma unroll
                     for (int e = 0; e < E; e++) {
                         const uint64_t w = r.weight(x[e]);
-                        above += b[e] < bin && w >= r.least ? w : 0;
+                        above += (b[e] < bin) & (w >= r.least) ? w : 0;
                     }
             });
             r.set_regions(above);
@@ -578,6 +590,8 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
         }
         r.cut(mass, need);
     }
+    if (r.key == 0x007fffffu)
+        r.last = -1; // a score of -infinity is never taken
     const uint64_t least = RAW + r.least;
     const float border = score_of(r.key);
 #pragma unroll 1
@@ -585,28 +599,17 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
         const int index = r.locate(
             known,
             [&](const float(&x)[E], int i, uint64_t *each_one) INLINE -> uint64_t {
-                bool in[E], any = false;
-#pragma unroll
-                for (int e = 0; e < E; e++)
-                    any |= in[e] = last == 0 ? x[e] == border : x[e] > border || (x[e] == border && i + e <= r.last);
+                const int upto = last == 0 ? 0x7fffffff : r.last;
                 uint64_t sum = 0;
-                if (any) {
-                    uint64_t w[E];
 #pragma unroll
-                    for (int e = 0; e < E; e++)
-                        w[e] = last == 0 ? RAW + 1 : r.raw_weight(x[e]);
-#pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        w[e] = in[e] && (last == 0 || w[e] >= least) ? w[e] : RAW;
-                        sum += w[e];
-                        if (each_one)
-                            each_one[e] = w[e] - RAW;
-                    }
-                    sum -= RAW * E;
-                } else if (each_one)
-#pragma unroll
-                    for (int e = 0; e < E; e++)
-                        each_one[e] = 0;
+                for (int e = 0; e < E; e++) {
+                    const bool in = ((x[e] > border) & (last != 0)) | ((x[e] == border) & (i + e <= upto));
+                    uint64_t w = last == 0 ? RAW + 1 : r.raw_weight(x[e]);
+                    w = in & (w >= (last == 0 ? RAW : least)) ? w - RAW : 0;
+                    sum += w;
+                    if (each_one)
+                        each_one[e] = w;
+                }
                 return sum;
             },
             [&](uint64_t all) INLINE -> uint64_t { return last == 0 ? r.ties - 1 : goal_of(all); });
