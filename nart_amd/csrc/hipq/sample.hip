@@ -337,10 +337,29 @@ struct Row {
         __syncthreads();
     }
 
-    // The threads' numbers, the first n of them, from the largest to the smallest (those behind are 0): exchanges over distances that
-    // halve, in the wave's registers where both ends are in it: 28 steps of 140 ns at 100 numbers
+    // The threads' numbers, the first n of them and all different, from the largest to the smallest (those behind are 0).  Few are each
+    // compared with all, by 4 to 16 threads; more by exchanges over distances that halve, in the wave's registers where both ends are in
+    // it.  (100 numbers: 1.5 us and 4; a step of the latter takes 140 ns.)
     __device__ __forceinline__ uint64_t sort(uint64_t v, int n)
     {
+        if (n <= 256) {
+            const int shift = n <= 64 ? 4 : n <= 128 ? 3 : 2, own = tid >> shift, part = tid & ((1 << shift) - 1);
+            __syncthreads();
+            s.few[tid] = v;
+            __syncthreads();
+            v = s.few[own];
+            int rank = 0;
+#pragma unroll 4
+            for (int i = part; i < n; i += 1 << shift)
+                rank += s.few[i] > v;
+            for (int o = 1; o < 1 << shift; o *= 2)
+                rank += __shfl_xor(rank, o);
+            __syncthreads();
+            if (own < n && part == 0)
+                s.few[rank] = v;
+            __syncthreads();
+            return tid < n ? s.few[tid] : 0;
+        }
         const bool some = wave * 64 < 2 * n; // waves that can hold some on their way
 #pragma unroll 1
         for (int size = 2; size < 2 * n; size *= 2)
@@ -421,6 +440,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
         for (int e = 0; e < E; e++)
             top = fmaxf(top, x[e]);
     });
+    float own = top; // the largest of this thread's scores
 #pragma unroll
     for (int o = 1; o < 64; o *= 2)
         top = fmaxf(top, __shfl_xor(top, o));
@@ -435,6 +455,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
     __syncthreads();
     r.infinite = top == __builtin_inff();
     r.top = r.infinite ? 0.0f : top;
+    own = !r.infinite ? own : own == top ? 0.0f : none;
     const float t = a.temperature ? a.temperature[blockIdx.x] : 1.0f;
     if (top == none) {
         if (tid == 0)
@@ -486,32 +507,38 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
     };
     constexpr uint64_t RAW = Row<TYPE>::RAW;
 #pragma unroll 1
-    for (int filter = 0; filter < 2; filter++) { // top-k, then top-p among what it keeps
-        const bool mass = filter == 1;
-        if (!(mass ? by_mass : by_count))
+    for (int step = 0; step < 3; step++) { // top-k, then top-p among what it keeps
+        // The first k are not below the k-th largest of the threads' largest scores, and hardly more scores are above that: where k
+        // is small it is looked for among those alone (0), and in all scores (1) only if that was no use.
+        const bool mass = step == 2;
+        if (!(mass ? by_mass : by_count && (step == 1 || k <= FEW / 2)))
             continue;
         r.clear_bins();
         __syncthreads();
         const uint32_t key = r.key, ties = r.ties;
         const float border = score_of(key);
         const bool all_ties = ties == 0xffffffffu && border > none;
-        r.each([&](const float(&x)[E], int) INLINE {
-            bool in[E], any = false;
-#pragma unroll
-            for (int e = 0; e < E; e++)
-                any |= in[e] = (x[e] > border) | ((x[e] == border) & all_ties); // no branches: a loop of them took twice the instructions
-            if (any) {
-                uint64_t w[E];
-                if (mass)
-#pragma unroll
-                    for (int e = 0; e < E; e++)
-                        w[e] = r.weight(x[e]);
+        if (step == 0) {
+            if (own > none)
+                atomicAdd((unsigned long long *)&s.bins[r.bin_of(own)], 1ull);
+        } else
+            r.each([&](const float(&x)[E], int) INLINE {
+                bool in[E], any = false;
 #pragma unroll
                 for (int e = 0; e < E; e++)
-                    if (in[e])
-                        atomicAdd((unsigned long long *)&s.bins[r.bin_of(x[e])], mass ? (unsigned long long)w[e] : 1ull);
-            }
-        });
+                    any |= in[e] = (x[e] > border) | ((x[e] == border) & all_ties); // no branches: a loop of them took twice the instructions
+                if (any) {
+                    uint64_t w[E];
+                    if (mass)
+#pragma unroll
+                        for (int e = 0; e < E; e++)
+                            w[e] = r.weight(x[e]);
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+                        if (in[e])
+                            atomicAdd((unsigned long long *)&s.bins[r.bin_of(x[e])], mass ? (unsigned long long)w[e] : 1ull);
+                }
+            });
         if (tid == 0 && ties != 0xffffffffu)
             atomicAdd((unsigned long long *)&s.bins[r.bin_of(score_of(key))], (unsigned long long)(mass ? r.weight(score_of(key)) * ties : ties));
         __syncthreads();
@@ -532,29 +559,30 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
                 s.listed = 0, s.low = 0xffffffffu, s.index = -1;
             __syncthreads();
             uint64_t above = 0;
+            const float first = mass ? (float)bin : 0.0f, behind = (float)(bin + 1); // the intervals that are listed
             r.each(r.from(), r.to(), r.lane, 64, [&](const float(&x)[E], int i) INLINE {
-                int b[E], least_b = BINS;
-                bool here = false;
-                const int from = mass ? bin : 0; // the intervals that are listed
+                // in place of intervals, what their numbers are the whole part of
+                float v[E];
+                bool here = false, over = false;
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    b[e] = x[e] > none ? r.bin_of(x[e]) : BINS;
-                    least_b = min(least_b, b[e]);
-                    here |= (b[e] >= from) & (b[e] <= bin);
+                    v[e] = (r.top - x[e]) * r.per_bin; // infinite or NaN where a score is never taken
+                    here |= (v[e] >= first) & (v[e] < behind);
+                    over |= v[e] < first;
                 }
                 if (here)
 #pragma unroll
                     for (int e = 0; e < E; e++)
-                        if ((b[e] >= from) & (b[e] <= bin)) {
+                        if ((v[e] >= first) & (v[e] < behind)) {
                             const uint32_t at = atomicAdd(&s.listed, 1u);
                             if (at < FEW)
                                 s.few[at] = (uint64_t)key_of(x[e]) << 32 | ~(uint32_t)(i + e); // a larger one comes first
                         }
-                if (mass && least_b < bin)
+                if (mass && over)
 #pragma unroll
                     for (int e = 0; e < E; e++) {
                         const uint64_t w = r.weight(x[e]);
-                        above += (b[e] < bin) & (w >= r.least) ? w : 0;
+                        above += (v[e] < first) & (w >= r.least) ? w : 0;
                     }
             });
             r.set_regions(above);
@@ -579,7 +607,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
                 const uint64_t most = by_mass ? need_of(r.sum) : ~0ull;
                 w = front < most && w >= r.least ? w : 0;
                 // in the order of their indices
-                const uint64_t at = r.sort(w ? (uint64_t)(MOST_VOCAB - 1 - index) << (FRACTION + 1) | w : 0, min(n, k));
+                const uint64_t at = r.sort(tid < min(n, k) ? (uint64_t)(MOST_VOCAB - 1 - index) << (FRACTION + 1) | w : 0, min(n, k));
                 w = at & ((2ull << FRACTION) - 1);
                 const uint64_t run = r.scan(w);
                 const uint64_t goal = goal_of(r.sum);
@@ -588,7 +616,8 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
                 return;
             }
         }
-        r.cut(mass, need);
+        if (step > 0)
+            r.cut(mass, need);
     }
     if (r.key == 0x007fffffu)
         r.last = -1; // a score of -infinity is never taken
