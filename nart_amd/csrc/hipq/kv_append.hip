@@ -6,7 +6,7 @@
 // as four of its heads: lanes take up to 8 heads of one token in turn and keep them, the norm's weights multiplied in, the next head on
 // its way.  With a division for each 8-bit code and weights read anew for each head its arithmetic took longer than its bytes: 5000 tokens of
 // 40 + 8 + 8 heads of 128, fp16 into int8, 50 us; now 35.5 (133 MB at 3.7 TB/s; 2, 4 or 28 heads a lane: 44.5, 36.7, 40.2).
-// 32 tokens of 32 + 8 + 8 heads: 3.5 us.
+// 32 tokens of 32 + 8 + 8 heads: 3.3 us.
 #include "real16.h"
 
 namespace hipq {
