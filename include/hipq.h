@@ -514,8 +514,8 @@ int hipq_w4_plan_create(const hipq_w4_desc *desc, const uint8_t *q, const void *
 void hipq_w4_plan_destroy(hipq_w4_plan *plan);
 /* Name of the kernel that hipq_w4_run launches for M rows ("" for a number of rows that it refuses).  The string is static. */
 const char *hipq_w4_plan_kernel(const hipq_w4_plan *plan, int M);
-/* x: M rows of K, x_stride elements apart (a multiple of 8 below 2^23, the first row at a multiple of 16 bytes); y: M rows of N, y_stride apart.
- * M may be 0.  The plan belongs to the device that it was created on.  workspace: hipq_w4_workspace bytes at a multiple of 16 (0: none,
+/* x: M rows of K, x_stride elements apart (a multiple of 8 below 2^23, the first row at a multiple of 16 bytes); y: M rows of N, y_stride apart,
+ * not over x.  M may be 0.  The plan belongs to the device that it was created on.  workspace: hipq_w4_workspace bytes at a multiple of 16 (0: none,
  * may be NULL), whose content is of no interest before and after; calls that may run at the same time need one each. */
 size_t hipq_w4_workspace(const hipq_w4_plan *plan, int M);
 int hipq_w4_run(const hipq_w4_plan *plan, const void *x, int64_t x_stride, void *y, int64_t y_stride, int M, void *workspace,
@@ -565,7 +565,7 @@ int hipq_kv_append(const hipq_kv_cache *cache, const hipq_kv_append_desc *desc, 
  * Rows of o that belong to no sequence are left as they are.  Entries of blocks behind a sequence's end are not read; a block outside
  * the cache holds no tokens (they are not seen).  `longest` and `most_new` are the caller's bounds, from which the host divides the work:
  * of a sequence that is longer, or has more new tokens, nothing outside is read or written, and its rows mean nothing.
- * The scale is above 0.  o may be q itself (same strides).  Weights are rounded to 16 bits for the product with the values.  A value that is
+ * A sequence's blocks hold up to 2^30 tokens.  The scale is above 0.  o may be q itself (same strides).  Weights are rounded to 16 bits for the product with the values.  A value that is
  * infinite or NaN reaches the rows that see its token, as NaN or as an infinity.
  * workspace: hipq_kv_attend_workspace bytes at a multiple of 16 (0: none, may be NULL), whose content is of no interest before and after;
  * calls that may run at the same time need one each.

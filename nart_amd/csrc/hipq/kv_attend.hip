@@ -845,7 +845,7 @@ static int check_attend(const hipq_kv_cache *c, const hipq_kv_attend_desc *d)
     HIPQ_REQUIRE(d->q_heads >= 1 && d->q_heads <= 65536 && d->q_heads % c->heads == 0, "attend: %d query heads on %d heads of the cache", d->q_heads, c->heads);
     HIPQ_REQUIRE(d->most_new >= 0 && d->most_new <= (1 << 20), "attend: %d new tokens of a sequence", d->most_new);
     HIPQ_REQUIRE(!d->mask || d->most_new <= 64, "attend: a mask has bits for 64 new tokens of a sequence, not %d", d->most_new);
-    HIPQ_REQUIRE(d->blocks_per_sequence >= 0 && (int64_t)d->blocks_per_sequence * c->page < ((int64_t)1 << 31), "attend: %d blocks of a sequence", d->blocks_per_sequence);
+    HIPQ_REQUIRE(d->blocks_per_sequence >= 0 && (int64_t)d->blocks_per_sequence * c->page <= ((int64_t)1 << 30), "attend: %d blocks of a sequence", d->blocks_per_sequence);
     HIPQ_REQUIRE(d->blocks_stride >= d->blocks_per_sequence || d->sequences <= 1, "attend: rows of blocks overlap");
     HIPQ_REQUIRE(d->longest >= 0, "attend: the longest sequence has %d tokens", d->longest);
     HIPQ_REQUIRE(d->scale > 0 && d->scale < 1e30f, "attend: scale %g", (double)d->scale);

@@ -1,10 +1,12 @@
 // Products with 4-bit weights and group scales (hipq_w4_*): y[m][n] = sum_g s[n][g] sum_{k in g} x[m][k] (q[n][k] - z[n][g]).  gfx950 only.
 //
 // The arithmetic of every kernel here.  A weight's four bits become a 16-bit float without a conversion: with the bits at the right place
-// of a half dword, one v_and_or makes two floats 16 + q (16 = 2^4 has q's unit at mantissa bit 3 of a bfloat16, bit 6 of a float16), exactly;
-// seven instructions make eight of them.  The 16 and the zero point come off behind the product, where x is already summed: with
-// X = sum of x over the group, sum x (q - z) = sum x (16 + q) - (16 + z) X.  Both sums are float32; the terms are at most 31 / 8 as
-// large as with centred weights, so the difference keeps 21 bits.  The group's sum is then scaled and added in float32: the
+// of a half dword, one v_and_or makes two floats 32 + q (32 = 2^5 has q's unit at mantissa bit 2 of a bfloat16, bit 5 of a float16), exactly;
+// seven instructions make eight of them.  The 32 and the zero point come off behind the product, where x is already summed: with
+// X = sum of x over the group, sum x (q - z) = sum x (32 + q) - (32 + z) X.  Where a zero point would then cost more instructions for the sums
+// than for the weights, 16 - z is added to the mantissas as an integer (to 48 + q - z, below 64), and 48 X comes off for all columns alike,
+// as the matrix product's own initial value.  Both sums are float32; the terms are at most 63 / 8 as
+// large as with centred weights, so the difference keeps 20 bits.  The group's sum is then scaled and added in float32: the
 // weights themselves are never rounded.
 //
 // Layout.  k runs in blocks of 128, rows of weights in tiles of 16.  The 1 KB of a tile and block lies together (weights_at), a lane's 16 bytes the
@@ -26,7 +28,7 @@ struct W4Args {
     uint16_t *y;
     int64_t x_stride, y_stride;
     const uint16_t *nothing; // 16 bytes of zeros: in the place of x behind the last k
-    const float *xsum; // tile kernel: [block][group of the block][m_pad], minus the sums of x (times 24 where there are no zero points)
+    const float *xsum; // tile kernel: [block][group of the block][m_pad], sums of x times what the kernel adds them with (W4Tile::FACTOR)
     int M, N, K, blocks, m_pad;
     int activation; // with one, tiles 2 i and 2 i + 1 hold rows 16 i .. 16 i + 15 of the gate and of the other projection
 };
@@ -35,16 +37,16 @@ template <int TYPE>
 struct Nibbles;
 template <>
 struct Nibbles<HIPQ_REAL_BF16> {
-    static constexpr int SHIFT = 3;
-    static constexpr uint32_t MASK = 0x00780078u, BASE = 0x41804180u, MINUS_ONE = 0xbf80bf80u, MINUS_24 = 0xc1c0c1c0u;
+    static constexpr int SHIFT = 2;
+    static constexpr uint32_t MASK = 0x003c003cu, BASE = 0x42004200u, MINUS_ONE = 0xbf80bf80u, MINUS_40 = 0xc220c220u, MINUS_48 = 0xc240c240u;
 };
 template <>
 struct Nibbles<HIPQ_REAL_F16> {
-    static constexpr int SHIFT = 6;
-    static constexpr uint32_t MASK = 0x03c003c0u, BASE = 0x4c004c00u, MINUS_ONE = 0xbc00bc00u, MINUS_24 = 0xce00ce00u;
+    static constexpr int SHIFT = 5;
+    static constexpr uint32_t MASK = 0x01e001e0u, BASE = 0x50005000u, MINUS_ONE = 0xbc00bc00u, MINUS_40 = 0xd100d100u, MINUS_48 = 0xd200d200u;
 };
 
-// eight floats 16 + q.  The two constants sit in registers that the compiler knows nothing about: as literals they would not fit one
+// eight floats 32 + q.  The two constants sit in registers that the compiler knows nothing about: as literals they would not fit one
 // v_and_or, and two instructions would do its work
 template <int TYPE>
 struct Spread {
@@ -74,7 +76,7 @@ __device__ static __forceinline__ float activate(float v, int activation)
 template <int TYPE>
 __device__ static __forceinline__ uint16_t rounded(float v) { return (uint16_t)Real16<TYPE>::pack(v, 0.0f); }
 
-// The scales of a row and block: GPB of them, 16 bits each; with zero points GPB words, the scale below, 16 + z above.
+// The scales of a row and block: GPB of them, 16 bits each; with zero points GPB words, the scale below, 16 - z at SHIFT of the half above.
 template <int TYPE, int GPB, bool ZEROS>
 struct Scales {
     static constexpr int DWORDS = ZEROS ? GPB : (GPB + 1) / 2, BYTES = ZEROS ? 4 * GPB : 2 * GPB;
@@ -92,9 +94,17 @@ struct Scales {
     __device__ __forceinline__ float offset(int g) const
     {
         if constexpr (ZEROS)
-            return Real16<TYPE>::high(w[g]);
+            return 80.0f - Real16<TYPE>::high(w[g] | (Nibbles<TYPE>::BASE & 0xffff0000u));
         else
-            return 24.0f;
+            return 40.0f;
+    }
+    // what makes two floats 48 + q - z of two 32 + q, by an integer addition
+    __device__ __forceinline__ uint32_t less_zero(int g) const
+    {
+        if constexpr (ZEROS)
+            return __builtin_amdgcn_perm(w[g], w[g], 0x03020302u);
+        else
+            return 0;
     }
 };
 // where the weights of a tile and block begin, in KB: eight tiles lie together, so that what a work-group reads at once lies side by side
@@ -264,7 +274,7 @@ __global__ __launch_bounds__(256) void w4_xsum_kernel(const W4Args a, float *xsu
 // What bounds it: up to some dozen rows the weights (17 rows of 14336 x 4096 gated, groups of 64, 18.6 us: 3.5 TB/s in one round of
 // work-groups); above, the vector instructions that unpack weights (7 for 8 of them and 16 MT rows) and scale sums (one for an output and group,
 // two with zero points), which do not overlap the matrix unit's on a SIMD: 2048 rows of 8192 x 8192 in float16, 265 us with the sums of x,
-// 1.03 PFLOP/s, 49 % of the time the matrix unit's and 43 % theirs; 100 rows of 5000 x 5504 in groups of 32, 25 us.
+// 1.03 PFLOP/s, 49 % of the time the matrix unit's and 43 % theirs; 100 rows of 5000 x 5504 in groups of 32, 23 us.
 template <int TYPE, int GPB, bool ZEROS, int MT, int NT, int WM, int WN, int WK, int STAGES, bool XSUM>
 struct W4Tile {
     static constexpr int WAVES = WM * WN, BM = 16 * MT * WM, TILES = NT * WN, PER = 4 / GPB; // WAVES: of a group
@@ -275,7 +285,13 @@ struct W4Tile {
     static constexpr int W_AT = BM * 256, S_AT = W_AT + TILES * 1024, XS_AT = S_AT + S_ALL * 256, BLOCK = XS_AT + XS_ALL * 256;
     static constexpr int STAGE = WK * BLOCK, RED = (WK - 1) * WAVES * MT * NT * 1024, LDS = STAGES * STAGE > RED ? STAGES * STAGE : RED;
     static_assert(BM % (4 * WAVES) == 0 && TILES % WAVES == 0 && S_ALL >= 1 && (STAGES - 1) * LOADS < 64 && LDS <= 160 * 1024, "shape");
-    static_assert(!XSUM || MT * NT >= 16, "only there a stage's sums are read before it is filled again");
+    static_assert(XSUM == (MT * NT >= 16), "only there a stage's sums are read before it is filled again, and only there they are needed");
+    // Zero points in the weights (one instruction more for two) instead of in the sums (one more for each group and output), and sums of x as the
+    // products' initial values: us, 100 rows of 5000 x 5504 in groups of 32, 25.2 against 27.7; 24 of 14336 x 4096 gated, 26.0 against 27.2; 2048 of
+    // 8192 x 8192, 446 against 472, in groups of 64 352 against 376; the initial values alone, without zero points, 128 of 14336 x 4096
+    // gated, 61 against 72
+    static constexpr bool WHOLE = ZEROS && (XSUM ? MT * GPB >= 8 : GPB == 4 && MT >= 2), OFFSETS = ZEROS && !WHOLE, DIRECT = !OFFSETS && GPB == 4;
+    static constexpr float FACTOR = WHOLE ? -48.0f : ZEROS ? -1.0f : -40.0f;
 };
 
 template <int TYPE, int GPB, bool ZEROS, int MT, int NT, int WM, int WN, int WK, int STAGES, bool XSUM>
@@ -348,7 +364,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void w4_tile_kernel(const W4Args
         for (int nt = 0; nt < NT; nt++)
             total[mt][nt] = f32x4{0, 0, 0, 0};
     const Spread<TYPE> spread;
-    const uint32_t one = ZEROS ? Nibbles<TYPE>::MINUS_ONE : Nibbles<TYPE>::MINUS_24;
+    const uint32_t one = T::WHOLE ? Nibbles<TYPE>::MINUS_48 : ZEROS ? Nibbles<TYPE>::MINUS_ONE : Nibbles<TYPE>::MINUS_40;
     const u32x4 ones = {one, one, one, one};
     // With 64 x 64 results a wave there is no room for that: a group's rows are read at once, and multiplied with one tile after the other
     constexpr bool TIGHT = MT * NT >= 16;
@@ -373,17 +389,18 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void w4_tile_kernel(const W4Args
         if (begin)
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
-                less[mt] = XSUM ? *(const f32x4 *)(from + T::XS_AT + (g * T::BM + (wm * MT + mt) * 16 + j * 4) * 4) : f32x4{0, 0, 0, 0};
-        if (!XSUM)
+                less[mt] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-                less[mt] = R::mfma(x[t & 1][mt], ones, less[mt]);
+        for (int mt = 0; mt < MT; mt++)
+            less[mt] = R::mfma(x[t & 1][mt], ones, less[mt]);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const u32x4 f = spread(w[d][nt][t]);
+            u32x4 f = spread(w[d][nt][t]);
+            if (T::WHOLE)
+                f += s[d][nt].less_zero(g);
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
-                sum[mt][nt] = R::mfma(x[t & 1][mt], f, !begin ? sum[mt][nt] : !XSUM ? f32x4{0, 0, 0, 0} : ZEROS ? less[mt] * s[d][nt].offset(g) : less[mt]);
+                sum[mt][nt] = R::mfma(x[t & 1][mt], f, !begin ? sum[mt][nt] : T::DIRECT ? less[mt] : f32x4{0, 0, 0, 0});
         }
         if (end)
 #pragma unroll
@@ -393,7 +410,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void w4_tile_kernel(const W4Args
                 for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const float v = XSUM ? sum[mt][nt][r] : ZEROS ? __builtin_fmaf(less[mt][r], s[d][nt].offset(g), sum[mt][nt][r]) : sum[mt][nt][r] + less[mt][r];
+                        const float v = T::DIRECT ? sum[mt][nt][r] : T::OFFSETS ? __builtin_fmaf(less[mt][r], s[d][nt].offset(g), sum[mt][nt][r]) : sum[mt][nt][r] + less[mt][r];
                         total[mt][nt][r] = __builtin_fmaf(scale, v, total[mt][nt][r]);
                     }
             }
@@ -402,22 +419,18 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void w4_tile_kernel(const W4Args
         f32x4 first[MT];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++)
-            first[mt] = XSUM ? *(const f32x4 *)(from + T::XS_AT + (g * T::BM + (wm * MT + mt) * 16 + j * 4) * 4) : f32x4{0, 0, 0, 0};
-        if (!XSUM)
-#pragma unroll
-            for (int t = 0; t < PER; t++)
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++)
-                    first[mt] = R::mfma(x[t][mt], ones, first[mt]);
+            first[mt] = *(const f32x4 *)(from + T::XS_AT + (g * T::BM + (wm * MT + mt) * 16 + j * 4) * 4);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             f32x4 v[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
-                v[mt] = ZEROS ? first[mt] * s[0][nt].offset(g) : first[mt];
+                v[mt] = T::OFFSETS ? first[mt] * s[0][nt].offset(g) : first[mt];
 #pragma unroll
             for (int t = 0; t < PER; t++) {
-                const u32x4 f = spread(w[0][nt][g * PER + t]);
+                u32x4 f = spread(w[0][nt][g * PER + t]);
+                if (T::WHOLE)
+                    f += s[0][nt].less_zero(g);
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++)
                     v[mt] = R::mfma(x[t][mt], f, v[mt]);
@@ -583,7 +596,7 @@ struct PackArgs {
     uint16_t *to_scales, *to_bias;
     u32x4 *to_nothing;
     int rows, K, group, groups, blocks, tiles, gated; // rows: of one projection
-    int shift, bf16;
+    int shift;
 };
 
 // the row of the caller's arrays that row r of a tile holds, -1: none
@@ -623,8 +636,8 @@ __global__ __launch_bounds__(256) void w4_pack_kernel(const PackArgs p)
                 const uint32_t s = there ? p.scales[row * p.groups + from] : 0;
                 const size_t at = (scales_at(tile, kb, p.blocks) + c) * gpb + g;
                 if (p.zeros) {
-                    const float z = 16.0f + (float)(there ? p.zeros[row * p.groups + from] & 15 : 8);
-                    ((uint32_t *)p.to_scales)[at] = s | (p.bf16 ? Real16<HIPQ_REAL_BF16>::pack(z, 0.0f) : Real16<HIPQ_REAL_F16>::pack(z, 0.0f)) << 16;
+                    const uint32_t z = there ? p.zeros[row * p.groups + from] & 15 : 8;
+                    ((uint32_t *)p.to_scales)[at] = s | (16 - z) << (16 + p.shift);
                 } else
                     p.to_scales[at] = (uint16_t)s;
             }
@@ -676,7 +689,7 @@ extern "C" int hipq_w4_plan_create(const hipq_w4_desc *d, const uint8_t *q, cons
     k.to_q = p->memory, k.to_nothing = (u32x4 *)(p->memory + q_bytes + s_bytes + b_bytes), k.to_scales = (uint16_t *)(p->memory + q_bytes);
     k.to_bias = (uint16_t *)(p->memory + q_bytes + s_bytes);
     k.rows = d->N, k.K = d->K, k.group = d->group, k.groups = (d->K + d->group - 1) / d->group, k.blocks = p->blocks, k.tiles = (int)tiles, k.gated = gated;
-    k.bf16 = d->type == HIPQ_REAL_BF16, k.shift = d->type == HIPQ_REAL_BF16 ? Nibbles<HIPQ_REAL_BF16>::SHIFT : Nibbles<HIPQ_REAL_F16>::SHIFT;
+    k.shift = d->type == HIPQ_REAL_BF16 ? Nibbles<HIPQ_REAL_BF16>::SHIFT : Nibbles<HIPQ_REAL_F16>::SHIFT;
     const size_t groups = (pieces + 3) / 4;
     w4_pack_kernel<<<dim3((unsigned)(groups < 16384 ? groups : 16384)), dim3(256), 0, (hipStream_t)stream>>>(k);
     int bad = launch_status("w4_pack_kernel");
@@ -797,7 +810,7 @@ static int launch(const hipq_w4_plan *p, W4Args &a, float *workspace, hipStream_
         a.m_pad = round_up(a.M, SHAPE[s.kernel].rows);
         a.xsum = workspace;
         const int64_t threads = (int64_t)a.m_pad * a.blocks * 16;
-        w4_xsum_kernel<TYPE, GPB><<<dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st>>>(a, workspace, ZEROS ? -1.0f : -24.0f);
+        w4_xsum_kernel<TYPE, GPB><<<dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st>>>(a, workspace, W4Tile<TYPE, GPB, ZEROS, 4, 4, 2, 4, 1, GPB == 4 && ZEROS ? 2 : 3, true>::FACTOR);
         if (launch_status("w4_xsum_kernel"))
             return 1;
         workspace += (size_t)a.m_pad * a.blocks * GPB;
@@ -859,6 +872,7 @@ extern "C" int hipq_w4_run(const hipq_w4_plan *p, const void *x, int64_t x_strid
     HIPQ_REQUIRE(x && y, "w4: a null pointer");
     HIPQ_REQUIRE((uintptr_t)x % 16 == 0 && x_stride % 8 == 0, "w4: rows of x have to start at multiples of 16 bytes");
     HIPQ_REQUIRE((uintptr_t)y % 2 == 0, "w4: y is not aligned to its type");
+    HIPQ_REQUIRE(x != y, "w4: y lies over x");
     HIPQ_REQUIRE(x_stride < (1 << 23), "w4: rows of x are %lld elements apart", (long long)x_stride);
     HIPQ_REQUIRE(M == 1 || (x_stride >= p->desc.K && y_stride >= p->desc.N), "w4: rows overlap (strides %lld and %lld)", (long long)x_stride, (long long)y_stride);
     const size_t need = hipq_w4_workspace(p, M);

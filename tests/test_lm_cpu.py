@@ -72,14 +72,14 @@ def runs_of_4_bit_weights():
     rc, h = plan(K=2048)
     assert rc == 0
 
-    def call(plan=h, x=P, x_stride=2048, y=P, y_stride=512, M=8, workspace=None, size=0):
+    def call(plan=h, x=P, x_stride=2048, y=4 * P, y_stride=512, M=8, workspace=None, size=0):
         return lib.hipq_w4_run(plan, x, x_stride, y, y_stride, M, workspace, size, None)
     need = lib.hipq_w4_workspace(h, 8)
     assert need == 0
     r = Refusals(call, 1)
     r.takes(0, M=0, x=None, y=None)
     r.takes(1, M=1, x_stride=0, y_stride=0)
-    r.takes(1, x_stride=2056, y_stride=513, y=P + 2)
+    r.takes(1, x_stride=2056, y_stride=513, y=4 * P + 2)
     for M in (-1, (1 << 24) + 1):
         r.refuses("rows", M=M)
         assert lib.hipq_w4_plan_kernel(h, M) == b"" and lib.hipq_w4_workspace(h, M) == 0
@@ -89,7 +89,8 @@ def runs_of_4_bit_weights():
         r.refuses("null pointer", **{name: None})
     for changes in (dict(x=P + 8), dict(x_stride=2052)):
         r.refuses("multiples of 16 bytes", **changes)
-    r.refuses("aligned", y=P + 1)
+    r.refuses("aligned", y=4 * P + 1)
+    r.refuses("over x", y=P)
     for changes in (dict(x_stride=2040), dict(y_stride=511), dict(x_stride=-2048), dict(y_stride=0)):
         r.refuses("overlap", **changes)
     r.refuses("elements apart", x_stride=1 << 23)
@@ -197,7 +198,8 @@ def attention_over_the_cache():
     r.refuses("sequences", sequences=-1)
     r.refuses("new tokens", tokens=-1)
     r.refuses("longest", longest=-1)
-    for n in (-1, 1 << 27):
+    r.takes(1, blocks_per_sequence=1 << 26, blocks_stride=1 << 26)
+    for n in (-1, (1 << 26) + 1, 1 << 27):
         r.refuses("blocks of a sequence", blocks_per_sequence=n)
     r.refuses("overlap", blocks_stride=9)
     for scale in (0.0, -0.1, float("nan"), float("inf")):
@@ -255,7 +257,7 @@ class Tensor:
         return self.device
 
     def data_ptr(self):
-        return P
+        return P * (1 + len(self.dtype)) * (1 + self.shape[-1])
 
 
 def calls_with_tensors():
