@@ -271,7 +271,7 @@ __global__ __launch_bounds__(256) void w4_xsum_kernel(const W4Args a, float *xsu
 // block as well: all waves reading at once and multiplying afterwards left the multiplier idle for a third of the time.
 // gridDim.y work-groups share the blocks of k: then float32 sums go to `part`, and w4_join_kernel adds them.
 // XSUM: the sums of x come from w4_xsum_kernel, otherwise from a multiply by ones.
-// What bounds it: up to some dozen rows the weights (17 rows of 14336 x 4096 gated, groups of 64, 18.6 us: 3.5 TB/s in one round of
+// What bounds it: up to some dozen rows the weights (17 rows of 14336 x 4096 gated, groups of 64, 18.9 us: 3.4 TB/s in one round of
 // work-groups); above, the vector instructions that unpack weights (7 for 8 of them and 16 MT rows) and scale sums (one for an output and group,
 // two with zero points), which do not overlap the matrix unit's on a SIMD: 2048 rows of 8192 x 8192 in float16, 265 us with the sums of x,
 // 1.03 PFLOP/s, 49 % of the time the matrix unit's and 43 % theirs; 100 rows of 5000 x 5504 in groups of 32, 23 us.
