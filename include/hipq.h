@@ -591,8 +591,9 @@ int hipq_kv_attend(const hipq_kv_cache *cache, const hipq_kv_attend_desc *desc, 
  *   and have less than top_p of the weight of those in front of them (the first always; top_p >= 1: all),
  *   and have w_i >= min_p (the first always).
  * The token is the first one, by index, at which the running sum of the kept weights exceeds uniform * their sum (uniform in [0, 1)).
- * A temperature that is not above 0 takes the highest score, the lowest index among equal ones.  Scores of -infinity and NaN are never
- * taken: a row of nothing else gives -1; of +infinities each has the same weight, and nothing else has any.
+ * A top_p or min_p that is NaN filters nothing.  A temperature that is not above 0 takes the highest score, the lowest index among
+ * equal ones.  Scores of -infinity and NaN are never taken: a row of nothing else gives -1; of +infinities each has the same weight,
+ * and nothing else has any.
  * Weights are summed in 64-bit fixed point, so that no order of summation shows in a result; one below 2^-44 of the largest counts as 0.
  * temperature, top_k, top_p, min_p: a value per row, or NULL (1, all, all, all).  logits: rows of `vocab` of `type` (HIPQ_REAL_*), `stride`
  * elements apart, at any address that the type allows; vocab: up to 2^20.
