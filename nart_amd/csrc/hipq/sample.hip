@@ -587,7 +587,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
 #pragma unroll
                     for (int e = 0; e < E; e++) {
                         const uint64_t w = r.weight(x[e]);
-                        above += (v[e] < first) & (w >= r.least) ? w : 0;
+                        above += ((v[e] < first) & (w >= r.least)) ? w : 0;
                     }
             });
             r.set_regions(above);
@@ -642,7 +642,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a)
                 for (int e = 0; e < E; e++) {
                     const bool in = ((x[e] > border) & (last != 0)) | ((x[e] == border) & (i + e <= upto));
                     uint64_t w = last == 0 ? RAW + 1 : raw[e];
-                    w = in & (w >= (last == 0 ? RAW : least)) ? w - RAW : 0;
+                    w = (in & (w >= (last == 0 ? RAW : least))) ? w - RAW : 0;
                     sum += w;
                     if (each_one)
                         each_one[e] = w;
