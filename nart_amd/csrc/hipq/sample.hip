@@ -56,7 +56,8 @@ struct SampleShared {
     uint64_t before;
     uint32_t bin, listed, low, high;
     float top;
-    int index;
+    int index; // of a border
+    int found; // locate's alone: a border's index may still be read when locate begins
 };
 
 template <int TYPE>
@@ -399,7 +400,7 @@ struct Row {
         uint64_t front = w ? of_lane(regions, w - 1) : 0;
         const int begin = w * part, end = min(a.vocab, begin + part);
         if (tid == 0)
-            s.index = -1;
+            s.found = -1;
 #pragma unroll 1
         for (int base = begin; base < end; base += THREADS * E) {
             float x[E];
@@ -418,14 +419,14 @@ struct Row {
                     run += each_one[e];
                     at += run <= goal;
                 }
-                s.index = at;
+                s.found = at;
             }
             __syncthreads();
             front += sum;
-            if ((int)uniform((uint32_t)s.index) >= 0)
+            if ((int)uniform((uint32_t)s.found) >= 0)
                 break;
         }
-        return (int)uniform((uint32_t)s.index);
+        return (int)uniform((uint32_t)s.found);
     }
 };
 

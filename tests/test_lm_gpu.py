@@ -613,6 +613,23 @@ def test_sample_infinities_and_nan(dtype):
     assert got[0] == -1 and got[2] == 2 and got[12] == -1
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_sample_last_token_that_top_p_keeps(dtype):
+    """Rows with top-p alone whose border is a heavy token, which is the answer as often as not: left out by any part of the work-group, it
+    would make another token of the row.  Every call gives the same."""
+    rng = np.random.default_rng(12)
+    r, v = 320, 700
+    x = torch.from_numpy(rng.standard_normal((r, v)) * 0.1 - 9.0)
+    heavy = rng.integers(2, 6, r)
+    for i in range(r):  # the heavy tokens weigh about the same, the others all together 700 e^-9 of one
+        x[i, torch.from_numpy(rng.choice(v, heavy[i], replace=False))] = torch.from_numpy(rng.uniform(-0.2, 0.2, heavy[i]))
+    x, u, p = x.to(dtype).cuda(), rng.random(r).astype(np.float32).tolist(), (rng.uniform(0.2, 0.95, r)).tolist()
+    first = check_sample(x, u, p=p)
+    f = lambda n: torch.tensor(n, dtype=F32, device="cuda")  # noqa: E731
+    for _ in range(20):
+        assert hipq.sample(x, f(u), top_p=f(p)).tolist() == first
+
+
 def test_sample_rows_with_gaps_and_odd_addresses():
     g = gen(4)
     wide = (torch.randn((9, 1003), device="cuda", generator=g) * 2).to(BF16)
