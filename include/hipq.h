@@ -565,8 +565,10 @@ int hipq_kv_append(const hipq_kv_cache *cache, const hipq_kv_append_desc *desc, 
  * Rows of o that belong to no sequence are left as they are.  Entries of blocks behind a sequence's end are not read; a block outside
  * the cache holds no tokens (they are not seen).  `longest` and `most_new` are the caller's bounds, from which the host divides the work:
  * of a sequence that is longer, or has more new tokens, nothing outside is read or written, and its rows mean nothing.
- * A sequence's blocks hold up to 2^30 tokens.  The scale is above 0.  o may be q itself (same strides).  Weights are rounded to 16 bits for the product with the values.  A value that is
- * infinite or NaN reaches the rows that see its token, as NaN or as an infinity.
+ * A sequence's blocks hold up to 2^30 tokens.  The scale is above 0.  o may be q itself (same strides). 
+ * Weights - over codes, weights times their tokens' value scales - are rounded to 16 bits for the product with the values: by at most half a
+ * unit in the last place, in float16 by up to 2^-32 of the row's largest where that is more.
+ * A value or value scale that is infinite or NaN reaches the rows that see its token, as NaN or as an infinity, and no others.
  * workspace: hipq_kv_attend_workspace bytes at a multiple of 16 (0: none, may be NULL), whose content is of no interest before and after;
  * calls that may run at the same time need one each.
  */

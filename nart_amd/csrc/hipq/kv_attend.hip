@@ -1,8 +1,8 @@
 // Attention of new tokens over a paged cache (hipq_kv_attend).  gfx950 only.
 //
 // The cache is read once and every other thing is small: a query head's scores are never written.  With a reference m that is at least the
-// running maximum less 8, each tile of tokens adds p_t = 2^(s_t - m) to the sum l and p_t v_t to the output o, all in float32 (p is
-// rounded to 16 bits for the product, half a unit in the last place each, as the values themselves are); when a score passes m + 8, m moves there and l
+// running maximum less 8, each tile of tokens adds p_t = 2^(s_t - m) to the sum l and p_t v_t to the output o, all in float32 (p, over codes
+// p times the token's value scale, is rounded to 16 bits for the product, half a unit in the last place each; see softmax_step for float16's small ones); when a score passes m + 8, m moves there and l
 // and o are scaled, which keeps the result and leaves most tiles without any exchange between lanes.
 //
 // What carries it:
@@ -185,13 +185,25 @@ __device__ static __forceinline__ void not_finite(u32x4 &v, const uint32_t (&see
     }
 }
 
+// Float16 has few small numbers: below 2^-14 they lose bits, below 2^-25 they are 0, while weights are at most 2^8 and half of its range lies above.
+// Over 16 bits they are therefore 2^7 times as large, in their sum as in the outputs, so that a weight is off by at most half a unit in its last
+// place or 2^-32 of the row's largest.  Over codes what is rounded is a weight times its token's value scale, whose size has nothing to
+// do with the weight's: it has a reference of its own, `unit`, a power of two that it passes by 2^8 at most, and is
+// multiplied by 2^7 / unit; outputs are in units of unit / 2^7.  unit is a row's, from what the row sees, and moves with m as the outputs would.
+// (With one unit for a wave, its largest value scale, rows of 8192 tokens with some dominant ones were off by up to 94 times what roundings leave.  us, now against
+// then, of float16 over codes: one token of 8 sequences of up to 2000 15.4 and 16.3, 16 trees of 32 tokens on up to 8000 117 and 117.)
+template <int TYPE, bool QUANT>
+constexpr bool UNITS = QUANT && TYPE == HIPQ_REAL_F16;
+constexpr float RAISED = 128.0f, LEAST_UNIT = 0x1p-100f; // what lies below that is 0 in float16, however many tokens there are
+
 // A row's weights p of 8 tokens a lane from its scores s: the reference m moves where a score passes it by more than 8, and with it the sums (l
 // of codes, lsum of 16-bit values) and outputs are scaled.
 template <int TYPE, bool QUANT, bool MASKED, int VD>
 __device__ static __forceinline__ void softmax_step(float scale2, const f32x4 (&s)[2], const f32x4 (&kscale)[2], const f32x4 (&vsc)[2], uint32_t sees, float &m, float &l,
-                                                    f32x4 &lsum, f32x4 (&o)[VD], u32x4 &p)
+                                                    f32x4 &lsum, float &unit, float &per_unit, f32x4 (&o)[VD], u32x4 &p)
 {
     using R = Real16<TYPE>;
+    constexpr bool units = UNITS<TYPE, QUANT>;
     float x[8], top = NONE;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -206,16 +218,22 @@ __device__ static __forceinline__ void softmax_step(float scale2, const f32x4 (&
         top = fmaxf(top, m);
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
+        if (units)
+            top = ceilf(top); // units stay powers of two, and scaling exact
         const float f = top == NONE ? 1.0f : exp2_fast(m - top);
         m = top;
         l *= f;
         lsum *= f;
+        if (units) {
+            unit *= f;
+            per_unit = unit >= LEAST_UNIT ? RAISED / unit : 0.0f;
+        } else
 #pragma unroll
-        for (int i = 0; i < VD; i++)
-            o[i] *= f;
+            for (int i = 0; i < VD; i++)
+                o[i] *= f;
     }
-    const float ref = m == NONE ? 0.0f : m;
-    float y[8];
+    const float ref = (m == NONE ? 0.0f : m) - (!QUANT && TYPE == HIPQ_REAL_F16 ? 7.0f : 0.0f);
+    float y[8], most = 0;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         y[e] = exp2_fast(QUANT ? x[e] - ref : __builtin_fmaf(x[e], scale2, -ref));
@@ -224,7 +242,25 @@ __device__ static __forceinline__ void softmax_step(float scale2, const f32x4 (&
             y[e] *= vsc[e / 4][e % 4];
             if (MASKED)
                 y[e] = (sees >> e) & 1 ? y[e] : 0.0f;
+            if (units)
+                most = fmaxf(most, fabsf(y[e]));
         }
+    }
+    if (units) {
+        if (__any(most > unit * 256.0f)) {
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            most = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, most) & 0x7f800000u); // the power of two below
+            most = fmaxf(fminf(fmaxf(most, LEAST_UNIT), 0x1p126f), unit);
+            const float f = unit / most; // 0 at the first, where nothing is there to be scaled
+            unit = most, per_unit = RAISED / most;
+#pragma unroll
+            for (int i = 0; i < VD; i++)
+                o[i] *= f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            y[e] *= per_unit;
     }
 #pragma unroll
     for (int e = 0; e < 4; e++)
@@ -288,11 +324,12 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
 
     float m[RT], l[RT];
     f32x4 lsum[RT]; // 16 bits: the sums of p, by a multiply by ones
-    float unit = 0, per_unit = 0; // float16 codes: p is multiplied by value scale / unit, unit the largest scale so far or more, to stay in range
+    float unit[RT], per_unit[RT];
     f32x4 o[RT][VD];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         m[rt] = NONE, l[rt] = 0;
+        unit[rt] = per_unit[rt] = 0;
         lsum[rt] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < VD; i++)
@@ -375,26 +412,6 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
                 }
             }
         }
-        if (QUANT && TYPE == HIPQ_REAL_F16) {
-            float top = 0;
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                top = fmaxf(top, vsc[e / 4][e % 4]);
-            if (__any(top > unit)) {
-#pragma unroll
-                for (int s = 1; s < 64; s *= 2)
-                    top = fmaxf(top, __shfl_xor(top, s));
-                top = fminf(fmaxf(top, 1e-30f), 3e38f);
-                const float f = unit / top; // 0 at the first, where nothing is there to be scaled
-                unit = top, per_unit = 1.0f / top;
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                    for (int i = 0; i < VD; i++)
-                        o[rt][i] *= f;
-            }
-            vsc[0] *= per_unit, vsc[1] *= per_unit;
-        }
         u32x4 p[RT];
         uint32_t sees[RT]; // a bit for each of the lane's 8 tokens: seen by the row
 #pragma unroll
@@ -407,7 +424,7 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
                     s[half] = R::mfma(k[half][ks], Q_LDS ? lq[(rt * KS + ks) * 64 + lane] : q[Q_LDS ? 0 : rt][Q_LDS ? 0 : ks], s[half]);
             if (masked)
                 sees[rt] = seen_by(a, seq, own[rt], t, j, now);
-            softmax_step<TYPE, QUANT, masked, VD>(a.scale2, s, kscale, vsc, masked ? sees[rt] : 0, m[rt], l[rt], lsum[rt], o[rt], p[rt]);
+            softmax_step<TYPE, QUANT, masked, VD>(a.scale2, s, kscale, vsc, masked ? sees[rt] : 0, m[rt], l[rt], lsum[rt], unit[rt], per_unit[rt], o[rt], p[rt]);
         }
         __builtin_amdgcn_sched_barrier(0);
         // output
@@ -459,10 +476,10 @@ __global__ __launch_bounds__(256, DIM == 256 || (QUANT && TYPE == HIPQ_REAL_F16 
         if (QUANT) {
             l[rt] += __shfl_xor(l[rt], 16);
             l[rt] += __shfl_xor(l[rt], 32);
-            if (TYPE == HIPQ_REAL_F16)
+            if (UNITS<TYPE, QUANT>)
 #pragma unroll
                 for (int i = 0; i < VD; i++)
-                    o[rt][i] *= unit;
+                    o[rt][i] *= unit[rt] * (1 / RAISED);
         } else
             l[rt] = lsum[rt][0];
         if (j == 0)
@@ -571,11 +588,12 @@ __global__ __launch_bounds__(256, 2) void kv_attend_wide_kernel(const AttendArgs
         for (int ks = 0; ks < KS; ks++)
             q[rt][ks] = *(const u32x4 *)(x + ks * 32 + j * 8);
     }
-    float m[RT], l[RT], unit = 0, per_unit = 0;
+    float m[RT], l[RT], unit[RT], per_unit[RT];
     f32x4 lsum[RT], o[RT][VD];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         m[rt] = NONE, l[rt] = 0;
+        unit[rt] = per_unit[rt] = 0;
         lsum[rt] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < VD; i++)
@@ -665,26 +683,6 @@ __global__ __launch_bounds__(256, 2) void kv_attend_wide_kernel(const AttendArgs
 #pragma unroll
             for (int s = 0; s < 2; s++)
                 kscale[s] = lsc[from][s * 4 + j], vsc[s] = lsc[from][8 + s * 4 + j];
-        if (QUANT && TYPE == HIPQ_REAL_F16) {
-            float top = 0;
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                top = fmaxf(top, vsc[e / 4][e % 4]);
-            if (__any(top > unit)) {
-#pragma unroll
-                for (int s = 1; s < 64; s *= 2)
-                    top = fmaxf(top, __shfl_xor(top, s));
-                top = fminf(fmaxf(top, 1e-30f), 3e38f);
-                const float f = unit / top;
-                unit = top, per_unit = 1.0f / top;
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                    for (int i = 0; i < VD; i++)
-                        o[rt][i] *= f;
-            }
-            vsc[0] *= per_unit, vsc[1] *= per_unit;
-        }
         f32x4 s[RT][2];
 #pragma unroll
         for (int half = 0; half < 2; half++)
@@ -701,7 +699,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_wide_kernel(const AttendArgs
         for (int rt = 0; rt < RT; rt++) {
             if (masked)
                 sees[rt] = seen_by(a, seq, own[rt], t, j, now);
-            softmax_step<TYPE, QUANT, masked, VD>(a.scale2, s[rt], kscale, vsc, masked ? sees[rt] : 0, m[rt], l[rt], lsum[rt], o[rt], p[rt]);
+            softmax_step<TYPE, QUANT, masked, VD>(a.scale2, s[rt], kscale, vsc, masked ? sees[rt] : 0, m[rt], l[rt], lsum[rt], unit[rt], per_unit[rt], o[rt], p[rt]);
         }
 #pragma unroll
         for (int i = 0; i < VD; i++) {
@@ -758,7 +756,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_wide_kernel(const AttendArgs
         const int row = r0 + 16 * rt + c;
         if (row >= rows)
             continue;
-        const float f = (QUANT && TYPE == HIPQ_REAL_F16 ? unit : 1.0f) * (a.splits > 1 ? 1.0f : l[rt] > 0 ? 1.0f / l[rt] : l[rt] == 0 ? 0.0f : l[rt]);
+        const float f = (UNITS<TYPE, QUANT> ? unit[rt] * (1 / RAISED) : 1.0f) * (a.splits > 1 ? 1.0f : l[rt] > 0 ? 1.0f / l[rt] : l[rt] == 0 ? 0.0f : l[rt]);
         const int64_t at = (((int64_t)b * a.cache.heads + h) * a.splits + split) * a.rows + row;
         if (a.splits > 1 && j == 0)
             a.part_ml[2 * at] = m[rt], a.part_ml[2 * at + 1] = l[rt];

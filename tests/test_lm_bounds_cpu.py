@@ -1,0 +1,65 @@
+"""The spreads of lm_bounds.py, on the CPU: results that are computed as the kernels say they compute them keep to them, results with a mistake
+that the worst case of a sum would hide do not."""
+import numpy as np
+import pytest
+import torch
+
+import lm_bounds
+
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def normals(rng, dtype, *shape):
+    return torch.from_numpy(rng.standard_normal(shape)).to(dtype)
+
+
+def tiles(q, k, v, ks, vs, scale, how):
+    """One row over the cache with weights in 16 bits."""
+    dtype, n = q.dtype, k.shape[0]
+    s = ((k.double() @ q.double()) * (1 if ks is None else ks.double()) * scale * 1.4426950408889634).float()
+    p = torch.exp2(s - s.max().ceil())
+    w = p if vs is None else p * vs
+    shift = 1.0
+    if dtype == F16:
+        shift = 2.0 ** 7 if vs is None else 2.0 ** 7 / 2.0 ** float(torch.log2(w.max()).floor())
+        if how == "weights by the largest scale":
+            shift = 1 / float(vs.max())
+        if how == "weights of 1 and less":
+            shift = 1.0
+    w = (w * shift).to(dtype).float() / shift
+    total = (w if vs is None else p).clone()
+    if how in ("a tile lost", "the first tile lost", "the last tokens lost"):
+        at = {"a tile lost": n // 64 * 32, "the first tile lost": 0, "the last tokens lost": n - 32}[how]
+        w[at:at + 32], total[at:at + 32] = 0, 0
+    o = (w.double() @ v.double()) / total.double().sum()
+    return (o * (1.01 if how == "scaled" else 1)).to(dtype)
+
+
+# one score far above the rest, one value scale many times the others'
+@pytest.mark.parametrize("n, gap, ratio", [(8192, 9, 4096), (131072, 12, 256), (131072, 15, 16)])
+def test_attention_float16_codes_of_many_sizes(n, gap, ratio):
+    rng, dim = np.random.default_rng(n), 64
+    q = torch.ones((1, 1, dim), dtype=F16)
+    k = torch.full((n, dim), 1, dtype=torch.int8)
+    ks = torch.from_numpy((rng.standard_normal(n) * 0.5).astype(np.float32))
+    ks[n // 3] = gap
+    v = torch.from_numpy(rng.integers(1, 128, (n, dim)).astype(np.int8))
+    vs = torch.from_numpy(rng.random(n).astype(np.float32) * 0.01 + 0.01)
+    vs[n // 2] *= ratio
+    args = (q, [k[None]], [v[None]], [0, 1], [n], None, 1 / dim, 1, [ks[None]], [vs[None]])
+    want, off = lm_bounds.attend_spread(*args)
+    lm_bounds.check_attend_spread(tiles(q[0, 0], k, v, ks, vs, 1 / dim, "")[None, None], want, off)
+    with pytest.raises(AssertionError, match="roundings leave"):
+        lm_bounds.check_attend_spread(tiles(q[0, 0], k, v, ks, vs, 1 / dim, "weights by the largest scale")[None, None], want, off)
+
+
+def test_attention_float16_long_tail():
+    """The same over 16 bits: many tokens of small weights that have a mean of their own."""
+    rng, dim, n = np.random.default_rng(3), 64, 131072
+    q, k, v = torch.ones((1, 1, dim), dtype=F16), torch.zeros((n, dim), dtype=F16), normals(rng, F16, n, dim) + 1
+    k[n // 3], v[n // 3] = 17.4, -1
+    args = (q, [k[None]], [v[None]], [0, 1], [n], None, 1 / dim, 1)
+    want, off = lm_bounds.attend_spread(*args)
+    lm_bounds.check_attend_spread(tiles(q[0, 0], k, v, None, None, 1 / dim, "")[None, None], want, off)
+    with pytest.raises(AssertionError, match="roundings leave"):
+        lm_bounds.check_attend_spread(tiles(q[0, 0], k, v, None, None, 1 / dim, "weights of 1 and less")[None, None], want, off)

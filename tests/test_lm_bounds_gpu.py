@@ -1,0 +1,140 @@
+"""The operators of language models on the GPU against lm_bounds.py: what roundings leave, and no more."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import lm_bounds
+from nart_amd import hipq
+from test_lm_gpu import fill_cache, gen, randn, tokens_of, trees
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def index(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def starts_of(counts):
+    return np.concatenate(([0], np.cumsum(counts))).tolist()
+
+
+# ---- attention over the cache ---------------------------------------------------------------------------------------------
+def check(cache, blocks, q, counts, lens, mask=None, scale=None):
+    heads, dim = cache.k.shape[1], cache.k.shape[-1]
+    starts = starts_of(counts)
+    got = cache.attend(q, index(starts), index(lens), blocks, max(counts), mask=mask, scale=scale)
+    k, v = ([tokens_of(p, blocks[b], n) for b, n in enumerate(lens)] for p in (cache.k, cache.v))
+    ks, vs = ([tokens_of(p[..., None], blocks[b], n)[..., 0] for b, n in enumerate(lens)] if p is not None else None for p in (cache.k_scale, cache.v_scale))
+    lm_bounds.check_attend_spread(got, *lm_bounds.attend_spread(q, k, v, starts, lens, mask, dim ** -0.5 if scale is None else scale, q.shape[1] // heads, ks, vs))
+    return got
+
+
+def cache_with_scores(g, dtype, heads, dim, scores, int8, page=64):
+    """One sequence whose token t has score scores[t] for queries of ones and a scale of 1 / dim; values are positive."""
+    n = len(scores)
+    cache, blocks = fill_cache(g, dtype, 1, heads, page, dim, n, int8, spare=0)
+    at = torch.arange(n, device="cuda")
+    pages, places = blocks[0].long()[at // page], at % page
+    if int8:
+        cache.k.fill_(1)
+        cache.k_scale[pages, :, places] = scores.float()[:, None].cuda()
+        cache.v.copy_(torch.randint(1, 128, cache.v.shape, dtype=torch.int8, device="cuda", generator=g))
+    else:
+        cache.k[pages, :, places] = scores.to(dtype)[:, None, None].cuda()
+        cache.v.copy_((torch.randn(cache.v.shape, device="cuda", generator=g) + 1).to(dtype))
+    return cache, blocks, pages, places
+
+
+# rows: single tokens, a chain, many rows (each kernel), whose queries are ones
+ROWS = [(1, 1, 4, 64), (1, 1, 4, 128), (9, 1, 4, 256), (40, 8, 32, 128)]
+FRONT = [3, 35, 67, 99]  # a token for each wave of a work-group that takes tiles of 32 in turn
+
+
+def check_alike(cache, blocks, rows, hq, dim, n, dtype):
+    """Queries of ones: one sequence alone, divided among as many work-groups as there can be, and as many sequences over the same pages as make
+    every work-group go over all of one."""
+    heads = cache.k.shape[1]
+    for sequences in (1, 512 // heads):
+        q = torch.ones((sequences * rows, hq, dim), dtype=dtype, device="cuda")
+        got = cache.attend(q, index(list(range(0, sequences * rows + 1, rows))), index([n] * sequences), blocks.expand(sequences, -1).contiguous(), rows, scale=1 / dim)
+        assert (got.view(sequences, rows, hq, dim) == got[:rows]).all()
+        k, v, ks, vs = (None if p is None else [tokens_of(p, blocks[0], n)] for p in (cache.k, cache.v, *(None if t is None else t[..., None] for t in (cache.k_scale, cache.v_scale))))
+        ks, vs = (None if t is None else [t[0][..., 0]] for t in (ks, vs))
+        lm_bounds.check_attend_spread(got[:rows], *lm_bounds.attend_spread(q[:rows], k, v, [0, rows], [n], None, 1 / dim, hq // heads, ks, vs), rows=1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows, heads, hq, dim", ROWS)
+@pytest.mark.parametrize("n, gap, ratio", [(8192, 9, 4096), (32768, 12, 256), (32768, 11, 16), (8192, 9, 1e-4)])
+def test_attend_codes_of_many_sizes(n, gap, ratio, rows, heads, hq, dim, dtype):
+    """An int8 cache with some scores far above the others and some value scales many times the others' (or 10^-4 of them)."""
+    g = gen(n + dim)
+    scores = torch.from_numpy(np.random.default_rng(n).standard_normal(n) * 0.5)
+    scores[FRONT] = gap
+    cache, blocks, pages, places = cache_with_scores(g, dtype, heads, dim, scores, True)
+    for shift in (2, n // 2):
+        at = torch.tensor(FRONT) + shift
+        before = cache.v_scale[pages[at], :, places[at]].clone()
+        cache.v_scale[pages[at], :, places[at]] *= ratio
+        check_alike(cache, blocks, rows, hq, dim, n, dtype)
+        cache.v_scale[pages[at], :, places[at]] = before
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("rows, heads, hq, dim", ROWS)
+@pytest.mark.parametrize("gap", [15, 17])
+def test_attend_long_tail(gap, rows, heads, hq, dim, int8, dtype):
+    """Many tokens behind some whose scores are 15 or 17 above theirs: together they are some hundredths or thousandths of the result."""
+    g, n = gen(gap), 131072 if heads == 1 else 32768
+    scores = torch.zeros(n)
+    scores[FRONT] = gap
+    cache, blocks, pages, places = cache_with_scores(g, dtype, heads, dim, scores, int8)
+    cache.v[pages[FRONT], :, places[FRONT]] = -1
+    check_alike(cache, blocks, rows, hq, dim, n, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows, heads, hq, dim", [(1, 1, 4, 64), (5, 2, 6, 128), (40, 8, 32, 128), (12, 1, 2, 256)])
+def test_attend_value_scales_over_four_decades(rows, heads, hq, dim, dtype):
+    """Scales from 10^-3 to 10 of single tokens, and of tokens that follow each other by size, up and down, beside scores that fall and rise."""
+    g = gen(rows + dim)
+    n = 3000
+    cache, blocks = fill_cache(g, dtype, 1, heads, 64, dim, n, True, spare=0)
+    at = torch.arange(n, device="cuda")
+    pages, places = blocks[0].long()[at // 64], at % 64
+    q = randn(g, dtype, rows, hq, dim)
+    by_size = 10.0 ** (at.double() / n * 4 - 3)
+    for scales in (10.0 ** (torch.rand(n, device="cuda", generator=g).double() * 4 - 3), by_size, by_size.flip(0)):
+        cache.v_scale[pages, :, places] = scales.float()[:, None]
+        check(cache, blocks, q, [rows], [n])
+    cache.k.fill_(1)
+    for scores in (at.double() / n * 9, 9 - at.double() / n * 9):  # the scores undo the scales, and the other way round
+        cache.k_scale[pages, :, places] = scores.float()[:, None]
+        check_alike(cache, blocks, rows, hq, dim, n, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows, heads, hq, n", [(3, 1, 4, 1000), (40, 8, 32, 9000), (17, 2, 2, 100)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_attend_scales_of_tokens_that_are_not_seen(rows, heads, hq, n, tree, dtype):
+    """A drafted token's value scale of 2^12 to 2^100 times the others', or infinite: rows that do not see it get what they got."""
+    g = gen(rows)
+    cache, blocks = fill_cache(g, dtype, 1, heads, 64, 128, n, True, spare=0)
+    q = randn(g, dtype, rows, hq, 128)
+    words = [1 | 1 << i for i in range(rows)] if tree else None  # the first token, and branches of one
+    mask = torch.tensor(words, dtype=torch.int64, device="cuda") if tree else None
+    call = lambda: cache.attend(q, index([0, rows]), index([n]), blocks, rows, mask=mask)  # noqa: E731
+    want = call()
+    new = rows - 1 if not tree else 1
+    at = n - rows + new
+    page, place = blocks[0, at // 64].long(), at % 64
+    others = [r for r in range(rows) if r != new]
+    for factor in (2.0 ** 12, 2.0 ** 40, 2.0 ** 100, math.inf, math.nan):
+        before = cache.v_scale[page, :, place].clone()
+        cache.v_scale[page, :, place] *= factor
+        assert torch.equal(call()[others], want[others]), factor
+        cache.v_scale[page, :, place] = before
