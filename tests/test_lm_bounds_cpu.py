@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import lm_bounds
+import lm_reference as ref
 
 BF16, F16 = torch.bfloat16, torch.float16
 
@@ -13,6 +14,7 @@ def normals(rng, dtype, *shape):
     return torch.from_numpy(rng.standard_normal(shape)).to(dtype)
 
 
+# ---- attention ---------------------------------------------------------------------------------------------------------
 def tiles(q, k, v, ks, vs, scale, how):
     """One row over the cache with weights in 16 bits."""
     dtype, n = q.dtype, k.shape[0]
@@ -33,6 +35,29 @@ def tiles(q, k, v, ks, vs, scale, how):
         w[at:at + 32], total[at:at + 32] = 0, 0
     o = (w.double() @ v.double()) / total.double().sum()
     return (o * (1.01 if how == "scaled" else 1)).to(dtype)
+
+
+MISTAKES = ["a tile lost", "the first tile lost", "the last tokens lost", "scaled"]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("n", [700, 4096, 20000])
+def test_attention(n, int8, dtype):
+    rng, dim, rows = np.random.default_rng(n), 128, 4
+    q = normals(rng, dtype, rows, 1, dim)
+    k, v = (torch.from_numpy(rng.integers(-127, 128, (n, dim)).astype(np.int8)) if int8 else normals(rng, dtype, n, dim) for _ in range(2))
+    ks, vs = (torch.from_numpy(rng.random(n).astype(np.float32) * 0.02 + 0.001) if int8 else None for _ in range(2))
+    one = lambda t: None if t is None else t[None]  # noqa: E731
+    many = lambda t: None if t is None else [one(t)] * rows  # noqa: E731
+    want, off = lm_bounds.attend_spread(q, many(k), many(v), list(range(rows + 1)), [n] * rows, None, dim ** -0.5, 1, many(ks), many(vs))
+    worst = ref.attend(q, many(k), many(v), list(range(rows + 1)), [n] * rows, None, dim ** -0.5, 1, many(ks), many(vs))[0]
+    assert torch.allclose(want, worst, rtol=1e-12, atol=1e-14)
+    run = lambda how: torch.stack([tiles(q[r, 0], k, v, ks, vs, dim ** -0.5, how) for r in range(rows)])[:, None]  # noqa: E731
+    lm_bounds.check_attend_spread(run(""), want, off)
+    for how in MISTAKES:
+        with pytest.raises(AssertionError, match="roundings leave"):
+            lm_bounds.check_attend_spread(run(how), want, off)
 
 
 # one score far above the rest, one value scale many times the others'

@@ -6,11 +6,10 @@ import pytest
 import torch
 
 import lm_bounds
-from nart_amd import hipq
 from test_lm_gpu import fill_cache, gen, randn, tokens_of, trees
 
 pytestmark = pytest.mark.gpu
-BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+BF16, F16 = torch.bfloat16, torch.float16
 
 
 def index(v):
@@ -30,6 +29,54 @@ def check(cache, blocks, q, counts, lens, mask=None, scale=None):
     ks, vs = ([tokens_of(p[..., None], blocks[b], n)[..., 0] for b, n in enumerate(lens)] if p is not None else None for p in (cache.k_scale, cache.v_scale))
     lm_bounds.check_attend_spread(got, *lm_bounds.attend_spread(q, k, v, starts, lens, mask, dim ** -0.5 if scale is None else scale, q.shape[1] // heads, ks, vs))
     return got
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("dim, hq, hkv, counts, lens, tree", [
+    (64, 6, 2, [1] * 5, [2000, 700, 33, 129, 1024], False), (128, 8, 2, [1] * 3, [9000, 257, 5000], False), (256, 4, 1, [1] * 3, [600, 4000, 31], False),
+    (64, 4, 1, [40, 3, 1], [300, 1000, 77], False), (128, 16, 4, [16, 9, 30], [2500, 40, 1111], True), (256, 6, 2, [5, 20], [800, 300], True),
+    (128, 32, 8, [34, 20, 64, 5], [1000, 1900, 600, 1024], True), (128, 16, 8, [300, 129], [300, 4000], False)])
+def test_attend_spread(dim, hq, hkv, counts, lens, tree, int8, dtype):
+    """All kernels: single tokens, chains, trees, prompts, many rows; scores that are close together and, with a larger scale, far apart."""
+    g, rng = gen(sum(lens)), np.random.default_rng(sum(lens))
+    cache, blocks = fill_cache(g, dtype, len(lens), hkv, 48, dim, max(lens), int8)
+    q, mask = randn(g, dtype, sum(counts), hq, dim), trees(rng, counts) if tree else None
+    for scale in (None, 2.0):
+        check(cache, blocks, q, counts, lens, mask, scale)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("int8", [False, True])
+def test_attend_spread_long(int8, dtype):
+    """Many parts and their joins: a lost tile of 32 tokens would be 4 % of the result, ten times what is allowed."""
+    g = gen(80)
+    lens = [20000, 19999, 131072]
+    cache, blocks = fill_cache(g, dtype, 3, 1, 64, 128, max(lens), int8)
+    for counts in ([1, 1, 1], [1, 2, 9]):
+        check(cache, blocks, randn(g, dtype, sum(counts), 4, 128), counts, lens)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("n, rows, heads", [(20000, 1, 1), (3001, 1, 1), (4500, 40, 8)])
+def test_attend_every_token_is_found(n, rows, heads, int8):
+    """One token's score is far above the others', at places over the whole sequence: its value is the result."""
+    g = gen(n)
+    cache, blocks = fill_cache(g, F16, 1, heads, 64, 128, n, int8, spare=0)
+    q = torch.full((rows, 4 * heads, 128), 1.0, dtype=F16, device="cuda")
+    cache.k.fill_(0)
+    if int8:
+        cache.k_scale.fill_(0.25)
+    old = n - rows
+    where = sorted({t for t in list(range(0, old, max(1, old // 70))) + [31, 32, 127, 128, 255, 256, old // 2 // 128 * 128, old - 33, old - 32, old - 1] if 0 <= t < old})
+    for t in where:
+        page, at = blocks[0, t // 64].long(), t % 64
+        cache.k[page, :, at] = 100
+        got = cache.attend(q, index([0, rows]), index([n]), blocks, rows)
+        v = cache.v[page, :, at].double() * (cache.v_scale[page, :, at, None].double() if int8 else 1)
+        want = v.repeat_interleave(4, 0)[None].expand(rows, -1, -1)
+        assert ((got.double() - want).abs() <= 2.0 ** -10 * want.abs() + 2.0 ** -24).all(), t  # two roundings: the weight's, the result's
+        cache.k[page, :, at] = 0
 
 
 def cache_with_scores(g, dtype, heads, dim, scores, int8, page=64):
