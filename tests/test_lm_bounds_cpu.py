@@ -14,6 +14,35 @@ def normals(rng, dtype, *shape):
     return torch.from_numpy(rng.standard_normal(shape)).to(dtype)
 
 
+# ---- products ----------------------------------------------------------------------------------------------------------
+def product(x, q, scales, group, zeros, how):
+    x, y = x.float(), 0
+    for g, at in enumerate(range(0, q.shape[1], group)):
+        w, s = q[:, at:at + group].float() - zeros[:, g:g + 1].float(), scales[:, g].float()
+        if how == "rounded weights":
+            y = y + x[:, at:at + group] @ (w * s[:, None]).to(scales.dtype).float().t()
+        else:
+            y = y + (x[:, at:at + group] @ w.t()) * s
+        if how == "16-bit sums":
+            y = y.to(scales.dtype).float()
+        if how == "sums of x with a wrong zero" and g == 1:
+            y = y + x[:, at:at + group].sum(1, keepdim=True) * s * 2.0 ** -4
+    return y.to(scales.dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("k, group", [(1056, 128), (4128, 128), (2112, 64), (1024, 32)])
+def test_products(k, group, dtype):
+    rng = np.random.default_rng(k)
+    groups = -(-k // group)
+    x, q = normals(rng, dtype, 16, k), torch.from_numpy(rng.integers(0, 16, (96, k)).astype(np.uint8))
+    scales, zeros = torch.from_numpy(rng.random((96, groups)) * 0.02 + 0.002).to(dtype), torch.from_numpy(rng.integers(0, 16, (96, groups)).astype(np.uint8))
+    lm_bounds.check_linear_spread(product(x, q, scales, group, zeros, ""), x, q, scales, group, zeros)
+    for how in ("rounded weights", "16-bit sums", "sums of x with a wrong zero"):
+        with pytest.raises(AssertionError, match="away"):
+            lm_bounds.check_linear_spread(product(x, q, scales, group, zeros, how), x, q, scales, group, zeros)
+
+
 # ---- attention ---------------------------------------------------------------------------------------------------------
 def tiles(q, k, v, ks, vs, scale, how):
     """One row over the cache with weights in 16 bits."""

@@ -6,7 +6,9 @@ import pytest
 import torch
 
 import lm_bounds
-from test_lm_gpu import fill_cache, gen, randn, tokens_of, trees
+from nart_amd import hipq
+from lm_reference import pack_rows
+from test_lm_gpu import fill_cache, gen, randn, tokens_of, trees, weights
 
 pytestmark = pytest.mark.gpu
 BF16, F16 = torch.bfloat16, torch.float16
@@ -18,6 +20,34 @@ def index(v):
 
 def starts_of(counts):
     return np.concatenate(([0], np.cumsum(counts))).tolist()
+
+
+# ---- products with 4-bit weights ----------------------------------------------------------------------------------------
+KERNELS = [(16, 200, 1056, "w4_stream_16"), (3, 20500, 1056, "w4_tile_16x128"), (24, 9000, 2080, "w4_tile_32x128"), (33, 300, 2112, "w4_tile_32x128"), (60, 16400, 160, "w4_tile_64x128"),
+           (100, 400, 4128, "w4_tile_64x128"), (90, 16400, 160, "w4_tile_128x128"), (200, 300, 2112, "w4_tile_128x128"), (140, 8200, 1056, "w4_tile_128x256")]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("group, zeros", [(128, False), (128, True), (64, False), (64, True), (32, False), (32, True)])
+@pytest.mark.parametrize("m, n, k, kernel", KERNELS)
+def test_linear_spread(m, n, k, kernel, group, zeros, dtype):
+    """Every kernel rounds once: weights that were rounded, or sums in 16 bits, would not keep to this."""
+    g = gen(m + group)
+    q, scales, z, b = weights(g, dtype, n, k, group, zeros=zeros)
+    x = randn(g, dtype, m, k)
+    plan = hipq.LinearW4(pack_rows(q), scales, group, zeros=z, bias=b)
+    assert plan.kernel(m) == kernel
+    lm_bounds.check_linear_spread(plan(x), x, q, scales, group, z, b)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype, group", [(BF16, 128), (F16, 64), (BF16, 32)])
+@pytest.mark.parametrize("m, n, k", [(16, 330, 160), (20, 100, 512), (7, 10300, 1056), (60, 8200, 160), (100, 200, 2112), (140, 4200, 160)])
+def test_linear_gated_spread(m, n, k, dtype, group, act):
+    g = gen(m)
+    q, scales, z, b = weights(g, dtype, 2 * n, k, group)
+    x = randn(g, dtype, m, k)
+    lm_bounds.check_linear_spread(hipq.LinearW4(pack_rows(q), scales, group, zeros=z, bias=b, activation=act)(x), x, q, scales, group, z, b, act)
 
 
 # ---- attention over the cache ---------------------------------------------------------------------------------------------
