@@ -493,7 +493,9 @@ int hipq_copy_bytes(const void *src, void *dst, size_t count, void *stream);
 /* ---- products with 4-bit weights (beside the fully-connected layers above, whose weights have 8)
  *   y[m][n] = sum over groups g of scale[n][g] * sum over k in g of x[m][k] * (q[n][k] - zero[n][g]),  + bias[n]
  * With an activation the plan holds two projections of N outputs each, the gate's rows first:
- *   y[m][n] = act(y_gate[m][n]) * y_up[m][n]                         (each with its bias; one launch). */
+ *   y[m][n] = act(y_gate[m][n]) * y_up[m][n]                         (each with its bias; one launch).
+ * Weights are not rounded.  The float32 sums are those of x times numbers of up to 63, and of x, which comes off: beside the rounding to 16 bits a group is
+ * off by a few 2^-24 of 63 sum |x| times its scale.  */
 typedef struct hipq_w4_desc {
     int32_t N, K;       /* outputs (of each projection) and inputs; K a multiple of 32 */
     int32_t group;      /* weights that share a scale: 32, 64 or 128; the last group of a row may be shorter */

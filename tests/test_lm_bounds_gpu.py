@@ -40,6 +40,24 @@ def test_linear_spread(m, n, k, kernel, group, zeros, dtype):
     lm_bounds.check_linear_spread(plan(x), x, q, scales, group, z, b)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("group, zeros", [(128, False), (64, True), (32, True)])
+@pytest.mark.parametrize("m, n, k, kernel", KERNELS)
+def test_linear_large_x_at_zero_points(m, n, k, kernel, group, zeros, dtype):
+    """Some x of 10^3 to 10^4 meet codes that are their zero points, which they do nothing to but in the roundings: those of sums of 63 |x|."""
+    g = gen(m + group)
+    q, scales, z, b = weights(g, dtype, n, k, group, zeros=zeros)
+    x = randn(g, dtype, m, k)
+    at = torch.randperm(k, device="cuda", generator=g)[:k // 40 + 1]
+    x[:, at] = (x[:, at] * 3000).to(dtype)
+    q[:, at] = 8 if z is None else z[:, at // group]
+    got = hipq.LinearW4(pack_rows(q), scales, group, zeros=z, bias=b)(x)
+    lm_bounds.check_linear_spread(got, x, q, scales, group, z, b)
+    want, off = lm_bounds.linear_spread(x, q, scales, group, z, b)
+    half = torch.finfo(dtype).eps / 2
+    assert ((got.double() - want).abs() <= half * want.abs() + 8 * off + torch.finfo(dtype).smallest_normal).all()  # 8: of some million normal ones
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 @pytest.mark.parametrize("dtype, group", [(BF16, 128), (F16, 64), (BF16, 32)])
 @pytest.mark.parametrize("m, n, k", [(16, 330, 160), (20, 100, 512), (7, 10300, 1056), (60, 8200, 160), (100, 200, 2112), (140, 4200, 160)])
