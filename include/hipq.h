@@ -495,7 +495,8 @@ int hipq_copy_bytes(const void *src, void *dst, size_t count, void *stream);
  * With an activation the plan holds two projections of N outputs each, the gate's rows first:
  *   y[m][n] = act(y_gate[m][n]) * y_up[m][n]                         (each with its bias; one launch).
  * Weights are not rounded.  The float32 sums are those of x times numbers of up to 63, and of x, which comes off: beside the rounding to 16 bits a group is
- * off by a few 2^-24 of 63 sum |x| times its scale.  */
+ * off by a few 2^-24 of 63 sum |x| times its scale.  A row of x with an infinity or NaN in it gives NaN in all its results, as may one of numbers
+ * whose sum, 63 times as large, is beyond float32. */
 typedef struct hipq_w4_desc {
     int32_t N, K;       /* outputs (of each projection) and inputs; K a multiple of 32 */
     int32_t group;      /* weights that share a scale: 32, 64 or 128; the last group of a row may be shorter */

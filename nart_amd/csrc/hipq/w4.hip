@@ -7,7 +7,7 @@
 // than for the weights, 16 - z is added to the mantissas as an integer (to 48 + q - z, below 64), and 48 X comes off for all columns alike,
 // as the matrix product's own initial value.  Both sums are float32: a term is up to 63 |x|, however little of it is left, so beside the
 // rounding to 16 bits a group's result is off by a few 2^-24 of 63 sum |x| times its scale (of numbers of either sign, whose running sums are
-// smaller, of 63 sqrt(sum x^2)).
+// smaller, of 63 sqrt(sum x^2)).  Infinities meet their opposites, and are NaN.
 // The group's sum is then scaled and added in float32: the weights themselves are never rounded.
 //
 // Layout.  k runs in blocks of 128, rows of weights in tiles of 16.  The 1 KB of a tile and block lies together (weights_at), a lane's 16 bytes the

@@ -58,6 +58,22 @@ def test_linear_large_x_at_zero_points(m, n, k, kernel, group, zeros, dtype):
     assert ((got.double() - want).abs() <= half * want.abs() + 8 * off + torch.finfo(dtype).smallest_normal).all()  # 8: of some million normal ones
 
 
+@pytest.mark.parametrize("act", [None, "silu", "gelu"])
+@pytest.mark.parametrize("group, zeros", [(128, False), (64, True), (32, True)])
+@pytest.mark.parametrize("m, n, k, kernel", KERNELS)
+def test_linear_rows_that_are_not_finite(m, n, k, kernel, group, zeros, act):
+    """A row with an infinity, with two of either sign, or with NaN: NaN throughout; the other rows get what they got."""
+    g = gen(m + group)
+    q, scales, z, b = weights(g, BF16, n if act is None else n // 2 * 2, k, group, zeros=zeros)
+    plan, x = hipq.LinearW4(pack_rows(q), scales, group, zeros=z, bias=b, activation=act), randn(g, BF16, m, k)
+    want, bad = plan(x), x.clone()
+    bad[0, 5], bad[m // 2, k - 1], bad[m - 1, 7], bad[m - 1, k // 2] = math.inf, math.nan, -math.inf, math.inf
+    got = plan(bad)
+    rows = [0, m // 2, m - 1]
+    others = [r for r in range(m) if r not in rows]
+    assert torch.isnan(got[rows]).all() and torch.equal(got[others], want[others])
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 @pytest.mark.parametrize("dtype, group", [(BF16, 128), (F16, 64), (BF16, 32)])
 @pytest.mark.parametrize("m, n, k", [(16, 330, 160), (20, 100, 512), (7, 10300, 1056), (60, 8200, 160), (100, 200, 2112), (140, 4200, 160)])
