@@ -518,8 +518,9 @@ void hipq_w4_plan_destroy(hipq_w4_plan *plan);
 /* Name of the kernel that hipq_w4_run launches for M rows ("" for a number of rows that it refuses).  The string is static. */
 const char *hipq_w4_plan_kernel(const hipq_w4_plan *plan, int M);
 /* x: M rows of K, x_stride elements apart (a multiple of 8 below 2^23, the first row at a multiple of 16 bytes); y: M rows of N, y_stride apart,
- * not over x.  M may be 0.  The plan belongs to the device that it was created on.  workspace: hipq_w4_workspace bytes at a multiple of 16 (0: none,
- * may be NULL), whose content is of no interest before and after; calls that may run at the same time need one each. */
+ * none of them over a row of x (between them they may lie).  M may be 0.  The plan belongs to the device that it was created on.
+ * workspace: hipq_w4_workspace bytes at a multiple of 16 (0: none, may be NULL), whose content is of no interest before and after; calls that
+ * may run at the same time need one each. */
 size_t hipq_w4_workspace(const hipq_w4_plan *plan, int M);
 int hipq_w4_run(const hipq_w4_plan *plan, const void *x, int64_t x_stride, void *y, int64_t y_stride, int M, void *workspace,
                 size_t workspace_bytes, void *stream);

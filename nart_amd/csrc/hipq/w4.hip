@@ -16,6 +16,7 @@
 #include <new>
 #include <type_traits>
 
+#include "overlap.h"
 #include "real16.h"
 
 namespace hipq {
@@ -873,9 +874,10 @@ extern "C" int hipq_w4_run(const hipq_w4_plan *p, const void *x, int64_t x_strid
     HIPQ_REQUIRE(x && y, "w4: a null pointer");
     HIPQ_REQUIRE((uintptr_t)x % 16 == 0 && x_stride % 8 == 0, "w4: rows of x have to start at multiples of 16 bytes");
     HIPQ_REQUIRE((uintptr_t)y % 2 == 0, "w4: y is not aligned to its type");
-    HIPQ_REQUIRE(x != y, "w4: y lies over x");
     HIPQ_REQUIRE(x_stride < (1 << 23), "w4: rows of x are %lld elements apart", (long long)x_stride);
     HIPQ_REQUIRE(M == 1 || (x_stride >= p->desc.K && y_stride >= p->desc.N), "w4: rows overlap (strides %lld and %lld)", (long long)x_stride, (long long)y_stride);
+    const ByteRows read = {(int64_t)(uintptr_t)x, M > 1 ? x_stride * 2 : 0, p->desc.K * 2ll, M}, written = {(int64_t)(uintptr_t)y, M > 1 ? y_stride * 2 : 0, p->desc.N * 2ll, M};
+    HIPQ_REQUIRE(!overlap(read, written), "w4: y lies over x");
     const size_t need = hipq_w4_workspace(p, M);
     HIPQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0), "w4: a workspace of %zu bytes is needed", need);
     int device;
