@@ -545,7 +545,8 @@ typedef struct hipq_kv_cache {
  * (2 i, 2 i + 1) where interleaved: (a, b) -> (a c - b s, b c + a s).  What lies behind `rot` is not turned.
  * slots[t]: page * page size + place.  A token whose slot lies outside the cache (-1 marks a padded row) or whose position lies outside
  * the table is left alone: neither its row of q_out nor the cache is written.  Two tokens of one call must not have the same slot.
- * q_out may be q itself (same strides).  Strides are in elements, multiples of 8; all pointers at multiples of 16 bytes.
+ * q_out may be q itself (same strides); otherwise none of its heads may lie over one of q, k or v, which is not looked at.  Strides are in
+ * elements, multiples of 8; all pointers at multiples of 16 bytes.
  */
 typedef struct hipq_kv_append_desc {
     const void *q, *k, *v; /* [tokens][heads][dim] */
@@ -569,7 +570,8 @@ int hipq_kv_append(const hipq_kv_cache *cache, const hipq_kv_append_desc *desc, 
  * Rows of o that belong to no sequence are left as they are.  Entries of blocks behind a sequence's end are not read; a block outside
  * the cache holds no tokens (they are not seen).  `longest` and `most_new` are the caller's bounds, from which the host divides the work:
  * of a sequence that is longer, or has more new tokens, nothing outside is read or written, and its rows mean nothing.
- * A sequence's blocks hold up to 2^30 tokens.  The scale is above 0.  o may be q itself (same strides). 
+ * A sequence's blocks hold up to 2^30 tokens.  The scale is above 0.  o may be q itself (same strides); otherwise none of its heads
+ * may lie over one of q, which is not looked at.
  * Weights - over codes, weights times their tokens' value scales - are rounded to 16 bits for the product with the values: by at most half a
  * unit in the last place, in float16 by up to 2^-32 of the row's largest where that is more.
  * A value or value scale that is infinite or NaN reaches the rows that see its token, as NaN or as an infinity, and no others.
