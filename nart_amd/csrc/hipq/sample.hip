@@ -23,6 +23,7 @@ namespace hipq {
 
 constexpr int THREADS = 1024, WAVES = THREADS / 64, BINS = 2048, LIST = 4096, FEW = THREADS, FRACTION = 43;
 constexpr int MOST_VOCAB = 1 << 20; // sums of weights fit 64 bits
+constexpr int MOST_ROWS = 1 << 21;  // of a launch
 
 // 2^(i / 32) and 2^(i / 1024)
 __constant__ const double POWERS[2][32] = {
@@ -678,12 +679,21 @@ extern "C" int hipq_sample(const void *logits, int type, int rows, int vocab, in
     SampleArgs a = {};
     a.logits = logits, a.stride = stride, a.uniform = uniform, a.temperature = temperature, a.top_p = top_p, a.min_p = min_p, a.top_k = top_k;
     a.tokens = tokens, a.vocab = vocab;
-    const dim3 grid(rows), block(THREADS);
-    if (type == HIPQ_REAL_F32)
-        sample_kernel<HIPQ_REAL_F32><<<grid, block, 0, (hipStream_t)stream>>>(a);
-    else if (type == HIPQ_REAL_F16)
-        sample_kernel<HIPQ_REAL_F16><<<grid, block, 0, (hipStream_t)stream>>>(a);
-    else
-        sample_kernel<HIPQ_REAL_BF16><<<grid, block, 0, (hipStream_t)stream>>>(a);
-    return launch_status("sample_kernel");
+    // of 2^32 work-items and more only what is left over would run
+    for (int done = 0; done < rows; done += MOST_ROWS) {
+        const dim3 grid(rows - done < MOST_ROWS ? rows - done : MOST_ROWS), block(THREADS);
+        if (type == HIPQ_REAL_F32)
+            sample_kernel<HIPQ_REAL_F32><<<grid, block, 0, (hipStream_t)stream>>>(a);
+        else if (type == HIPQ_REAL_F16)
+            sample_kernel<HIPQ_REAL_F16><<<grid, block, 0, (hipStream_t)stream>>>(a);
+        else
+            sample_kernel<HIPQ_REAL_BF16><<<grid, block, 0, (hipStream_t)stream>>>(a);
+        if (launch_status("sample_kernel"))
+            return 1;
+        a.logits = (const uint8_t *)a.logits + MOST_ROWS * stride * (type == HIPQ_REAL_F32 ? 4 : 2);
+        a.uniform += MOST_ROWS, a.tokens += MOST_ROWS;
+        a.temperature += a.temperature ? MOST_ROWS : 0, a.top_k += a.top_k ? MOST_ROWS : 0;
+        a.top_p += a.top_p ? MOST_ROWS : 0, a.min_p += a.min_p ? MOST_ROWS : 0;
+    }
+    return 0;
 }

@@ -642,6 +642,22 @@ def test_sample_large_vocabulary():
     check_sample(x, [0.1, 0.5, 0.9, 0.999], t=[1.0, 0.7, 1.5, 1.0], k=[0, 0, 20000, 50], p=[0.95, 0.999, 0.9, 0.8], m=[0, 1e-3, 0, 0])
 
 
+def test_sample_millions_of_rows():
+    """More rows than one launch has: 2^22 and some of them, the last with filters of their own."""
+    g, r = gen(13), (1 << 22) + 3
+    x, u = (torch.randn((r, 2), device="cuda", generator=g) * 2).to(F16), torch.rand(r, device="cuda", generator=g)
+    p = torch.ones(r, device="cuda")
+    p[-2:] = 0.0  # the first alone
+    w = torch.softmax(x.double(), 1)
+    want = (u.double() >= w[:, 0]).long()  # (a number as near to a border as 2^-40 may fall on either side: none does)
+    want[-2:] = x[-2:].argmax(1)
+    assert ((u.double() - w[:, 0]).abs() > 2.0 ** -36).all()
+    assert torch.equal(hipq.sample(x, u, top_p=p), want)
+    k = torch.zeros(r, dtype=torch.int32, device="cuda")
+    k[-2:] = 1
+    assert torch.equal(hipq.sample(x, u, temperature=torch.ones(r, device="cuda"), top_k=k, min_p=torch.zeros(r, device="cuda")), want)
+
+
 # ---- together, on streams and in graphs ------------------------------------------------------------------------------------
 def decoder(g, dtype, hidden=256, hq=4, hkv=2, dim=64, inner=320, vocab=1000, page=16, pages=40, int8=False):
     mk = lambda n, k, **kw: hipq.LinearW4(ref.pack_rows(torch.randint(0, 16, (n, k), dtype=torch.uint8, device="cuda", generator=g)),  # noqa: E731
