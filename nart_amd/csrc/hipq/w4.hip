@@ -244,13 +244,15 @@ __global__ __launch_bounds__(WAVES * 64) void w4_stream_kernel(const W4Args a)
 typedef const uint32_t __attribute__((address_space(1))) *gptr_t;
 typedef uint32_t __attribute__((address_space(3))) *lptr_t;
 
+constexpr int64_t XSUM_ROW = 1 << 23; // work-groups side by side
+
 // Minus the sums of x over each group, for the tile kernel: a thread has 8 of x, the group's threads are neighbours.
 template <int TYPE, int GPB>
 __global__ __launch_bounds__(256) void w4_xsum_kernel(const W4Args a, float *xsum, float factor)
 {
     using R = Real16<TYPE>;
     const int per_row = a.blocks * 16;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, m = id / per_row;
+    const int64_t id = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x, m = id / per_row;
     const int k8 = (int)(id - m * per_row);
     float s = 0;
     if (m < a.M && k8 * 8 < a.K) {
@@ -811,8 +813,10 @@ static int launch(const hipq_w4_plan *p, W4Args &a, float *workspace, hipStream_
     if (SHAPE[s.kernel].xsum) {
         a.m_pad = round_up(a.M, SHAPE[s.kernel].rows);
         a.xsum = workspace;
-        const int64_t threads = (int64_t)a.m_pad * a.blocks * 16;
-        w4_xsum_kernel<TYPE, GPB><<<dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st>>>(a, workspace, W4Tile<TYPE, GPB, ZEROS, 4, 4, 2, 4, 1, GPB == 4 && ZEROS ? 2 : 3, true>::FACTOR);
+        // of 2^32 work-items side by side and more only what is left over would run
+        const int64_t groups = ((int64_t)a.m_pad * a.blocks * 16 + 255) / 256;
+        const dim3 grid((unsigned)(groups < XSUM_ROW ? groups : XSUM_ROW), (unsigned)((groups + XSUM_ROW - 1) / XSUM_ROW));
+        w4_xsum_kernel<TYPE, GPB><<<grid, dim3(256), 0, st>>>(a, workspace, W4Tile<TYPE, GPB, ZEROS, 4, 4, 2, 4, 1, GPB == 4 && ZEROS ? 2 : 3, true>::FACTOR);
         if (launch_status("w4_xsum_kernel"))
             return 1;
         workspace += (size_t)a.m_pad * a.blocks * GPB;

@@ -28,7 +28,19 @@ def samples():
         assert sum(x for x, _ in run(rows)) == 1024 * rows
 
 
-CASES = [samples]
+def sums_of_x():
+    """Of 2^35 numbers, eight for each work-item."""
+    lib = base.hipq.lib()
+    for K, M in ((2048, 1 << 24), (16384, 1 << 21), (16384, (1 << 21) - 1), (4096, 1024)):
+        plan = base.plan(N=2048, K=K)[1]
+        launched(0)
+        assert lib.hipq_w4_plan_kernel(plan, M) == b"w4_tile_128x256"
+        (side, rows), _ = launched(lib.hipq_w4_run(plan, P, K, 1 << 50, 2048, M, P << 20, 1 << 60, None))
+        items = -(-M // 128) * 128 * K // 8
+        assert items <= side * rows < items + side
+
+
+CASES = [samples, sums_of_x]
 
 
 @pytest.fixture(scope="module")
