@@ -35,7 +35,7 @@ def sums_of_x():
         plan = base.plan(N=2048, K=K)[1]
         launched(0)
         assert lib.hipq_w4_plan_kernel(plan, M) == b"w4_tile_128x256"
-        (side, rows), _ = launched(lib.hipq_w4_run(plan, P, K, 1 << 50, 2048, M, P << 20, 1 << 60, None))
+        (side, rows), *_ = launched(lib.hipq_w4_run(plan, P, K, 1 << 50, 2048, M, P << 20, 1 << 60, None))
         items = -(-M // 128) * 128 * K // 8
         assert items <= side * rows < items + side
 
