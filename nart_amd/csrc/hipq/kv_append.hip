@@ -215,7 +215,8 @@ static int launch_append(AppendArgs &a, hipStream_t st)
 {
     const int all = a.d.q_heads + 2 * a.cache.heads, chunks = (all + a.per_chunk - 1) / a.per_chunk;
     a.blocks = (int)(((int64_t)a.d.tokens * (DIM / 8) + 255) / 256);
-    HIPQ_REQUIRE((int64_t)a.blocks * chunks < ((int64_t)1 << 31), "append: %d tokens of %d heads", a.d.tokens, all);
+    // of 2^32 work-items and more only what is left over would run
+    HIPQ_REQUIRE((int64_t)a.blocks * chunks < (1 << 24), "append: %d tokens of %d heads", a.d.tokens, all);
     const dim3 grid((unsigned)(a.blocks * chunks));
     if (a.cache.quantized)
         kv_append_kernel<TYPE, DIM, true><<<grid, dim3(256), 0, st>>>(a);

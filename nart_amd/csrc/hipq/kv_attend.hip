@@ -944,7 +944,8 @@ extern "C" int hipq_kv_attend(const hipq_kv_cache *cache, const hipq_kv_attend_d
     HIPQ_REQUIRE(((uintptr_t)d->q | (uintptr_t)d->o) % 16 == 0 && (d->q_token | d->q_head | d->o_token | d->o_head) % 8 == 0,
                  "attend: heads have to start at multiples of 16 bytes");
     HIPQ_REQUIRE(s.workspace == 0 || (workspace && workspace_bytes >= s.workspace && (uintptr_t)workspace % 16 == 0), "attend: a workspace of %zu bytes is needed", s.workspace);
-    HIPQ_REQUIRE(items * s.splits * 16 * s.rt < ((int64_t)1 << 31), "attend: %lld work-groups", (long long)items * s.splits);
+    // item numbers are 32 bits, and of 2^32 work-items and more only what is left over would run
+    HIPQ_REQUIRE(items * s.splits * 16 * s.rt < ((int64_t)1 << 31) && items * s.splits <= (1 << 24) - 8, "attend: %lld work-groups", (long long)items * s.splits);
     AttendArgs a = {};
     a.cache = *cache, a.d = *d;
     if (cache->pages == 0)

@@ -40,7 +40,42 @@ def sums_of_x():
         assert items <= side * rows < items + side
 
 
-CASES = [samples, sums_of_x]
+def refused(rc, message):
+    assert rc != 0 and message in base.hipq.lib().hipq_last_error(), (rc, base.hipq.lib().hipq_last_error())
+    assert C.c_long.in_dll(base.STUB, "stub_launches").value == 0
+
+
+def attention():
+    """A work-group for each sequence, head, block of rows and part: 2^24 of 256 are too many."""
+    lib = base.hipq.lib()
+
+    def run(sequences, heads, most_new=1, dim=64, blocks=1, longest=16):
+        c = base.cache(dict(heads=heads, dim=dim))
+        d = base.hipq.KvAttendDesc(q=P, o=P, q_token=heads * dim, q_head=dim, o_token=heads * dim, o_head=dim, starts=P, lens=P, blocks=P, blocks_stride=blocks,
+                                   sequences=sequences, tokens=sequences, q_heads=heads, blocks_per_sequence=blocks, most_new=most_new, longest=longest, scale=0.1)
+        return lib.hipq_kv_attend(C.byref(c), C.byref(d), P, 1 << 60, None)
+    for sequences, heads, more in ((1 << 20, 15, {}), (1 << 12, 4095, {}), (1 << 10, 512, dict(most_new=1 << 9)), (300, 64, dict(dim=128, most_new=4096, longest=1 << 14, blocks=1 << 10))):
+        launched(run(sequences, heads, **more))
+    for sequences, heads, more in ((1 << 20, 16, {}), (1 << 12, 4096, {}), (1 << 20, 64, {}), (1 << 10, 512, dict(most_new=1 << 10))):
+        refused(run(sequences, heads, **more), b"work-groups")
+
+
+def new_tokens():
+    """A work-item for eight elements of a token, for each eight of its heads."""
+    lib = base.hipq.lib()
+
+    def run(tokens, heads, dim=256):
+        c = base.cache(dict(heads=heads, dim=dim))
+        d = base.hipq.KvAppendDesc(k=P, v=P, k_head=dim, v_head=dim, positions=P, slots=P, tokens=tokens, eps=1e-6)
+        return lib.hipq_kv_append(C.byref(c), C.byref(d), None)
+    for tokens, heads in ((1 << 24, 28), (1 << 20, 508), (5, 4096)):
+        (side, rows), = launched(run(tokens, heads))
+        assert side >= tokens * 32 * -(-2 * heads // 8) or tokens == 5
+    for tokens, heads in ((1 << 24, 32), (1 << 24, 4096), (1 << 20, 512)):
+        refused(run(tokens, heads), b"tokens of")
+
+
+CASES = [samples, sums_of_x, attention, new_tokens]
 
 
 @pytest.fixture(scope="module")
