@@ -754,7 +754,7 @@ static W4Shape shape_of(const hipq_w4_plan *p, int M)
         s.kernel = M <= 16 ? TILE_16 : TILE_32;
     else if (M <= 128)
         s.kernel = M <= 64 ? (columns < 128 ? TILE_32 : TILE_64) : (columns < 128 ? TILE_64 : TILE_128);
-    else if ((M + 127) / 128 * ((p->tiles + 15) / 16) < 64)
+    else if ((int64_t)((M + 127) / 128) * ((p->tiles + 15) / 16) < 64)
         s.kernel = TILE_128;
     if (s.kernel != STREAM_16) {
         const int64_t groups = (int64_t)((M + SHAPE[s.kernel].rows - 1) / SHAPE[s.kernel].rows) * ((p->tiles + SHAPE[s.kernel].tiles - 1) / SHAPE[s.kernel].tiles);
@@ -880,6 +880,8 @@ extern "C" int hipq_w4_run(const hipq_w4_plan *p, const void *x, int64_t x_strid
     HIPQ_REQUIRE((uintptr_t)y % 2 == 0, "w4: y is not aligned to its type");
     HIPQ_REQUIRE(x_stride < (1 << 23), "w4: rows of x are %lld elements apart", (long long)x_stride);
     HIPQ_REQUIRE(M == 1 || (x_stride >= p->desc.K && y_stride >= p->desc.N), "w4: rows overlap (strides %lld and %lld)", (long long)x_stride, (long long)y_stride);
+    // the widest work-groups' number: of 2^32 work-items and more only what is left over would run
+    HIPQ_REQUIRE((int64_t)((M + 127) / 128) * ((p->tiles + 15) / 16) <= (1 << 23) - 8, "w4: %d rows of %d outputs", M, p->desc.N);
     const ByteRows read = {(int64_t)(uintptr_t)x, M > 1 ? x_stride * 2 : 0, p->desc.K * 2ll, M}, written = {(int64_t)(uintptr_t)y, M > 1 ? y_stride * 2 : 0, p->desc.N * 2ll, M};
     HIPQ_REQUIRE(!overlap(read, written), "w4: y lies over x");
     const size_t need = hipq_w4_workspace(p, M);

@@ -40,6 +40,20 @@ def sums_of_x():
         assert items <= side * rows < items + side
 
 
+def products():
+    """A work-group of 512 for 128 rows of 256 outputs: 2^23 are too many."""
+    lib = base.hipq.lib()
+    plans = {n: base.plan(N=n, K=32)[1] for n in (16384, 16128, 1 << 20)}
+    gated = base.plan(N=8192, K=32, activation=1)[1]
+    launched(0)
+    run = lambda plan, M: lib.hipq_w4_run(plan, P, 32, 1 << 50, 1 << 20, M, P << 20, 1 << 60, None)  # noqa: E731
+    for n, M in ((16384, (1 << 24) - 256), (16128, 1 << 24), (1 << 20, 1 << 17)):
+        launched(run(plans[n], M))
+        refused(run(plans[n], 1 << 24), b"outputs") if n != 16128 else None
+    launched(run(gated, (1 << 24) - 256))
+    refused(run(gated, 1 << 24), b"outputs")
+
+
 def refused(rc, message):
     assert rc != 0 and message in base.hipq.lib().hipq_last_error(), (rc, base.hipq.lib().hipq_last_error())
     assert C.c_long.in_dll(base.STUB, "stub_launches").value == 0
@@ -75,7 +89,7 @@ def new_tokens():
         refused(run(tokens, heads), b"tokens of")
 
 
-CASES = [samples, sums_of_x, attention, new_tokens]
+CASES = [samples, sums_of_x, products, attention, new_tokens]
 
 
 @pytest.fixture(scope="module")
