@@ -569,7 +569,8 @@ int hipq_kv_append(const hipq_kv_cache *cache, const hipq_kv_append_desc *desc, 
  *   o = sum_t softmax_t(scale * q . k_t) v_t over the tokens seen; 0 where there is none.
  * Rows of o that belong to no sequence are left as they are.  Entries of blocks behind a sequence's end are not read; a block outside
  * the cache holds no tokens (they are not seen).  `longest` and `most_new` are the caller's bounds, from which the host divides the work:
- * of a sequence that is longer, or has more new tokens, nothing outside is read or written, and its rows mean nothing.
+ * of a sequence that is longer, or has more new tokens, nothing outside is read or written, and its rows mean nothing.  Rows that
+ * starts names outside of q, or that end before they begin, are left out.
  * A sequence's blocks hold up to 2^30 tokens.  The scale is above 0.  o may be q itself (same strides); otherwise none of its heads
  * may lie over one of q, which is not looked at.
  * Weights - over codes, weights times their tokens' value scales - are rounded to 16 bits for the product with the values: by at most half a

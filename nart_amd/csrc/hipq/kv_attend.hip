@@ -74,7 +74,7 @@ struct Sequence {
     int row0, count, len, old; // first row of q, new tokens, tokens in the cache, those before the new ones
     __device__ __forceinline__ Sequence(const AttendArgs &a, int b)
     {
-        const int end = min(a.d.starts[b + 1], a.d.tokens);
+        const int end = max(min(a.d.starts[b + 1], a.d.tokens), 0); // end - row0 fits whatever is in starts
         row0 = max(a.d.starts[b], 0);
         len = max(min(min(a.d.lens[b], a.d.longest), a.d.blocks_per_sequence * a.cache.page), 0);
         count = max(min(end - row0, a.d.most_new), 0);

@@ -504,6 +504,22 @@ def test_pages_beyond_32_bits(int8):
     check_attend(g, cache, blocks, [3], [n], 16, BF16)
 
 
+@pytest.mark.parametrize("heads, hq, n", [(2, 4, 100), (1, 4, 5000), (8, 64, 4000)])
+def test_attend_rows_that_are_not_there(heads, hq, n):
+    """Starts in front of the first row, behind the last, falling, at both ends of 32 bits: no row outside is read or written, and the rows of a sequence that is
+    in order are what they are among others in order."""
+    g = gen(n)
+    cache, blocks = fill_cache(g, BF16, 8, heads, 16, 128, n, False)
+    index = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    q = randn(g, BF16, 30, hq, 128)
+    top, low = (1 << 31) - 1, -(1 << 31)
+    call = lambda starts, lens: cache.attend(q, index(starts), index(lens), blocks, 12, out=torch.full_like(q, 11.0))  # noqa: E731
+    want = call([0, 0, 3, 12, 12, 12, 12, 12, 12], [n] * 8)[3:12]
+    for starts, end in (([top, low, 3, 12, low, low + 7, -5, -9, low], 12), ([low, low, 3, 12, top, low, 0, -1, low], 24)):
+        got = call(starts, [n, top, n, n, low, -1, n, top])
+        assert torch.equal(got[3:12], want) and (got[end:] == 11).all() and torch.isfinite(got).all()
+
+
 def test_attend_over_its_queries():
     """The outputs may lie where the queries lay."""
     g = gen(71)
