@@ -1,9 +1,10 @@
 // Attention of new tokens over a paged cache (hipq_kv_attend).  gfx950 only.
 //
 // The cache is read once and every other thing is small: a query head's scores are never written.  With a reference m that is at least the
-// running maximum less 8, each tile of tokens adds p_t = 2^(s_t - m) to the sum l and p_t v_t to the output o, all in float32 (p, over codes
-// p times the token's value scale, is rounded to 16 bits for the product, half a unit in the last place each; see softmax_step for float16's small ones); when a score passes m + 8, m moves there and l
-// and o are scaled, which keeps the result and leaves most tiles without any exchange between lanes.
+// running maximum less 8, each tile of tokens adds p_t = 2^(s_t - m) to the sum l and p_t v_t to the output o, all in float32; when a score
+// passes m + 8, m moves there and l and o are scaled, which keeps the result and leaves most tiles without any exchange between lanes.
+// For the product p - over codes p times the token's value scale - is rounded to 16 bits, which is what the matrix unit takes (in two parts it
+// would do twice the work): half a unit in the last place each, and for float16's small ones see softmax_step.
 //
 // What carries it:
 //   * The rows of a work-group are the new tokens of one sequence times the query heads that share a cache head: up to 16 RT of them read

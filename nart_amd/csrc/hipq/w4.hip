@@ -119,7 +119,7 @@ __device__ __host__ static __forceinline__ size_t scales_at(int tile, int block,
 // Every weight is used by at most 16 MT rows, so the time is what it takes to read the weights, and what counts is how much of them is
 // in flight: a work-group owns NT tiles and 16 MT rows, its waves take the blocks of k in turn, each DEPTH blocks ahead and straight
 // into registers (a tile's block is 1 KB, in one load), and their sums meet once, in LDS.  No barrier in the loop.  One row of 4096 x 4096: 4.8 us,
-// a launch and two rounds of loads; the tile kernel and its join take 9.3.
+// a launch and one round of loads (all of k is asked for before the first multiply); the tile kernel and its join take 9.3.
 template <int TYPE, int GPB, bool ZEROS, int MT, int NT, int WAVES, int DEPTH>
 __global__ __launch_bounds__(WAVES * 64) void w4_stream_kernel(const W4Args a)
 {
@@ -277,8 +277,9 @@ __global__ __launch_bounds__(256) void w4_xsum_kernel(const W4Args a, float *xsu
 // XSUM: the sums of x come from w4_xsum_kernel, otherwise from a multiply by ones.
 // What bounds it: up to some dozen rows the weights (17 rows of 14336 x 4096 gated, groups of 64, 18.9 us: 3.4 TB/s in one round of
 // work-groups); above, the vector instructions that unpack weights (7 for 8 of them and 16 MT rows) and scale sums (one for an output and group,
-// two with zero points), which do not overlap the matrix unit's on a SIMD: 2048 rows of 8192 x 8192 in float16, 265 us with the sums of x,
-// 1.03 PFLOP/s, 49 % of the time the matrix unit's and 43 % theirs; 100 rows of 5000 x 5504 in groups of 32, 23 us.
+// two with zero points), which take turns with the multiplies, as the waves of a SIMD are in step: 2048 rows of 8192 x 8192 in float16, 265 to 297 us
+// on different cards with the sums of x, 0.93 to 1.03 PFLOP/s, 49 % of the time the matrix unit's and 43 % theirs; 100 rows of 5000 x 5504 in groups
+// of 32, 23 us.
 template <int TYPE, int GPB, bool ZEROS, int MT, int NT, int WM, int WN, int WK, int STAGES, bool XSUM>
 struct W4Tile {
     static constexpr int WAVES = WM * WN, BM = 16 * MT * WM, TILES = NT * WN, PER = 4 / GPB; // WAVES: of a group
