@@ -525,6 +525,42 @@ size_t hipq_w4_workspace(const hipq_w4_plan *plan, int M);
 int hipq_w4_run(const hipq_w4_plan *plan, const void *x, int64_t x_stride, void *y, int64_t y_stride, int M, void *workspace,
                 size_t workspace_bytes, void *stream);
 
+/* ---- a layer of experts with 4-bit weights
+ * Each token takes the `top` experts with the largest scores (logits; the lowest index among equal ones; scores of -infinity and NaN are never taken, so that
+ * a token may have fewer, and with none y = 0):
+ *   y[t] = sum over them of share[e] * down_e(act(gate_e x[t]) * up_e x[t])
+ * with products as above, and
+ *   HIPQ_SCORES_SOFTMAX: share[e] = exp(logit_e) / sum of exp(logit) over all experts, or with normalize over the token's (of +infinities each counts as much, and
+ *                        nothing else does),
+ *   HIPQ_SCORES_SIGMOID: share[e] = 1 / (1 + exp(-logit_e)), with normalize divided by the sum of the token's.
+ * The hidden rows are rounded to 16 bits between the products; in float16 one beyond 65504 is an infinity there. */
+#define HIPQ_SCORES_SOFTMAX 0
+#define HIPQ_SCORES_SIGMOID 1
+
+typedef struct hipq_w4_experts_desc {
+    int32_t experts, top; /* up to 1024, and 16 of them for a token */
+    int32_t N, K, inner;  /* outputs, inputs and hidden values of an expert; K and inner multiples of 32 */
+    int32_t group, type;  /* as above */
+    int32_t activation;   /* HIPQ_ACT_SILU or HIPQ_ACT_GELU */
+    int32_t scores, normalize;
+} hipq_w4_experts_desc;
+
+typedef struct hipq_w4_experts_plan hipq_w4_experts_plan;
+
+/* Setup, as hipq_w4_plan_create.  gate_up: for each expert the gate's `inner` rows of K / 2 bytes, then those of the other projection; down: for each N rows of
+ * inner / 2 bytes; scales and zeros (for both products or NULL for both) in that order. */
+int hipq_w4_experts_create(const hipq_w4_experts_desc *desc, const uint8_t *gate_up, const void *gate_up_scales, const uint8_t *gate_up_zeros, const uint8_t *down,
+                           const void *down_scales, const uint8_t *down_zeros, void *stream, hipq_w4_experts_plan **plan_out);
+void hipq_w4_experts_destroy(hipq_w4_experts_plan *plan);
+/* Name of the kernel that multiplies M rows ("" for a number of rows that is refused).  The string is static. */
+const char *hipq_w4_experts_kernel(const hipq_w4_experts_plan *plan, int M);
+/* x and y as for hipq_w4_run, with M times x_stride below 2^31 and M times `top` times `inner` as well; logits: M rows of `experts` of logits_type (HIPQ_REAL_*),
+ * logits_stride elements apart.  y lies over neither.  workspace: hipq_w4_experts_workspace bytes at a multiple of 16, whose content is of no interest before and
+ * after; calls that may run at the same time need one each. */
+size_t hipq_w4_experts_workspace(const hipq_w4_experts_plan *plan, int M);
+int hipq_w4_experts_run(const hipq_w4_experts_plan *plan, const void *x, int64_t x_stride, const void *logits, int logits_type, int64_t logits_stride, void *y,
+                        int64_t y_stride, int M, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- a paged cache of keys and values, and the attention that reads it
  * Keys and values lie in pages: element (page p, head h, token t of the page, i) at ((p * heads + h) * page + t) * dim + i.  In 8 bits
  * (quantized = 1) the value is code * scale with one float scale for each (p, h, t); codes are int8 in -127..127. */
@@ -609,6 +645,31 @@ int hipq_kv_attend(const hipq_kv_cache *cache, const hipq_kv_attend_desc *desc, 
  */
 int hipq_sample(const void *logits, int type, int rows, int vocab, int64_t stride, const float *uniform, const float *temperature,
                 const int32_t *top_k, const float *top_p, const float *min_p, int64_t *tokens, void *stream);
+
+/*
+ * What a row's scores become before a token is drawn from them, in this order:
+ *   a token that has occurred - one of tokens[row][0 .. lens[row] - 1] - has its score x divided by repetition where x > 0, otherwise multiplied by it;
+ *   one that has occurred n > 0 times behind the row's first prompt_lens[row] loses n * frequency + presence;
+ *   a token of bias_tokens[row] gains its bias (of several entries for one token the last counts);
+ *   a token whose bit - bit v % 32 of allowed[row][v / 32] - is not set has -infinity.
+ * In 32 bits, rounded once to `type`.  Numbers of tokens outside 0 .. vocab - 1 (-1 marks an empty entry) mean nothing.  All but logits and out may be NULL:
+ * lens (all of `longest`), prompt_lens (0), a penalty (none), tokens where longest is 0, bias and bias_tokens where biases is, allowed.
+ * out may be logits (same strides), otherwise it lies over none of its rows, nor over any other array, which is not looked at.  Strides are in elements, of
+ * `bias_tokens` and `bias` the same.
+ */
+typedef struct hipq_penalize_desc {
+    const void *logits;
+    void *out; /* rows of `vocab` of `type`, at any address that the type allows */
+    int64_t stride, out_stride;
+    const int32_t *tokens, *lens, *prompt_lens;         /* [rows][longest], [rows], [rows] */
+    const float *repetition, *frequency, *presence;     /* [rows] */
+    const int32_t *bias_tokens;                         /* [rows][biases] */
+    const float *bias;
+    const uint32_t *allowed;                            /* [rows][ceil(vocab / 32)] */
+    int64_t tokens_stride, bias_stride, allowed_stride;
+    int32_t type, rows, vocab, longest, biases;         /* vocab: up to 2^20 */
+} hipq_penalize_desc;
+int hipq_penalize(const hipq_penalize_desc *desc, void *stream);
 
 #ifdef __cplusplus
 }

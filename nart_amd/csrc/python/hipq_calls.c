@@ -479,6 +479,16 @@ static int whole_tensor(PyObject *t, const char *name, int dims, unsigned allowe
     return 1;
 }
 
+/* with gaps between rows; None: a null pointer */
+static int tensor_or_none(PyObject *t, const char *name, int dims, unsigned allowed, int device, view_t *v)
+{
+    if (t == Py_None) {
+        memset(v, 0, sizeof *v);
+        return 1;
+    }
+    return tensor(t, name, dims, allowed, device, v);
+}
+
 static int shaped(const view_t *v, const char *name, int dims, int64_t s0, int64_t s1, int64_t s2)
 {
     const int64_t s[3] = {s0, s1, s2};
@@ -521,6 +531,37 @@ static PyObject *py_w4_run(ARGS)
         || !current_stream(&st))
         return NULL;
     CALL(hipq_w4_run((const hipq_w4_plan *)plan, x.p, x.stride[0], y.p, y.stride[0], (int)x.shape[0], w.p, (size_t)w.shape[0], st));
+}
+
+/* plan, M */
+static PyObject *py_experts_workspace(ARGS)
+{
+    (void)self;
+    if (!expect(n, 2))
+        return NULL;
+    void *plan = PyLong_AsVoidPtr(a[0]);
+    int m;
+    if ((plan == NULL && PyErr_Occurred()) || !whole(a[1], &m))
+        return NULL;
+    return PyLong_FromSize_t(hipq_w4_experts_workspace((const hipq_w4_experts_plan *)plan, m));
+}
+
+/* plan, type, N, K, experts, x, logits, y, workspace or None */
+static PyObject *py_experts_run(ARGS)
+{
+    (void)self;
+    view_t x, l, y, w;
+    int device, type, N, K, experts;
+    void *st;
+    if (!expect(n, 9))
+        return NULL;
+    void *plan = PyLong_AsVoidPtr(a[0]);
+    if ((plan == NULL && PyErr_Occurred()) || !whole(a[1], &type) || !whole(a[2], &N) || !whole(a[3], &K) || !whole(a[4], &experts) || !current_device(&device)
+        || !tensor(a[5], "x", 2, 1u << type, device, &x) || !tensor(a[6], "logits", 2, HALVES | 1u << F32, device, &l) || !tensor(a[7], "y", 2, 1u << type, device, &y)
+        || !whole_tensor(a[8], "workspace", 1, 1u << U8, device, 1, &w) || !shaped(&x, "x", 2, x.shape[0], K, 0) || !shaped(&l, "logits", 2, x.shape[0], experts, 0)
+        || !shaped(&y, "y", 2, x.shape[0], N, 0) || !current_stream(&st))
+        return NULL;
+    CALL(hipq_w4_experts_run((const hipq_w4_experts_plan *)plan, x.p, x.stride[0], l.p, l.dtype, l.stride[0], y.p, y.stride[0], (int)x.shape[0], w.p, (size_t)w.shape[0], st));
 }
 
 static void free_cache(PyObject *c) { PyMem_Free(PyCapsule_GetPointer(c, "hipq_kv_cache")); }
@@ -707,11 +748,54 @@ static PyObject *py_sample(ARGS)
     CALL(hipq_sample(x.p, x.dtype, (int)r, (int)x.shape[1], x.stride[0], u.p, t.p, k.p, p.p, m.p, out.p, st));
 }
 
+/* logits, out, tokens, lens, prompt_lens, repetition, frequency, presence, bias_tokens, bias, allowed (all but the first two: or None) */
+static PyObject *py_penalize(ARGS)
+{
+    (void)self;
+    hipq_penalize_desc d;
+    view_t x, out, tokens, lens, prompt, rep, freq, pres, at, bias, bits;
+    int device;
+    void *st;
+    memset(&d, 0, sizeof d);
+    if (!expect(n, 11) || !current_device(&device) || !tensor(a[0], "logits", 2, HALVES | 1u << F32, device, &x) || !tensor(a[1], "out", 2, 1u << x.dtype, device, &out)
+        || !tensor_or_none(a[2], "tokens", 2, 1u << I32, device, &tokens) || !whole_tensor(a[3], "lens", 1, 1u << I32, device, 1, &lens)
+        || !whole_tensor(a[4], "prompt_lens", 1, 1u << I32, device, 1, &prompt) || !whole_tensor(a[5], "repetition", 1, 1u << F32, device, 1, &rep)
+        || !whole_tensor(a[6], "frequency", 1, 1u << F32, device, 1, &freq) || !whole_tensor(a[7], "presence", 1, 1u << F32, device, 1, &pres)
+        || !tensor_or_none(a[8], "bias_tokens", 2, 1u << I32, device, &at) || !tensor_or_none(a[9], "bias", 2, 1u << F32, device, &bias)
+        || !tensor_or_none(a[10], "allowed", 2, 1u << I32, device, &bits))
+        return NULL;
+    const int64_t r = x.shape[0], v = x.shape[1];
+    if (!shaped(&out, "out", 2, r, v, 0) || !shaped(&tokens, "tokens", 1, r, 0, 0) || !shaped(&lens, "lens", 1, r, 0, 0) || !shaped(&prompt, "prompt_lens", 1, r, 0, 0)
+        || !shaped(&rep, "repetition", 1, r, 0, 0) || !shaped(&freq, "frequency", 1, r, 0, 0) || !shaped(&pres, "presence", 1, r, 0, 0)
+        || !shaped(&at, "bias_tokens", 1, r, 0, 0) || !shaped(&bias, "bias", 2, r, at.shape[1], 0) || !shaped(&bits, "allowed", 2, r, (v + 31) / 32, 0)
+        || !current_stream(&st))
+        return NULL;
+    if (bias.there && r > 1 && bias.stride[0] != at.stride[0]) {
+        PyErr_SetString(PyExc_ValueError, "bias: rows as far apart as those of bias_tokens are expected");
+        return NULL;
+    }
+    if (!tokens.there && (lens.there || prompt.there || rep.there || freq.there || pres.there)) {
+        PyErr_SetString(PyExc_ValueError, "tokens: a tensor is expected where lengths or penalties are given");
+        return NULL;
+    }
+    if (at.there != bias.there) {
+        PyErr_SetString(PyExc_ValueError, "bias and bias_tokens belong together");
+        return NULL;
+    }
+    d.logits = x.p, d.out = out.p, d.stride = x.stride[0], d.out_stride = out.stride[0];
+    d.tokens = tokens.p, d.lens = lens.p, d.prompt_lens = prompt.p, d.repetition = rep.p, d.frequency = freq.p, d.presence = pres.p;
+    d.bias_tokens = at.p, d.bias = bias.p, d.allowed = bits.p;
+    d.tokens_stride = tokens.stride[0], d.bias_stride = at.stride[0], d.allowed_stride = bits.stride[0];
+    d.type = x.dtype, d.rows = (int)r, d.vocab = (int)v, d.longest = (int)tokens.shape[1], d.biases = (int)at.shape[1];
+    CALL(hipq_penalize(&d, st));
+}
+
 #define METHOD(NAME) {#NAME, (PyCFunction)(void (*)(void))py_##NAME, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {
     METHOD(init),        METHOD(conv2d_run),  METHOD(add_u8),      METHOD(eltwise_u8),    METHOD(relu_u8),       METHOD(concat_u8), METHOD(softmax_u8),
     METHOD(pool_u8),     METHOD(quantize_u8), METHOD(quantize_i8), METHOD(dequantize_u8), METHOD(dequantize_i8),
-    METHOD(types),       METHOD(w4_workspace), METHOD(w4_run),     METHOD(kv_cache),      METHOD(kv_append),     METHOD(kv_attend), METHOD(sample),
+    METHOD(types),       METHOD(w4_workspace), METHOD(w4_run),     METHOD(experts_workspace), METHOD(experts_run), METHOD(kv_cache),      METHOD(kv_append),     METHOD(kv_attend), METHOD(sample),
+    METHOD(penalize),
     {NULL, NULL, 0, NULL},
 };
 

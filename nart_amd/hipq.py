@@ -33,6 +33,10 @@ class W4Desc(C.Structure):  # hipq_w4_desc
     _fields_ = [(n, C.c_int32) for n in ("N", "K", "group", "type", "activation")]
 
 
+class W4ExpertsDesc(C.Structure):  # hipq_w4_experts_desc
+    _fields_ = [(n, C.c_int32) for n in ("experts", "top", "N", "K", "inner", "group", "type", "activation", "scores", "normalize")]
+
+
 class KvCacheStruct(C.Structure):  # hipq_kv_cache
     _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] \
         + [(n, C.c_int32) for n in ("pages", "heads", "page", "dim", "type", "quantized")]
@@ -49,6 +53,12 @@ class KvAttendDesc(C.Structure):  # hipq_kv_attend_desc
     _fields_ = [(n, C.c_void_p) for n in ("q", "o")] + [(n, C.c_int64) for n in ("q_token", "q_head", "o_token", "o_head")] \
         + [(n, C.c_void_p) for n in ("starts", "lens", "blocks", "mask")] + [("blocks_stride", C.c_int64)] \
         + [(n, C.c_int32) for n in ("sequences", "tokens", "q_heads", "blocks_per_sequence", "most_new", "longest")] + [("scale", C.c_float)]
+
+
+class PenalizeDesc(C.Structure):  # hipq_penalize_desc
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "out")] + [(n, C.c_int64) for n in ("stride", "out_stride")] \
+        + [(n, C.c_void_p) for n in ("tokens", "lens", "prompt_lens", "repetition", "frequency", "presence", "bias_tokens", "bias", "allowed")] \
+        + [(n, C.c_int64) for n in ("tokens_stride", "bias_stride", "allowed_stride")] + [(n, C.c_int32) for n in ("type", "rows", "vocab", "longest", "biases")]
 
 
 TILE_INDEX = {"128x128": 0, "256x64": 1, "128x64": 2, "64x128": 3, "64x64": 4}  # hipq_conv2d_plan_select
@@ -137,10 +147,16 @@ _SIGS = {
     "hipq_w4_plan_destroy": (None, [C.c_void_p]),
     "hipq_w4_plan_kernel": (C.c_char_p, [C.c_void_p, C.c_int]),
     "hipq_w4_workspace": (C.c_size_t, [C.c_void_p, C.c_int]),
+    "hipq_w4_experts_create": (C.c_int, [C.POINTER(W4ExpertsDesc)] + [C.c_void_p] * 7 + [C.POINTER(C.c_void_p)]),
+    "hipq_w4_experts_destroy": (None, [C.c_void_p]),
+    "hipq_w4_experts_kernel": (C.c_char_p, [C.c_void_p, C.c_int]),
+    "hipq_w4_experts_workspace": (C.c_size_t, [C.c_void_p, C.c_int]),
+    "hipq_w4_experts_run": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
     "hipq_w4_run": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
     "hipq_kv_append": (C.c_int, [C.POINTER(KvCacheStruct), C.POINTER(KvAppendDesc), C.c_void_p]),
     "hipq_kv_attend_workspace": (C.c_size_t, [C.POINTER(KvCacheStruct), C.POINTER(KvAttendDesc)]),
     "hipq_kv_attend": (C.c_int, [C.POINTER(KvCacheStruct), C.POINTER(KvAttendDesc), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "hipq_penalize": (C.c_int, [C.POINTER(PenalizeDesc), C.c_void_p]),
     "hipq_sample": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int64] + [C.c_void_p] * 7),
 }
 EXPORTS = tuple(_SIGS)
@@ -668,6 +684,95 @@ class LinearW4:
             pass
 
 
+_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+class ExpertsW4:
+    """A layer of experts with 4-bit weights and group scales: each token's `top` experts with the largest scores, their gated pairs, the second product of each, and
+    the sum of those times the experts' shares (include/hipq.h: "a layer of experts").
+
+    gate_up: uint8 [experts, 2 inner, K / 2], an expert's gate rows first; down: uint8 [experts, N, inner / 2]; scales: [experts, rows, ceil(columns / group)] of each
+    in float16 or bfloat16, which x and y then are as well; zeros: uint8 like the scales, for both or None (8 everywhere).  scores: "softmax" or "sigmoid";
+    normalize: the shares of a token's experts sum to 1.  All on the current device; the plan keeps a copy of its own."""
+
+    def __init__(self, gate_up, gate_up_scales, down, down_scales, top, group=128, gate_up_zeros=None, down_zeros=None, activation="silu", scores="softmax", normalize=True):
+        import torch
+        self.handle, self._address = None, 0
+        types = {torch.float16: REAL_F16, torch.bfloat16: REAL_BF16}
+        if activation not in ("silu", "gelu"):
+            raise ValueError("activation: 'silu' or 'gelu' is expected")
+        if scores not in _SCORES:
+            raise ValueError("scores: 'softmax' or 'sigmoid' is expected")
+        for t, name in ((gate_up, "gate_up"), (down, "down")):
+            if t.dim() != 3 or t.dtype != torch.uint8:
+                raise ValueError("%s: uint8 with three dimensions is expected" % name)
+        if gate_up_scales.dtype not in types:
+            raise ValueError("gate_up_scales: float16 or bfloat16 is expected")
+        if group not in (32, 64, 128):
+            raise ValueError("group: 32, 64 or 128 is expected")
+        experts, rows, k = gate_up.shape[0], gate_up.shape[1], 2 * gate_up.shape[2]
+        n, inner = down.shape[1], 2 * down.shape[2]
+        if not 1 <= experts or rows != 2 * inner or down.shape[0] != experts:
+            raise ValueError("down: [%d, N, %d] is expected, it is %s" % (experts, rows // 4, tuple(down.shape)))
+        if not 1 <= top <= min(16, experts):
+            raise ValueError("top: 1 to %d experts of a token are expected" % min(16, experts))
+        if (gate_up_zeros is None) != (down_zeros is None):
+            raise ValueError("zeros: for both products or for neither")
+        dtype = gate_up_scales.dtype
+        up, low = (experts, rows, -(-k // group)), (experts, n, -(-inner // group))
+        for t, name, shape, of in ((gate_up_scales, "gate_up_scales", up, dtype), (down_scales, "down_scales", low, dtype), (gate_up_zeros, "gate_up_zeros", up, torch.uint8),
+                                   (down_zeros, "down_zeros", low, torch.uint8)):
+            if t is not None and (tuple(t.shape) != shape or t.dtype != of):
+                raise ValueError("%s: %s of shape %s is expected" % (name, of, shape))
+        tensors = (gate_up, gate_up_scales, gate_up_zeros, down, down_scales, down_zeros)
+        current = torch.cuda.current_device()
+        for t, name in zip(tensors, ("gate_up", "gate_up_scales", "gate_up_zeros", "down", "down_scales", "down_zeros")):
+            if t is not None and t.get_device() != current:
+                raise ValueError("%s is not on the current device" % name)
+        tensors = [None if t is None else t.contiguous() for t in tensors]
+        self.experts, self.top, self.N, self.K, self.inner, self.type, self.dtype = experts, int(top), n, k, inner, types[dtype], dtype
+        d = W4ExpertsDesc(experts=experts, top=top, N=n, K=k, inner=inner, group=group, type=self.type, activation=_ACTIVATIONS[activation], scores=_SCORES[scores],
+                          normalize=int(bool(normalize)))
+        h = C.c_void_p()
+        check(lib().hipq_w4_experts_create(C.byref(d), *(_ptr(t) for t in tensors), _stream(), C.byref(h)))
+        self.handle, self._address = h, h.value
+
+    def kernel(self, m):
+        """Name of the kernel that multiplies m rows."""
+        return lib().hipq_w4_experts_kernel(self.handle, int(m)).decode()
+
+    def __call__(self, x, logits, y=None):
+        """y [M, N] of x [M, K] (or with more dimensions in front) and the experts' scores, logits [M, experts] in float32, float16 or bfloat16; rows may have gaps
+        between them."""
+        if not self._address:
+            raise ValueError("the plan is closed")
+        if x.dim() != 2:
+            front = x.shape[:-1]
+            if y is not None:
+                raise ValueError("y: only with an x of two dimensions")
+            return self(x.reshape(-1, x.shape[-1]), logits.reshape(-1, logits.shape[-1])).view(*front, self.N)
+        calls = _CALLS or _calls()
+        m = x.shape[0]
+        if y is None:
+            y = x.new_empty((m, self.N))
+        need = calls.experts_workspace(self._address, m)
+        rc = calls.experts_run(self._address, self.type, self.N, self.K, self.experts, x, logits, y, _bytes_like(x, need) if need else None)
+        if rc:
+            check(rc)
+        return y
+
+    def close(self):
+        if self.handle:
+            lib().hipq_w4_experts_destroy(self.handle)
+            self.handle, self._address = None, 0
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 def _bytes_like(t, count):
     import torch
     return torch.empty(count, dtype=torch.uint8, device=t.device)
@@ -719,6 +824,19 @@ def rotation_table(positions, rot, base=10000.0):
     angle = torch.arange(positions, dtype=torch.float64, device="cuda")[:, None] * float(base) ** -(
         torch.arange(0, rot, 2, dtype=torch.float64, device="cuda") / rot)
     return torch.cat((angle.cos(), angle.sin()), 1).float()
+
+
+def penalize(logits, tokens=None, lens=None, prompt_lens=None, repetition=None, frequency=None, presence=None, bias_tokens=None, bias=None, allowed=None, out=None):
+    """Scores for sample(): logits [rows, vocab] (float32, float16 or bfloat16) with penalties for tokens that have occurred, biases and a grammar's bits, to `out`
+    (may be logits) (include/hipq.h: hipq_penalize).  tokens: int32 [rows, longest], a row's first lens[row] count, the first prompt_lens[row] of them as its prompt;
+    repetition, frequency, presence: float32 [rows]; bias_tokens, bias: int32 and float32 [rows, entries]; allowed: int32 [rows, ceil(vocab / 32)].  Each may be None."""
+    calls = _CALLS or _calls()
+    if out is None:
+        out = logits.new_empty(logits.shape)
+    rc = calls.penalize(logits, out, tokens, lens, prompt_lens, repetition, frequency, presence, bias_tokens, bias, allowed)
+    if rc:
+        check(rc)
+    return out
 
 
 def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
