@@ -630,6 +630,48 @@ size_t hipq_kv_attend_workspace(const hipq_kv_cache *cache, const hipq_kv_attend
 int hipq_kv_attend(const hipq_kv_cache *cache, const hipq_kv_attend_desc *desc, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
+ * The attention that each token of the cache receives: for each of a sequence's tokens t and heads h
+ *   out[t][h] = (t before the new tokens ? weights[t][h] : 0) + sum of softmax_t(scale * q . k_t) over the new tokens' query heads that read h,
+ * with what hipq_kv_attend says of sequences, masks, scales and bounds, over the same tokens: its softmax.  weights and out lie in pages as the scales of a
+ * quantized cache do, float32 at ((p * heads + h) * page + t); out may be weights, otherwise it lies over none of it.  A page belongs to one sequence: of one that
+ * several have, the content afterwards means nothing.  A sequence without new tokens is left alone, as is what belongs to no sequence or lies behind its end.  A row
+ * that sees nothing adds nothing; one with a score of +infinity or NaN makes the weights of what it sees NaN.  Sums are over rows in a fixed order.
+ * workspace: as for hipq_kv_attend, hipq_kv_weigh_workspace bytes.
+ */
+typedef struct hipq_kv_weigh_desc {
+    const void *q;
+    int64_t q_token, q_head;
+    const int32_t *starts, *lens, *blocks;
+    const uint64_t *mask;
+    const float *weights;
+    float *out;
+    int64_t blocks_stride;
+    int32_t sequences, tokens, q_heads;
+    int32_t blocks_per_sequence, most_new, longest;
+    float scale;
+} hipq_kv_weigh_desc;
+size_t hipq_kv_weigh_workspace(const hipq_kv_cache *cache, const hipq_kv_weigh_desc *desc);
+int hipq_kv_weigh(const hipq_kv_cache *cache, const hipq_kv_weigh_desc *desc, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Holds every sequence to `budget` tokens.  One of more keeps, for each head on its own, its first `first` tokens, its last `recent` ones, and of those between them the
+ * heaviest (the first of equal ones; NaN below every number) until there are `budget`; one of no more keeps all.  The kept tokens, in their order, become
+ * tokens 0, 1, ... of the blocks to[b]: keys, values, scales and weights move there.  left[b] = min(lens[b], budget), the sequence's new length, may be lens[b]
+ * itself.  kept[b][h][j]: the place that token j had, -1 behind the last.
+ * to may be blocks (same stride): in place.  Otherwise none of its pages is one of any sequence's in blocks.  No page stands twice in either, so that a page that several
+ * sequences share is not to be evicted from.  A token whose block, or whose new one, lies outside the cache is not moved, and counts as one whose weight is NaN.
+ * Keys keep the rotation of the positions that they had.  Sequences' lengths count up to `longest`.  `to` holds at least min(budget, longest) tokens of a sequence.
+ */
+typedef struct hipq_kv_evict_desc {
+    float *weights;                     /* as for hipq_kv_weigh */
+    const int32_t *lens, *blocks, *to;  /* [sequences], [sequences][blocks_stride], [sequences][to_stride] */
+    int64_t blocks_stride, to_stride;
+    int32_t *kept, *left;               /* [sequences][heads][budget], [sequences] */
+    int32_t sequences, blocks_per_sequence, to_per_sequence, longest, budget, recent, first;
+} hipq_kv_evict_desc;
+int hipq_kv_evict(const hipq_kv_cache *cache, const hipq_kv_evict_desc *desc, void *stream);
+
+/*
  * A token of every row of scores (beside hipq_softmax_u8, which makes them probabilities).  With w_i = exp((x_i - max x) / temperature), and the
  * row's tokens ordered by score, equal ones by index, those are kept that
  *   are among the first top_k (top_k <= 0: all),

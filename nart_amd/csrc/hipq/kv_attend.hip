@@ -24,129 +24,11 @@
 // codes; the kernel without shared tiles takes 121, a third of its 360 for that).
 #include <type_traits>
 
-#include "real16.h"
+#include "kv_frag.h"
 
 namespace hipq {
 
-int check_cache(const hipq_kv_cache *c);
-
-struct AttendArgs {
-    hipq_kv_cache cache;
-    hipq_kv_attend_desc d;
-    float scale2;            // scale * log2(e)
-    int group, splits;       // query heads of a cache head; parts of a sequence
-    int row_blocks, rows;    // work-groups and rows (new tokens x group) of a sequence and cache head at most
-    uint32_t page_magic;     // of page / 16
-    int page_shift;
-    float *part_o, *part_ml; // [sequence][head][split][row][dim], [...][row][2]
-};
-
-// an address that is the same in all lanes, kept in scalar registers: a lane's part of it is then 32 bits that stay
-typedef const uint8_t __attribute__((address_space(1))) *gbytes_t;
-__device__ static __forceinline__ gbytes_t uniform(const void *p)
-{
-    gbytes_t g = (gbytes_t)p;
-    asm("" : "+s"(g));
-    return g;
-}
-template <class T>
-__device__ static __forceinline__ T at(gbytes_t p, uint32_t offset)
-{
-    return *(const __attribute__((address_space(1))) T *)(p + offset);
-}
-
-constexpr float NONE = -__builtin_inff();
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-
-// codes 0..7 of two dwords, as 16-bit floats
-template <int TYPE>
-__device__ static __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi)
-{
-    u32x4 o;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t w = i < 2 ? lo : hi;
-        o[i] = Real16<TYPE>::pack_exact((float)(int8_t)(w >> (16 * (i & 1))), (float)(int8_t)(w >> (16 * (i & 1) + 8)));
-    }
-    return o;
-}
-
-struct Sequence {
-    int row0, count, len, old; // first row of q, new tokens, tokens in the cache, those before the new ones
-    __device__ __forceinline__ Sequence(const AttendArgs &a, int b)
-    {
-        const int end = max(min(a.d.starts[b + 1], a.d.tokens), 0); // end - row0 fits whatever is in starts
-        row0 = max(a.d.starts[b], 0);
-        len = max(min(min(a.d.lens[b], a.d.longest), a.d.blocks_per_sequence * a.cache.page), 0);
-        count = max(min(end - row0, a.d.most_new), 0);
-        old = len - count;
-    }
-    // the tokens of a part: an equal share in whole rounds of the four waves
-    __device__ __forceinline__ int share(int splits) const { return ((len + splits - 1) / splits + 127) / 128 * 128; }
-};
-
-// a tile: two halves of 16 tokens, each in one page
-struct Pages {
-    int page[2]; // -1: not there
-    int place[2];
-};
-// where the tokens of a sequence lie
-struct Paging {
-    const int32_t *blocks;
-    int halves, page16, page, pages, heads, shift;
-    uint32_t magic;
-    __device__ __forceinline__ Paging(const AttendArgs &a, const int32_t *blocks_, int len)
-        : blocks(blocks_), halves((len + 15) / 16), page16(a.cache.page / 16), page(a.cache.page), pages(a.cache.pages), heads(a.cache.heads), shift(a.page_shift), magic(a.page_magic)
-    {
-    }
-    __device__ __forceinline__ Pages of(int t) const
-    {
-        Pages p;
-#pragma unroll
-        for (int s = 0; s < 2; s++) {
-            const int t16 = t / 16 + s;
-            const int at = magic ? (int)(((uint64_t)(uint32_t)t16 * magic) >> 32) >> shift : t16;
-            // through the scalar cache: behind a barrier the compiler would take a vector load, and wait for all those before it
-            const int number = __builtin_amdgcn_readfirstlane(t16 < halves ? ((const int32_t __attribute__((address_space(4))) *)(uintptr_t)blocks)[at] : -1);
-            p.page[s] = number >= 0 && number < pages ? number : -1;
-            p.place[s] = (t16 - at * page16) * 16;
-        }
-        return p;
-    }
-    // of a half's first token in the cache; some page's where there is none
-    __device__ __forceinline__ int64_t row(const Pages &p, int s, int h) const { return ((int64_t)max(p.page[s], 0) * heads + h) * page + p.place[s]; }
-    // All rows see a whole tile unless it holds a new token, the end, or a page that is not there; from the first such tile on each is looked
-    // at token by token.  Which that is, is found beforehand: a loop that ends on what it reads kept two sets of all its registers.
-    // The first token from t0 on that is not in a page, at most clear.
-    __device__ __forceinline__ int clear_until(int clear, int t0, int lane) const
-    {
-        for (int at = t0 / page + lane; (int64_t)at * page < clear; at += 64)
-            if (blocks[at] < 0 || blocks[at] >= pages)
-                clear = min(clear, at * page);
-#pragma unroll
-        for (int s = 1; s < 64; s *= 2)
-            clear = min(clear, __shfl_xor(clear, s));
-        return __builtin_amdgcn_readfirstlane(clear);
-    }
-};
-
-// a bit for each of a lane's 8 tokens of the tile at t: seen by new token `own` of the sequence
-__device__ static __forceinline__ uint32_t seen_by(const AttendArgs &a, const Sequence &seq, int own, int t, int j, const Pages &now)
-{
-    const uint64_t mask = a.d.mask ? a.d.mask[seq.row0 + own] : 0;
-    uint32_t sees = 0;
-#pragma unroll
-    for (int half = 0; half < 2; half++) { // four tokens from `first` on
-        const int first = t + half * 16 + j * 4, fresh = first - seq.old;
-        const int there = now.page[half] >= 0 ? min(max(seq.len - first, 0), 4) : 0;
-        uint32_t bits = (1u << min(max(own + 1 - fresh, 0), 4)) - 1;
-        if (a.d.mask)
-            bits = fresh >= 0 ? (uint32_t)(mask >> min(fresh, 63)) & (fresh < 64 ? 15u : 0u)
-                              : (uint32_t)mask << min(-fresh, 4) | ((1u << min(-fresh, 4)) - 1);
-        sees |= (bits & ((1u << there) - 1)) << (4 * half);
-    }
-    return sees;
-}
 
 // infinities or NaN among an operand's 16-bit values
 template <int TYPE>
@@ -834,22 +716,22 @@ struct AttendShape {
     size_t workspace;
 };
 
-static int check_attend(const hipq_kv_cache *c, const hipq_kv_attend_desc *d)
+int check_attend(const char *name, const hipq_kv_cache *c, const hipq_kv_attend_desc *d)
 {
     if (check_cache(c))
         return 1;
-    HIPQ_REQUIRE(d, "attend: a null pointer");
-    HIPQ_REQUIRE(d->sequences >= 0 && d->sequences <= (1 << 20), "attend: %d sequences", d->sequences);
-    HIPQ_REQUIRE(d->tokens >= 0 && d->tokens <= (1 << 24), "attend: %d new tokens", d->tokens);
-    HIPQ_REQUIRE(d->q_heads >= 1 && d->q_heads <= 65536 && d->q_heads % c->heads == 0, "attend: %d query heads on %d heads of the cache", d->q_heads, c->heads);
-    HIPQ_REQUIRE(d->most_new >= 0 && d->most_new <= (1 << 20), "attend: %d new tokens of a sequence", d->most_new);
-    HIPQ_REQUIRE(!d->mask || d->most_new <= 64, "attend: a mask has bits for 64 new tokens of a sequence, not %d", d->most_new);
-    HIPQ_REQUIRE(d->blocks_per_sequence >= 0 && (int64_t)d->blocks_per_sequence * c->page <= ((int64_t)1 << 30), "attend: %d blocks of a sequence", d->blocks_per_sequence);
-    HIPQ_REQUIRE(d->blocks_stride >= d->blocks_per_sequence || d->sequences <= 1, "attend: rows of blocks overlap");
-    HIPQ_REQUIRE(d->longest >= 0, "attend: the longest sequence has %d tokens", d->longest);
-    HIPQ_REQUIRE(d->scale > 0 && d->scale < 1e30f, "attend: scale %g", (double)d->scale);
+    HIPQ_REQUIRE(d, "%s: a null pointer", name);
+    HIPQ_REQUIRE(d->sequences >= 0 && d->sequences <= (1 << 20), "%s: %d sequences", name, d->sequences);
+    HIPQ_REQUIRE(d->tokens >= 0 && d->tokens <= (1 << 24), "%s: %d new tokens", name, d->tokens);
+    HIPQ_REQUIRE(d->q_heads >= 1 && d->q_heads <= 65536 && d->q_heads % c->heads == 0, "%s: %d query heads on %d heads of the cache", name, d->q_heads, c->heads);
+    HIPQ_REQUIRE(d->most_new >= 0 && d->most_new <= (1 << 20), "%s: %d new tokens of a sequence", name, d->most_new);
+    HIPQ_REQUIRE(!d->mask || d->most_new <= 64, "%s: a mask has bits for 64 new tokens of a sequence, not %d", name, d->most_new);
+    HIPQ_REQUIRE(d->blocks_per_sequence >= 0 && (int64_t)d->blocks_per_sequence * c->page <= ((int64_t)1 << 30), "%s: %d blocks of a sequence", name, d->blocks_per_sequence);
+    HIPQ_REQUIRE(d->blocks_stride >= d->blocks_per_sequence || d->sequences <= 1, "%s: rows of blocks overlap", name);
+    HIPQ_REQUIRE(d->longest >= 0, "%s: the longest sequence has %d tokens", name, d->longest);
+    HIPQ_REQUIRE(d->scale > 0 && d->scale < 1e30f, "%s: scale %g", name, (double)d->scale);
     const int64_t rows = (int64_t)d->most_new * (d->q_heads / c->heads);
-    HIPQ_REQUIRE(rows < (1 << 24), "attend: %lld rows of a sequence", (long long)rows);
+    HIPQ_REQUIRE(rows < (1 << 24), "%s: %lld rows of a sequence", name, (long long)rows);
     return 0;
 }
 
@@ -929,13 +811,13 @@ using namespace hipq;
 extern "C" size_t hipq_kv_attend_workspace(const hipq_kv_cache *cache, const hipq_kv_attend_desc *d)
 {
     clear_error();
-    return check_attend(cache, d) ? 0 : shape_of(cache, d).workspace;
+    return check_attend("attend", cache, d) ? 0 : shape_of(cache, d).workspace;
 }
 
 extern "C" int hipq_kv_attend(const hipq_kv_cache *cache, const hipq_kv_attend_desc *d, void *workspace, size_t workspace_bytes, void *stream)
 {
     clear_error();
-    if (check_attend(cache, d))
+    if (check_attend("attend", cache, d))
         return 1;
     const AttendShape s = shape_of(cache, d);
     const int64_t items = (int64_t)d->sequences * cache->heads * s.row_blocks;

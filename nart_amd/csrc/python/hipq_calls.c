@@ -729,6 +729,117 @@ static PyObject *py_kv_attend(ARGS)
     return PyLong_FromLong(rc);
 }
 
+/* a number of a longest sequence, or None: `capacity` */
+static int bounded(PyObject *o, int64_t capacity, int *out)
+{
+    *out = (int)capacity;
+    if (o != Py_None) {
+        const long long v = PyLong_AsLongLong(o);
+        if (v == -1 && PyErr_Occurred())
+            return 0;
+        *out = v < capacity ? (int)(v < -1 ? -1 : v) : (int)capacity;
+    }
+    return 1;
+}
+
+/* [pages][heads][page] of the cache */
+static int of_pages(const view_t *w, const char *name, const hipq_kv_cache *c) { return shaped(w, name, 3, c->pages, c->heads, c->page); }
+
+/* cache, its device, q, weights, out, starts, lens, blocks, mask or None, most_new, longest or None, scale, allocate: (bytes) -> uint8 tensor */
+static PyObject *py_kv_weigh(ARGS)
+{
+    (void)self;
+    hipq_kv_cache c;
+    hipq_kv_weigh_desc d;
+    view_t q, weights, out, starts, lens, blocks, mask, w;
+    int device;
+    void *st;
+    memset(&d, 0, sizeof d);
+    if (!expect(n, 13) || !current_device(&device) || !cache_device(a[1], device) || !tensor(a[2], "q", 3, HALVES, device, &q) || !cache_for(a[0], &q, &c)
+        || !whole_tensor(a[3], "weights", 3, 1u << F32, device, 0, &weights) || !whole_tensor(a[4], "out", 3, 1u << F32, device, 0, &out)
+        || !whole_tensor(a[5], "starts", 1, 1u << I32, device, 0, &starts) || !whole_tensor(a[6], "lens", 1, 1u << I32, device, 0, &lens)
+        || !tensor(a[7], "blocks", 2, 1u << I32, device, &blocks) || !whole_tensor(a[8], "mask", 1, 1u << I64, device, 1, &mask) || !number(a[11], &d.scale))
+        return NULL;
+    const long most_new = PyLong_AsLong(a[9]);
+    if (most_new == -1 && PyErr_Occurred())
+        return NULL;
+    d.most_new = most_new < -1 ? -1 : most_new > 0x7fffffff ? 0x7fffffff : (int)most_new;
+    const int64_t b = lens.shape[0], t = q.shape[0], capacity = blocks.shape[1] * c.page;
+    if (!shaped(&q, "q", 3, t, q.shape[1], c.dim) || !of_pages(&weights, "weights", &c) || !of_pages(&out, "out", &c) || !shaped(&starts, "starts", 1, b + 1, 0, 0)
+        || !shaped(&blocks, "blocks", 2, b, blocks.shape[1], 0) || !shaped(&mask, "mask", 1, t, 0, 0))
+        return NULL;
+    if (capacity > 0x7fffffff) {
+        PyErr_SetString(PyExc_ValueError, "blocks: a sequence has too many");
+        return NULL;
+    }
+    if (!bounded(a[10], capacity, &d.longest) || !current_stream(&st))
+        return NULL;
+    if (blocks.stride[0] == 0 && b > 1 && blocks.shape[1] > 0) {
+        PyErr_SetString(PyExc_ValueError, "blocks: rows overlap");
+        return NULL;
+    }
+    d.q = q.p, d.q_token = q.stride[0], d.q_head = q.stride[1], d.weights = weights.p, d.out = out.p;
+    d.starts = starts.p, d.lens = lens.p, d.blocks = blocks.p, d.mask = mask.p, d.blocks_stride = blocks.stride[0];
+    d.sequences = (int)b, d.tokens = (int)t, d.q_heads = (int)q.shape[1], d.blocks_per_sequence = (int)blocks.shape[1];
+    const size_t need = hipq_kv_weigh_workspace(&c, &d);
+    memset(&w, 0, sizeof w);
+    PyObject *workspace = NULL;
+    if (need > 0) {
+        PyObject *size = PyLong_FromSize_t(need);
+        workspace = size ? PyObject_CallOneArg(a[12], size) : NULL;
+        Py_XDECREF(size);
+        if (workspace == NULL)
+            return NULL;
+        if (!whole_tensor(workspace, "workspace", 1, 1u << U8, device, 0, &w)) {
+            Py_DECREF(workspace);
+            return NULL;
+        }
+    }
+    int rc;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = hipq_kv_weigh(&c, &d, w.p, (size_t)w.shape[0], st);
+    Py_END_ALLOW_THREADS;
+    Py_XDECREF(workspace);
+    return PyLong_FromLong(rc);
+}
+
+/* cache, its device, weights, lens, blocks, to, left, kept, budget, recent, first, longest or None */
+static PyObject *py_kv_evict(ARGS)
+{
+    (void)self;
+    hipq_kv_evict_desc d;
+    view_t weights, lens, blocks, to, left, kept;
+    int device;
+    void *st;
+    memset(&d, 0, sizeof d);
+    const hipq_kv_cache *c = n == 12 ? PyCapsule_GetPointer(a[0], "hipq_kv_cache") : NULL;
+    if (!expect(n, 12) || c == NULL || !current_device(&device) || !cache_device(a[1], device) || !whole_tensor(a[2], "weights", 3, 1u << F32, device, 0, &weights)
+        || !whole_tensor(a[3], "lens", 1, 1u << I32, device, 0, &lens) || !tensor(a[4], "blocks", 2, 1u << I32, device, &blocks)
+        || !tensor(a[5], "to", 2, 1u << I32, device, &to) || !whole_tensor(a[6], "left", 1, 1u << I32, device, 0, &left)
+        || !whole_tensor(a[7], "kept", 3, 1u << I32, device, 0, &kept) || !whole(a[8], &d.budget) || !whole(a[9], &d.recent) || !whole(a[10], &d.first))
+        return NULL;
+    const int64_t b = lens.shape[0], capacity = blocks.shape[1] * c->page;
+    if (!of_pages(&weights, "weights", c) || !shaped(&blocks, "blocks", 2, b, blocks.shape[1], 0) || !shaped(&to, "to", 2, b, to.shape[1], 0) || !shaped(&left, "left", 1, b, 0, 0)
+        || !shaped(&kept, "kept", 3, b, c->heads, d.budget))
+        return NULL;
+    if (capacity > 0x7fffffff) {
+        PyErr_SetString(PyExc_ValueError, "blocks: a sequence has too many");
+        return NULL;
+    }
+    if (!bounded(a[11], capacity, &d.longest) || !current_stream(&st))
+        return NULL;
+    if (b > 1 && ((blocks.stride[0] == 0 && blocks.shape[1] > 0) || (to.stride[0] == 0 && to.shape[1] > 0))) {
+        PyErr_SetString(PyExc_ValueError, "blocks: rows overlap");
+        return NULL;
+    }
+    hipq_kv_cache any = *c;
+    if (any.quantized)
+        any.type = BF16; /* codes are moved as they are */
+    d.weights = weights.p, d.lens = lens.p, d.blocks = blocks.p, d.to = to.p, d.left = left.p, d.kept = kept.p;
+    d.blocks_stride = blocks.stride[0], d.to_stride = to.stride[0], d.sequences = (int)b, d.blocks_per_sequence = (int)blocks.shape[1], d.to_per_sequence = (int)to.shape[1];
+    CALL(hipq_kv_evict(&any, &d, st));
+}
+
 /* logits, uniform, temperature, top_k, top_p, min_p (each or None), out */
 static PyObject *py_sample(ARGS)
 {
@@ -795,7 +906,7 @@ static PyMethodDef methods[] = {
     METHOD(init),        METHOD(conv2d_run),  METHOD(add_u8),      METHOD(eltwise_u8),    METHOD(relu_u8),       METHOD(concat_u8), METHOD(softmax_u8),
     METHOD(pool_u8),     METHOD(quantize_u8), METHOD(quantize_i8), METHOD(dequantize_u8), METHOD(dequantize_i8),
     METHOD(types),       METHOD(w4_workspace), METHOD(w4_run),     METHOD(experts_workspace), METHOD(experts_run), METHOD(kv_cache),      METHOD(kv_append),     METHOD(kv_attend), METHOD(sample),
-    METHOD(penalize),
+    METHOD(kv_weigh),    METHOD(kv_evict),    METHOD(penalize),
     {NULL, NULL, 0, NULL},
 };
 

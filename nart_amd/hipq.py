@@ -55,6 +55,17 @@ class KvAttendDesc(C.Structure):  # hipq_kv_attend_desc
         + [(n, C.c_int32) for n in ("sequences", "tokens", "q_heads", "blocks_per_sequence", "most_new", "longest")] + [("scale", C.c_float)]
 
 
+class KvWeighDesc(C.Structure):  # hipq_kv_weigh_desc
+    _fields_ = [("q", C.c_void_p)] + [(n, C.c_int64) for n in ("q_token", "q_head")] + [(n, C.c_void_p) for n in ("starts", "lens", "blocks", "mask", "weights", "out")] \
+        + [("blocks_stride", C.c_int64)] + [(n, C.c_int32) for n in ("sequences", "tokens", "q_heads", "blocks_per_sequence", "most_new", "longest")] + [("scale", C.c_float)]
+
+
+class KvEvictDesc(C.Structure):  # hipq_kv_evict_desc
+    _fields_ = [(n, C.c_void_p) for n in ("weights", "lens", "blocks", "to")] + [(n, C.c_int64) for n in ("blocks_stride", "to_stride")] \
+        + [(n, C.c_void_p) for n in ("kept", "left")] \
+        + [(n, C.c_int32) for n in ("sequences", "blocks_per_sequence", "to_per_sequence", "longest", "budget", "recent", "first")]
+
+
 class PenalizeDesc(C.Structure):  # hipq_penalize_desc
     _fields_ = [(n, C.c_void_p) for n in ("logits", "out")] + [(n, C.c_int64) for n in ("stride", "out_stride")] \
         + [(n, C.c_void_p) for n in ("tokens", "lens", "prompt_lens", "repetition", "frequency", "presence", "bias_tokens", "bias", "allowed")] \
@@ -156,6 +167,9 @@ _SIGS = {
     "hipq_kv_append": (C.c_int, [C.POINTER(KvCacheStruct), C.POINTER(KvAppendDesc), C.c_void_p]),
     "hipq_kv_attend_workspace": (C.c_size_t, [C.POINTER(KvCacheStruct), C.POINTER(KvAttendDesc)]),
     "hipq_kv_attend": (C.c_int, [C.POINTER(KvCacheStruct), C.POINTER(KvAttendDesc), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "hipq_kv_weigh_workspace": (C.c_size_t, [C.POINTER(KvCacheStruct), C.POINTER(KvWeighDesc)]),
+    "hipq_kv_weigh": (C.c_int, [C.POINTER(KvCacheStruct), C.POINTER(KvWeighDesc), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "hipq_kv_evict": (C.c_int, [C.POINTER(KvCacheStruct), C.POINTER(KvEvictDesc), C.c_void_p]),
     "hipq_penalize": (C.c_int, [C.POINTER(PenalizeDesc), C.c_void_p]),
     "hipq_sample": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int64] + [C.c_void_p] * 7),
 }
@@ -815,6 +829,35 @@ class KvCache:
         if rc:
             check(rc)
         return out
+
+
+    def weigh(self, q, starts, lens, blocks, most_new, weights, mask=None, scale=None, out=None, longest=None):
+        """The attention that every token of the cache receives from the new tokens q, added to `weights` float32 [pages, heads, page] (those of the new tokens begin
+        with it), in place or to `out`; the other arguments are attend()'s (include/hipq.h: hipq_kv_weigh)."""
+        calls = _CALLS or _calls()
+        if out is None:
+            out = weights
+        rc = calls.kv_weigh(self._struct, self._device, q, weights, out, starts, lens, blocks, mask, most_new, longest, self._scale if scale is None else scale,
+                            lambda count: _bytes_like(q, count))
+        if rc:
+            check(rc)
+        return out
+
+    def evict(self, weights, lens, blocks, budget, recent=0, first=0, to=None, longest=None, left=None, kept=None):
+        """Holds every sequence to `budget` tokens: its first `first`, its last `recent` and, for each head on its own, the heaviest of the others by `weights` float32
+        [pages, heads, page], moved in their order - with their weights - to the blocks `to` (int32 [sequences, blocks], other pages than the sequences'; None: in
+        place, to the front of their own).  Returns (left, kept): the new lengths, int32 [sequences], and the places that the kept tokens had, int32 [sequences, heads,
+        budget], -1 behind the last (include/hipq.h: hipq_kv_evict).  lens, blocks: int32; left may be lens."""
+        import torch
+        calls = _CALLS or _calls()
+        if left is None:
+            left = torch.empty(lens.shape, dtype=torch.int32, device=lens.device)
+        if kept is None:
+            kept = torch.empty((lens.shape[0], self.k.shape[1], budget), dtype=torch.int32, device=lens.device)
+        rc = calls.kv_evict(self._struct, self._device, weights, lens, blocks, blocks if to is None else to, left, kept, budget, recent, first, longest)
+        if rc:
+            check(rc)
+        return left, kept
 
 
 def rotation_table(positions, rot, base=10000.0):

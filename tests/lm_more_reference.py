@@ -95,3 +95,54 @@ def penalize(x, tokens=None, lens=None, prompt_lens=None, repetition=None, frequ
             y[r, bits == 0] = -np.inf
             off[r, bits == 0] = 0
     return torch.from_numpy(y), torch.from_numpy(off)
+
+
+def weigh(q, k, starts, lens, mask, scale, group, old, k_scale=None):
+    """[(weights [heads, len], how far)] of each sequence with new tokens, None of others: k: lists of [heads, len, dim] (codes with scales [heads, len]), old: of [heads, len]."""
+    got = []
+    dim = q.shape[-1]
+    for b, n in enumerate(lens):
+        lo, hi = starts[b], starts[b + 1]
+        new = hi - lo
+        if new == 0:
+            got.append(None)
+            continue
+        fresh = torch.arange(n, device=q.device) - (n - new)
+        row = torch.arange(new, device=q.device)[:, None]
+        seen = fresh <= row if mask is None else (fresh < 0) | (((mask[lo:hi, None] >> fresh.clamp(0, 63)) & 1) > 0)
+        before = torch.where(fresh < 0, old[b].double(), 0.0)
+        w, off = before.clone(), STEP32 * before.abs()
+        for h in range(k[b].shape[0]):
+            qs, kh = q[lo:hi, h * group:(h + 1) * group].double(), k[b][h].double()
+            ks = 1.0 if k_scale is None else k_scale[b][h].double()
+            x = torch.where(seen[:, None], (qs @ kh.t()) * ks * scale, -math.inf)
+            top = x.amax(-1, keepdim=True)
+            p = torch.exp(x - torch.where(top > -math.inf, top, 0.0))
+            p = p / torch.where(p.sum(-1, keepdim=True) > 0, p.sum(-1, keepdim=True), 1.0)
+            # a score's error is the relative error of its weight and, as largest of a row, of the sum (as for attention); the logarithm of the sum, and what is taken
+            # off in its place, are as large as the scores, and rounded
+            size = (qs.abs() @ kh.abs().t()) * ks * abs(scale)
+            d = (STEP32 * (dim + 10) * torch.where(seen[:, None], size, 0.0)).amax(-1, keepdim=True) + 2.0 ** -20
+            w[h] += p.sum((0, 1))
+            # sums of n terms in 32 bits, and of the rows
+            off[h] += (p * (3 * d + STEP32 * 64)).sum((0, 1)) + STEP32 * new * group * w[h].abs()
+        got.append((w, off))
+    return got
+
+
+def evict(weights, lens, budget, recent, first):
+    """For each sequence [heads, min(len, budget)]: the places of the tokens that stay.  weights: lists of [heads, len]."""
+    got = []
+    for w, n in zip(weights, lens):
+        rows = []
+        for h in range(w.shape[0]):
+            if n <= budget:
+                rows.append(np.arange(n))
+                continue
+            x = w[h].double().cpu().numpy()
+            middle = np.arange(first, n - recent)
+            key = np.where(np.isnan(x[middle]), -np.inf, x[middle])
+            order = np.lexsort((middle, -key, np.isnan(x[middle])))  # numbers before NaN, the heaviest first, of equal ones the first
+            rows.append(np.sort(np.concatenate((np.arange(first), middle[order[:budget - first - recent]], np.arange(n - recent, n)))))
+        got.append(np.stack(rows) if rows else np.zeros((0, 0), int))
+    return got

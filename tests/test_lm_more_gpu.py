@@ -257,3 +257,255 @@ def test_penalize_and_sample_in_a_graph():
         torch.cuda.synchronize()
         assert tokens[0] == only
         assert torch.equal(out, hipq.penalize(x, **kw)) and torch.equal(tokens, hipq.sample(out, uniform))
+
+
+# ---- the cache ----------------------------------------------------------------------------------------------------------
+class Sequences:
+    """Sequences of given lengths in a paged cache full of other things."""
+
+    def __init__(self, g, dtype, lens, heads, dim, page, int8, spare=3, more=0):
+        rng = np.random.default_rng(len(lens) + sum(lens))
+        self.lens, self.page, self.heads, self.dim = lens, page, heads, dim
+        per = max(1, -(-max(lens) // page)) + more
+        self.pages = len(lens) * per + spare
+        self.blocks = rng.permutation(self.pages)[:len(lens) * per].reshape(len(lens), per)
+        self.rest = np.setdiff1d(np.arange(self.pages), self.blocks)
+        shape = (self.pages, heads, page)
+        if int8:
+            k, v = (whole(g, -127, 128, torch.int8, *shape, dim) for _ in range(2))
+            self.scales = [torch.rand(shape, device="cuda", generator=g) * 0.02 + 0.002 for _ in range(2)]
+        else:
+            k, v = randn(g, dtype, *shape, dim), randn(g, dtype, *shape, dim)
+            self.scales = [None, None]
+        self.cache = hipq.KvCache(k, v, *self.scales)
+        self.weights = torch.exp(2 * randn(g, F32, *shape))
+        self.ints = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")  # noqa: E731
+
+    def of(self, pool, b):
+        """A sequence's tokens: [heads, len, ...]."""
+        n = self.lens[b]
+        x = pool[torch.from_numpy(self.blocks[b, :-(-n // self.page)]).long().cuda()]
+        return x.transpose(0, 1).reshape(self.heads, x.shape[0] * self.page, *x.shape[3:])[:, :n]
+
+    def all(self, pool):
+        return None if pool is None else [self.of(pool, b) for b in range(len(self.lens))]
+
+
+def check_weighed(g, s, dtype, counts, group, tree=False, scale=None, q_gap=0):
+    total = sum(counts)
+    q = randn(g, dtype, total + 2, s.heads * group + q_gap, s.dim)[:, :s.heads * group]  # rows of no sequence behind
+    starts = [0] + list(np.cumsum(counts))
+    mask = None
+    if tree:
+        rng = np.random.default_rng(total)
+        words = rng.integers(0, 2 ** 63, total + 2, dtype=np.int64)
+        words[::5] = 0  # rows that see no new token
+        mask = torch.from_numpy(words).cuda()
+    kw = dict(mask=mask, scale=scale)
+    before = s.weights.clone()
+    out = torch.full_like(before, 7.0)
+    got = s.cache.weigh(q, s.ints(starts), s.ints(s.lens), s.ints(s.blocks), max(counts), s.weights, out=out, **kw)
+    assert got is out and torch.equal(before, s.weights)
+    want = more.weigh(q, s.all(s.cache.k), starts, s.lens, mask, scale or s.dim ** -0.5, group, s.all(before), s.all(s.cache.k_scale))
+    left = torch.ones(before.shape, dtype=torch.bool, device="cuda")
+    for b, n in enumerate(s.lens):
+        if want[b] is None or n == 0:
+            continue
+        w, off = want[b]
+        have = s.of(out, b).double()
+        ok = (have - w).abs() <= off
+        assert ok.all(), "sequence %d: %g away, %g allowed" % (b, ((have - w).abs() - off).max() + off[~ok].max(), off[~ok].max())
+        for i, p in enumerate(s.blocks[b, :-(-n // s.page)]):
+            left[p, :, :min(s.page, n - i * s.page)] = False
+    assert (out[left] == 7).all()
+    again = s.cache.weigh(q, s.ints(starts), s.ints(s.lens), s.ints(s.blocks), max(counts), s.weights, **kw)  # in place
+    assert again is s.weights and torch.equal(again[~left], out[~left]) and torch.equal(again[left], before[left])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("lens, counts, heads, group, dim, page", [
+    ([1], [1], 1, 1, 64, 16), ([2, 33, 0, 17], [1, 1, 0, 1], 2, 4, 128, 16), ([700, 1, 90, 300], [1, 1, 0, 1], 2, 8, 64, 48), ([2500, 31], [3, 31], 1, 5, 128, 64),
+    ([64, 65, 300], [64, 40, 1], 2, 3, 256, 32), ([5000], [2], 3, 1, 256, 128), ([1300, 200], [100, 129], 1, 7, 128, 64), ([130, 20], [70, 20], 4, 16, 64, 16)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_weigh(lens, counts, heads, group, dim, page, int8, dtype, tree):
+    if tree and max(counts) > 64:
+        pytest.skip("a mask has 64 bits")
+    g = gen(sum(lens))
+    check_weighed(g, Sequences(g, dtype, lens, heads, dim, page, int8), dtype, counts, group, tree, scale=0.3 if dim == 64 else None, q_gap=group % 3)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("new, group", [(1, 2), (1, 16), (2, 16), (30, 4)])
+def test_weigh_long(new, group, int8):
+    """Sequences shared by work-groups, as many of them as there may be."""
+    g = gen(new)
+    check_weighed(g, Sequences(g, BF16, [70001, 16385, 40000], 1, 128, 64, int8), BF16, [new, new // 2 + 1, 1], group)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_weigh_blocks_outside(new):
+    """Tokens of blocks outside the cache are not there; lengths beyond `longest` and beyond the blocks end there."""
+    g = gen(2)
+    s = Sequences(g, BF16, [100, 90], 2, 64, 16, False)
+    q = randn(g, BF16, 2 * new, 2, 64)
+    starts, blocks = [0, new, 2 * new], s.blocks.copy()
+    blocks[0, 1], blocks[1, 2] = -1, s.pages
+    out = s.cache.weigh(q, s.ints(starts), s.ints(s.lens), s.ints(blocks), new, s.weights, out=torch.full_like(s.weights, 7.0))
+    gone = {0: 1, 1: 2}
+    for b in range(2):
+        keep = np.array([t for t in range(s.lens[b]) if t // 16 != gone[b]])
+        k, old = (s.of(x, b)[:, torch.from_numpy(keep).cuda()] for x in (s.cache.k, s.weights))
+        seen = torch.from_numpy(keep[None] - (s.lens[b] - new) <= np.arange(new)[:, None]).cuda()
+        for h in range(2):
+            x = torch.where(seen, q[starts[b]:starts[b + 1], h].double() @ k[h].double().t() / 8, -math.inf)
+            want = torch.softmax(x, -1).sum(0) + torch.where(torch.from_numpy(keep < s.lens[b] - new).cuda(), old[h].double(), 0.0)
+            assert ((s.of(out, b)[h, torch.from_numpy(keep).cuda()].double() - want).abs() <= 2.0 ** -17 * want).all()
+        page = torch.from_numpy(s.blocks[b, gone[b]:gone[b] + 1]).long().cuda()
+        assert (out[page] == 7).all()
+    short = s.cache.weigh(q, s.ints(starts), s.ints([1000, 1 << 30]), s.ints(s.blocks), new, s.weights, out=torch.full_like(s.weights, 7.0), longest=50)
+    s.lens = [50, 50]
+    same = s.cache.weigh(q, s.ints(starts), s.ints(s.lens), s.ints(s.blocks), new, s.weights, out=torch.full_like(s.weights, 7.0))
+    assert torch.equal(short, same)
+
+
+def test_weigh_rows_that_are_not_finite():
+    """A row of NaN makes the weights of what it sees NaN, and no others."""
+    g = gen(3)
+    for new in (2, 50):
+        s = Sequences(g, BF16, [200], 1, 64, 16, False)
+        q = randn(g, BF16, new, 1, 64)
+        q[0] = math.nan
+        s.cache.weigh(q, s.ints([0, new]), s.ints([200]), s.ints(s.blocks), new, s.weights)
+        got = s.of(s.weights, 0)[0]
+        assert torch.isnan(got[:200 - new + 1]).all() and torch.isfinite(got[200 - new + 1:]).all()
+
+
+def same(a, b):
+    """Equal, and NaN in the same places."""
+    return torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num()) if a.is_floating_point() else torch.equal(a, b)
+
+
+def check_evicted(s, budget, recent, first, in_place, longest=None):
+    pools = [p for p in (s.cache.k, s.cache.v, s.cache.k_scale, s.cache.v_scale, s.weights) if p is not None]
+    tokens = [s.all(p) for p in pools]
+    tokens = [[x.clone() for x in pool] for pool in tokens]
+    before = [p.clone() for p in pools]
+    lens = [min(n, longest) if longest else n for n in s.lens]
+    want = more.evict([w[:, :n] for w, n in zip(tokens[-1], lens)], lens, budget, recent, first)
+    need = -(-min(budget, max(max(lens), 1)) // s.page)
+    to = s.blocks if in_place else np.random.default_rng(1).permutation(s.rest)[:len(lens) * need].reshape(len(lens), need)
+    given = s.ints(s.lens)
+    blocks = s.ints(s.blocks)
+    left, kept = s.cache.evict(s.weights, given, blocks, budget, recent=recent, first=first, to=None if in_place else s.ints(to), longest=longest, left=given if in_place else None)
+    assert left.tolist() == [min(n, budget) for n in lens]
+    touched = torch.zeros((s.pages, s.heads, s.page), dtype=torch.bool, device="cuda")
+    for b, n in enumerate(lens):
+        many = min(n, budget)
+        assert (kept[b, :, many:] == -1).all()
+        assert np.array_equal(kept[b, :, :many].cpu().numpy(), want[b][:, :many])
+        if many == 0:
+            continue
+        j = np.arange(many)
+        at, place = torch.from_numpy(to[b][j // s.page]).long().cuda(), torch.from_numpy(j % s.page).cuda()
+        index = torch.from_numpy(want[b]).long().cuda()
+        touched[at, :, place] = True
+        for pool, mine in zip(pools, tokens):
+            have = pool[at, :, place].transpose(0, 1)
+            x = mine[b]
+            assert same(have, torch.gather(x, 1, index if x.dim() == 2 else index[..., None].expand(-1, -1, x.shape[2])))
+    for pool, was in zip(pools, before):
+        assert same(pool[~touched], was[~touched])
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("lens, budget, recent, first, heads, dim, page", [
+    ([1], 1, 0, 0, 1, 64, 16), ([5, 0, 40], 4, 1, 1, 2, 64, 16), ([300, 17, 100, 101], 100, 30, 4, 3, 128, 48), ([1000, 2000], 999, 999, 0, 1, 128, 64), ([700], 50, 0, 50, 2, 256, 16),
+    ([5000, 4097, 9000], 4096, 100, 3, 2, 64, 128), ([20000], 19999, 5000, 0, 1, 128, 32), ([40000, 33000], 3001, 17, 0, 2, 64, 64), ([100], 700, 20, 4, 2, 128, 16)])
+def test_evict(lens, budget, recent, first, heads, dim, page, int8, in_place):
+    g = gen(sum(lens))
+    s = Sequences(g, BF16, lens, heads, dim, page, int8, spare=len(lens) * (-(-budget // page) + 1))
+    check_evicted(s, budget, recent, first, in_place)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("what", ["equal", "few values", "zeros", "not finite", "either sign", "close"])
+def test_evict_ties(what, in_place):
+    g = gen(9)
+    s = Sequences(g, F16, [6000, 501, 77], 2, 64, 32, False, spare=60)
+    w = s.weights
+    if what == "equal":
+        w.fill_(0.25)
+    elif what == "few values":
+        w.copy_(whole(g, 0, 3, torch.int32, *w.shape).float())
+    elif what == "zeros":
+        w.copy_(torch.where(torch.rand(w.shape, device="cuda", generator=g) < 0.97, 0.0, w))
+        w[::2] *= -1  # zeros of either sign are equal
+    elif what == "not finite":
+        u = torch.rand(w.shape, device="cuda", generator=g)
+        w.copy_(torch.where(u < 0.3, math.nan, torch.where(u < 0.8, -math.inf, torch.where(u < 0.85, math.inf, w))))
+    elif what == "either sign":
+        w.copy_(randn(g, F32, *w.shape))
+    else:
+        w.copy_(1 + whole(g, 0, 200, torch.int32, *w.shape).float() * 2.0 ** -23)
+    check_evicted(s, 500, 20, 5, in_place)
+
+
+def test_evict_longest_and_blocks_outside():
+    g = gen(4)
+    s = Sequences(g, BF16, [300, 200], 2, 64, 16, False, spare=40)
+    check_evicted(s, 40, 5, 0, False, longest=100)
+    # tokens of blocks that are not there are the lightest, and are not moved
+    s = Sequences(g, BF16, [300, 200], 1, 64, 16, False, spare=40)
+    blocks, to = s.blocks.copy(), s.rest[:8].reshape(2, 4)
+    blocks[0, 2], blocks[1, 12] = -1, s.pages + 7
+    to[1, 0] = -5
+    before = s.weights.clone()
+    w = [s.of(before, b).clone() for b in range(2)]
+    w[0][:, 32:48] = math.nan
+    w[1][:, 192:] = math.nan
+    want = more.evict(w, s.lens, 64, 10, 0)
+    left, kept = s.cache.evict(s.weights, s.ints(s.lens), s.ints(blocks), 64, recent=10, to=s.ints(to))
+    assert left.tolist() == [64, 64] and all(np.array_equal(kept[b].cpu().numpy(), want[b]) for b in range(2))
+    changed = (s.weights != before).any(-1).any(-1).nonzero().flatten().tolist()
+    assert set(changed) <= set(to.flatten().tolist()) - {-5}
+    for j in range(16, 64):  # of the second sequence, in blocks that are there
+        t = want[1][0, j]
+        if t < 192:
+            assert s.weights[int(to[1, j // 16]), 0, j % 16] == w[1][0, t]
+
+
+def test_weigh_and_evict_in_a_graph():
+    """A step of a conversation, captured: attention, its weights, and every few steps the budget; replayed with other tokens it gives what eager calls give."""
+    g = gen(6)
+    s = Sequences(g, BF16, [400, 90], 2, 128, 16, False)
+    q, starts, lens, blocks = randn(g, BF16, 2, 8, 128), s.ints([0, 1, 2]), s.ints(s.lens), s.ints(s.blocks)
+    out, kept = torch.zeros_like(q), torch.zeros((2, 2, 64), dtype=torch.int32, device="cuda")
+    pools = (s.cache.k, s.cache.v, s.weights, lens)
+    start = [p.clone() for p in pools]
+
+    def step():
+        s.cache.attend(q, starts, lens, blocks, 1, out=out)
+        s.cache.weigh(q, starts, lens, blocks, 1, s.weights)
+        s.cache.evict(s.weights, lens, blocks, 64, recent=8, left=lens, kept=kept)
+
+    def reset():
+        for p, was in zip(pools, start):
+            p.copy_(was)
+    step()
+    reset()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(4):
+        q.copy_(randn(g, BF16, 2, 8, 128))
+        reset()
+        step()
+        want = [p.clone() for p in (*pools, out, kept)]
+        reset()
+        out.zero_(), kept.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((*pools, out, kept), want))
+        assert lens.tolist() == [64, 64]
