@@ -661,6 +661,7 @@ int hipq_kv_weigh(const hipq_kv_cache *cache, const hipq_kv_weigh_desc *desc, vo
  * to may be blocks (same stride): in place.  Otherwise none of its pages is one of any sequence's in blocks.  No page stands twice in either, so that a page that several
  * sequences share is not to be evicted from.  A token whose block, or whose new one, lies outside the cache is not moved, and counts as one whose weight is NaN.
  * Keys keep the rotation of the positions that they had.  Sequences' lengths count up to `longest`.  `to` holds at least min(budget, longest) tokens of a sequence.
+ * workspace: as for hipq_kv_attend, hipq_kv_evict_workspace bytes.
  */
 typedef struct hipq_kv_evict_desc {
     float *weights;                     /* as for hipq_kv_weigh */
@@ -669,7 +670,8 @@ typedef struct hipq_kv_evict_desc {
     int32_t *kept, *left;               /* [sequences][heads][budget], [sequences] */
     int32_t sequences, blocks_per_sequence, to_per_sequence, longest, budget, recent, first;
 } hipq_kv_evict_desc;
-int hipq_kv_evict(const hipq_kv_cache *cache, const hipq_kv_evict_desc *desc, void *stream);
+size_t hipq_kv_evict_workspace(const hipq_kv_cache *cache, const hipq_kv_evict_desc *desc);
+int hipq_kv_evict(const hipq_kv_cache *cache, const hipq_kv_evict_desc *desc, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
  * A token of every row of scores (beside hipq_softmax_u8, which makes them probabilities).  With w_i = exp((x_i - max x) / temperature), and the

@@ -1,8 +1,8 @@
 // A paged cache held to a budget (hipq_kv_evict): of every sequence and head the first, the last and the heaviest tokens stay.  gfx950 only.
 //
-// Two launches.  The first finds a sequence's and head's tokens: a work-group looks for the weight with which the budget is used up, digit by digit of the
-// weights' bits (counts in LDS, which are integers, so that the order does not matter), and writes the kept ones' places in their order; of equal weights the first
-// tokens stay.  The second moves them.  In place a token moves to the front or not at all, so that work-groups may each have a stretch of the heads' width
+// First a sequence's and head's tokens are chosen: a work-group looks for the weight with which the budget is used up, digit by digit of the weights' bits (counts
+// in LDS, which are integers, so that the order does not matter), and writes the kept ones' places in their order; of equal weights the first tokens stay.  The next
+// launch moves them.  In place a token moves to the front or not at all, so that work-groups may each have a stretch of the heads' width
 // and go through the tokens in order: what a step reads lies behind all that steps before it have written.  Into other pages the tokens are shared out as well.
 #include "real16.h"
 
@@ -15,7 +15,10 @@ struct EvictArgs {
     hipq_kv_evict_desc d;
     uint32_t page_magic; // of page / 16
     int page_shift;
-    int parts, kinds;    // of the second launch: work-groups that share the tokens, and those that share a token's row
+    int parts, kinds;    // moving: work-groups that share the tokens, and those that share a token's row
+    // choosing by several work-groups, `chunks` for a sequence and head
+    int chunks;
+    uint32_t *hist, *above, *found; // [digit][sequence and head][chunk][bin], [digit][..][chunk], [digit][..][2]
 };
 
 // 0: a NaN, or in no page; otherwise in the order of the weights
@@ -37,109 +40,249 @@ __device__ static __forceinline__ int length(const EvictArgs &a, int b)
     return max(min(min(a.d.lens[b], a.d.longest), a.d.blocks_per_sequence * a.cache.page), 0);
 }
 
-constexpr int CHOOSERS = 1024, BINS = 2048;
+constexpr int CHOOSERS = 1024, BINS = 2048, DIGITS = 3;
+__device__ static __forceinline__ int digit_of(int pass) { return pass < 2 ? 11 : 10; }
+__device__ static __forceinline__ int shift_of(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
 
+// What a sequence and head has to keep: of tokens lo..hi - 1 the `want` heaviest, and all others.
+struct Middle {
+    int len, lo, hi, want;
+    __device__ __forceinline__ Middle(const EvictArgs &a, int b) : len(length(a, b)), lo(a.d.first), hi(len - a.d.recent), want(a.d.budget - a.d.first - a.d.recent) {}
+};
+
+// Ranks of four tokens from t on (a multiple of four); what is no middle token has 0 as well.
+__device__ static __forceinline__ void ranks_of(const EvictArgs &a, const Middle &m, const int32_t *blocks, int h, int t, uint32_t (&rank)[4])
+{
+    f32x4 w = {0, 0, 0, 0};
+    int64_t at = -1;
+    if (t < m.hi && t + 4 > m.lo) {
+        at = row_of(a, blocks, h, t);
+        if (at >= 0)
+            w = *(const f32x4 *)(a.d.weights + at);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        rank[e] = at >= 0 ? rank_of(w[e]) : 0;
+}
+
+struct Found {
+    uint32_t bin, left;
+};
+// The bin in which the `left`-th largest is, and how many of that bin's are among them: thread i brings the numbers of bins BINS - 1 - 2 i and BINS - 2 - 2 i.
+__device__ static __forceinline__ Found find_bin(uint32_t n0, uint32_t n1, uint32_t left, uint32_t (&totals)[16], uint32_t (&found)[2])
+{
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t run = n0 + n1;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const uint32_t u = (uint32_t)__shfl_up((int)run, o);
+        run += lane >= o ? u : 0;
+    }
+    if (lane == 63)
+        totals[wave] = run;
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < 16; v++)
+        run += v < wave ? totals[v] : 0;
+    const uint32_t before = run - n0 - n1;
+    if (before < left && left <= before + n0)
+        found[0] = BINS - 1 - 2 * tid, found[1] = left - before;
+    else if (before + n0 < left && left <= run)
+        found[0] = BINS - 2 - 2 * tid, found[1] = left - before - n0;
+    __syncthreads();
+    const Found f = {found[0], found[1]};
+    __syncthreads();
+    return f;
+}
+
+// a number of each thread's, summed over the work-group
+__device__ static __forceinline__ uint32_t sum_of(uint32_t n, uint32_t (&totals)[16])
+{
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2)
+        n += (uint32_t)__shfl_xor((int)n, o);
+    if ((threadIdx.x & 63) == 0)
+        totals[threadIdx.x >> 6] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int v = 0; v < 16; v++)
+        n += totals[v];
+    __syncthreads();
+    return n;
+}
+
+// Writes the kept of four tokens a thread: the forced ones, those above the border, and of those at it the first `left`.  above, equal: how many there are before these
+// 4096, and behind them afterwards.
+__device__ static __forceinline__ void write_kept(const Middle &m, int t, const uint32_t (&rank)[4], uint32_t border, uint32_t left, uint32_t &above, uint32_t &equal,
+                                                  int32_t *kept, uint32_t (&totals)[16])
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t is[4], mine = 0; // above in the lower half, equal in the upper one
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const bool middle = t + e >= m.lo && t + e < m.hi;
+        is[e] = t + e >= m.len ? 0u : !middle ? 1u : m.want == 0 ? 0u : rank[e] > border ? 1u : rank[e] == border ? 1u << 16 : 0u;
+        mine += is[e];
+    }
+    uint32_t run = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const uint32_t u = (uint32_t)__shfl_up((int)run, o);
+        run += lane >= o ? u : 0;
+    }
+    if (lane == 63)
+        totals[wave] = run;
+    __syncthreads();
+    uint32_t all = 0, over = 0;
+#pragma unroll
+    for (int v = 0; v < 16; v++) {
+        over += v < wave ? totals[v] : 0;
+        all += totals[v];
+    }
+    const uint32_t start = over + run - mine;
+    uint32_t g = above + (start & 0xffff), q = equal + (start >> 16);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if (is[e] == 1 || (is[e] && q < left))
+            kept[g + min(q, left)] = t + e;
+        g += is[e] & 0xffff, q += is[e] >> 16;
+    }
+    above += all & 0xffff, equal += all >> 16;
+    __syncthreads();
+}
+
+__device__ static __forceinline__ void keep_all(const EvictArgs &a, int len, int32_t *kept)
+{
+    for (int j = threadIdx.x; j < a.d.budget; j += CHOOSERS)
+        kept[j] = j < len ? j : -1;
+}
+
+// A work-group for a sequence and head of up to 4096 HELD tokens, whose ranks stay in registers.
+template <int HELD>
 __global__ __launch_bounds__(CHOOSERS) void kv_choose_kernel(const EvictArgs a)
 {
     __shared__ uint32_t bins[BINS], totals[16], found[2];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int h = blockIdx.x % a.cache.heads, b = blockIdx.x / a.cache.heads, len = length(a, b), budget = a.d.budget;
-    int32_t *const kept = a.d.kept + (int64_t)blockIdx.x * budget;
-    if (len <= budget) {
-        for (int j = tid; j < budget; j += CHOOSERS)
-            kept[j] = j < len ? j : -1;
-        return;
-    }
+    const int tid = threadIdx.x, h = blockIdx.x % a.cache.heads, b = blockIdx.x / a.cache.heads;
+    int32_t *const kept = a.d.kept + (int64_t)blockIdx.x * a.d.budget;
+    const Middle m(a, b);
+    if (m.len <= a.d.budget)
+        return keep_all(a, m.len, kept);
     const int32_t *const blocks = a.d.blocks + (int64_t)b * a.d.blocks_stride;
-    const int lo = a.d.first, hi = len - a.d.recent, want = budget - a.d.first - a.d.recent; // of tokens lo .. hi - 1, which are more than that
-    auto four = [&](int t, uint32_t (&rank)[4]) __attribute__((always_inline)) { // of tokens t..t + 3
-        const int64_t at = row_of(a, blocks, h, t);
-        const f32x4 w = at < 0 ? f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")} : *(const f32x4 *)(a.d.weights + at);
+    uint32_t rank[HELD][4];
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            rank[e] = rank_of(w[e]);
-    };
-    // the rank of the last one that stays, from its highest digit on, and how many of those with that rank stay
-    uint32_t border = 0, left = (uint32_t)want;
-    int known = 0; // bits
-    while (known < 32 && left > 0) {
-        const int digit = known < 22 ? 11 : 10, shift = 32 - known - digit;
+    for (int i = 0; i < HELD; i++)
+        ranks_of(a, m, blocks, h, (i * CHOOSERS + tid) * 4, rank[i]);
+    uint32_t border = 0, left = (uint32_t)m.want;
+    for (int pass = 0; pass < DIGITS && m.want > 0; pass++) {
+        const int digit = digit_of(pass), shift = shift_of(pass);
         for (int i = tid; i < BINS; i += CHOOSERS)
             bins[i] = 0;
         __syncthreads();
-        for (int t = (lo & ~3) + tid * 4; t < hi; t += CHOOSERS * 4) {
-            uint32_t rank[4];
-            four(t, rank);
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (t + e >= lo && t + e < hi && (known == 0 || (rank[e] >> (32 - known)) == border))
-                    atomicAdd(&bins[(rank[e] >> shift) & ((1u << digit) - 1)], 1u);
-        }
-        __syncthreads();
-        // the bin in which the number wanted is reached, from the highest on: thread i has bins 2 i and 2 i + 1 from above
-        const uint32_t n0 = bins[BINS - 1 - 2 * tid], n1 = bins[BINS - 2 - 2 * tid];
-        uint32_t run = n0 + n1;
+        for (int i = 0; i < HELD; i++)
 #pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const uint32_t u = (uint32_t)__shfl_up((int)run, o);
-            run += lane >= o ? u : 0;
-        }
-        if (lane == 63)
-            totals[wave] = run;
+            for (int e = 0; e < 4; e++) {
+                const int t = (i * CHOOSERS + tid) * 4 + e;
+                if (t >= m.lo && t < m.hi && (pass == 0 || rank[i][e] >> (shift + digit) == border))
+                    atomicAdd(&bins[(rank[i][e] >> shift) & ((1u << digit) - 1)], 1u);
+            }
         __syncthreads();
-        for (int v = 0; v < wave; v++)
-            run += totals[v];
-        const uint32_t before = run - n0 - n1;
-        if (before < left && left <= before + n0)
-            found[0] = BINS - 1 - 2 * tid, found[1] = left - before;
-        else if (before + n0 < left && left <= run)
-            found[0] = BINS - 2 - 2 * tid, found[1] = left - before - n0;
-        __syncthreads();
-        border = border << digit | found[0];
-        left = found[1];
-        known += digit;
-        __syncthreads();
+        const Found f = find_bin(bins[BINS - 1 - 2 * tid], bins[BINS - 2 - 2 * tid], left, totals, found);
+        border = border << digit | f.bin, left = f.left;
     }
-    // kept: the forced ones, those above the border, and the first `left` of those at it
-    const bool none = want == 0;
-    uint32_t above = 0, equal = 0; // so far, of all waves
-    for (int t0 = 0; t0 < len; t0 += CHOOSERS * 4) {
-        const int t = t0 + tid * 4;
-        uint32_t rank[4] = {0, 0, 0, 0}, mine = 0; // above in the lower half, equal in the upper one
-        if (t < hi && t + 4 > lo)
-            four(t, rank);
-        uint32_t is[4];
+    uint32_t above = 0, equal = 0;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const bool middle = t + e >= lo && t + e < hi;
-            is[e] = t + e >= len ? 0u : !middle || (!none && rank[e] > border) ? 1u : !none && rank[e] == border ? 1u << 16 : 0u;
-            mine += is[e];
-        }
-        uint32_t run = mine;
+    for (int i = 0; i < HELD; i++)
+        if (i * CHOOSERS * 4 < m.len)
+            write_kept(m, (i * CHOOSERS + tid) * 4, rank[i], border, left, above, equal, kept, totals);
+}
+
+// The same for longer ones, shared by work-groups of 4096 QUADS tokens each: a launch for each digit, which leaves the part's numbers of every bin, and one that writes.
+// Every work-group finds the bins from all parts' numbers itself; what was found of earlier digits, and how many of a part's tokens are above them, the launches pass on.
+constexpr int QUADS = 2;
+template <int PASS>
+__global__ __launch_bounds__(CHOOSERS) void kv_rank_kernel(const EvictArgs a)
+{
+    __shared__ uint32_t bins[BINS], totals[16], found[2];
+    const int tid = threadIdx.x, part = blockIdx.x % a.chunks, bh = blockIdx.x / a.chunks, h = bh % a.cache.heads, b = bh / a.cache.heads;
+    const int heads = a.d.sequences * a.cache.heads, from = part * (QUADS * CHOOSERS * 4);
+    const Middle m(a, b);
+    int32_t *const kept = a.d.kept + (int64_t)bh * a.d.budget;
+    if (m.len <= a.d.budget) {
+        if (PASS == DIGITS && part == 0)
+            keep_all(a, m.len, kept);
+        return;
+    }
+    const int parts = (m.len + QUADS * CHOOSERS * 4 - 1) / (QUADS * CHOOSERS * 4); // of this sequence
+    if (part >= parts || (m.want == 0 && PASS < DIGITS))
+        return;
+    const int32_t *const blocks = a.d.blocks + (int64_t)b * a.d.blocks_stride;
+    uint32_t rank[QUADS][4];
 #pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const uint32_t u = (uint32_t)__shfl_up((int)run, o);
-            run += lane >= o ? u : 0;
+    for (int i = 0; i < QUADS; i++)
+        ranks_of(a, m, blocks, h, from + (i * CHOOSERS + tid) * 4, rank[i]);
+    uint32_t border = 0, left = (uint32_t)m.want, before = 0, equal_before = 0;
+    if (PASS > 0 && m.want > 0) {
+        if (PASS > 1)
+            border = a.found[2 * ((PASS - 2) * heads + bh)], left = a.found[2 * ((PASS - 2) * heads + bh) + 1];
+        const u32x2 *const hist = (const u32x2 *)(a.hist + ((int64_t)((PASS - 1) * heads + bh) * a.chunks) * BINS) + BINS / 2 - 1 - tid;
+        u32x2 all = {0, 0}, ours = {0, 0};
+#pragma unroll 8
+        for (int p = 0; p < parts; p++) {
+            const u32x2 n = hist[(int64_t)p * (BINS / 2)];
+            all += n;
+            if (PASS == DIGITS && p < part)
+                ours += n;
         }
-        if (lane == 63)
-            totals[wave] = run;
+        const Found f = find_bin(all[1], all[0], left, totals, found);
+        constexpr int digit = PASS - 1 < 2 ? 11 : 10;
+        if (PASS == DIGITS) {
+            const uint32_t b1 = BINS - 1 - 2 * tid, b0 = b1 - 1;
+            before = sum_of((b1 > f.bin ? ours[1] : 0) + (b0 > f.bin ? ours[0] : 0), totals);
+            equal_before = sum_of((b1 == f.bin ? ours[1] : 0) + (b0 == f.bin ? ours[0] : 0), totals);
+            for (int p = 0; p < part; p++)
+                before += a.above[(int64_t)bh * a.chunks + p] + a.above[(int64_t)(heads + bh) * a.chunks + p];
+        }
+        border = border << digit | f.bin, left = f.left;
+        if (PASS < DIGITS) {
+            if (part == 0 && tid == 0)
+                a.found[2 * ((PASS - 1) * heads + bh)] = border, a.found[2 * ((PASS - 1) * heads + bh) + 1] = left;
+            uint32_t n = 0; // above the border in this digit, at it in those before
+            constexpr int shift = PASS == 1 ? 21 : 10;
+#pragma unroll
+            for (int i = 0; i < QUADS; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int t = from + (i * CHOOSERS + tid) * 4 + e;
+                    const uint32_t r = rank[i][e] >> shift;
+                    n += t >= m.lo && t < m.hi && r > border && (PASS == 1 || r >> 11 == border >> 11) ? 1 : 0;
+                }
+            n = sum_of(n, totals);
+            if (tid == 0)
+                a.above[(int64_t)((PASS - 1) * heads + bh) * a.chunks + part] = n;
+        }
+    }
+    if constexpr (PASS < DIGITS) {
+        constexpr int digit = PASS < 2 ? 11 : 10, shift = PASS == 0 ? 21 : PASS == 1 ? 10 : 0;
+        for (int i = tid; i < BINS; i += CHOOSERS)
+            bins[i] = 0;
         __syncthreads();
-        uint32_t all = 0, over = 0;
 #pragma unroll
-        for (int v = 0; v < 16; v++) {
-            over += v < wave ? totals[v] : 0;
-            all += totals[v];
-        }
-        const uint32_t start = over + run - mine;
-        uint32_t g = above + (start & 0xffff), q = equal + (start >> 16);
+        for (int i = 0; i < QUADS; i++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (is[e] == 1 || (is[e] && q < left))
-                kept[g + min(q, left)] = t + e;
-            g += is[e] & 0xffff, q += is[e] >> 16;
-        }
-        above += all & 0xffff, equal += all >> 16;
+            for (int e = 0; e < 4; e++) {
+                const int t = from + (i * CHOOSERS + tid) * 4 + e;
+                if (t >= m.lo && t < m.hi && (PASS == 0 || rank[i][e] >> ((shift + digit) & 31) == border))
+                    atomicAdd(&bins[(rank[i][e] >> shift) & ((1u << digit) - 1)], 1u);
+            }
         __syncthreads();
+        ((u32x2 *)(a.hist + ((int64_t)(PASS * heads + bh) * a.chunks + part) * BINS))[tid] = ((const u32x2 *)bins)[tid];
+    } else {
+        uint32_t above = before + min(from, m.lo) + max(from - m.hi, 0);
+#pragma unroll
+        for (int i = 0; i < QUADS; i++)
+            write_kept(m, from + (i * CHOOSERS + tid) * 4, rank[i], border, left, above, equal_before, kept, totals);
     }
 }
 
@@ -204,6 +347,29 @@ __global__ __launch_bounds__(MOVERS) void kv_move_kernel(const EvictArgs a)
         }
 }
 
+static int choose(const EvictArgs &a, int64_t longest, hipStream_t st)
+{
+    const unsigned heads = (unsigned)(a.d.sequences * a.cache.heads);
+    if (a.chunks == 1) {
+        if (longest <= 4 * CHOOSERS || longest <= a.d.budget)
+            kv_choose_kernel<1><<<dim3(heads), dim3(CHOOSERS), 0, st>>>(a);
+        else
+            kv_choose_kernel<4><<<dim3(heads), dim3(CHOOSERS), 0, st>>>(a);
+        return launch_status("kv_choose_kernel");
+    }
+    kv_rank_kernel<0><<<dim3(heads * a.chunks), dim3(CHOOSERS), 0, st>>>(a);
+    if (launch_status("kv_rank_kernel"))
+        return 1;
+    kv_rank_kernel<1><<<dim3(heads * a.chunks), dim3(CHOOSERS), 0, st>>>(a);
+    if (launch_status("kv_rank_kernel"))
+        return 1;
+    kv_rank_kernel<2><<<dim3(heads * a.chunks), dim3(CHOOSERS), 0, st>>>(a);
+    if (launch_status("kv_rank_kernel"))
+        return 1;
+    kv_rank_kernel<3><<<dim3(heads * a.chunks), dim3(CHOOSERS), 0, st>>>(a);
+    return launch_status("kv_rank_kernel");
+}
+
 template <int STRETCH>
 static int launch_move(EvictArgs &a, bool in_place, hipStream_t st)
 {
@@ -221,9 +387,28 @@ static int launch_move(EvictArgs &a, bool in_place, hipStream_t st)
 
 using namespace hipq;
 
-extern "C" int hipq_kv_evict(const hipq_kv_cache *cache, const hipq_kv_evict_desc *d, void *stream)
+namespace hipq {
+
+struct EvictShape {
+    int chunks; // 1: one work-group chooses
+    size_t hist, above, workspace;
+};
+
+static EvictShape shape_of(const hipq_kv_cache *c, const hipq_kv_evict_desc *d)
 {
-    clear_error();
+    const int64_t tokens = (int64_t)d->blocks_per_sequence * c->page, longest = d->longest < tokens ? d->longest : tokens;
+    const size_t heads = (size_t)d->sequences * c->heads;
+    EvictShape s = {1, 0, 0, 0};
+    if (longest > 4 * 4 * CHOOSERS && longest > d->budget) {
+        s.chunks = (int)((longest + QUADS * CHOOSERS * 4 - 1) / (QUADS * CHOOSERS * 4));
+        s.hist = heads * DIGITS * s.chunks * BINS * 4, s.above = s.hist + (heads * 2 * s.chunks * 4 + 15) / 16 * 16;
+        s.workspace = s.above + heads * 2 * 2 * 4;
+    }
+    return s;
+}
+
+static int check_evict(const hipq_kv_cache *cache, const hipq_kv_evict_desc *d)
+{
     if (check_cache(cache))
         return 1;
     HIPQ_REQUIRE(d, "evict: a null pointer");
@@ -238,19 +423,39 @@ extern "C" int hipq_kv_evict(const hipq_kv_cache *cache, const hipq_kv_evict_des
     HIPQ_REQUIRE(!in_place || (d->to_stride == d->blocks_stride && d->to_per_sequence <= d->blocks_per_sequence) || d->sequences <= 1, "evict: in place the blocks are the same");
     const int64_t tokens = (int64_t)d->blocks_per_sequence * cache->page, longest = d->longest < tokens ? d->longest : tokens, most = d->budget < longest ? d->budget : longest;
     HIPQ_REQUIRE(d->to_per_sequence >= 0 && (int64_t)d->to_per_sequence * cache->page >= most, "evict: %d blocks for %lld tokens that stay", d->to_per_sequence, (long long)most);
+    // of 2^32 work-items and more only what is left over would run
+    HIPQ_REQUIRE((int64_t)d->sequences * cache->heads * shape_of(cache, d).chunks < (1 << 22), "evict: %d sequences of %d heads", d->sequences, cache->heads);
+    return 0;
+}
+
+} // namespace hipq
+
+extern "C" size_t hipq_kv_evict_workspace(const hipq_kv_cache *cache, const hipq_kv_evict_desc *d)
+{
+    clear_error();
+    return check_evict(cache, d) ? 0 : shape_of(cache, d).workspace;
+}
+
+extern "C" int hipq_kv_evict(const hipq_kv_cache *cache, const hipq_kv_evict_desc *d, void *workspace, size_t workspace_bytes, void *stream)
+{
+    clear_error();
+    if (check_evict(cache, d))
+        return 1;
     if (d->sequences == 0)
         return 0;
+    const bool in_place = d->to == d->blocks;
+    const int64_t tokens = (int64_t)d->blocks_per_sequence * cache->page, longest = d->longest < tokens ? d->longest : tokens, most = d->budget < longest ? d->budget : longest;
     HIPQ_REQUIRE(d->lens && d->kept && d->left && (most == 0 || (d->weights && d->blocks && d->to)), "evict: a null pointer");
     HIPQ_REQUIRE((uintptr_t)d->weights % 16 == 0, "evict: weights are not at multiples of 16 bytes");
-    const int64_t heads = (int64_t)d->sequences * cache->heads;
-    // of 2^32 work-items and more only what is left over would run
-    HIPQ_REQUIRE(heads < (1 << 22), "evict: %d sequences of %d heads", d->sequences, cache->heads);
+    const EvictShape s = shape_of(cache, d);
+    HIPQ_REQUIRE(s.workspace == 0 || (workspace && workspace_bytes >= s.workspace && (uintptr_t)workspace % 16 == 0), "evict: a workspace of %zu bytes is needed", s.workspace);
     EvictArgs a = {};
     a.cache = *cache, a.d = *d;
     if (hipq_div_magic((uint32_t)cache->page / 16, &a.page_magic, &a.page_shift))
         return fail("evict: pages of %d tokens", cache->page);
-    kv_choose_kernel<<<dim3((unsigned)heads), dim3(CHOOSERS), 0, (hipStream_t)stream>>>(a);
-    if (launch_status("kv_choose_kernel"))
+    a.chunks = s.chunks;
+    a.hist = (uint32_t *)workspace, a.above = (uint32_t *)((uint8_t *)workspace + s.hist), a.found = (uint32_t *)((uint8_t *)workspace + s.above);
+    if (choose(a, longest, (hipStream_t)stream))
         return 1;
     return cache->dim * (cache->quantized ? 1 : 2) == 64 ? launch_move<64>(a, in_place, (hipStream_t)stream) : launch_move<128>(a, in_place, (hipStream_t)stream);
 }

@@ -22,7 +22,7 @@ struct WeighArgs {
     float *scores;          // [sequence][head][row][stride], or nullptr
     float *lse;             // [sequence][head][row]: without scores
     int64_t stride;
-    int splits;             // the second launch's
+    int splits, chunk;      // the second launch's work-groups for a sequence and head, and their tokens
 };
 
 // Scores of a tile's 8 tokens of a lane and one of its rows, to the base 2; -infinity: not seen.
@@ -67,13 +67,15 @@ struct Keys {
     __device__ static __forceinline__ const u32x4 *query(const uint16_t *q, int ks, int j) { return (const u32x4 *)(q + (QUANT ? ks / 2 * 64 + j * 16 + ks % 2 * 8 : ks * 32 + j * 8)); }
 };
 
-// Rows' maxima and sums over a part, and with SCORES their scores.  A lane keeps both for its own tokens; they meet at the end.
+// Rows' maxima and sums over a part, and with SCORES their scores.  A lane keeps both for its own tokens; they meet at the end.  More than two blocks of 16 rows are
+// in LDS, in operand order.
 template <int TYPE, int DIM, bool QUANT, int RT, bool SCORES>
 __global__ __launch_bounds__(256, 2) void kv_scores_kernel(const WeighArgs w)
 {
     using R = Real16<TYPE>;
     using K = Keys<TYPE, DIM, QUANT>;
     constexpr int KS = K::KS;
+    constexpr bool Q_LDS = RT > 2;
     const AttendArgs &a = w.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, j = lane >> 4;
@@ -91,8 +93,10 @@ __global__ __launch_bounds__(256, 2) void kv_scores_kernel(const WeighArgs w)
     const int most = a.d.mask ? seq.len : min(seq.len, seq.old + min(rows - 1, r0 + 16 * RT - 1) / a.group + 1);
     const int t1 = min(t0 + share, most);
     __shared__ float lm[4][RT * 16], ll[4][RT * 16];
+    __shared__ u32x4 lq[Q_LDS ? RT * KS * 64 : 1];
 
-    u32x4 q[RT][KS];
+    u32x4 q[Q_LDS ? 1 : RT][Q_LDS ? 1 : KS];
+    const int live = (min(rows - r0, RT * 16) + 15) / 16; // blocks of rows that are there
     int own[RT]; // the lane's rows (the last one again behind it): new token
     float m[RT], l[RT];
     float *to[RT];
@@ -103,10 +107,15 @@ __global__ __launch_bounds__(256, 2) void kv_scores_kernel(const WeighArgs w)
         const uint16_t *x = (const uint16_t *)a.d.q + (int64_t)(seq.row0 + own[rt]) * a.d.q_token + (int64_t)(h * a.group + row - own[rt] * a.group) * a.d.q_head;
 #pragma unroll
         for (int ks = 0; ks < KS; ks++)
-            q[rt][ks] = *K::query(x, ks, j);
+            if (!Q_LDS)
+                q[Q_LDS ? 0 : rt][Q_LDS ? 0 : ks] = *K::query(x, ks, j);
+            else if ((rt * KS + ks) % 4 == wave)
+                lq[(rt * KS + ks) * 64 + lane] = *K::query(x, ks, j);
         m[rt] = NONE, l[rt] = 0;
         to[rt] = SCORES && at < rows ? w.scores + (((int64_t)b * a.cache.heads + h) * a.rows + row) * w.stride + j * 4 : nullptr;
     }
+    if (Q_LDS)
+        __syncthreads();
     const Paging paging(a, a.d.blocks + (int64_t)b * a.d.blocks_stride, seq.len);
     K keys;
     auto tile = [&](int t, const Pages &now, const Pages &next, auto MASKED) __attribute__((always_inline)) {
@@ -119,12 +128,14 @@ __global__ __launch_bounds__(256, 2) void kv_scores_kernel(const WeighArgs w)
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
+            if (rt > 0 && rt >= live)
+                break;
             f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
                 for (int half = 0; half < 2; half++)
-                    s[half] = R::mfma(k[half][ks], q[rt][ks], s[half]);
+                    s[half] = R::mfma(k[half][ks], Q_LDS ? lq[(rt * KS + ks) * 64 + lane] : q[Q_LDS ? 0 : rt][Q_LDS ? 0 : ks], s[half]);
             float x[8], top = m[rt];
             scaled<QUANT, masked>(s, ksc, a.scale2, masked ? seen_by(a, seq, own[rt], t, j, now) : 0, x);
 #pragma unroll
@@ -280,85 +291,105 @@ __global__ __launch_bounds__(256) void kv_lse_kernel(const WeighArgs w)
         w.lse[id] = v;
 }
 
-// From the keys: a wave has 32 tokens', and the rows go by, 16 at a time.
+// From the keys: a wave has 32 tokens', and the rows go by, 16 at a time, from LDS, where BLOCKS such blocks are at once, in operand order, with their sums.
 template <int TYPE, int DIM, bool QUANT>
 __global__ __launch_bounds__(256, 2) void kv_sum_keys_kernel(const WeighArgs w)
 {
     using R = Real16<TYPE>;
     using K = Keys<TYPE, DIM, QUANT>;
-    constexpr int KS = K::KS;
+    constexpr int KS = K::KS, BLOCKS = DIM == 256 ? 4 : 8;
     const AttendArgs &a = w.a;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), c = lane & 15, j = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, j = lane >> 4;
     const int eighth = gridDim.x / 8, item = (int)(blockIdx.x % 8) * eighth + (int)(blockIdx.x / 8), chunk = item % w.splits, bh = item / w.splits;
     const int h = bh % a.cache.heads, b = bh / a.cache.heads;
     if (b >= a.d.sequences)
         return;
     const Sequence seq(a, b);
-    const int rows = seq.count * a.group, t = chunk * 128 + wave * 32;
-    if (rows == 0 || t >= seq.len)
+    const int rows = seq.count * a.group, from = chunk * w.chunk, to = min(seq.len, from + w.chunk);
+    if (rows == 0 || from >= to)
         return;
+    __shared__ u32x4 lq[BLOCKS * KS * 64];
+    __shared__ float ls[BLOCKS * 16];
     const Paging paging(a, a.d.blocks + (int64_t)b * a.d.blocks_stride, seq.len);
-    const Pages now = paging.of(t);
-    K keys;
-    keys.load(a, paging, now, h, c, j);
-    u32x4 k[2][KS];
-    keys.operands(k);
-    if (QUANT)
-        keys.scale[0] *= a.scale2, keys.scale[1] *= a.scale2;
-    const bool masked = t + 32 > min(seq.old, seq.len) || now.page[0] < 0 || now.page[1] < 0;
-    // the first row that sees something of the tile: those of earlier tokens see none of it
-    const int first = a.d.mask || t < seq.old ? 0 : (t - seq.old) * a.group / 16 * 16;
-    f32x4 sum[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-    u32x4 q[KS];
-    float lse = 0;
-    int own = 0;
-    auto load = [&](int r) __attribute__((always_inline)) {
-        const int row = min(r + c, rows - 1);
-        own = row / a.group;
-        const uint16_t *x = (const uint16_t *)a.d.q + (int64_t)(seq.row0 + own) * a.d.q_token + (int64_t)(h * a.group + row - own * a.group) * a.d.q_head;
+    auto fetch = [&](int r0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++)
-            q[ks] = *K::query(x, ks, j);
-        lse = r + c < rows ? w.lse[(int64_t)bh * a.rows + row] : __builtin_inff();
-    };
-    load(first);
-#pragma unroll 1
-    for (int r = first; r < rows; r += 16) {
-        f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-            for (int half = 0; half < 2; half++)
-                s[half] = R::mfma(k[half][ks], q[ks], s[half]);
-        const float ref = lse;
-        const uint32_t sees = masked ? seen_by(a, seq, own, t, j, now) : 255u;
-        load(min(r + 16, rows - 1));
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float x = s[e / 4][e % 4] * (QUANT ? keys.scale[e / 4][e % 4] : a.scale2);
-            sum[e / 4][e % 4] += (sees >> e) & 1 ? exp2_fast(x - ref) : 0.0f;
+        for (int i = 0; i < BLOCKS * KS / 4; i++) {
+            const int rb = (i * 4 + wave) / KS, ks = (i * 4 + wave) % KS, row = min(r0 + rb * 16 + c, rows - 1), own = row / a.group;
+            const uint16_t *x = (const uint16_t *)a.d.q + (int64_t)(seq.row0 + own) * a.d.q_token + (int64_t)(h * a.group + row - own * a.group) * a.d.q_head;
+            if (r0 + rb * 16 < rows)
+                lq[(i * 4 + wave) * 64 + lane] = *K::query(x, ks, j);
         }
-    }
+        if (tid < BLOCKS * 16)
+            ls[tid] = r0 + tid < rows ? w.lse[(int64_t)bh * a.rows + r0 + tid] : __builtin_inff();
+    };
+    K keys;
+    Pages now = paging.of(from + wave * 32);
+    keys.load(a, paging, now, h, c, j);
+    fetch(0);
+    __syncthreads();
+#pragma unroll 1
+    for (int t0 = from; t0 < to; t0 += 128) { // all waves alike, as they share the rows
+        const int t = t0 + wave * 32;
+        u32x4 k[2][KS];
+        keys.operands(k);
+        f32x4 ksc[2];
+        if (QUANT)
+            ksc[0] = keys.scale[0] * a.scale2, ksc[1] = keys.scale[1] * a.scale2;
+        const Pages next = paging.of(t + 128);
+        __builtin_amdgcn_sched_barrier(0);
+        keys.load(a, paging, next, h, c, j);
+        __builtin_amdgcn_sched_barrier(0);
+        const bool masked = t + 32 > min(seq.old, seq.len) || now.page[0] < 0 || now.page[1] < 0;
+        // rows of tokens before the tile's first see none of it
+        const int first = a.d.mask || t < seq.old ? 0 : (t - seq.old) * a.group / 16 * 16;
+        f32x4 sum[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += BLOCKS * 16) {
+            if (rows > BLOCKS * 16 && (r0 > 0 || t0 > from)) {
+                __syncthreads();
+                fetch(r0);
+                __syncthreads();
+            }
+            const int end = min(BLOCKS, (rows - r0 + 15) / 16);
+#pragma unroll 1
+            for (int rb = max(first - r0, 0) / 16; rb < end; rb++) {
+                f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-    for (int o = 1; o < 16; o *= 2)
+                for (int ks = 0; ks < KS; ks++) {
+                    const u32x4 q = lq[(rb * KS + ks) * 64 + lane];
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-            sum[e / 4][e % 4] += __shfl_xor(sum[e / 4][e % 4], o);
-    if (c < 2) { // a half each
+                    for (int half = 0; half < 2; half++)
+                        s[half] = R::mfma(k[half][ks], q, s[half]);
+                }
+                const float lse = ls[rb * 16 + c];
+                const uint32_t sees = masked ? seen_by(a, seq, min(r0 + rb * 16 + c, rows - 1) / a.group, t, j, now) : 255u;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float p = exp2_fast(__builtin_fmaf(s[e / 4][e % 4], QUANT ? ksc[e / 4][e % 4] : a.scale2, -lse));
+                    sum[e / 4][e % 4] += (sees >> e) & 1 ? p : 0.0f;
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o *= 2)
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                sum[e / 4][e % 4] += __shfl_xor(sum[e / 4][e % 4], o);
         const int t4 = t + 16 * c + 4 * j;
-        if (t4 < seq.len) {
+        if (c < 2 && t4 < seq.len) { // a half each
             const int64_t at = weight_at(a, b, h, t4);
             f32x4 old = {0, 0, 0, 0};
             if (at >= 0 && t4 < seq.old)
                 old = *(const f32x4 *)(w.old + at);
             put(w, seq, at, t4, c ? sum[1] : sum[0], old);
         }
+        now = next;
     }
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------
 struct WeighShape {
-    int rt, row_blocks, rows, splits, chunks;
+    int rt, row_blocks, rows, splits, chunks, chunk;
     bool scores;
     int64_t stride;
     size_t part, lse, workspace; // bytes: of the parts; where the rest begins; of all
@@ -369,15 +400,18 @@ static WeighShape shape_of(const hipq_kv_cache *c, const hipq_kv_attend_desc *d)
     WeighShape s = {};
     const int group = d->q_heads / c->heads, width = c->quantized ? c->dim : 2 * c->dim;
     s.rows = d->most_new * group;
-    s.rt = s.rows <= 16 ? 1 : 2;
+    s.rt = s.rows <= 16 ? 1 : s.rows <= 32 ? 2 : s.rows <= 64 ? 4 : 8;
+    if (c->dim == 256 && s.rt == 8)
+        s.rt = 4; // of LDS without asking
     s.row_blocks = (s.rows + 16 * s.rt - 1) / (16 * s.rt);
     const int64_t longest = d->longest < (int64_t)d->blocks_per_sequence * c->page ? d->longest : (int64_t)d->blocks_per_sequence * c->page;
     const int64_t items = (int64_t)d->sequences * c->heads * s.row_blocks;
-    const int64_t target = items < 256 ? 256 : 512, want = items ? (target + items - 1) / items : 1, most = (longest + 255) / 256;
+    const int64_t want = items ? (1024 + items - 1) / items : 1, most = (longest + 255) / 256;
     s.splits = (int)(want < most ? want : most);
-    s.splits = s.splits < 1 ? 1 : s.splits > 64 ? 64 : s.splits;
+    s.splits = s.splits < 1 ? 1 : s.splits > 256 ? 256 : s.splits;
     s.scores = s.rows <= 32 && s.rows * 8 <= width;
-    s.chunks = (int)((longest + (s.scores ? 1023 : 127)) / (s.scores ? 1024 : 128));
+    s.chunk = s.scores ? 1024 : 512;
+    s.chunks = (int)((longest + s.chunk - 1) / s.chunk);
     const size_t heads = (size_t)d->sequences * c->heads;
     s.stride = (longest + 31) / 32 * 32;
     s.part = (heads * s.splits * s.rows * 8 + 255) / 256 * 256;
@@ -396,8 +430,12 @@ static int launch_weigh(const WeighArgs &w, const WeighShape &s, hipStream_t st)
         kv_scores_kernel<TYPE, DIM, QUANT, 2, true><<<grid, dim3(256), 0, st>>>(w);
     else if (s.rt == 1)
         kv_scores_kernel<TYPE, DIM, QUANT, 1, false><<<grid, dim3(256), 0, st>>>(w);
-    else
+    else if (s.rt == 2)
         kv_scores_kernel<TYPE, DIM, QUANT, 2, false><<<grid, dim3(256), 0, st>>>(w);
+    else if (s.rt == 4)
+        kv_scores_kernel<TYPE, DIM, QUANT, 4, false><<<grid, dim3(256), 0, st>>>(w);
+    else if constexpr (DIM < 256)
+        kv_scores_kernel<TYPE, DIM, QUANT, 8, false><<<grid, dim3(256), 0, st>>>(w);
     if (launch_status("kv_scores_kernel"))
         return 1;
     if (s.scores) {
@@ -470,7 +508,7 @@ extern "C" int hipq_kv_weigh(const hipq_kv_cache *cache, const hipq_kv_weigh_des
     w.a.group = d.q_heads / cache->heads, w.a.splits = s.splits, w.a.row_blocks = s.row_blocks, w.a.rows = s.rows;
     if (hipq_div_magic((uint32_t)cache->page / 16, &w.a.page_magic, &w.a.page_shift))
         return fail("weigh: pages of %d tokens", cache->page);
-    w.old = desc->weights, w.out = desc->out, w.stride = s.stride, w.splits = s.chunks;
+    w.old = desc->weights, w.out = desc->out, w.stride = s.stride, w.splits = s.chunks, w.chunk = s.chunk;
     w.a.part_ml = (float *)workspace;
     (s.scores ? w.scores : w.lse) = (float *)((uint8_t *)workspace + s.part);
     return cache->type == HIPQ_REAL_BF16 ? launch_weigh<HIPQ_REAL_BF16>(w, s, (hipStream_t)stream) : launch_weigh<HIPQ_REAL_F16>(w, s, (hipStream_t)stream);

@@ -742,6 +742,21 @@ static int bounded(PyObject *o, int64_t capacity, int *out)
     return 1;
 }
 
+/* a workspace of `need` bytes from the caller's function; NULL where none is needed */
+static int allocated(PyObject *allocate, size_t need, int device, PyObject **workspace, view_t *w)
+{
+    memset(w, 0, sizeof *w);
+    *workspace = NULL;
+    if (need == 0)
+        return 1;
+    PyObject *size = PyLong_FromSize_t(need);
+    *workspace = size ? PyObject_CallOneArg(allocate, size) : NULL;
+    Py_XDECREF(size);
+    if (*workspace != NULL && !whole_tensor(*workspace, "workspace", 1, 1u << U8, device, 0, w))
+        Py_CLEAR(*workspace);
+    return *workspace != NULL;
+}
+
 /* [pages][heads][page] of the cache */
 static int of_pages(const view_t *w, const char *name, const hipq_kv_cache *c) { return shaped(w, name, 3, c->pages, c->heads, c->page); }
 
@@ -781,20 +796,9 @@ static PyObject *py_kv_weigh(ARGS)
     d.q = q.p, d.q_token = q.stride[0], d.q_head = q.stride[1], d.weights = weights.p, d.out = out.p;
     d.starts = starts.p, d.lens = lens.p, d.blocks = blocks.p, d.mask = mask.p, d.blocks_stride = blocks.stride[0];
     d.sequences = (int)b, d.tokens = (int)t, d.q_heads = (int)q.shape[1], d.blocks_per_sequence = (int)blocks.shape[1];
-    const size_t need = hipq_kv_weigh_workspace(&c, &d);
-    memset(&w, 0, sizeof w);
-    PyObject *workspace = NULL;
-    if (need > 0) {
-        PyObject *size = PyLong_FromSize_t(need);
-        workspace = size ? PyObject_CallOneArg(a[12], size) : NULL;
-        Py_XDECREF(size);
-        if (workspace == NULL)
-            return NULL;
-        if (!whole_tensor(workspace, "workspace", 1, 1u << U8, device, 0, &w)) {
-            Py_DECREF(workspace);
-            return NULL;
-        }
-    }
+    PyObject *workspace;
+    if (!allocated(a[12], hipq_kv_weigh_workspace(&c, &d), device, &workspace, &w))
+        return NULL;
     int rc;
     Py_BEGIN_ALLOW_THREADS;
     rc = hipq_kv_weigh(&c, &d, w.p, (size_t)w.shape[0], st);
@@ -803,17 +807,17 @@ static PyObject *py_kv_weigh(ARGS)
     return PyLong_FromLong(rc);
 }
 
-/* cache, its device, weights, lens, blocks, to, left, kept, budget, recent, first, longest or None */
+/* cache, its device, weights, lens, blocks, to, left, kept, budget, recent, first, longest or None, allocate: (bytes) -> uint8 tensor */
 static PyObject *py_kv_evict(ARGS)
 {
     (void)self;
     hipq_kv_evict_desc d;
-    view_t weights, lens, blocks, to, left, kept;
+    view_t weights, lens, blocks, to, left, kept, w;
     int device;
     void *st;
     memset(&d, 0, sizeof d);
-    const hipq_kv_cache *c = n == 12 ? PyCapsule_GetPointer(a[0], "hipq_kv_cache") : NULL;
-    if (!expect(n, 12) || c == NULL || !current_device(&device) || !cache_device(a[1], device) || !whole_tensor(a[2], "weights", 3, 1u << F32, device, 0, &weights)
+    const hipq_kv_cache *c = n == 13 ? PyCapsule_GetPointer(a[0], "hipq_kv_cache") : NULL;
+    if (!expect(n, 13) || c == NULL || !current_device(&device) || !cache_device(a[1], device) || !whole_tensor(a[2], "weights", 3, 1u << F32, device, 0, &weights)
         || !whole_tensor(a[3], "lens", 1, 1u << I32, device, 0, &lens) || !tensor(a[4], "blocks", 2, 1u << I32, device, &blocks)
         || !tensor(a[5], "to", 2, 1u << I32, device, &to) || !whole_tensor(a[6], "left", 1, 1u << I32, device, 0, &left)
         || !whole_tensor(a[7], "kept", 3, 1u << I32, device, 0, &kept) || !whole(a[8], &d.budget) || !whole(a[9], &d.recent) || !whole(a[10], &d.first))
@@ -837,7 +841,15 @@ static PyObject *py_kv_evict(ARGS)
         any.type = BF16; /* codes are moved as they are */
     d.weights = weights.p, d.lens = lens.p, d.blocks = blocks.p, d.to = to.p, d.left = left.p, d.kept = kept.p;
     d.blocks_stride = blocks.stride[0], d.to_stride = to.stride[0], d.sequences = (int)b, d.blocks_per_sequence = (int)blocks.shape[1], d.to_per_sequence = (int)to.shape[1];
-    CALL(hipq_kv_evict(&any, &d, st));
+    PyObject *workspace;
+    if (!allocated(a[12], hipq_kv_evict_workspace(&any, &d), device, &workspace, &w))
+        return NULL;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = hipq_kv_evict(&any, &d, w.p, (size_t)w.shape[0], st);
+    Py_END_ALLOW_THREADS;
+    Py_XDECREF(workspace);
+    return PyLong_FromLong(rc);
 }
 
 /* logits, uniform, temperature, top_k, top_p, min_p (each or None), out */

@@ -169,7 +169,8 @@ _SIGS = {
     "hipq_kv_attend": (C.c_int, [C.POINTER(KvCacheStruct), C.POINTER(KvAttendDesc), C.c_void_p, C.c_size_t, C.c_void_p]),
     "hipq_kv_weigh_workspace": (C.c_size_t, [C.POINTER(KvCacheStruct), C.POINTER(KvWeighDesc)]),
     "hipq_kv_weigh": (C.c_int, [C.POINTER(KvCacheStruct), C.POINTER(KvWeighDesc), C.c_void_p, C.c_size_t, C.c_void_p]),
-    "hipq_kv_evict": (C.c_int, [C.POINTER(KvCacheStruct), C.POINTER(KvEvictDesc), C.c_void_p]),
+    "hipq_kv_evict_workspace": (C.c_size_t, [C.POINTER(KvCacheStruct), C.POINTER(KvEvictDesc)]),
+    "hipq_kv_evict": (C.c_int, [C.POINTER(KvCacheStruct), C.POINTER(KvEvictDesc), C.c_void_p, C.c_size_t, C.c_void_p]),
     "hipq_penalize": (C.c_int, [C.POINTER(PenalizeDesc), C.c_void_p]),
     "hipq_sample": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int64] + [C.c_void_p] * 7),
 }
@@ -854,7 +855,8 @@ class KvCache:
             left = torch.empty(lens.shape, dtype=torch.int32, device=lens.device)
         if kept is None:
             kept = torch.empty((lens.shape[0], self.k.shape[1], budget), dtype=torch.int32, device=lens.device)
-        rc = calls.kv_evict(self._struct, self._device, weights, lens, blocks, blocks if to is None else to, left, kept, budget, recent, first, longest)
+        rc = calls.kv_evict(self._struct, self._device, weights, lens, blocks, blocks if to is None else to, left, kept, budget, recent, first, longest,
+                            lambda count: _bytes_like(weights, count))
         if rc:
             check(rc)
         return left, kept
