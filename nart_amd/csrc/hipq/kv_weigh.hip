@@ -20,22 +20,24 @@ struct WeighArgs {
     const float *old;
     float *out;
     float *scores;          // [sequence][head][row][stride], or nullptr
-    float *lse;             // [sequence][head][row]: without scores
+    float *lse;             // [sequence][head][row]; nullptr: the second launch joins the parts itself
     int64_t stride;
+    uint32_t group_magic;   // of a.group
+    int group_shift;
     int splits, chunk;      // the second launch's work-groups for a sequence and head, and their tokens
 };
 
-// Scores of a tile's 8 tokens of a lane and one of its rows, to the base 2; -infinity: not seen.
-template <bool QUANT, bool MASKED>
-__device__ static __forceinline__ void scaled(const f32x4 (&s)[2], const f32x4 (&ksc)[2], float scale2, uint32_t sees, float (&x)[8])
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+__device__ static __forceinline__ int new_token(const WeighArgs &w, int row) { return w.group_magic ? (int)(((uint64_t)(uint32_t)row * w.group_magic) >> 32) >> w.group_shift : row; }
+// a row's query
+__device__ static __forceinline__ const uint16_t *query(const WeighArgs &w, const Sequence &seq, int h, int row)
 {
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        x[e] = s[e / 4][e % 4] * (QUANT ? ksc[e / 4][e % 4] * scale2 : scale2);
-        if (MASKED)
-            x[e] = (sees >> e) & 1 ? x[e] : NONE;
-    }
+    const int own = new_token(w, row);
+    return (const uint16_t *)w.a.d.q + (int64_t)(seq.row0 + own) * w.a.d.q_token + (int64_t)(h * w.a.group + row - own * w.a.group) * w.a.d.q_head;
 }
+
+constexpr float LOWEST = -0x1.fffffep127f; // a reference where nothing has been seen: finite, so that differences are numbers
 
 template <int TYPE, int DIM, bool QUANT>
 struct Keys {
@@ -67,15 +69,13 @@ struct Keys {
     __device__ static __forceinline__ const u32x4 *query(const uint16_t *q, int ks, int j) { return (const u32x4 *)(q + (QUANT ? ks / 2 * 64 + j * 16 + ks % 2 * 8 : ks * 32 + j * 8)); }
 };
 
-// Rows' maxima and sums over a part, and with SCORES their scores.  A lane keeps both for its own tokens; they meet at the end.  More than two blocks of 16 rows are
-// in LDS, in operand order.
+// Up to 32 rows: their maxima and sums over a part, and with SCORES their scores.  A lane keeps both for its own tokens; they meet at the end.
 template <int TYPE, int DIM, bool QUANT, int RT, bool SCORES>
 __global__ __launch_bounds__(256, 2) void kv_scores_kernel(const WeighArgs w)
 {
     using R = Real16<TYPE>;
     using K = Keys<TYPE, DIM, QUANT>;
     constexpr int KS = K::KS;
-    constexpr bool Q_LDS = RT > 2;
     const AttendArgs &a = w.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, j = lane >> 4;
@@ -93,62 +93,57 @@ __global__ __launch_bounds__(256, 2) void kv_scores_kernel(const WeighArgs w)
     const int most = a.d.mask ? seq.len : min(seq.len, seq.old + min(rows - 1, r0 + 16 * RT - 1) / a.group + 1);
     const int t1 = min(t0 + share, most);
     __shared__ float lm[4][RT * 16], ll[4][RT * 16];
-    __shared__ u32x4 lq[Q_LDS ? RT * KS * 64 : 1];
 
-    u32x4 q[Q_LDS ? 1 : RT][Q_LDS ? 1 : KS];
-    const int live = (min(rows - r0, RT * 16) + 15) / 16; // blocks of rows that are there
-    int own[RT]; // the lane's rows (the last one again behind it): new token
-    float m[RT], l[RT];
+    u32x4 q[RT][KS];
+    float m[RT], l[RT]; // of the lane's rows (the last one again behind it)
     float *to[RT];
+    auto row_of = [&](int rt) __attribute__((always_inline)) { return min(r0 + 16 * rt + c, rows - 1); };
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        const int at = r0 + 16 * rt + c, row = min(at, rows - 1);
-        own[rt] = row / a.group;
-        const uint16_t *x = (const uint16_t *)a.d.q + (int64_t)(seq.row0 + own[rt]) * a.d.q_token + (int64_t)(h * a.group + row - own[rt] * a.group) * a.d.q_head;
+        m[rt] = LOWEST, l[rt] = 0;
+        to[rt] = SCORES && r0 + 16 * rt + c < rows ? w.scores + (((int64_t)b * a.cache.heads + h) * a.rows + row_of(rt)) * w.stride + j * 4 : nullptr;
 #pragma unroll
         for (int ks = 0; ks < KS; ks++)
-            if (!Q_LDS)
-                q[Q_LDS ? 0 : rt][Q_LDS ? 0 : ks] = *K::query(x, ks, j);
-            else if ((rt * KS + ks) % 4 == wave)
-                lq[(rt * KS + ks) * 64 + lane] = *K::query(x, ks, j);
-        m[rt] = NONE, l[rt] = 0;
-        to[rt] = SCORES && at < rows ? w.scores + (((int64_t)b * a.cache.heads + h) * a.rows + row) * w.stride + j * 4 : nullptr;
+            q[rt][ks] = *K::query(query(w, seq, h, row_of(rt)), ks, j);
     }
-    if (Q_LDS)
-        __syncthreads();
     const Paging paging(a, a.d.blocks + (int64_t)b * a.d.blocks_stride, seq.len);
     K keys;
     auto tile = [&](int t, const Pages &now, const Pages &next, auto MASKED) __attribute__((always_inline)) {
         constexpr bool masked = decltype(MASKED)::value;
         u32x4 k[2][KS];
         keys.operands(k);
-        const f32x4 ksc[2] = {keys.scale[0], keys.scale[1]};
+        f32x4 ksc[2];
+        if (QUANT)
+            ksc[0] = keys.scale[0] * a.scale2, ksc[1] = keys.scale[1] * a.scale2;
         __builtin_amdgcn_sched_barrier(0);
         keys.load(a, paging, next, h, c, j);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
-            if (rt > 0 && rt >= live)
-                break;
             f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
                 for (int half = 0; half < 2; half++)
-                    s[half] = R::mfma(k[half][ks], Q_LDS ? lq[(rt * KS + ks) * 64 + lane] : q[Q_LDS ? 0 : rt][Q_LDS ? 0 : ks], s[half]);
-            float x[8], top = m[rt];
-            scaled<QUANT, masked>(s, ksc, a.scale2, masked ? seen_by(a, seq, own[rt], t, j, now) : 0, x);
+                    s[half] = R::mfma(k[half][ks], q[rt][ks], s[half]);
+            // scores to the base 2; of 16-bit keys, where nothing needs them, as they are
+            constexpr bool RAW = !QUANT && !SCORES;
+            const uint32_t sees = masked ? seen_by(a, seq, new_token(w, row_of(rt)), t, j, now) : 255u;
+            float x[8], p[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                top = fmaxf(top, x[e]);
-            if (__any(top > m[rt] + 8.0f)) { // the reference moves, as in attention
-                l[rt] *= top == NONE ? 1.0f : exp2_fast(m[rt] - top);
-                m[rt] = top;
+            for (int e = 0; e < 8; e++) {
+                x[e] = RAW ? s[e / 4][e % 4] : s[e / 4][e % 4] * (QUANT ? ksc[e / 4][e % 4] : a.scale2);
+                if (masked)
+                    x[e] = (sees >> e) & 1 ? x[e] : NONE;
             }
-            const float ref = m[rt] == NONE ? 0.0f : m[rt];
+            // no branch for a reference that stays: blocks of rows would wait for each other's
+            float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+            top = fmaxf(RAW ? top * a.scale2 : top, m[rt]);
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                l[rt] += exp2_fast(x[e] - ref);
+                p[e] = exp2_fast(RAW ? __builtin_fmaf(x[e], a.scale2, -top) : x[e] - top);
+            l[rt] = __builtin_fmaf(l[rt], exp2_fast(m[rt] - top), ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
+            m[rt] = top;
             if (SCORES && to[rt])
 #pragma unroll
                 for (int half = 0; half < 2; half++)
@@ -179,8 +174,8 @@ __global__ __launch_bounds__(256, 2) void kv_scores_kernel(const WeighArgs w)
     for (int rt = 0; rt < RT; rt++) {
 #pragma unroll
         for (int o = 16; o < 64; o *= 2) {
-            const float om = __shfl_xor(m[rt], o), ol = __shfl_xor(l[rt], o), top = fmaxf(m[rt], om), ref = top == NONE ? 0.0f : top;
-            l[rt] = l[rt] * exp2_fast(m[rt] - ref) + ol * exp2_fast(om - ref);
+            const float om = __shfl_xor(m[rt], o), ol = __shfl_xor(l[rt], o), top = fmaxf(m[rt], om);
+            l[rt] = l[rt] * exp2_fast(m[rt] - top) + ol * exp2_fast(om - top);
             m[rt] = top;
         }
         if (j == 0)
@@ -188,33 +183,162 @@ __global__ __launch_bounds__(256, 2) void kv_scores_kernel(const WeighArgs w)
     }
     __syncthreads();
     if (tid < RT * 16 && r0 + tid < rows) {
-        float top = NONE, sum = 0;
+        float top = LOWEST, sum = 0;
 #pragma unroll
         for (int v = 0; v < 4; v++)
             top = fmaxf(top, lm[v][tid]);
-        const float ref = top == NONE ? 0.0f : top;
 #pragma unroll
         for (int v = 0; v < 4; v++)
-            sum += ll[v][tid] * exp2_fast(lm[v][tid] - ref);
-        const int64_t at = (((int64_t)b * a.cache.heads + h) * a.splits + split) * a.rows + r0 + tid;
-        a.part_ml[2 * at] = top, a.part_ml[2 * at + 1] = sum;
+            sum += ll[v][tid] * exp2_fast(lm[v][tid] - top);
+        ((f32x2 *)a.part_ml)[(((int64_t)b * a.cache.heads + h) * a.rows + r0 + tid) * a.splits + split] = f32x2{top, sum};
     }
 }
 
-// log2 of a row's sum, by 8 neighbouring lanes of which each takes some of the parts; +infinity for a row that sees nothing, so that its weights are 0
-__device__ static __forceinline__ float joined(const AttendArgs &a, int bh, int row, int lane8)
+// More rows: BLOCKS blocks of 16 at once in LDS, in operand order, put there by the load unit; a wave has a tile's keys in registers and the rows go by, two blocks at a
+// time, whose maxima and sums wait in LDS meanwhile.  (With those in registers, for which all blocks are unrolled, the code alone took longer to arrive than the work.)
+template <int DIM>
+constexpr int BLOCKS = DIM == 256 ? 4 : 8;
+typedef const uint32_t __attribute__((address_space(1))) *gptr_t;
+typedef uint32_t __attribute__((address_space(3))) *lptr_t;
+
+// rows r0 .. of a sequence, the last one again behind it, and waits for this wave's part
+template <int TYPE, int DIM, bool QUANT>
+__device__ static __forceinline__ void fetch_rows(const WeighArgs &w, const Sequence &seq, int h, int r0, int rows, u32x4 *to, int wave, int c, int j)
 {
-    const int64_t at = (int64_t)bh * a.splits * a.rows + row;
-    float top = NONE, sum = 0;
-    for (int s = lane8; s < a.splits; s += 8) {
-        const float m = a.part_ml[2 * (at + (int64_t)s * a.rows)], l = a.part_ml[2 * (at + (int64_t)s * a.rows) + 1], both = fmaxf(top, m), ref = both == NONE ? 0.0f : both;
-        sum = sum * exp2_fast(top - ref) + l * exp2_fast(m - ref);
+    using K = Keys<TYPE, DIM, QUANT>;
+#pragma unroll 1
+    for (int i = wave; i < BLOCKS<DIM> * K::KS; i += 4)
+        __builtin_amdgcn_global_load_lds((gptr_t)K::query(query(w, seq, h, min(r0 + i / K::KS * 16 + c, rows - 1)), i % K::KS, j), (lptr_t)(to + i * 64), 16, 0, 0);
+}
+
+// two blocks' products with a tile
+template <int TYPE, int KS>
+__device__ static __forceinline__ void two_blocks(const u32x4 (&k)[2][KS], const u32x4 *q, int lane, f32x4 (&s)[2][2])
+{
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+        s[u][0] = s[u][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const u32x4 v = q[(u * KS + ks) * 64 + lane];
+#pragma unroll
+            for (int half = 0; half < 2; half++)
+                s[u][half] = Real16<TYPE>::mfma(k[half][ks], v, s[u][half]);
+        }
+}
+
+template <int TYPE, int DIM, bool QUANT>
+__global__ __launch_bounds__(256, 2) void kv_row_sums_kernel(const WeighArgs w)
+{
+    using K = Keys<TYPE, DIM, QUANT>;
+    constexpr int KS = K::KS, ROWS = 16 * BLOCKS<DIM>;
+    const AttendArgs &a = w.a;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, j = lane >> 4;
+    const int eighth = gridDim.x / 8, item = (int)(blockIdx.x % 8) * eighth + (int)(blockIdx.x / 8);
+    const int rb = item % a.row_blocks, split = item / a.row_blocks % a.splits, bh = item / a.row_blocks / a.splits, h = bh % a.cache.heads, b = bh / a.cache.heads;
+    if (b >= a.d.sequences)
+        return;
+    const Sequence seq(a, b);
+    const int rows = seq.count * a.group, r0 = rb * ROWS;
+    if (r0 >= rows)
+        return;
+    const int share = seq.share(a.splits), t0 = split * share;
+    const int most = a.d.mask ? seq.len : min(seq.len, seq.old + new_token(w, min(rows, r0 + ROWS) - 1) + 1), t1 = min(t0 + share, most);
+    __shared__ u32x4 lq[BLOCKS<DIM> * KS * 64];
+    __shared__ f32x2 lml[4][BLOCKS<DIM>][64]; // a wave's own: maxima and sums
+    const Paging paging(a, a.d.blocks + (int64_t)b * a.d.blocks_stride, seq.len);
+    const int blocks = (min(rows - r0, ROWS) + 15) / 16;
+    K keys;
+    Pages now = paging.of(t0 + wave * 32);
+    fetch_rows<TYPE, DIM, QUANT>(w, seq, h, r0, rows, lq, wave, c, j);
+    keys.load(a, paging, now, h, c, j);
+#pragma unroll 1
+    for (int i = 0; i < BLOCKS<DIM>; i++)
+        lml[wave][i][lane] = f32x2{LOWEST, 0};
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+#pragma unroll 1
+    for (int t = t0 + wave * 32; t < t1; t += 128) {
+        u32x4 k[2][KS];
+        keys.operands(k);
+        f32x4 ksc[2];
+        if (QUANT)
+            ksc[0] = keys.scale[0] * a.scale2, ksc[1] = keys.scale[1] * a.scale2;
+        const Pages next = paging.of(t + 128);
+        __builtin_amdgcn_sched_barrier(0);
+        keys.load(a, paging, next, h, c, j);
+        __builtin_amdgcn_sched_barrier(0);
+        const bool masked = t + 32 > min(seq.old, seq.len) || now.page[0] < 0 || now.page[1] < 0;
+#pragma unroll 1
+        for (int i = 0; i < blocks; i += 2) {
+            f32x4 s[2][2];
+            f32x2 ml[2] = {lml[wave][i][lane], lml[wave][i + 1][lane]};
+            two_blocks<TYPE, KS>(k, lq + i * KS * 64, lane, s);
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                float x[8], p[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    x[e] = QUANT ? s[u][e / 4][e % 4] * ksc[e / 4][e % 4] : s[u][e / 4][e % 4];
+                if (masked) {
+                    const uint32_t sees = seen_by(a, seq, new_token(w, min(r0 + (i + u) * 16 + c, rows - 1)), t, j, now);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        x[e] = (sees >> e) & 1 ? x[e] : NONE;
+                }
+                float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+                top = fmaxf(QUANT ? top : top * a.scale2, ml[u][0]);
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    p[e] = exp2_fast(QUANT ? x[e] - top : __builtin_fmaf(x[e], a.scale2, -top));
+                lml[wave][i + u][lane] = f32x2{top, __builtin_fmaf(ml[u][1], exp2_fast(ml[u][0] - top), ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])))};
+            }
+        }
+        now = next;
+    }
+    __syncthreads();
+    // a row's four lanes of each of the four waves
+    if (tid < ROWS && r0 + tid < rows) {
+        float top = LOWEST, sum = 0;
+#pragma unroll 1
+        for (int i = 0; i < 16; i++) {
+            const f32x2 ml = lml[i / 4][tid / 16][i % 4 * 16 + tid % 16];
+            const float both = fmaxf(top, ml[0]);
+            sum = sum * exp2_fast(top - both) + ml[1] * exp2_fast(ml[0] - both);
+            top = both;
+        }
+        ((f32x2 *)a.part_ml)[((int64_t)bh * a.rows + r0 + tid) * a.splits + split] = f32x2{top, sum};
+    }
+}
+
+// log2 of a row's sum, by LANES neighbouring lanes of which each takes some of the parts; +infinity for a row that sees nothing, so that its weights are 0
+template <int LANES>
+__device__ static __forceinline__ float joined(const AttendArgs &a, int bh, int row, int lane)
+{
+    const f32x2 *const part = (const f32x2 *)a.part_ml + ((int64_t)bh * a.rows + row) * a.splits;
+    float top = LOWEST, sum = 0;
+#pragma unroll 1
+    for (int s0 = lane; s0 < a.splits; s0 += 8 * LANES) { // eight on their way at once
+        f32x2 ml[8];
+        float both = top, more = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            ml[i] = part[min(s0 + i * LANES, a.splits - 1)];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            both = fmaxf(both, ml[i][0]);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            more += s0 + i * LANES < a.splits ? ml[i][1] * exp2_fast(ml[i][0] - both) : 0.0f;
+        sum = __builtin_fmaf(sum, exp2_fast(top - both), more);
         top = both;
     }
 #pragma unroll
-    for (int o = 1; o < 8; o *= 2) {
-        const float m = __shfl_xor(top, o), l = __shfl_xor(sum, o), both = fmaxf(top, m), ref = both == NONE ? 0.0f : both;
-        sum = sum * exp2_fast(top - ref) + l * exp2_fast(m - ref);
+    for (int o = 1; o < LANES; o *= 2) {
+        const float m = __shfl_xor(top, o), l = __shfl_xor(sum, o), both = fmaxf(top, m);
+        sum = sum * exp2_fast(top - both) + l * exp2_fast(m - both);
         top = both;
     }
     return sum == 0 ? __builtin_inff() : top + log2f(sum);
@@ -226,6 +350,15 @@ __device__ static __forceinline__ int64_t weight_at(const AttendArgs &a, int b, 
     const int t16 = t / 16, page16 = a.cache.page / 16, block = a.page_magic ? (int)(((uint64_t)(uint32_t)t16 * a.page_magic) >> 32) >> a.page_shift : t16;
     const int page = a.d.blocks[(int64_t)b * a.d.blocks_stride + block];
     return page < 0 || page >= a.cache.pages ? -1 : ((int64_t)page * a.cache.heads + h) * a.cache.page + t - block * (page16 * 16);
+}
+
+// the sum over 16 neighbouring lanes, in all of them
+__device__ static __forceinline__ float over_rows(float v)
+{
+    v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x128, 0xf, 0xf, true)); // turned round by 8, ...
+    v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x124, 0xf, 0xf, true));
+    v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x122, 0xf, 0xf, true));
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x121, 0xf, 0xf, true));
 }
 
 // four tokens' sums, into the cache: to those before the new ones what they had is added
@@ -261,7 +394,7 @@ __global__ __launch_bounds__(256) void kv_sum_scores_kernel(const WeighArgs w)
     if (at >= 0 && t < seq.old)
         old = *(const f32x4 *)(w.old + at);
     const int row = threadIdx.x / 8;
-    const float own = joined(a, bh, min(row, rows - 1), threadIdx.x % 8);
+    const float own = joined<8>(a, bh, min(row, rows - 1), threadIdx.x % 8);
     if (threadIdx.x % 8 == 0)
         lse[row] = own;
     __syncthreads();
@@ -286,18 +419,17 @@ __global__ __launch_bounds__(256) void kv_lse_kernel(const WeighArgs w)
     if (bh >= a.d.sequences * a.cache.heads)
         return;
     const Sequence seq(a, bh / a.cache.heads);
-    const float v = row < seq.count * a.group ? joined(a, bh, row, threadIdx.x % 8) : __builtin_inff();
+    const float v = row < seq.count * a.group ? joined<8>(a, bh, row, threadIdx.x % 8) : __builtin_inff();
     if (threadIdx.x % 8 == 0)
         w.lse[id] = v;
 }
 
-// From the keys: a wave has 32 tokens', and the rows go by, 16 at a time, from LDS, where BLOCKS such blocks are at once, in operand order, with their sums.
+// From the keys: as the first launch of more rows.
 template <int TYPE, int DIM, bool QUANT>
 __global__ __launch_bounds__(256, 2) void kv_sum_keys_kernel(const WeighArgs w)
 {
-    using R = Real16<TYPE>;
     using K = Keys<TYPE, DIM, QUANT>;
-    constexpr int KS = K::KS, BLOCKS = DIM == 256 ? 4 : 8;
+    constexpr int KS = K::KS, ROWS = 16 * BLOCKS<DIM>;
     const AttendArgs &a = w.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, j = lane >> 4;
     const int eighth = gridDim.x / 8, item = (int)(blockIdx.x % 8) * eighth + (int)(blockIdx.x / 8), chunk = item % w.splits, bh = item / w.splits;
@@ -308,25 +440,26 @@ __global__ __launch_bounds__(256, 2) void kv_sum_keys_kernel(const WeighArgs w)
     const int rows = seq.count * a.group, from = chunk * w.chunk, to = min(seq.len, from + w.chunk);
     if (rows == 0 || from >= to)
         return;
-    __shared__ u32x4 lq[BLOCKS * KS * 64];
-    __shared__ float ls[BLOCKS * 16];
+    __shared__ u32x4 lq[BLOCKS<DIM> * KS * 64];
+    __shared__ float ls[ROWS];
     const Paging paging(a, a.d.blocks + (int64_t)b * a.d.blocks_stride, seq.len);
     auto fetch = [&](int r0) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < BLOCKS * KS / 4; i++) {
-            const int rb = (i * 4 + wave) / KS, ks = (i * 4 + wave) % KS, row = min(r0 + rb * 16 + c, rows - 1), own = row / a.group;
-            const uint16_t *x = (const uint16_t *)a.d.q + (int64_t)(seq.row0 + own) * a.d.q_token + (int64_t)(h * a.group + row - own * a.group) * a.d.q_head;
-            if (r0 + rb * 16 < rows)
-                lq[(i * 4 + wave) * 64 + lane] = *K::query(x, ks, j);
-        }
-        if (tid < BLOCKS * 16)
-            ls[tid] = r0 + tid < rows ? w.lse[(int64_t)bh * a.rows + r0 + tid] : __builtin_inff();
+        fetch_rows<TYPE, DIM, QUANT>(w, seq, h, r0, rows, lq, wave, c, j);
+        constexpr int LANES = 256 / ROWS;
+        const int row = r0 + tid / LANES;
+        float lse;
+        if (w.lse)
+            lse = w.lse[(int64_t)bh * a.rows + min(row, rows - 1)];
+        else
+            lse = joined<LANES>(a, bh, min(row, rows - 1), tid % LANES);
+        ls[tid / LANES] = row < rows ? lse : __builtin_inff();
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
     };
     K keys;
     Pages now = paging.of(from + wave * 32);
     keys.load(a, paging, now, h, c, j);
     fetch(0);
-    __syncthreads();
 #pragma unroll 1
     for (int t0 = from; t0 < to; t0 += 128) { // all waves alike, as they share the rows
         const int t = t0 + wave * 32;
@@ -336,53 +469,55 @@ __global__ __launch_bounds__(256, 2) void kv_sum_keys_kernel(const WeighArgs w)
         if (QUANT)
             ksc[0] = keys.scale[0] * a.scale2, ksc[1] = keys.scale[1] * a.scale2;
         const Pages next = paging.of(t + 128);
+        // lanes 0 and 1 of 16 write a half's sums each
+        const int t4 = t + 16 * c + 4 * j;
+        const bool there = c < 2 && t4 < seq.len && (c ? now.page[1] : now.page[0]) >= 0;
+        const int64_t at = (c ? paging.row(now, 1, h) : paging.row(now, 0, h)) + 4 * j;
+        f32x4 old = {0, 0, 0, 0};
+        if (there && t4 < seq.old)
+            old = *(const f32x4 *)(w.old + at);
         __builtin_amdgcn_sched_barrier(0);
         keys.load(a, paging, next, h, c, j);
         __builtin_amdgcn_sched_barrier(0);
         const bool masked = t + 32 > min(seq.old, seq.len) || now.page[0] < 0 || now.page[1] < 0;
         // rows of tokens before the tile's first see none of it
-        const int first = a.d.mask || t < seq.old ? 0 : (t - seq.old) * a.group / 16 * 16;
+        const int first = a.d.mask || t < seq.old ? 0 : (t - seq.old) * a.group / 32 * 2;
         f32x4 sum[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll 1
-        for (int r0 = 0; r0 < rows; r0 += BLOCKS * 16) {
-            if (rows > BLOCKS * 16 && (r0 > 0 || t0 > from)) {
+        for (int r0 = 0; r0 < rows; r0 += ROWS) {
+            if (rows > ROWS && (r0 > 0 || t0 > from)) {
                 __syncthreads();
                 fetch(r0);
-                __syncthreads();
             }
-            const int end = min(BLOCKS, (rows - r0 + 15) / 16);
+            const int end = min(BLOCKS<DIM>, (rows - r0 + 15) / 16);
+            // two blocks at once, the second of which may be the last row again with a sum of infinity
 #pragma unroll 1
-            for (int rb = max(first - r0, 0) / 16; rb < end; rb++) {
-                f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+            for (int i = max(first - r0 / 16, 0); i < end; i += 2) {
+                f32x4 s[2][2];
+                two_blocks<TYPE, KS>(k, lq + i * KS * 64, lane, s);
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) {
-                    const u32x4 q = lq[(rb * KS + ks) * 64 + lane];
+                for (int u = 0; u < 2; u++) {
+                    const float lse = ls[(i + u) * 16 + c];
+                    float p[8];
 #pragma unroll
-                    for (int half = 0; half < 2; half++)
-                        s[half] = R::mfma(k[half][ks], q, s[half]);
-                }
-                const float lse = ls[rb * 16 + c];
-                const uint32_t sees = masked ? seen_by(a, seq, min(r0 + rb * 16 + c, rows - 1) / a.group, t, j, now) : 255u;
+                    for (int e = 0; e < 8; e++)
+                        p[e] = exp2_fast(__builtin_fmaf(s[u][e / 4][e % 4], QUANT ? ksc[e / 4][e % 4] : a.scale2, -lse));
+                    if (masked) {
+                        const uint32_t sees = seen_by(a, seq, new_token(w, min(r0 + (i + u) * 16 + c, rows - 1)), t, j, now);
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float p = exp2_fast(__builtin_fmaf(s[e / 4][e % 4], QUANT ? ksc[e / 4][e % 4] : a.scale2, -lse));
-                    sum[e / 4][e % 4] += (sees >> e) & 1 ? p : 0.0f;
+                        for (int e = 0; e < 8; e++)
+                            p[e] = (sees >> e) & 1 ? p[e] : 0.0f;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        sum[e / 4][e % 4] += p[e];
                 }
             }
         }
 #pragma unroll
-        for (int o = 1; o < 16; o *= 2)
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                sum[e / 4][e % 4] += __shfl_xor(sum[e / 4][e % 4], o);
-        const int t4 = t + 16 * c + 4 * j;
-        if (c < 2 && t4 < seq.len) { // a half each
-            const int64_t at = weight_at(a, b, h, t4);
-            f32x4 old = {0, 0, 0, 0};
-            if (at >= 0 && t4 < seq.old)
-                old = *(const f32x4 *)(w.old + at);
-            put(w, seq, at, t4, c ? sum[1] : sum[0], old);
-        }
+        for (int e = 0; e < 8; e++)
+            sum[e / 4][e % 4] = over_rows(sum[e / 4][e % 4]);
+        put(w, seq, there ? at : -1, t4, c ? sum[1] : sum[0], old);
         now = next;
     }
 }
@@ -390,9 +525,9 @@ __global__ __launch_bounds__(256, 2) void kv_sum_keys_kernel(const WeighArgs w)
 // ---- host ----------------------------------------------------------------------------------------------------------------------
 struct WeighShape {
     int rt, row_blocks, rows, splits, chunks, chunk;
-    bool scores;
+    bool scores, lse;
     int64_t stride;
-    size_t part, lse, workspace; // bytes: of the parts; where the rest begins; of all
+    size_t part, workspace; // bytes: of the parts; of all
 };
 
 static WeighShape shape_of(const hipq_kv_cache *c, const hipq_kv_attend_desc *d)
@@ -400,22 +535,25 @@ static WeighShape shape_of(const hipq_kv_cache *c, const hipq_kv_attend_desc *d)
     WeighShape s = {};
     const int group = d->q_heads / c->heads, width = c->quantized ? c->dim : 2 * c->dim;
     s.rows = d->most_new * group;
-    s.rt = s.rows <= 16 ? 1 : s.rows <= 32 ? 2 : s.rows <= 64 ? 4 : 8;
-    if (c->dim == 256 && s.rt == 8)
-        s.rt = 4; // of LDS without asking
+    s.rt = s.rows <= 16 ? 1 : s.rows <= 32 ? 2 : c->dim == 256 ? BLOCKS<256> : BLOCKS<128>;
     s.row_blocks = (s.rows + 16 * s.rt - 1) / (16 * s.rt);
     const int64_t longest = d->longest < (int64_t)d->blocks_per_sequence * c->page ? d->longest : (int64_t)d->blocks_per_sequence * c->page;
     const int64_t items = (int64_t)d->sequences * c->heads * s.row_blocks;
-    const int64_t want = items ? (1024 + items - 1) / items : 1, most = (longest + 255) / 256;
+    // all work-groups that fit at once: three or four a CU, and of those that bring their rows into LDS first each with four tiles for a wave at least
+    const int64_t target = s.rt <= 2 ? 1024 : 768, least = s.rt <= 2 ? 256 : 512, want = items ? target / items : 1, most = (longest + least - 1) / least;
     s.splits = (int)(want < most ? want : most);
     s.splits = s.splits < 1 ? 1 : s.splits > 256 ? 256 : s.splits;
     s.scores = s.rows <= 32 && s.rows * 8 <= width;
-    s.chunk = s.scores ? 1024 : 512;
+    // once all rows are in LDS at once the second launch joins the parts itself
+    s.lse = !s.scores && s.rows > 16 * (c->dim == 256 ? BLOCKS<256> : BLOCKS<128>);
+    // from scores, four tokens a thread; from keys, as many tokens of a work-group as fill the chip once, with three a CU
+    const int64_t share = (longest * d->sequences * c->heads / 768 + 127) / 128 * 128;
+    s.chunk = s.scores ? 1024 : (int)(share < 128 ? 128 : share > 1024 ? 1024 : share);
     s.chunks = (int)((longest + s.chunk - 1) / s.chunk);
     const size_t heads = (size_t)d->sequences * c->heads;
     s.stride = (longest + 31) / 32 * 32;
     s.part = (heads * s.splits * s.rows * 8 + 255) / 256 * 256;
-    s.workspace = s.part + (s.scores ? heads * s.rows * s.stride * 4 : heads * s.rows * 4);
+    s.workspace = s.part + (s.scores ? heads * s.rows * s.stride * 4 : s.lse ? heads * s.rows * 4 : 0);
     return s;
 }
 
@@ -432,19 +570,19 @@ static int launch_weigh(const WeighArgs &w, const WeighShape &s, hipStream_t st)
         kv_scores_kernel<TYPE, DIM, QUANT, 1, false><<<grid, dim3(256), 0, st>>>(w);
     else if (s.rt == 2)
         kv_scores_kernel<TYPE, DIM, QUANT, 2, false><<<grid, dim3(256), 0, st>>>(w);
-    else if (s.rt == 4)
-        kv_scores_kernel<TYPE, DIM, QUANT, 4, false><<<grid, dim3(256), 0, st>>>(w);
-    else if constexpr (DIM < 256)
-        kv_scores_kernel<TYPE, DIM, QUANT, 8, false><<<grid, dim3(256), 0, st>>>(w);
+    else
+        kv_row_sums_kernel<TYPE, DIM, QUANT><<<grid, dim3(256), 0, st>>>(w);
     if (launch_status("kv_scores_kernel"))
         return 1;
     if (s.scores) {
         kv_sum_scores_kernel<<<dim3((unsigned)(heads * s.chunks)), dim3(256), 0, st>>>(w);
         return launch_status("kv_sum_scores_kernel");
     }
-    kv_lse_kernel<<<dim3((unsigned)((heads * s.rows + 31) / 32)), dim3(256), 0, st>>>(w);
-    if (launch_status("kv_lse_kernel"))
-        return 1;
+    if (w.lse) {
+        kv_lse_kernel<<<dim3((unsigned)((heads * s.rows + 31) / 32)), dim3(256), 0, st>>>(w);
+        if (launch_status("kv_lse_kernel"))
+            return 1;
+    }
     kv_sum_keys_kernel<TYPE, DIM, QUANT><<<dim3((unsigned)((heads * s.chunks + 7) / 8 * 8)), dim3(256), 0, st>>>(w);
     return launch_status("kv_sum_keys_kernel");
 }
@@ -508,8 +646,13 @@ extern "C" int hipq_kv_weigh(const hipq_kv_cache *cache, const hipq_kv_weigh_des
     w.a.group = d.q_heads / cache->heads, w.a.splits = s.splits, w.a.row_blocks = s.row_blocks, w.a.rows = s.rows;
     if (hipq_div_magic((uint32_t)cache->page / 16, &w.a.page_magic, &w.a.page_shift))
         return fail("weigh: pages of %d tokens", cache->page);
+    if (hipq_div_magic((uint32_t)w.a.group, &w.group_magic, &w.group_shift))
+        return fail("weigh: %d query heads on %d heads of the cache", d.q_heads, cache->heads);
     w.old = desc->weights, w.out = desc->out, w.stride = s.stride, w.splits = s.chunks, w.chunk = s.chunk;
     w.a.part_ml = (float *)workspace;
-    (s.scores ? w.scores : w.lse) = (float *)((uint8_t *)workspace + s.part);
+    if (s.scores)
+        w.scores = (float *)((uint8_t *)workspace + s.part);
+    if (s.lse)
+        w.lse = (float *)((uint8_t *)workspace + s.part);
     return cache->type == HIPQ_REAL_BF16 ? launch_weigh<HIPQ_REAL_BF16>(w, s, (hipStream_t)stream) : launch_weigh<HIPQ_REAL_F16>(w, s, (hipStream_t)stream);
 }
