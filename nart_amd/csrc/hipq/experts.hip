@@ -4,8 +4,7 @@
 //   y[t] = sum over the chosen e of share[t][e] * down_e (act(gate_e x[t]) * up_e x[t])
 //
 // A pair is a token and one of its experts.  Choosing and numbering: a wave finds a token's experts (the largest of its scores, `top` times); one work-group then
-// counts the pairs of each expert and numbers them, an expert's side by side in the order of their tokens, so that the same rows meet in the same work-groups
-// every time.  Both products are those of w4_tile.h, whose blocks of rows then have an expert each; the hidden rows between them are rounded to 16
+// counts the pairs of each expert and numbers them, an expert's side by side.  Both products are those of w4_tile.h, whose blocks of rows then have an expert each; the hidden rows between them are rounded to 16
 // bits, as the matrix unit takes them.  The second product's float32 sums go to memory, and a last kernel adds a token's, each times its share.
 #include <cmath>
 #include <new>
@@ -27,13 +26,29 @@ struct RouteArgs {
     int32_t *row;    // [pairs]: its token
     W4Block *block;
     int32_t *count;  // of blocks
+    float *placed_share; // [pairs]: by number, or nullptr
+    int most_blocks;
 };
 
-// A token's experts, its scores over the lanes of a wave: lane l has those of experts l, l + 64, ..., EACH of them
-template <int EACH>
-__device__ static __forceinline__ void choose(const RouteArgs &a, int t, int lane)
+// the largest of a wave's numbers, within groups of 16 lanes by turning them round
+__device__ static __forceinline__ uint32_t largest_of(uint32_t v)
 {
-    uint32_t key[EACH]; // in the order of the scores; 0: never taken
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x124, 0xf, 0xf, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x122, 0xf, 0xf, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x121, 0xf, 0xf, true));
+    const uint32_t a = max((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16));
+    return max(a, max((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48)));
+}
+
+struct Choice {
+    int expert; // -1: none
+    float share;
+};
+// A token's experts, lane s has the s-th; its scores over the lanes of a wave: lane l has those of experts l, l + 64, ..., EACH of them
+template <int EACH>
+__device__ static __forceinline__ void load_scores(const RouteArgs &a, int t, int lane, uint32_t (&key)[EACH]) // in the order of the scores; 0: never taken
+{
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
         const int e = i * 64 + lane;
@@ -47,15 +62,17 @@ __device__ static __forceinline__ void choose(const RouteArgs &a, int t, int lan
             key[i] = !(x > -__builtin_inff()) ? 0 : u & 0x80000000u ? ~u : u | 0x80000000u;
         }
     }
+}
+
+template <int EACH>
+__device__ static __forceinline__ Choice choose(const RouteArgs &a, uint32_t (&key)[EACH], int lane)
+{
     auto largest = [&] {
         uint32_t most = 0;
 #pragma unroll
         for (int i = 0; i < EACH; i++)
             most = max(most, key[i]);
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2)
-            most = max(most, (uint32_t)__shfl_xor((int)most, o));
-        return most;
+        return largest_of(most);
     };
     auto score = [](uint32_t k) { return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k); };
     const uint32_t most = largest();
@@ -95,61 +112,27 @@ __device__ static __forceinline__ void choose(const RouteArgs &a, int t, int lan
         if (lane == s)
             mine = e, share = w;
     }
-    if (lane < a.top) {
-        a.chosen[(int64_t)t * a.top + lane] = mine;
-        a.share[(int64_t)t * a.top + lane] = mine < 0 ? 0.0f : share / (a.normalize ? sum : a.sigmoid ? 1.0f : all);
-    }
+    return {mine, mine < 0 ? 0.0f : share / (a.normalize ? sum : a.sigmoid ? 1.0f : all)};
 }
 
 template <int EACH>
 __global__ __launch_bounds__(256) void experts_choose_kernel(const RouteArgs a)
 {
     const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (t < a.M)
-        choose<EACH>(a, (int)t, threadIdx.x & 63);
+    const int lane = threadIdx.x & 63;
+    if (t >= a.M)
+        return;
+    uint32_t key[EACH];
+    load_scores<EACH>(a, (int)t, lane, key);
+    const Choice own = choose<EACH>(a, key, lane);
+    if (lane < a.top)
+        a.chosen[t * a.top + lane] = own.expert, a.share[t * a.top + lane] = own.share;
 }
 
-// Numbers the pairs, by expert and then by token, and lists the blocks of rows.  Each of 16 waves has a contiguous part of the pairs, and goes through it 64 at a time
-// twice: to count each expert's, and to number them from where the waves before it end.  EACH above 0: it chooses as well.
-template <int EACH>
-__global__ __launch_bounds__(1024) void experts_number_kernel(const RouteArgs a)
+// an expert's pairs and blocks of rows, by thread, and those before it; lists the blocks, and returns where the expert's pairs begin
+__device__ static __forceinline__ int list_blocks(const RouteArgs &a, int pairs_of, int *scan)
 {
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    int32_t *const counts = (int32_t *)lds, *const scan = counts + 16 * a.experts; // [wave][expert]; pairs and blocks of [wave]
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    for (int i = tid; i < 16 * a.experts; i += 1024)
-        counts[i] = 0;
-    if constexpr (EACH > 0)
-        for (int t = wave; t < a.M; t += 16)
-            choose<EACH>(a, t, lane);
-    __syncthreads(); // the work-group's own writes to memory are in order behind it
-    const int pairs = a.M * a.top, share = (pairs + 1023) / 1024 * 64, from = wave * share, to = min(pairs, from + share);
-    auto same = [&](int e) { // the lanes with the same expert
-        uint64_t lanes = __ballot(e >= 0);
-#pragma unroll
-        for (int bit = 0; bit < 10; bit++)
-            if (a.experts > 1 << bit) {
-                const uint64_t set = __ballot((e >> bit) & 1);
-                lanes &= (e >> bit) & 1 ? set : ~set;
-            }
-        return lanes;
-    };
-    for (int p = from; p < to; p += 64) {
-        const int e = p + lane < to ? a.chosen[p + lane] : -1;
-        const uint64_t lanes = same(e);
-        if (e >= 0 && lane == __builtin_ctzll(lanes))
-            counts[wave * a.experts + e] += __builtin_popcountll(lanes);
-    }
-    __syncthreads();
-    // an expert's pairs and blocks, and those before it
-    int pairs_of = 0, blocks_of = 0;
-    if (tid < a.experts)
-        for (int w = 0; w < 16; w++) {
-            const int n = counts[w * a.experts + tid];
-            counts[w * a.experts + tid] = pairs_of;
-            pairs_of += n;
-        }
-    blocks_of = (pairs_of + a.block_rows - 1) / a.block_rows;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, blocks_of = (pairs_of + a.block_rows - 1) / a.block_rows;
     int first = pairs_of, base = blocks_of;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
@@ -159,30 +142,140 @@ __global__ __launch_bounds__(1024) void experts_number_kernel(const RouteArgs a)
     if (lane == 63)
         scan[wave] = first, scan[16 + wave] = base;
     __syncthreads();
-    for (int w = 0; w < wave; w++)
-        first += scan[w], base += scan[16 + w];
+#pragma unroll
+    for (int w = 0; w < 16; w++)
+        first += w < wave ? scan[w] : 0, base += w < wave ? scan[16 + w] : 0;
     if (tid == 1023)
         *a.count = base;
     first -= pairs_of, base -= blocks_of;
-    if (tid < a.experts) {
-        for (int w = 0; w < 16; w++)
-            counts[w * a.experts + tid] += first;
-        for (int i = 0; i < blocks_of; i++)
-            a.block[base + i] = W4Block{tid, first + i * a.block_rows, min(first + pairs_of, first + (i + 1) * a.block_rows), base, blocks_of};
+#pragma unroll 1
+    for (int i = 0; i < blocks_of; i++)
+        a.block[base + i] = W4Block{tid, first + i * a.block_rows, min(first + pairs_of, first + (i + 1) * a.block_rows), base, blocks_of};
+    return first;
+}
+
+// Few tokens: chooses their experts and numbers the pairs, by expert and then by token: a row's block, and with it the order of its sums, is the same every time.  Each of 16
+// waves has a contiguous part of the pairs, and goes through it 64 at a time twice: to count each expert's, and to number them from where the waves before it end.
+constexpr int CHOOSE_TOKENS = 128;
+template <int EACH>
+__global__ __launch_bounds__(1024) void experts_route_kernel(const RouteArgs a)
+{
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    int32_t *const counts = (int32_t *)lds; // [wave][expert]
+    __shared__ int32_t scan[32], chosen[CHOOSE_TOKENS * MOST_TOP];
+    __shared__ float share[CHOOSE_TOKENS * MOST_TOP];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr bool AHEAD = EACH <= 4; // more than that are too many registers
+    uint32_t key[EACH], next[EACH];
+    load_scores<EACH>(a, min(wave, a.M - 1), lane, next);
+#pragma unroll 1
+    for (int t = wave; t < a.M; t += 16) {
+        if (!AHEAD)
+            load_scores<EACH>(a, t, lane, next);
+#pragma unroll
+        for (int i = 0; i < EACH; i++)
+            key[i] = next[i];
+        if (AHEAD)
+            load_scores<EACH>(a, min(t + 16, a.M - 1), lane, next);
+        const Choice own = choose<EACH>(a, key, lane);
+        if (lane < a.top)
+            chosen[t * a.top + lane] = own.expert, share[t * a.top + lane] = a.share[t * a.top + lane] = own.share;
     }
+    for (int i = tid; i < 16 * a.experts; i += 1024)
+        counts[i] = 0;
     __syncthreads();
-    for (int p = from; p < to; p += 64) {
-        const int e = p + lane < to ? a.chosen[p + lane] : -1;
-        const uint64_t lanes = same(e);
-        int at = -1;
-        if (e >= 0) {
-            at = counts[wave * a.experts + e] + __builtin_popcountll(lanes & ((1ull << lane) - 1));
-            a.row[at] = (p + lane) / a.top;
+    const int pairs = a.M * a.top, part = (pairs + 1023) / 1024 * 64, from = wave * part, to = min(pairs, from + part);
+    auto same = [&](int e) { // the lanes with the same expert
+        uint64_t lanes = __ballot(e >= 0);
+#pragma unroll 1
+        for (int bit = 0; a.experts > 1 << bit; bit++) {
+            const uint64_t set = __ballot((e >> bit) & 1);
+            lanes &= (e >> bit) & 1 ? set : ~set;
         }
-        if (p + lane < to)
-            a.place[p + lane] = at;
+        return lanes;
+    };
+#pragma unroll 1
+    for (int p = from + lane; p - lane < to; p += 64)
+        if (p < to && chosen[p] >= 0)
+            atomicAdd(&counts[wave * a.experts + chosen[p]], 1);
+    __syncthreads();
+    int n[16], all = 0;
+    if (tid < a.experts) {
+#pragma unroll
+        for (int w = 0; w < 16; w++)
+            n[w] = counts[w * a.experts + tid];
+#pragma unroll
+        for (int w = 0; w < 16; w++)
+            all += n[w];
+    }
+    int at = list_blocks(a, all, scan);
+    if (tid < a.experts)
+#pragma unroll
+        for (int w = 0; w < 16; w++) {
+            counts[w * a.experts + tid] = at;
+            at += n[w];
+        }
+    __syncthreads();
+#pragma unroll 1
+    for (int p = from + lane; p - lane < to; p += 64) {
+        const int e = p < to ? chosen[p] : -1;
+        const uint64_t lanes = same(e);
+        int place = -1;
+        if (e >= 0) {
+            place = counts[wave * a.experts + e] + __builtin_popcountll(lanes & ((1ull << lane) - 1));
+            a.row[place] = p / a.top;
+            if (a.placed_share)
+                a.placed_share[place] = share[p];
+        }
+        if (p < to)
+            a.place[p] = place;
         if (e >= 0 && lane == __builtin_ctzll(lanes)) // in order behind the reads above: a wave's LDS accesses are
             counts[wave * a.experts + e] += __builtin_popcountll(lanes);
+    }
+}
+
+// More tokens, whose experts are chosen: a pair's place among its expert's is the one that it gets first.  Which row of a block it then is does not show in its result, and
+// neither does the block: all blocks of an expert's rows go through k from the same place on.
+__global__ __launch_bounds__(1024) void experts_number_kernel(const RouteArgs a)
+{
+    __shared__ int32_t counts[MOST_EXPERTS], scan[32];
+    const int tid = threadIdx.x, pairs = a.M * a.top;
+    constexpr int STEPS = 8; // on their way at once
+    counts[tid] = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int p0 = tid; p0 < pairs; p0 += 1024 * STEPS) {
+        int e[STEPS];
+#pragma unroll
+        for (int k = 0; k < STEPS; k++)
+            e[k] = p0 + 1024 * k < pairs ? a.chosen[p0 + 1024 * k] : -1;
+#pragma unroll
+        for (int k = 0; k < STEPS; k++)
+            if (e[k] >= 0)
+                a.place[p0 + 1024 * k] = atomicAdd(&counts[e[k]], 1);
+    }
+    __syncthreads();
+    const int first = list_blocks(a, tid < a.experts ? counts[tid] : 0, scan);
+    __syncthreads();
+    counts[tid] = first;
+    __syncthreads();
+#pragma unroll 1
+    for (int p0 = tid; p0 < pairs; p0 += 1024 * STEPS) {
+        int e[STEPS], place[STEPS];
+#pragma unroll
+        for (int k = 0; k < STEPS; k++) {
+            const int p = p0 + 1024 * k;
+            e[k] = p < pairs ? a.chosen[p] : -1, place[k] = p < pairs ? a.place[p] : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < STEPS; k++) {
+            const int p = p0 + 1024 * k;
+            if (p < pairs) {
+                if (e[k] >= 0)
+                    place[k] += counts[e[k]], a.row[place[k]] = p / a.top;
+                a.place[p] = e[k] >= 0 ? place[k] : -1;
+            }
+        }
     }
 }
 
@@ -211,6 +304,250 @@ __global__ __launch_bounds__(256) void experts_join_kernel(const RouteArgs a, co
             y[t * y_stride + n + e] = rounded<TYPE>(v[e]);
 }
 
+// ---- few tokens: streams of weights --------------------------------------------------------------------------------------------------
+// An expert has some rows, so the time is what it takes to read the chosen experts' weights, and to begin with it: they go straight into registers, several blocks
+// of k ahead, and no wave waits for another before its end.  A block has up to ROWS rows.  Of 4 rows 128 k are one load, lane c + 16 j of which has row c % 4 and k = 32 (c / 4) +
+// 8 j + 0..7, and turning it round within 16 lanes brings the next operand's to lanes 0..3; of 16 rows they are four loads, more than the weights are.
+constexpr int FEW_TOKENS = 64, FEW_PAIRS = FEW_TOKENS * MOST_TOP;
+
+template <int N>
+__device__ static __forceinline__ u32x4 turned(const u32x4 &v)
+{
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t w = v[i];
+        o[i] = (uint32_t)__builtin_amdgcn_mov_dpp((int)w, 0x120 + N, 0xf, 0xf, true);
+    }
+    return o;
+}
+
+// Blocks of 128 k of NT tiles and of ROWS rows, DEPTH of them on their way (w4_stream_kernel's arithmetic)
+template <int TYPE, int GPB, bool ZEROS, int ROWS, int NT, int DEPTH>
+struct Stream {
+    using R = Real16<TYPE>;
+    static constexpr int PIECES = ROWS == 4 ? 1 : 4;
+    u32x4 w[DEPTH][NT], x[DEPTH][PIECES];
+    Scales<TYPE, GPB, ZEROS> s[DEPTH][NT];
+    f32x4 total[NT];
+    Spread<TYPE> spread;
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+            total[nt] = f32x4{0, 0, 0, 0};
+    }
+    // the row that a lane reads, and where in it
+    static __device__ __forceinline__ int row_of(int c) { return ROWS == 4 ? c % 4 : c; }
+    static __device__ __forceinline__ int k_of(int c, int j) { return 8 * j + (ROWS == 4 ? c / 4 * 32 : 0); }
+    // q, scales: an array's; row: the lane's row of x, k_of elements into it
+    __device__ __forceinline__ void load(int d, const W4Args &a, const uint8_t *q, const uint8_t *scales, const uint16_t *row, int tile, int kb, int lane)
+    {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            w[d][nt] = *(const u32x4 *)(q + weights_at(tile + nt, kb, a.blocks) * 1024 + lane * 16);
+            s[d][nt].load(scales + (scales_at(tile + nt, kb, a.blocks) + (lane & 15)) * s[d][nt].BYTES);
+        }
+#pragma unroll
+        for (int t = 0; t < PIECES; t++) {
+            x[d][t] = u32x4{0, 0, 0, 0};
+            if (kb * 128 + (ROWS == 4 ? (lane & 15) / 4 : t) * 32 < a.K)
+                x[d][t] = *(const u32x4 *)(row + kb * 128 + t * 32);
+        }
+    }
+    __device__ __forceinline__ void multiply(int d)
+    {
+        const u32x4 minus_one = {Nibbles<TYPE>::MINUS_ONE, Nibbles<TYPE>::MINUS_ONE, Nibbles<TYPE>::MINUS_ONE, Nibbles<TYPE>::MINUS_ONE};
+        u32x4 a[4];
+        if constexpr (ROWS == 4)
+            a[0] = x[d][0], a[1] = turned<12>(x[d][0]), a[2] = turned<8>(x[d][0]), a[3] = turned<4>(x[d][0]);
+        else
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                a[t] = x[d][t % PIECES];
+#pragma unroll
+        for (int g = 0; g < GPB; g++) {
+            f32x4 less = {0, 0, 0, 0}; // minus the sums of x, in every column
+#pragma unroll
+            for (int t = g * 4 / GPB; t < (g + 1) * 4 / GPB; t++)
+                less = R::mfma(a[t], minus_one, less);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                f32x4 sum = less * s[d][nt].offset(g);
+#pragma unroll
+                for (int t = g * 4 / GPB; t < (g + 1) * 4 / GPB; t++)
+                    sum = R::mfma(a[t], spread(w[d][nt][t]), sum);
+                const float scale = s[d][nt].scale(g);
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    total[nt][r] = __builtin_fmaf(scale, sum[r], total[nt][r]);
+            }
+        }
+    }
+};
+
+struct FewArgs {
+    RouteArgs r;
+    W4Args a; // x and y: of the launch
+    size_t q_bytes, s_bytes; // of an expert
+    int groups;              // work-groups of a block of rows
+    float *part;             // [split][token][column] of the second launch, where work-groups share a tile
+};
+
+// The hidden rows: a work-group has two tiles of the gate and their two of the other projection, for a block of rows, and WAVES waves take the blocks of k in turn.
+template <int TYPE, int GPB, bool ZEROS, int ROWS, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, GPB == 1 ? 3 : 2) void experts_few_up_kernel(const FewArgs f)
+{
+    constexpr int NT = 4, DEPTH = ROWS == 4 && GPB == 1 ? 3 : 2;
+    using S = Stream<TYPE, GPB, ZEROS, ROWS, NT, DEPTH>;
+    __shared__ f32x4 red[WAVES][NT][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, j = lane >> 4;
+    const W4Args &a = f.a;
+    const int block = blockIdx.x / f.groups, tile0 = (int)(blockIdx.x - block * f.groups) * NT;
+    const W4Block b = f.r.block[block]; // read before it is known whether it is there
+    if (block >= *f.r.count)
+        return;
+    const int first = b.first, rows = b.end - first, expert = b.array;
+    const uint8_t *const q = a.q + expert * f.q_bytes, *const scales = a.scales + expert * f.s_bytes;
+    const uint16_t *const row = a.x + (int64_t)f.r.row[first + min(S::row_of(c), rows - 1)] * a.x_stride + S::k_of(c, j);
+    S stream;
+    stream.clear();
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++)
+        if (wave + d * WAVES < a.blocks)
+            stream.load(d, a, q, scales, row, tile0, wave + d * WAVES, lane);
+    for (int kb = wave; kb < a.blocks; kb += DEPTH * WAVES)
+#pragma unroll
+        for (int d = 0; d < DEPTH; d++)
+            if (kb + d * WAVES < a.blocks) {
+                stream.multiply(d);
+                if (kb + (d + DEPTH) * WAVES < a.blocks)
+                    stream.load(d, a, q, scales, row, tile0, kb + (d + DEPTH) * WAVES, lane);
+            }
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+        red[wave][nt][lane] = stream.total[nt];
+    __syncthreads();
+    if (tid < NT / 2 * 64) {
+        f32x4 gate = red[0][wave * 2][lane], up = red[0][wave * 2 + 1][lane];
+#pragma unroll
+        for (int o = 1; o < WAVES; o++)
+            gate += red[o][wave * 2][lane], up += red[o][wave * 2 + 1][lane];
+        const int n = (tile0 / 2 + wave) * 16 + c;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (n < a.N && 4 * j + i < rows)
+                a.y[(int64_t)(first + 4 * j + i) * a.y_stride + n] = rounded<TYPE>(activate(gate[i], a.activation) * up[i]);
+    }
+}
+
+// The result: a work-group has a tile of outputs, its 16 waves the same number of blocks each - of all blocks of rows and k, one after the other - and every
+// wave adds up what it has of each token, in LDS, where they meet.  Where there are fewer tiles than CUs, and much to read, gridDim.y work-groups share them, and
+// another launch adds up what they leave.  (The last of them to end could do that, but to have written what others read takes a write-back of the L2: 90 us.)
+template <int TYPE, int GPB, bool ZEROS, int ROWS>
+__global__ __launch_bounds__(1024) void experts_few_down_kernel(const FewArgs f)
+{
+    constexpr int WAVES = 16, DEPTH = ROWS == 4 ? (GPB == 4 ? 5 : 6) : GPB == 1 ? 4 : 3;
+    using S = Stream<TYPE, GPB, ZEROS, ROWS, 1, DEPTH>;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const RouteArgs &r = f.r;
+    const W4Args &a = f.a;
+    const int pairs = r.M * r.top;
+    float *const sums = (float *)lds;                     // [wave][token][16]
+    float *const share = sums + WAVES * r.M * 16;         // [pair]
+    int32_t *const token = (int32_t *)(share + pairs);    // [pair]
+    int32_t *const block = token + pairs;                 // [block]: expert, first, end
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, j = lane >> 4;
+    const int tile = blockIdx.x, items = __builtin_amdgcn_readfirstlane(*r.count) * a.blocks;
+    if (tid < pairs) { // what lies behind their ends is not looked at
+        share[tid] = r.placed_share[tid], token[tid] = r.row[tid];
+        if (tid < r.most_blocks)
+            block[3 * tid] = r.block[tid].array, block[3 * tid + 1] = r.block[tid].first, block[3 * tid + 2] = r.block[tid].end;
+    }
+    for (int i = tid; i < WAVES * r.M * 16; i += 1024)
+        sums[i] = 0;
+    __syncthreads();
+    const int split = blockIdx.y, splits = gridDim.y, own = split * WAVES + wave, all = splits * WAVES;
+    const int from = (int)((int64_t)items * own / all), to = (int)((int64_t)items * (own + 1) / all);
+    S stream;
+    stream.clear();
+    // the block that is loaded next, and the one that is multiplied next
+    int load_at = from / a.blocks, load_kb = from - load_at * a.blocks, at = load_at, kb = load_kb;
+    const uint8_t *q = nullptr, *scales = nullptr;
+    const uint16_t *row = nullptr;
+    auto enter = [&] {
+        const int expert = __builtin_amdgcn_readfirstlane(block[3 * load_at]), first = block[3 * load_at + 1], end = block[3 * load_at + 2];
+        q = a.q + expert * f.q_bytes, scales = a.scales + expert * f.s_bytes;
+        row = a.x + (int64_t)min(first + S::row_of(c), end - 1) * a.x_stride + S::k_of(c, j);
+    };
+    auto load = [&](int d) {
+        stream.load(d, a, q, scales, row, tile, load_kb, lane);
+        if (++load_kb == a.blocks) {
+            load_kb = 0, load_at++;
+            if (load_at * a.blocks < to)
+                enter();
+        }
+    };
+    auto leave = [&] { // a block of rows: what they have is added to their tokens'
+        const int first = block[3 * at + 1], end = block[3 * at + 2];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (first + 4 * j + i < end)
+                sums[(wave * r.M + token[first + 4 * j + i]) * 16 + c] += share[first + 4 * j + i] * stream.total[0][i];
+        stream.clear();
+    };
+    if (from < to) {
+        enter();
+#pragma unroll
+        for (int d = 0; d < DEPTH; d++)
+            if (from + d < to)
+                load(d);
+        for (int i = from; i < to; i += DEPTH)
+#pragma unroll
+            for (int d = 0; d < DEPTH; d++)
+                if (i + d < to) {
+                    stream.multiply(d);
+                    if (i + d + DEPTH < to)
+                        load(d);
+                    if (++kb == a.blocks || i + d + 1 == to) {
+                        leave();
+                        kb = 0, at++;
+                    }
+                }
+    }
+    __syncthreads();
+    float v = 0;
+    if (tid < r.M * 16) { // up to 64 tokens: one value a thread
+#pragma unroll
+        for (int o = 0; o < WAVES; o++)
+            v += sums[o * r.M * 16 + tid];
+    }
+    if (splits > 1) {
+        if (tid < r.M * 16)
+            f.part[((int64_t)split * r.M + tid / 16) * (gridDim.x * 16) + tile * 16 + tid % 16] = v;
+        return;
+    }
+    const int n = tile * 16 + tid % 16;
+    if (tid < r.M * 16 && n < a.N)
+        a.y[(int64_t)(tid / 16) * a.y_stride + n] = rounded<TYPE>(v);
+}
+
+template <int TYPE>
+__global__ __launch_bounds__(256) void experts_few_join_kernel(const float *part, int splits, int M, int columns, uint16_t *y, int64_t y_stride, int N)
+{
+    const int per_row = (N + 3) / 4, id = (int)blockIdx.x * 256 + threadIdx.x, t = id / per_row, n = (id - t * per_row) * 4;
+    if (t >= M)
+        return;
+    f32x4 v = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int s = 0; s < splits; s++)
+        v += *(const f32x4 *)(part + ((int64_t)s * M + t) * columns + n);
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (n + e < N)
+            y[t * y_stride + n + e] = rounded<TYPE>(v[e]);
+}
+
 } // namespace hipq
 
 using namespace hipq;
@@ -227,16 +564,16 @@ namespace hipq {
 
 // What lies in a caller's workspace.
 struct ExpertsLayout {
-    size_t chosen, share, place, row, block, count, hidden, part, xsum, bytes;
+    size_t chosen, share, place, row, block, count, hidden, part, xsum, share_by_number, bytes;
     int kernel, splits, block_rows;
     int64_t pairs, blocks; // at most
     int columns;
 };
-enum { TILE_16, TILE_32, TILE_64, TILE_128_WIDE, SHAPES };
+enum { FEW_4, FEW_16, TILE_16, TILE_32, TILE_64, TILE_128_WIDE, SHAPES };
 static const struct {
     const char *name;
     int rows, tiles; // of a work-group
-} SHAPE[SHAPES] = {{"w4_experts_16x128", 16, 8}, {"w4_experts_32x128", 32, 8}, {"w4_experts_64x128", 64, 8}, {"w4_experts_128x256", 128, 16}};
+} SHAPE[SHAPES] = {{"w4_experts_stream_4", 4, 1}, {"w4_experts_stream_16", 16, 1}, {"w4_experts_16x128", 16, 8}, {"w4_experts_32x128", 32, 8}, {"w4_experts_64x128", 64, 8}, {"w4_experts_128x256", 128, 16}};
 
 static ExpertsLayout layout_of(const hipq_w4_experts_plan *p, int M)
 {
@@ -244,12 +581,15 @@ static ExpertsLayout layout_of(const hipq_w4_experts_plan *p, int M)
     ExpertsLayout l = {};
     l.pairs = (int64_t)M * d.top;
     const int64_t each = l.pairs / d.experts; // an expert's, were all chosen as often
-    l.kernel = each <= 16 ? TILE_16 : each <= 32 ? TILE_32 : each <= 64 ? TILE_64 : TILE_128_WIDE;
+    if (M <= 16 || (M <= FEW_TOKENS && each <= 6))
+        l.kernel = M <= 4 || each <= 3 ? FEW_4 : FEW_16;
+    else
+        l.kernel = each <= 16 ? TILE_16 : each <= 32 ? TILE_32 : each <= 64 ? TILE_64 : TILE_128_WIDE;
     l.block_rows = SHAPE[l.kernel].rows;
     const int64_t used = l.pairs < d.experts ? l.pairs : d.experts;
     l.blocks = used + l.pairs / l.block_rows;
     l.blocks = l.blocks < l.pairs ? l.blocks : l.pairs;
-    const int64_t groups = l.blocks * ((p->tiles[1] + SHAPE[l.kernel].tiles - 1) / SHAPE[l.kernel].tiles);
+    const int64_t groups = l.blocks * ((p->tiles[1] + SHAPE[l.kernel].tiles - 1) / SHAPE[l.kernel].tiles); // of the second product
     const int most = p->args[1].blocks / 4;
     l.splits = groups < 256 ? (int)(256 / groups) : 1;
     l.splits = l.splits < most ? l.splits : most;
@@ -263,6 +603,17 @@ static ExpertsLayout layout_of(const hipq_w4_experts_plan *p, int M)
     };
     l.chosen = take(l.pairs * 4), l.share = take(l.pairs * 4), l.place = take(l.pairs * 4), l.row = take(l.pairs * 4), l.block = take(l.blocks * sizeof(W4Block)), l.count = take(4);
     l.hidden = take((size_t)l.pairs * d.inner * 2);
+    if (l.kernel <= FEW_16) {
+        l.share_by_number = take(l.pairs * 4);
+        // a work-group of 16 waves is what a CU holds; with less than 16 KB for each wave the launch that joins takes longer
+        const int64_t kb = used * p->args[1].blocks / 16;
+        l.splits = kb / 16 < 256 / p->tiles[1] ? (int)(kb / 16) : 256 / p->tiles[1];
+        l.splits = l.splits < 1 ? 1 : l.splits > 8 ? 8 : l.splits;
+        if (l.splits > 1)
+            l.part = take((size_t)p->tiles[1] * l.splits * M * 16 * 4);
+        l.bytes = at;
+        return l;
+    }
     l.part = take((size_t)l.splits * l.pairs * l.columns * 4);
     if (l.kernel == TILE_128_WIDE) {
         const size_t x = (size_t)round_up(M, 128) * p->args[0].blocks, h = (size_t)((l.pairs + 127) / 128 * 128) * p->args[1].blocks;
@@ -322,29 +673,85 @@ static int launch_experts(const hipq_w4_experts_plan *p, const ExpertsLayout &l,
                                  : launch_experts<TYPE, 4>(p, l, a, g, tiles, splits, ws, part, st);
 }
 
+template <int TYPE, int GPB, bool ZEROS, int ROWS>
+static int launch_few(const hipq_w4_experts_plan *p, FewArgs f, const uint16_t *x, int64_t x_stride, uint16_t *hidden, float *part, int splits, uint16_t *y, int64_t y_stride, hipStream_t st)
+{
+    f.a = p->args[0], f.q_bytes = p->groups[0].q_bytes, f.s_bytes = p->groups[0].s_bytes, f.groups = (p->tiles[0] + 3) / 4;
+    f.a.x = x, f.a.x_stride = x_stride, f.a.y = hidden, f.a.y_stride = p->desc.inner;
+    const int groups = f.r.most_blocks * f.groups;
+    // 2000 waves and more, however few blocks of k there are for each
+    if (groups >= 512)
+        experts_few_up_kernel<TYPE, GPB, ZEROS, ROWS, 4><<<dim3(groups), dim3(256), 0, st>>>(f);
+    else
+        experts_few_up_kernel<TYPE, GPB, ZEROS, ROWS, 8><<<dim3(groups), dim3(512), 0, st>>>(f);
+    if (launch_status("experts_few_up_kernel"))
+        return 1;
+    f.a = p->args[1], f.q_bytes = p->groups[1].q_bytes, f.s_bytes = p->groups[1].s_bytes;
+    f.a.x = hidden, f.a.x_stride = p->desc.inner, f.a.y = y, f.a.y_stride = y_stride, f.part = part;
+    constexpr int MOST = (16 * FEW_TOKENS * 16 + 5 * FEW_PAIRS) * 4;
+    const int lds = (16 * f.r.M * 16 + 5 * f.r.M * f.r.top) * 4;
+    static thread_local bool done[64] = {};
+    if (lds > 65536 && allow_lds((const void *)experts_few_down_kernel<TYPE, GPB, ZEROS, ROWS>, MOST, p->device, done))
+        return 1;
+    experts_few_down_kernel<TYPE, GPB, ZEROS, ROWS><<<dim3(p->tiles[1], splits), dim3(1024), lds, st>>>(f);
+    if (launch_status("experts_few_down_kernel"))
+        return 1;
+    if (splits == 1)
+        return 0;
+    const int64_t threads = (int64_t)f.r.M * ((p->desc.N + 3) / 4);
+    experts_few_join_kernel<TYPE><<<dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st>>>(part, splits, f.r.M, p->tiles[1] * 16, y, y_stride, p->desc.N);
+    return launch_status("experts_few_join_kernel");
+}
+
+template <int TYPE, int GPB, bool ZEROS>
+static int launch_few(const hipq_w4_experts_plan *p, const FewArgs &f, const uint16_t *x, int64_t x_stride, uint16_t *hidden, float *part, int splits, uint16_t *y, int64_t y_stride, hipStream_t st)
+{
+    return f.r.block_rows == 4 ? launch_few<TYPE, GPB, ZEROS, 4>(p, f, x, x_stride, hidden, part, splits, y, y_stride, st) : launch_few<TYPE, GPB, ZEROS, 16>(p, f, x, x_stride, hidden, part, splits, y, y_stride, st);
+}
+
+template <int TYPE, int GPB>
+static int launch_few(const hipq_w4_experts_plan *p, const FewArgs &f, const uint16_t *x, int64_t x_stride, uint16_t *hidden, float *part, int splits, uint16_t *y, int64_t y_stride, hipStream_t st)
+{
+    return p->args[0].zeros ? launch_few<TYPE, GPB, true>(p, f, x, x_stride, hidden, part, splits, y, y_stride, st) : launch_few<TYPE, GPB, false>(p, f, x, x_stride, hidden, part, splits, y, y_stride, st);
+}
+
+template <int TYPE>
+static int launch_few(const hipq_w4_experts_plan *p, const RouteArgs &r, const uint16_t *x, int64_t x_stride, uint16_t *hidden, float *part, int splits, uint16_t *y, int64_t y_stride, hipStream_t st)
+{
+    FewArgs f = {};
+    f.r = r;
+    return p->desc.group == 128  ? launch_few<TYPE, 1>(p, f, x, x_stride, hidden, part, splits, y, y_stride, st)
+           : p->desc.group == 64 ? launch_few<TYPE, 2>(p, f, x, x_stride, hidden, part, splits, y, y_stride, st)
+                                 : launch_few<TYPE, 4>(p, f, x, x_stride, hidden, part, splits, y, y_stride, st);
+}
+
 template <int EACH>
 static int route(const hipq_w4_experts_plan *p, const RouteArgs &r, hipStream_t st)
 {
-    const int lds = (16 * r.experts + 32) * 4, most = (16 * MOST_EXPERTS + 32) * 4;
-    const bool both = r.M <= 128; // 16 waves choose 128 tokens' experts in the time of a launch
-    static thread_local bool done[2][64] = {};
-    const auto kernel = both ? experts_number_kernel<EACH> : experts_number_kernel<0>;
-    if (!both) {
-        experts_choose_kernel<EACH><<<dim3((unsigned)((r.M + 3) / 4)), dim3(256), 0, st>>>(r);
-        if (launch_status("experts_choose_kernel"))
+    if (r.M <= CHOOSE_TOKENS) { // 16 waves choose so many tokens' experts in the time of a launch
+        const int lds = 16 * r.experts * 4;
+        static thread_local bool done[64] = {};
+        if (lds + CHOOSE_TOKENS * MOST_TOP * 8 + 128 > 65536 && allow_lds((const void *)experts_route_kernel<EACH>, 16 * MOST_EXPERTS * 4 + 1024, p->device, done))
             return 1;
+        experts_route_kernel<EACH><<<dim3(1), dim3(1024), lds, st>>>(r);
+        return launch_status("experts_route_kernel");
     }
-    if (lds > 65536 && allow_lds((const void *)kernel, most, p->device, done[both]))
+    experts_choose_kernel<EACH><<<dim3((unsigned)((r.M + 3) / 4)), dim3(256), 0, st>>>(r);
+    if (launch_status("experts_choose_kernel"))
         return 1;
-    kernel<<<dim3(1), dim3(1024), lds, st>>>(r);
+    experts_number_kernel<<<dim3(1), dim3(1024), 0, st>>>(r);
     return launch_status("experts_number_kernel");
 }
 
 template <int TYPE>
 static int run_experts(const hipq_w4_experts_plan *p, const ExpertsLayout &l, RouteArgs r, const void *x, int64_t x_stride, void *y, int64_t y_stride, uint8_t *ws, hipStream_t st)
 {
+    if (l.kernel <= FEW_16)
+        r.placed_share = (float *)(ws + l.share_by_number), r.most_blocks = (int)l.blocks;
     if (r.experts <= 64 ? route<1>(p, r, st) : r.experts <= 256 ? route<4>(p, r, st) : route<16>(p, r, st))
         return 1;
+    if (l.kernel <= FEW_16)
+        return launch_few<TYPE>(p, r, (const uint16_t *)x, x_stride, (uint16_t *)(ws + l.hidden), (float *)(ws + l.part), l.splits, (uint16_t *)y, y_stride, st);
     W4Args a = p->args[0];
     W4Groups g = p->groups[0];
     g.block = r.block, g.count = r.count, g.row = r.row;

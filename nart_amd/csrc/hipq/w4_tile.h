@@ -106,10 +106,13 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void w4_tile_kernel(const W4Args
         column = local / number;
         m0 = __builtin_amdgcn_readfirstlane(groups.block[base + block].first), end = __builtin_amdgcn_readfirstlane(groups.block[base + block].end);
         q += array * groups.q_bytes, scales += array * groups.s_bytes;
-        phase = number >= 8 ? block : item;
+        phase = column + array; // not the block's: which rows are in it may change from call to call
     }
     const int tile0 = column * T::TILES;
-    const int wm = wave % WM, wn = wave / WM;
+    // blocks of an array may have few rows: waves without any, which share their SIMDs with others, leave the multiplies to those (in groups of 64 the branch takes more
+    // registers than there are)
+    const int wm = G::GROUPS ? wave / WN : wave % WM, wn = G::GROUPS ? wave % WN : wave / WM;
+    const bool live = !G::GROUPS || GPB == 2 || m0 + wm * (16 * MT) < end;
     const int share = (a.blocks + (int)gridDim.y - 1) / (int)gridDim.y, kb0 = (int)blockIdx.y * share, mine = min(a.blocks - kb0, share);
     const int steps = mine > 0 ? (mine + WK - 1) / WK : 0;
     // Work-groups begin with different blocks, and go round: in step they would all ask for the same lines of x at once (5 % of 64 rows of
@@ -270,14 +273,16 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void w4_tile_kernel(const W4Args
                 asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * T::LOADS) : "memory");
                 issue(step + AHEAD, to);
                 const uint8_t *from = stage + wk * T::BLOCK;
-                read_weights(0, from);
+                if (live) {
+                    read_weights(0, from);
 #pragma unroll
-                for (int g = 0; g < GPB; g++) {
-                    asm volatile("" ::: "memory"); // two groups' rows at once are more than the registers hold
+                    for (int g = 0; g < GPB; g++) {
+                        asm volatile("" ::: "memory"); // two groups' rows at once are more than the registers hold
 #pragma unroll
-                    for (int t = 0; t < PER; t++)
-                        read_rows(g * PER + t, from);
-                    multiply_group(g, from);
+                        for (int t = 0; t < PER; t++)
+                            read_rows(g * PER + t, from);
+                        multiply_group(g, from);
+                    }
                 }
                 stage = stage == last ? lds : stage + T::STAGE;
                 to = to == last ? lds : to + T::STAGE;
