@@ -575,18 +575,26 @@ static const struct {
     int rows, tiles; // of a work-group
 } SHAPE[SHAPES] = {{"w4_experts_stream_4", 4, 1}, {"w4_experts_stream_16", 16, 1}, {"w4_experts_16x128", 16, 8}, {"w4_experts_32x128", 32, 8}, {"w4_experts_64x128", 64, 8}, {"w4_experts_128x256", 128, 16}};
 
+// Measured over 1 to 1024 tokens of 8 experts of 4096 x 14336 (two for a token), 64 of 2048 x 1408 (six), 128 of 2048 x 768 (eight), 13 of 1056 x 1120 and 32 of 4096 x 2048,
+// us:
+//   * up to 64 tokens and 8 rows of an expert the streams: 16 tokens of the first 164 against 167 with tiles of 16 rows, 64 of the second 98 against 106, but 64 of the
+//     first, 16 rows each, 280 against 253; with blocks of 4 rows up to 2 each: 4 of the first 77 against 84, but 32 of the second, 3 each, 83 against 78;
+//   * tiles of 16, 32, 64 and 128 x 256: 12 rows each 147, 146, 176, 217; 32 each 370, 327, 378, 486; 48 each 282, 239, 233, 253; 96 each 494, 374, 346, 312; but where the
+//     widest would have too few work-groups 71, 60, 53, 67 (333 tokens of the fourth, 77 each).
 static ExpertsLayout layout_of(const hipq_w4_experts_plan *p, int M)
 {
     const hipq_w4_experts_desc &d = p->desc;
     ExpertsLayout l = {};
     l.pairs = (int64_t)M * d.top;
     const int64_t each = l.pairs / d.experts; // an expert's, were all chosen as often
-    if (M <= 16 || (M <= FEW_TOKENS && each <= 6))
-        l.kernel = M <= 4 || each <= 3 ? FEW_4 : FEW_16;
-    else
-        l.kernel = each <= 16 ? TILE_16 : each <= 32 ? TILE_32 : each <= 64 ? TILE_64 : TILE_128_WIDE;
-    l.block_rows = SHAPE[l.kernel].rows;
     const int64_t used = l.pairs < d.experts ? l.pairs : d.experts;
+    // work-groups of the widest kernel in the first product, half a block of an expert's rows more than there are
+    const int64_t wide = (l.pairs / 128 + used / 2) * ((p->tiles[0] + 15) / 16);
+    if (M <= FEW_TOKENS && each <= 8)
+        l.kernel = each <= 2 ? FEW_4 : FEW_16;
+    else
+        l.kernel = each <= 16 ? TILE_16 : each <= 40 ? TILE_32 : each <= 64 || wide < 256 ? TILE_64 : TILE_128_WIDE;
+    l.block_rows = SHAPE[l.kernel].rows;
     l.blocks = used + l.pairs / l.block_rows;
     l.blocks = l.blocks < l.pairs ? l.blocks : l.pairs;
     const int64_t groups = l.blocks * ((p->tiles[1] + SHAPE[l.kernel].tiles - 1) / SHAPE[l.kernel].tiles); // of the second product

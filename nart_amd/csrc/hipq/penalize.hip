@@ -29,7 +29,7 @@ struct Piece<4> {
 
 // THREADS of a work-group, each with 16 tokens of a slice, 16 bytes of scores at a time
 template <int TYPE, int THREADS>
-__global__ __launch_bounds__(THREADS) void penalize_kernel(const PenalizeArgs a)
+__global__ __launch_bounds__(THREADS, 8) void penalize_kernel(const PenalizeArgs a)
 {
     constexpr int EACH = 16, SLICE = EACH * THREADS, WIDE = TYPE == HIPQ_REAL_F32 ? 4 : 8, PIECES = EACH / WIDE, BYTES = TYPE == HIPQ_REAL_F32 ? 4 : 2;
     using piece_t = typename Piece<BYTES>::type;
@@ -41,6 +41,17 @@ __global__ __launch_bounds__(THREADS) void penalize_kernel(const PenalizeArgs a)
     const int tid = threadIdx.x, first = (int)(group - row * a.slices) * SLICE, vocab = d.vocab;
     const uint8_t *const in = (const uint8_t *)d.logits + row * d.stride * BYTES;
     uint8_t *const out = (uint8_t *)d.out + row * d.out_stride * BYTES;
+
+    // the history is on its way before the scores, as loads are waited for in their order
+    constexpr int AHEAD = 4;
+    const bool history = d.tokens != nullptr, biases = d.bias != nullptr;
+    const int32_t *const tokens = d.tokens + row * d.tokens_stride;
+    const int len = !history ? 0 : min(d.lens ? max(d.lens[row], 0) : d.longest, d.longest), prompt = d.prompt_lens ? d.prompt_lens[row] : 0;
+    const float repetition = d.repetition ? d.repetition[row] : 1.0f, frequency = d.frequency ? d.frequency[row] : 0.0f, presence = d.presence ? d.presence[row] : 0.0f;
+    int32_t occurred[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++)
+        occurred[k] = tid + k * THREADS < len ? tokens[tid + k * THREADS] : -1;
 
     u32x4 x[PIECES];
     uint32_t bits[PIECES];
@@ -65,7 +76,6 @@ __global__ __launch_bounds__(THREADS) void penalize_kernel(const PenalizeArgs a)
     }
 
     uint32_t *const entry = counts + SLICE;
-    const bool history = d.tokens != nullptr, biases = d.bias != nullptr;
     if (history || biases) {
         const u32x4 none = {0, 0, 0, 0};
 #pragma unroll
@@ -76,19 +86,23 @@ __global__ __launch_bounds__(THREADS) void penalize_kernel(const PenalizeArgs a)
                 ((u32x4 *)entry)[i * THREADS + tid] = none;
         }
         __syncthreads();
-        if (history) {
-            const int len = min(d.lens ? max(d.lens[row], 0) : d.longest, d.longest), prompt = d.prompt_lens ? d.prompt_lens[row] : 0;
-            const int32_t *const tokens = d.tokens + row * d.tokens_stride;
-#pragma unroll 4
-            for (int i = tid; i < len; i += THREADS) {
-                const uint32_t at = (uint32_t)tokens[i] - (uint32_t)first; // outside of the slice: large
-                if (at < (uint32_t)SLICE) {
-                    if (i < prompt)
-                        atomicOr(&counts[at], OCCURRED);
-                    else
-                        atomicAdd(&counts[at], 1u);
-                }
+        auto count = [&](int i, int32_t token) {
+            const uint32_t at = (uint32_t)token - (uint32_t)first; // outside of the slice: large
+            if (at < (uint32_t)SLICE) {
+                if (i < prompt)
+                    atomicOr(&counts[at], OCCURRED);
+                else
+                    atomicAdd(&counts[at], 1u);
             }
+        };
+        if (history) {
+#pragma unroll
+            for (int k = 0; k < AHEAD; k++)
+                if (tid + k * THREADS < len)
+                    count(tid + k * THREADS, occurred[k]);
+#pragma unroll 4
+            for (int i = tid + AHEAD * THREADS; i < len; i += THREADS)
+                count(i, tokens[i]);
         }
         if (biases) {
             const int32_t *const tokens = d.bias_tokens + row * d.bias_stride;
@@ -100,7 +114,6 @@ __global__ __launch_bounds__(THREADS) void penalize_kernel(const PenalizeArgs a)
         }
         __syncthreads();
     }
-    const float repetition = d.repetition ? d.repetition[row] : 1.0f, frequency = d.frequency ? d.frequency[row] : 0.0f, presence = d.presence ? d.presence[row] : 0.0f;
 #pragma unroll
     for (int p = 0; p < PIECES; p++) {
         const int at = (p * THREADS + tid) * WIDE, v = first + at;
@@ -187,8 +200,9 @@ static int launch_penalize(PenalizeArgs &a, hipStream_t st)
 template <int TYPE>
 static int launch_penalize(PenalizeArgs &a, hipStream_t st)
 {
-    // large slices read a row's history less often, small ones fill the chip
-    return (int64_t)a.d.rows * ((a.d.vocab + 16383) / 16384) >= 512 ? launch_penalize<TYPE, 1024>(a, st) : launch_penalize<TYPE, 256>(a, st);
+    // large slices read a row's history less often, small ones fill the chip: us with 512 and 1024 threads, 8 rows of 128000 9.2 and 10.3, 32 rows 10.2 and 9.6, 256 rows 43 and
+    // 42 (with 256 threads 10.5, 11.7 and 52)
+    return (int64_t)a.d.rows * ((a.d.vocab + 16383) / 16384) >= 256 ? launch_penalize<TYPE, 1024>(a, st) : launch_penalize<TYPE, 512>(a, st);
 }
 
 } // namespace hipq
