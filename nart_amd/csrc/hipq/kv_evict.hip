@@ -370,15 +370,17 @@ static int choose(const EvictArgs &a, int64_t longest, hipStream_t st)
     return launch_status("kv_rank_kernel");
 }
 
+static int width_of(const hipq_kv_cache *c) { return c->dim * (c->quantized ? 1 : 2); }
+static int kinds_of(const hipq_kv_cache *c) { return 2 * ((width_of(c) + 127) / 128) + 1; }
+
 template <int STRETCH>
 static int launch_move(EvictArgs &a, bool in_place, hipStream_t st)
 {
     constexpr int TOKENS = MOVERS / (STRETCH / 16) * STEPS;
     const int64_t heads = (int64_t)a.d.sequences * a.cache.heads;
-    a.kinds = 2 * (a.cache.dim * (a.cache.quantized ? 1 : 2) / STRETCH) + 1;
+    a.kinds = kinds_of(&a.cache);
     const int64_t most = (a.d.budget + TOKENS - 1) / TOKENS, want = (4096 + heads * a.kinds - 1) / (heads * a.kinds);
     a.parts = in_place ? 1 : (int)(want < most ? want : most);
-    HIPQ_REQUIRE(heads * a.kinds * a.parts < (1 << 24), "evict: %d sequences of %d heads", a.d.sequences, a.cache.heads);
     kv_move_kernel<STRETCH><<<dim3((unsigned)(heads * a.kinds * a.parts)), dim3(MOVERS), 0, st>>>(a);
     return launch_status("kv_move_kernel");
 }
@@ -419,12 +421,13 @@ static int check_evict(const hipq_kv_cache *cache, const hipq_kv_evict_desc *d)
                  d->budget);
     HIPQ_REQUIRE(d->longest >= 0, "evict: the longest sequence has %d tokens", d->longest);
     HIPQ_REQUIRE(d->sequences <= 1 || (d->blocks_stride >= d->blocks_per_sequence && d->to_stride >= d->to_per_sequence), "evict: rows of blocks overlap");
-    const bool in_place = d->to == d->blocks;
+    const bool in_place = d->blocks && d->to == d->blocks;
     HIPQ_REQUIRE(!in_place || (d->to_stride == d->blocks_stride && d->to_per_sequence <= d->blocks_per_sequence) || d->sequences <= 1, "evict: in place the blocks are the same");
     const int64_t tokens = (int64_t)d->blocks_per_sequence * cache->page, longest = d->longest < tokens ? d->longest : tokens, most = d->budget < longest ? d->budget : longest;
     HIPQ_REQUIRE(d->to_per_sequence >= 0 && (int64_t)d->to_per_sequence * cache->page >= most, "evict: %d blocks for %lld tokens that stay", d->to_per_sequence, (long long)most);
     // of 2^32 work-items and more only what is left over would run
-    HIPQ_REQUIRE((int64_t)d->sequences * cache->heads * shape_of(cache, d).chunks < (1 << 22), "evict: %d sequences of %d heads", d->sequences, cache->heads);
+    const int64_t heads = (int64_t)d->sequences * cache->heads;
+    HIPQ_REQUIRE(heads * shape_of(cache, d).chunks < (1 << 22) && heads * kinds_of(cache) < (1 << 24) - 4096, "evict: %d sequences of %d heads", d->sequences, cache->heads);
     return 0;
 }
 
@@ -443,7 +446,7 @@ extern "C" int hipq_kv_evict(const hipq_kv_cache *cache, const hipq_kv_evict_des
         return 1;
     if (d->sequences == 0)
         return 0;
-    const bool in_place = d->to == d->blocks;
+    const bool in_place = d->blocks && d->to == d->blocks;
     const int64_t tokens = (int64_t)d->blocks_per_sequence * cache->page, longest = d->longest < tokens ? d->longest : tokens, most = d->budget < longest ? d->budget : longest;
     HIPQ_REQUIRE(d->lens && d->kept && d->left && (most == 0 || (d->weights && d->blocks && d->to)), "evict: a null pointer");
     HIPQ_REQUIRE((uintptr_t)d->weights % 16 == 0, "evict: weights are not at multiples of 16 bytes");
@@ -457,5 +460,5 @@ extern "C" int hipq_kv_evict(const hipq_kv_cache *cache, const hipq_kv_evict_des
     a.hist = (uint32_t *)workspace, a.above = (uint32_t *)((uint8_t *)workspace + s.hist), a.found = (uint32_t *)((uint8_t *)workspace + s.above);
     if (choose(a, longest, (hipStream_t)stream))
         return 1;
-    return cache->dim * (cache->quantized ? 1 : 2) == 64 ? launch_move<64>(a, in_place, (hipStream_t)stream) : launch_move<128>(a, in_place, (hipStream_t)stream);
+    return width_of(cache) == 64 ? launch_move<64>(a, in_place, (hipStream_t)stream) : launch_move<128>(a, in_place, (hipStream_t)stream);
 }

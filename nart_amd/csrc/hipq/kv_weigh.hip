@@ -10,6 +10,7 @@
 #include <type_traits>
 
 #include "kv_frag.h"
+#include "overlap.h"
 
 namespace hipq {
 
@@ -608,6 +609,20 @@ static hipq_kv_attend_desc attend_desc(const hipq_kv_weigh_desc *d)
     return t;
 }
 
+static int check_weigh(const hipq_kv_cache *cache, const hipq_kv_attend_desc &d, WeighShape *shape)
+{
+    if (check_attend("weigh", cache, &d))
+        return 1;
+    const WeighShape s = shape_of(cache, &d);
+    const int64_t heads = (int64_t)d.sequences * cache->heads;
+    // item numbers are 32 bits, and of 2^32 work-items and more only what is left over would run
+    HIPQ_REQUIRE(heads * s.row_blocks * s.splits * 16 * s.rt < ((int64_t)1 << 31) && heads * s.row_blocks * s.splits <= (1 << 24) - 8 && heads * s.chunks <= (1 << 24) - 8
+                     && heads * s.rows < ((int64_t)1 << 28),
+                 "weigh: %lld work-groups", (long long)(heads * (s.chunks > (int64_t)s.row_blocks * s.splits ? s.chunks : (int64_t)s.row_blocks * s.splits)));
+    *shape = s;
+    return 0;
+}
+
 } // namespace hipq
 
 using namespace hipq;
@@ -617,8 +632,8 @@ extern "C" size_t hipq_kv_weigh_workspace(const hipq_kv_cache *cache, const hipq
     clear_error();
     if (!desc)
         return 0;
-    const hipq_kv_attend_desc d = attend_desc(desc);
-    return check_attend("weigh", cache, &d) ? 0 : shape_of(cache, &d).workspace;
+    WeighShape s;
+    return check_weigh(cache, attend_desc(desc), &s) ? 0 : s.workspace;
 }
 
 extern "C" int hipq_kv_weigh(const hipq_kv_cache *cache, const hipq_kv_weigh_desc *desc, void *workspace, size_t workspace_bytes, void *stream)
@@ -626,20 +641,17 @@ extern "C" int hipq_kv_weigh(const hipq_kv_cache *cache, const hipq_kv_weigh_des
     clear_error();
     HIPQ_REQUIRE(desc, "weigh: a null pointer");
     const hipq_kv_attend_desc d = attend_desc(desc);
-    if (check_attend("weigh", cache, &d))
+    WeighShape s;
+    if (check_weigh(cache, d, &s))
         return 1;
-    const WeighShape s = shape_of(cache, &d);
-    const int64_t heads = (int64_t)d.sequences * cache->heads;
-    if (heads * s.rows == 0 || d.tokens == 0 || s.chunks == 0 || cache->pages == 0)
+    if (d.sequences == 0 || s.rows == 0 || d.tokens == 0 || s.chunks == 0 || cache->pages == 0)
         return 0;
     HIPQ_REQUIRE(d.q && d.starts && d.lens && d.blocks && desc->weights && desc->out, "weigh: a null pointer");
     HIPQ_REQUIRE((uintptr_t)d.q % 16 == 0 && (d.q_token | d.q_head) % 8 == 0, "weigh: heads have to start at multiples of 16 bytes");
     HIPQ_REQUIRE(((uintptr_t)desc->weights | (uintptr_t)desc->out) % 16 == 0, "weigh: weights are not at multiples of 16 bytes");
+    const int64_t pool = (int64_t)cache->pages * cache->heads * cache->page * 4;
+    HIPQ_REQUIRE(desc->out == desc->weights || !overlap({(int64_t)(uintptr_t)desc->weights, 0, pool, 1}, {(int64_t)(uintptr_t)desc->out, 0, pool, 1}), "weigh: out lies over the weights");
     HIPQ_REQUIRE(workspace && workspace_bytes >= s.workspace && (uintptr_t)workspace % 16 == 0, "weigh: a workspace of %zu bytes is needed", s.workspace);
-    // item numbers are 32 bits, and of 2^32 work-items and more only what is left over would run
-    HIPQ_REQUIRE(heads * s.row_blocks * s.splits * 16 * s.rt < ((int64_t)1 << 31) && heads * s.row_blocks * s.splits <= (1 << 24) - 8 && heads * s.chunks <= (1 << 24) - 8
-                     && heads * s.rows < ((int64_t)1 << 28),
-                 "weigh: %lld work-groups", (long long)(heads * (s.chunks > (int64_t)s.row_blocks * s.splits ? s.chunks : (int64_t)s.row_blocks * s.splits)));
     WeighArgs w = {};
     w.a.cache = *cache, w.a.d = d;
     w.a.scale2 = d.scale * 1.4426950408889634f;

@@ -854,7 +854,7 @@ class KvCache:
         if left is None:
             left = torch.empty(lens.shape, dtype=torch.int32, device=lens.device)
         if kept is None:
-            kept = torch.empty((lens.shape[0], self.k.shape[1], budget), dtype=torch.int32, device=lens.device)
+            kept = torch.empty((lens.shape[0], self.k.shape[1], max(0, budget)), dtype=torch.int32, device=lens.device)
         rc = calls.kv_evict(self._struct, self._device, weights, lens, blocks, blocks if to is None else to, left, kept, budget, recent, first, longest,
                             lambda count: _bytes_like(weights, count))
         if rc:
