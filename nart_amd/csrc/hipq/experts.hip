@@ -47,26 +47,28 @@ struct Choice {
 };
 // A token's experts, lane s has the s-th; its scores over the lanes of a wave: lane l has those of experts l, l + 64, ..., EACH of them
 template <int EACH>
-__device__ static __forceinline__ void load_scores(const RouteArgs &a, int t, int lane, uint32_t (&key)[EACH]) // in the order of the scores; 0: never taken
+__device__ static __forceinline__ void load_scores(const RouteArgs &a, int t, int lane, uint32_t (&raw)[EACH]) // as they are: nothing waits for them here
 {
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
-        const int e = i * 64 + lane;
-        key[i] = 0;
-        if (e < a.experts) {
-            const int64_t at = t * a.stride + e;
-            const float x = a.type == HIPQ_REAL_F32 ? ((const float *)a.logits)[at]
-                            : a.type == HIPQ_REAL_F16 ? Real16<HIPQ_REAL_F16>::low(((const uint16_t *)a.logits)[at])
-                                                      : Real16<HIPQ_REAL_BF16>::low(((const uint16_t *)a.logits)[at]);
-            const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f); // -0 is 0
-            key[i] = !(x > -__builtin_inff()) ? 0 : u & 0x80000000u ? ~u : u | 0x80000000u;
-        }
+        const int64_t at = t * a.stride + min(i * 64 + lane, a.experts - 1);
+        if (a.type == HIPQ_REAL_F32)
+            raw[i] = ((const uint32_t *)a.logits)[at];
+        else
+            raw[i] = ((const uint16_t *)a.logits)[at];
     }
 }
 
 template <int EACH>
-__device__ static __forceinline__ Choice choose(const RouteArgs &a, uint32_t (&key)[EACH], int lane)
+__device__ static __forceinline__ Choice choose(const RouteArgs &a, const uint32_t (&raw)[EACH], int lane)
 {
+    uint32_t key[EACH]; // in the order of the scores; 0: never taken
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        const float x = a.type == HIPQ_REAL_F32 ? __builtin_bit_cast(float, raw[i]) : a.type == HIPQ_REAL_F16 ? Real16<HIPQ_REAL_F16>::low(raw[i]) : Real16<HIPQ_REAL_BF16>::low(raw[i]);
+        const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f); // -0 is 0
+        key[i] = i * 64 + lane >= a.experts || !(x > -__builtin_inff()) ? 0 : u & 0x80000000u ? ~u : u | 0x80000000u;
+    }
     auto largest = [&] {
         uint32_t most = 0;
 #pragma unroll
@@ -122,9 +124,9 @@ __global__ __launch_bounds__(256) void experts_choose_kernel(const RouteArgs a)
     const int lane = threadIdx.x & 63;
     if (t >= a.M)
         return;
-    uint32_t key[EACH];
-    load_scores<EACH>(a, (int)t, lane, key);
-    const Choice own = choose<EACH>(a, key, lane);
+    uint32_t raw[EACH];
+    load_scores<EACH>(a, (int)t, lane, raw);
+    const Choice own = choose<EACH>(a, raw, lane);
     if (lane < a.top)
         a.chosen[t * a.top + lane] = own.expert, a.share[t * a.top + lane] = own.share;
 }
@@ -166,18 +168,19 @@ __global__ __launch_bounds__(1024) void experts_route_kernel(const RouteArgs a)
     __shared__ float share[CHOOSE_TOKENS * MOST_TOP];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     constexpr bool AHEAD = EACH <= 4; // more than that are too many registers
-    uint32_t key[EACH], next[EACH];
-    load_scores<EACH>(a, min(wave, a.M - 1), lane, next);
+    uint32_t raw[EACH], next[EACH];
+    if (wave < a.M)
+        load_scores<EACH>(a, wave, lane, next);
 #pragma unroll 1
     for (int t = wave; t < a.M; t += 16) {
-        if (!AHEAD)
-            load_scores<EACH>(a, t, lane, next);
 #pragma unroll
         for (int i = 0; i < EACH; i++)
-            key[i] = next[i];
-        if (AHEAD)
-            load_scores<EACH>(a, min(t + 16, a.M - 1), lane, next);
-        const Choice own = choose<EACH>(a, key, lane);
+            raw[i] = next[i];
+        if (AHEAD && t + 16 < a.M)
+            load_scores<EACH>(a, t + 16, lane, next);
+        const Choice own = choose<EACH>(a, raw, lane);
+        if (!AHEAD && t + 16 < a.M)
+            load_scores<EACH>(a, t + 16, lane, next);
         if (lane < a.top)
             chosen[t * a.top + lane] = own.expert, share[t * a.top + lane] = a.share[t * a.top + lane] = own.share;
     }

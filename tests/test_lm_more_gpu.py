@@ -75,7 +75,7 @@ def test_experts_shapes(m, experts, top, k, inner, n, group):
 
 
 @pytest.mark.parametrize("dtype, group, zeros", [(BF16, 128, False), (F16, 128, True), (BF16, 64, True), (F16, 64, False), (BF16, 32, True), (F16, 32, False)])
-@pytest.mark.parametrize("m, experts, top, kernel", [(3, 8, 2, "w4_experts_stream_4"), (24, 40, 3, "w4_experts_stream_4"), (16, 8, 4, "w4_experts_stream_16"), (60, 30, 3, "w4_experts_stream_16"), (40, 8, 2, "w4_experts_16x128"), (60, 4, 2, "w4_experts_32x128"), (100, 4, 2, "w4_experts_64x128"), (300, 4, 2, "w4_experts_128x256")])
+@pytest.mark.parametrize("m, experts, top, kernel", [(3, 8, 2, "w4_experts_stream_4"), (24, 40, 3, "w4_experts_stream_4"), (16, 8, 4, "w4_experts_stream_16"), (60, 30, 3, "w4_experts_stream_16"), (40, 8, 2, "w4_experts_16x128"), (60, 4, 2, "w4_experts_32x128"), (100, 4, 2, "w4_experts_64x128"), (1500, 4, 2, "w4_experts_128x256")])
 def test_experts_kernels(m, experts, top, kernel, dtype, group, zeros):
     """Every kernel, with reductions that end inside a block and are shared by work-groups."""
     g = gen(m + group)
