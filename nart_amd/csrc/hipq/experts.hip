@@ -835,12 +835,10 @@ extern "C" int hipq_w4_experts_create(const hipq_w4_experts_desc *d, const uint8
         PackArgs k = {};
         k.rows = a.N, k.K = a.K, k.group = d->group, k.groups = (a.K + d->group - 1) / d->group, k.blocks = a.blocks, k.tiles = round_up(p->tiles[i], 16), k.gated = !i;
         const size_t rows = (size_t)a.N * (i ? 1 : 2);
-        for (int x = 0; x < d->experts && !bad; x++) {
-            k.q = (i ? down : gate_up) + x * rows * (a.K / 2), k.scales = (const uint16_t *)(i ? down_scales : gate_up_scales) + x * rows * k.groups;
-            k.zeros = a.zeros ? (i ? down_zeros : gate_up_zeros) + x * rows * k.groups : nullptr;
-            k.to_q = const_cast<uint8_t *>(a.q) + x * q_bytes[i], k.to_scales = (uint16_t *)(a.scales + x * s_bytes[i]), k.to_nothing = (u32x4 *)p->memory;
-            bad = w4_pack(k, d->type, (hipStream_t)stream);
-        }
+        k.q = i ? down : gate_up, k.scales = (const uint16_t *)(i ? down_scales : gate_up_scales), k.zeros = i ? down_zeros : gate_up_zeros;
+        k.to_q = const_cast<uint8_t *>(a.q), k.to_scales = (uint16_t *)const_cast<uint8_t *>(a.scales), k.to_nothing = (u32x4 *)p->memory;
+        k.arrays = d->experts, k.q_step = rows * (a.K / 2), k.s_step = rows * k.groups, k.to_q_step = q_bytes[i], k.to_s_step = s_bytes[i];
+        bad = bad || w4_pack(k, d->type, (hipStream_t)stream);
     }
     if (!bad && (e = hipStreamSynchronize((hipStream_t)stream)) != hipSuccess)
         bad = fail("experts: laying the weights out failed: %s", hipGetErrorString(e));

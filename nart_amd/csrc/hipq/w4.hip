@@ -176,8 +176,11 @@ __device__ static __forceinline__ int64_t source_row(const PackArgs &p, int tile
     return n < p.rows ? (int64_t)n + (p.gated && tile % 2 ? p.rows : 0) : -1;
 }
 
-__global__ __launch_bounds__(256) void w4_pack_kernel(const PackArgs p)
+__global__ __launch_bounds__(256) void w4_pack_kernel(const PackArgs all)
 {
+    PackArgs p = all;
+    p.q += blockIdx.y * p.q_step, p.scales += blockIdx.y * p.s_step, p.zeros += p.zeros ? blockIdx.y * p.s_step : 0;
+    p.to_q += blockIdx.y * p.to_q_step, p.to_scales += blockIdx.y * p.to_s_step / 2;
     const int lane = threadIdx.x & 63, c = lane & 15, j = lane >> 4;
     const int gpb = 128 / p.group;
     if (blockIdx.x == 0 && threadIdx.x < 16)
@@ -220,7 +223,7 @@ int w4_pack(PackArgs p, int type, hipStream_t st)
 {
     p.shift = type == HIPQ_REAL_BF16 ? Nibbles<HIPQ_REAL_BF16>::SHIFT : Nibbles<HIPQ_REAL_F16>::SHIFT;
     const size_t groups = ((size_t)p.tiles * p.blocks + 3) / 4;
-    w4_pack_kernel<<<dim3((unsigned)(groups < 16384 ? groups : 16384)), dim3(256), 0, st>>>(p);
+    w4_pack_kernel<<<dim3((unsigned)(groups < 16384 ? groups : 16384), p.arrays > 1 ? p.arrays : 1), dim3(256), 0, st>>>(p);
     return launch_status("w4_pack_kernel");
 }
 

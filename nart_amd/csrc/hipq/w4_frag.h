@@ -124,8 +124,11 @@ struct PackArgs { // `shift` is w4_pack's
     u32x4 *to_nothing;
     int rows, K, group, groups, blocks, tiles, gated; // rows: of one projection
     int shift;
+    // several arrays of the same shape in one launch (0: one), and how far apart they lie: q and zeros in bytes, scales in numbers, where they go in bytes
+    int arrays;
+    size_t q_step, s_step, to_q_step, to_s_step;
 };
-int w4_pack(PackArgs p, int type, hipStream_t st); // a launch; `tiles` of 16 rows are written, those behind the last row as zeros
+int w4_pack(PackArgs p, int type, hipStream_t st); // a launch; `tiles` of 16 rows of each array are written, those behind the last row as zeros
 
 static int round_up(int v, int to) { return (v + to - 1) / to * to; }
 

@@ -31,9 +31,9 @@ def layers_of_experts():
         if rc == 0:
             hipq.lib().hipq_w4_experts_destroy(h)
         return rc
-    r = Refusals(call, 8)
+    r = Refusals(call, 2)
     r.takes(2, experts=1, top=1, N=1, K=32, inner=32, group=32, type=F16, activation=2, scores=1, normalize=0, gate_up_zeros=P, down_zeros=P)
-    r.takes(2048, experts=1024, top=16, N=16, K=32, inner=32)
+    r.takes(2, experts=1024, top=16, N=16, K=32, inner=32)
     for type in (F32, 3, -1):
         r.refuses("neither float16 nor bfloat16", type=type)
     for group in (0, 16, 256):
