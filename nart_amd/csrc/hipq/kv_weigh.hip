@@ -540,15 +540,16 @@ static WeighShape shape_of(const hipq_kv_cache *c, const hipq_kv_attend_desc *d)
     s.row_blocks = (s.rows + 16 * s.rt - 1) / (16 * s.rt);
     const int64_t longest = d->longest < (int64_t)d->blocks_per_sequence * c->page ? d->longest : (int64_t)d->blocks_per_sequence * c->page;
     const int64_t items = (int64_t)d->sequences * c->heads * s.row_blocks;
-    // all work-groups that fit at once: three or four a CU, and of those that bring their rows into LDS first each with four tiles for a wave at least
-    const int64_t target = s.rt <= 2 ? 1024 : 768, least = s.rt <= 2 ? 256 : 512, want = items ? target / items : 1, most = (longest + least - 1) / least;
+    // Two work-groups a CU, with two tiles for a wave at least, four where rows are brought into LDS first: us with 256, 512 and 1024, one token of 2 x up to 131072 157, 142,
+    // 142, of one of up to 20000 19, 19, 21, four of 4 x up to 8000 31, 29, 31; 32 of one of up to 30000 in 8 bits 41, with 1024 and two tiles 49
+    const int64_t target = 512, least = s.rt <= 2 ? 256 : 512, want = items ? target / items : 1, most = (longest + least - 1) / least;
     s.splits = (int)(want < most ? want : most);
     s.splits = s.splits < 1 ? 1 : s.splits > 256 ? 256 : s.splits;
     s.scores = s.rows <= 32 && s.rows * 8 <= width;
     // once all rows are in LDS at once the second launch joins the parts itself
     s.lse = !s.scores && s.rows > 16 * (c->dim == 256 ? BLOCKS<256> : BLOCKS<128>);
-    // from scores, four tokens a thread; from keys, as many tokens of a work-group as fill the chip once, with three a CU
-    const int64_t share = (longest * d->sequences * c->heads / 768 + 127) / 128 * 128;
+    // from scores, four tokens a thread; from keys, as many tokens of a work-group as fill the chip once with two a CU (us with 512, 768, 1536 of them: 41, 44, 44)
+    const int64_t share = (longest * d->sequences * c->heads / 512 + 127) / 128 * 128;
     s.chunk = s.scores ? 1024 : (int)(share < 128 ? 128 : share > 1024 ? 1024 : share);
     s.chunks = (int)((longest + s.chunk - 1) / s.chunk);
     const size_t heads = (size_t)d->sequences * c->heads;
