@@ -243,19 +243,23 @@ __global__ __launch_bounds__(1024) void experts_number_kernel(const RouteArgs a)
 {
     __shared__ int32_t counts[MOST_EXPERTS], scan[32];
     const int tid = threadIdx.x, pairs = a.M * a.top;
-    constexpr int STEPS = 8; // on their way at once
+    constexpr int STEPS = 8; // on their way at once; the first stay in registers, others' places wait in memory
+    int e[STEPS], place[STEPS];
     counts[tid] = 0;
     __syncthreads();
 #pragma unroll 1
-    for (int p0 = tid; p0 < pairs; p0 += 1024 * STEPS) {
-        int e[STEPS];
+    for (int p0 = tid + (pairs - 1) / (1024 * STEPS) * (1024 * STEPS); p0 >= 0; p0 -= 1024 * STEPS) { // the first last
 #pragma unroll
         for (int k = 0; k < STEPS; k++)
             e[k] = p0 + 1024 * k < pairs ? a.chosen[p0 + 1024 * k] : -1;
 #pragma unroll
         for (int k = 0; k < STEPS; k++)
-            if (e[k] >= 0)
-                a.place[p0 + 1024 * k] = atomicAdd(&counts[e[k]], 1);
+            place[k] = e[k] >= 0 ? atomicAdd(&counts[e[k]], 1) : 0;
+        if (p0 >= 1024 * STEPS)
+#pragma unroll
+            for (int k = 0; k < STEPS; k++)
+                if (p0 + 1024 * k < pairs)
+                    a.place[p0 + 1024 * k] = place[k];
     }
     __syncthreads();
     const int first = list_blocks(a, tid < a.experts ? counts[tid] : 0, scan);
@@ -264,12 +268,12 @@ __global__ __launch_bounds__(1024) void experts_number_kernel(const RouteArgs a)
     __syncthreads();
 #pragma unroll 1
     for (int p0 = tid; p0 < pairs; p0 += 1024 * STEPS) {
-        int e[STEPS], place[STEPS];
+        if (p0 >= 1024 * STEPS)
 #pragma unroll
-        for (int k = 0; k < STEPS; k++) {
-            const int p = p0 + 1024 * k;
-            e[k] = p < pairs ? a.chosen[p] : -1, place[k] = p < pairs ? a.place[p] : 0;
-        }
+            for (int k = 0; k < STEPS; k++) {
+                const int p = p0 + 1024 * k;
+                e[k] = p < pairs ? a.chosen[p] : -1, place[k] = p < pairs ? a.place[p] : 0;
+            }
 #pragma unroll
         for (int k = 0; k < STEPS; k++) {
             const int p = p0 + 1024 * k;
@@ -397,11 +401,13 @@ struct FewArgs {
     float *part;             // [split][token][column] of the second launch, where work-groups share a tile
 };
 
-// The hidden rows: a work-group has two tiles of the gate and their two of the other projection, for a block of rows, and WAVES waves take the blocks of k in turn.
-template <int TYPE, int GPB, bool ZEROS, int ROWS, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, GPB == 1 ? 3 : 2) void experts_few_up_kernel(const FewArgs f)
+// The hidden rows: a work-group has a tile of the gate and its one of the other projection, for a block of rows, and four waves take the blocks of k in turn, two
+// ahead each: little for one wave, but many are there.  us of the whole layer with 2 and 4 tiles, 4 and 8 waves, 2 and 3 or 4 blocks: one token through 2 of 8 experts of 4096 x 14336
+// 47.5; 48.1 with 4 tiles; 48.1 with 8 waves; 50.0 with 4 blocks; 54 with 4 tiles and 3 blocks; 16 tokens through 6 of 64 of 2048 x 1408 51.8, 52.5, 55.1, 53.2, 56.5.
+template <int TYPE, int GPB, bool ZEROS, int ROWS>
+__global__ __launch_bounds__(256) void experts_few_up_kernel(const FewArgs f)
 {
-    constexpr int NT = 4, DEPTH = ROWS == 4 && GPB == 1 ? 3 : 2;
+    constexpr int WAVES = 4, NT = 2, DEPTH = 2;
     using S = Stream<TYPE, GPB, ZEROS, ROWS, NT, DEPTH>;
     __shared__ f32x4 red[WAVES][NT][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, j = lane >> 4;
@@ -431,12 +437,12 @@ __global__ __launch_bounds__(WAVES * 64, GPB == 1 ? 3 : 2) void experts_few_up_k
     for (int nt = 0; nt < NT; nt++)
         red[wave][nt][lane] = stream.total[nt];
     __syncthreads();
-    if (tid < NT / 2 * 64) {
-        f32x4 gate = red[0][wave * 2][lane], up = red[0][wave * 2 + 1][lane];
+    if (wave == 0) {
+        f32x4 gate = red[0][0][lane], up = red[0][1][lane];
 #pragma unroll
         for (int o = 1; o < WAVES; o++)
-            gate += red[o][wave * 2][lane], up += red[o][wave * 2 + 1][lane];
-        const int n = (tile0 / 2 + wave) * 16 + c;
+            gate += red[o][0][lane], up += red[o][1][lane];
+        const int n = tile0 / 2 * 16 + c;
 #pragma unroll
         for (int i = 0; i < 4; i++)
             if (n < a.N && 4 * j + i < rows)
@@ -444,13 +450,13 @@ __global__ __launch_bounds__(WAVES * 64, GPB == 1 ? 3 : 2) void experts_few_up_k
     }
 }
 
-// The result: a work-group has a tile of outputs, its 16 waves the same number of blocks each - of all blocks of rows and k, one after the other - and every
+// The result: a work-group has a tile of outputs, its waves the same number of blocks each - of all blocks of rows and k, one after the other - and every
 // wave adds up what it has of each token, in LDS, where they meet.  Where there are fewer tiles than CUs, and much to read, gridDim.y work-groups share them, and
 // another launch adds up what they leave.  (The last of them to end could do that, but to have written what others read takes a write-back of the L2: 90 us.)
-template <int TYPE, int GPB, bool ZEROS, int ROWS>
-__global__ __launch_bounds__(1024) void experts_few_down_kernel(const FewArgs f)
+template <int TYPE, int GPB, bool ZEROS, int ROWS, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void experts_few_down_kernel(const FewArgs f)
 {
-    constexpr int WAVES = 16, DEPTH = ROWS == 4 ? (GPB == 4 ? 5 : 6) : GPB == 1 ? 4 : 3;
+    constexpr int DEPTH = 2;
     using S = Stream<TYPE, GPB, ZEROS, ROWS, 1, DEPTH>;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const RouteArgs &r = f.r;
@@ -462,12 +468,12 @@ __global__ __launch_bounds__(1024) void experts_few_down_kernel(const FewArgs f)
     int32_t *const block = token + pairs;                 // [block]: expert, first, end
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, j = lane >> 4;
     const int tile = blockIdx.x, items = __builtin_amdgcn_readfirstlane(*r.count) * a.blocks;
-    if (tid < pairs) { // what lies behind their ends is not looked at
-        share[tid] = r.placed_share[tid], token[tid] = r.row[tid];
-        if (tid < r.most_blocks)
-            block[3 * tid] = r.block[tid].array, block[3 * tid + 1] = r.block[tid].first, block[3 * tid + 2] = r.block[tid].end;
+    for (int i = tid; i < pairs; i += WAVES * 64) { // what lies behind their ends is not looked at
+        share[i] = r.placed_share[i], token[i] = r.row[i];
+        if (i < r.most_blocks)
+            block[3 * i] = r.block[i].array, block[3 * i + 1] = r.block[i].first, block[3 * i + 2] = r.block[i].end;
     }
-    for (int i = tid; i < WAVES * r.M * 16; i += 1024)
+    for (int i = tid; i < WAVES * r.M * 16; i += WAVES * 64)
         sums[i] = 0;
     __syncthreads();
     const int split = blockIdx.y, splits = gridDim.y, own = split * WAVES + wave, all = splits * WAVES;
@@ -519,20 +525,17 @@ __global__ __launch_bounds__(1024) void experts_few_down_kernel(const FewArgs f)
                 }
     }
     __syncthreads();
-    float v = 0;
-    if (tid < r.M * 16) { // up to 64 tokens: one value a thread
+    for (int i = tid; i < r.M * 16; i += WAVES * 64) {
+        float v = 0;
 #pragma unroll
         for (int o = 0; o < WAVES; o++)
-            v += sums[o * r.M * 16 + tid];
+            v += sums[o * r.M * 16 + i];
+        const int t = i / 16, n = tile * 16 + i % 16;
+        if (splits > 1)
+            f.part[((int64_t)split * r.M + t) * (gridDim.x * 16) + n] = v;
+        else if (n < a.N)
+            a.y[(int64_t)t * a.y_stride + n] = rounded<TYPE>(v);
     }
-    if (splits > 1) {
-        if (tid < r.M * 16)
-            f.part[((int64_t)split * r.M + tid / 16) * (gridDim.x * 16) + tile * 16 + tid % 16] = v;
-        return;
-    }
-    const int n = tile * 16 + tid % 16;
-    if (tid < r.M * 16 && n < a.N)
-        a.y[(int64_t)(tid / 16) * a.y_stride + n] = rounded<TYPE>(v);
 }
 
 template <int TYPE>
@@ -684,28 +687,32 @@ static int launch_experts(const hipq_w4_experts_plan *p, const ExpertsLayout &l,
                                  : launch_experts<TYPE, 4>(p, l, a, g, tiles, splits, ws, part, st);
 }
 
+template <int TYPE, int GPB, bool ZEROS, int ROWS, int WAVES>
+static int launch_few_down(const hipq_w4_experts_plan *p, const FewArgs &f, int splits, hipStream_t st)
+{
+    constexpr int MOST = (WAVES * FEW_TOKENS * 16 + 5 * FEW_PAIRS) * 4;
+    const int lds = (WAVES * f.r.M * 16 + 5 * f.r.M * f.r.top) * 4;
+    const auto kernel = experts_few_down_kernel<TYPE, GPB, ZEROS, ROWS, WAVES>;
+    static thread_local bool done[64] = {};
+    if (lds > 65536 && allow_lds((const void *)kernel, MOST, p->device, done))
+        return 1;
+    kernel<<<dim3(p->tiles[1], splits), dim3(WAVES * 64), lds, st>>>(f);
+    return launch_status("experts_few_down_kernel");
+}
+
+// 16 waves of a work-group where a CU has one, 8 where it has two: us, one token through one of 16 experts of 5120 x 8192 with 5120 outputs, 320 work-groups, 26 and 24; through 2 of 8
+// of 4096 x 14336, 256, 48 and 52
 template <int TYPE, int GPB, bool ZEROS, int ROWS>
 static int launch_few(const hipq_w4_experts_plan *p, FewArgs f, const uint16_t *x, int64_t x_stride, uint16_t *hidden, float *part, int splits, uint16_t *y, int64_t y_stride, hipStream_t st)
 {
-    f.a = p->args[0], f.q_bytes = p->groups[0].q_bytes, f.s_bytes = p->groups[0].s_bytes, f.groups = (p->tiles[0] + 3) / 4;
+    f.a = p->args[0], f.q_bytes = p->groups[0].q_bytes, f.s_bytes = p->groups[0].s_bytes, f.groups = p->tiles[0] / 2;
     f.a.x = x, f.a.x_stride = x_stride, f.a.y = hidden, f.a.y_stride = p->desc.inner;
-    const int groups = f.r.most_blocks * f.groups;
-    // 2000 waves and more, however few blocks of k there are for each
-    if (groups >= 512)
-        experts_few_up_kernel<TYPE, GPB, ZEROS, ROWS, 4><<<dim3(groups), dim3(256), 0, st>>>(f);
-    else
-        experts_few_up_kernel<TYPE, GPB, ZEROS, ROWS, 8><<<dim3(groups), dim3(512), 0, st>>>(f);
+    experts_few_up_kernel<TYPE, GPB, ZEROS, ROWS><<<dim3(f.r.most_blocks * f.groups), dim3(256), 0, st>>>(f);
     if (launch_status("experts_few_up_kernel"))
         return 1;
     f.a = p->args[1], f.q_bytes = p->groups[1].q_bytes, f.s_bytes = p->groups[1].s_bytes;
     f.a.x = hidden, f.a.x_stride = p->desc.inner, f.a.y = y, f.a.y_stride = y_stride, f.part = part;
-    constexpr int MOST = (16 * FEW_TOKENS * 16 + 5 * FEW_PAIRS) * 4;
-    const int lds = (16 * f.r.M * 16 + 5 * f.r.M * f.r.top) * 4;
-    static thread_local bool done[64] = {};
-    if (lds > 65536 && allow_lds((const void *)experts_few_down_kernel<TYPE, GPB, ZEROS, ROWS>, MOST, p->device, done))
-        return 1;
-    experts_few_down_kernel<TYPE, GPB, ZEROS, ROWS><<<dim3(p->tiles[1], splits), dim3(1024), lds, st>>>(f);
-    if (launch_status("experts_few_down_kernel"))
+    if (p->tiles[1] <= 256 ? launch_few_down<TYPE, GPB, ZEROS, ROWS, 16>(p, f, splits, st) : launch_few_down<TYPE, GPB, ZEROS, ROWS, 8>(p, f, splits, st))
         return 1;
     if (splits == 1)
         return 0;

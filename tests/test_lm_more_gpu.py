@@ -117,6 +117,36 @@ def test_experts_all_of_one(m):
     layer.check(randn(g, F16, m, 32), randn(g, F32, m, 1024))
 
 
+@pytest.mark.parametrize("m, experts, top", [(1, 5, 2), (9, 40, 3), (40, 60, 4), (60, 7, 1), (300, 3, 1)])
+def test_experts_wide_outputs(m, experts, top):
+    """More tiles of outputs than CUs, which other numbers of waves compute."""
+    g = gen(m)
+    layer = Layer(g, BF16, experts, 64, 160, 4200, top, 32)
+    layer.check(randn(g, BF16, m, 64), randn(g, F32, m, experts))
+
+
+@pytest.mark.parametrize("m, experts, top", [(3000, 5, 3), (9000, 300, 1)])
+def test_experts_many_pairs(m, experts, top):
+    """More pairs than one work-group numbers at once."""
+    g = gen(m)
+    layer = Layer(g, F16, experts, 64, 32, 40, top, 64)
+    layer.check(randn(g, F16, m, 64), randn(g, F32, m, experts))
+
+
+@pytest.mark.parametrize("m, experts", [(3, 4), (14, 4), (40, 30), (60, 3), (200, 4), (900, 4)])
+def test_experts_rows_that_are_not_finite(m, experts):
+    """An infinity or NaN in a row of x stays in its token's result."""
+    g = gen(m)
+    layer = Layer(g, BF16, experts, 256, 128, 90, 2, 64)
+    x, s = randn(g, BF16, m, 256), randn(g, F32, m, experts)
+    clean = layer.plan(x, s)
+    x[1, 5], x[m - 1, 200] = math.inf, math.nan
+    got = layer.plan(x, s)
+    assert torch.isnan(got[1]).all() and torch.isnan(got[m - 1]).all()
+    same = [i for i in range(m) if i not in (1, m - 1)]
+    assert torch.equal(got[same], clean[same])
+
+
 @pytest.mark.parametrize("m", [1, 5, 24, 200])
 def test_experts_rows_with_gaps(m):
     g = gen(m)
@@ -509,3 +539,59 @@ def test_weigh_and_evict_in_a_graph():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip((*pools, out, kept), want))
         assert lens.tolist() == [64, 64]
+
+
+# ---- together --------------------------------------------------------------------------------------------------------------
+def test_conversations_with_a_budget():
+    """Steps of a small model as a program makes them: queries, keys and values by 4-bit products into the cache, attention and its weights, the cache held to a budget,
+    experts, penalties on the scores, the next token.  Each operator is held against its formula on what it was given."""
+    g = gen(11)
+    b, heads, kv, dim, hidden, vocab, budget = 3, 4, 2, 64, 256, 300, 40
+    s = Sequences(g, BF16, [60, 33, 41], kv, dim, 16, False, more=3)
+    s.weights.zero_()
+    table = hipq.rotation_table(500, dim)
+    quant = lambda rows, k: (whole(g, 0, 256, torch.uint8, rows, k // 2), (torch.rand((rows, k // 64), device="cuda", generator=g) * 0.01).to(BF16))  # noqa: E731
+    wqkv, wo, head = (hipq.LinearW4(*quant(*shape), 64) for shape in (((heads + 2 * kv) * dim, hidden), (hidden, heads * dim), (vocab, hidden)))
+    layer = Layer(g, BF16, 6, hidden, 96, hidden, 2, 64, scores="sigmoid")
+    router, embedding = randn(g, BF16, hidden, 6) * 0.1, randn(g, BF16, vocab, hidden)
+    position, lens, blocks, starts = s.ints([100, 80, 200]), s.ints(s.lens), s.ints(s.blocks), s.ints(range(b + 1))
+    history, count = torch.full((b, 20), -1, dtype=torch.int32, device="cuda"), s.ints([0] * b)
+    value = lambda v: torch.full((b,), v, device="cuda")  # noqa: E731
+    kept = torch.zeros((b, kv, budget), dtype=torch.int32, device="cuda")
+    token = whole(g, 0, vocab, torch.int64, b)
+    rows = torch.arange(b, device="cuda")
+    evicted = 0
+    for step in range(12):
+        x = embedding[token]
+        qkv = wqkv(x).view(b, heads + 2 * kv, dim)
+        slots = (blocks.gather(1, (lens[:, None] // 16).long())[:, 0] * 16 + lens % 16).to(torch.int32)
+        q = s.cache.append(qkv[:, :heads], qkv[:, heads:-kv], qkv[:, -kv:], position, slots, table)
+        lens += 1
+        position += 1
+        s.lens = lens.tolist()
+        o = s.cache.attend(q, starts, lens, blocks, 1)
+        want, off = ref.attend(q, s.all(s.cache.k), s.all(s.cache.v), list(range(b + 1)), s.lens, None, dim ** -0.5, heads // kv)
+        assert ref.within(o, want, off)[0]
+        before = s.all(s.weights.clone())
+        s.cache.weigh(q, starts, lens, blocks, 1, s.weights)
+        for (w, off), have in zip(more.weigh(q, s.all(s.cache.k), list(range(b + 1)), s.lens, None, dim ** -0.5, heads // kv, before), s.all(s.weights)):
+            assert ((have.double() - w).abs() <= off).all()
+        if max(s.lens) > 48:
+            tokens, long = [t.clone() for t in s.all(s.cache.v)], list(s.lens)
+            want = more.evict([t.clone() for t in s.all(s.weights)], s.lens, budget, 8, 2)
+            s.cache.evict(s.weights, lens, blocks, budget, recent=8, first=2, left=lens, kept=kept)
+            s.lens = lens.tolist()
+            assert s.lens == [min(n, budget) for n in long]
+            for i in range(b):
+                assert np.array_equal(kept[i, :, :s.lens[i]].cpu().numpy(), want[i])
+                assert torch.equal(s.of(s.cache.v, i), torch.gather(tokens[i], 1, torch.from_numpy(want[i]).cuda()[..., None].expand(-1, -1, dim)))
+            evicted += 1
+        x = x + wo(o.flatten(1))
+        x = x + layer.check(x, (x @ router).float())
+        scores = head(x)
+        kw = dict(tokens=history, lens=count, repetition=value(1.3), frequency=value(0.2), presence=value(0.1))
+        scores = check_penalized(scores, **kw).cuda()
+        token = hipq.sample(scores, torch.rand(b, device="cuda", generator=g), temperature=value(0.8))
+        history[rows, count.long()] = token.to(torch.int32)
+        count += 1
+    assert evicted >= 2 and (history[:, :12] >= 0).all()
