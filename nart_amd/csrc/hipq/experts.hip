@@ -286,29 +286,52 @@ __global__ __launch_bounds__(1024) void experts_number_kernel(const RouteArgs a)
     }
 }
 
-// y[t] = sum of a token's pairs, four values a thread.
+// four neighbouring results, the first `left` of them
 template <int TYPE>
-__global__ __launch_bounds__(256) void experts_join_kernel(const RouteArgs a, const float *part, int splits, int64_t pairs, int columns, uint16_t *y, int64_t y_stride, int N)
+__device__ static __forceinline__ void put4(uint16_t *to, const f32x4 &v, int left)
 {
-    const int per_row = (N + 3) / 4;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, t = id / per_row;
-    const int n = (int)(id - t * per_row) * 4;
-    if (t >= a.M)
+    if (left >= 4 && (uintptr_t)to % 8 == 0)
+        *(u32x2 *)to = u32x2{Real16<TYPE>::pack(v[0], v[1]), Real16<TYPE>::pack(v[2], v[3])};
+    else
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (e < left)
+                to[e] = rounded<TYPE>(v[e]);
+}
+
+// y[t] = sum of a token's pairs, four values a thread and a token a work-group, whose pairs' numbers then are the same for all; four pairs on their way at once.
+template <int TYPE>
+__global__ __launch_bounds__(256) void experts_join_kernel(const RouteArgs a, const float *part, int splits, int64_t pairs, int columns, uint16_t *y, int64_t y_stride, int N, int stretches)
+{
+    const int t = blockIdx.x / stretches, n = ((int)(blockIdx.x - t * stretches) * 256 + (int)threadIdx.x) * 4;
+    if (n >= N)
         return;
     f32x4 v = {0, 0, 0, 0};
-    for (int s = 0; s < a.top; s++) {
-        const int p = a.place[t * a.top + s];
-        if (p < 0)
-            break;
-        f32x4 u = {0, 0, 0, 0};
-        for (int i = 0; i < splits; i++)
-            u += *(const f32x4 *)(part + (i * pairs + p) * columns + n);
-        v += a.share[t * a.top + s] * u;
-    }
+    for (int s = 0; s < a.top; s += 4) {
+        int p[4];
+        float share[4];
+        f32x4 u[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-        if (n + e < N)
-            y[t * y_stride + n + e] = rounded<TYPE>(v[e]);
+        for (int k = 0; k < 4; k++) {
+            p[k] = s + k < a.top ? a.place[(int64_t)t * a.top + s + k] : -1;
+            share[k] = s + k < a.top ? a.share[(int64_t)t * a.top + s + k] : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            u[k] = f32x4{0, 0, 0, 0};
+            if (p[k] >= 0)
+                u[k] = *(const f32x4 *)(part + (int64_t)p[k] * columns + n);
+        }
+        for (int i = 1; i < splits; i++)
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (p[k] >= 0)
+                    u[k] += *(const f32x4 *)(part + (i * pairs + p[k]) * columns + n);
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            v += share[k] * u[k];
+    }
+    put4<TYPE>(y + t * y_stride + n, v, N - n);
 }
 
 // ---- few tokens: streams of weights --------------------------------------------------------------------------------------------------
@@ -548,10 +571,7 @@ __global__ __launch_bounds__(256) void experts_few_join_kernel(const float *part
 #pragma unroll 4
     for (int s = 0; s < splits; s++)
         v += *(const f32x4 *)(part + ((int64_t)s * M + t) * columns + n);
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-        if (n + e < N)
-            y[t * y_stride + n + e] = rounded<TYPE>(v[e]);
+    put4<TYPE>(y + t * y_stride + n, v, N - n);
 }
 
 } // namespace hipq
@@ -785,9 +805,9 @@ static int run_experts(const hipq_w4_experts_plan *p, const ExpertsLayout &l, Ro
     a.x = (const uint16_t *)(ws + l.hidden), a.x_stride = p->desc.inner, a.M = (int)l.pairs;
     if (launch_experts<TYPE>(p, l, a, g, p->tiles[1], l.splits, ws, (float *)(ws + l.part), st))
         return 1;
-    const int64_t threads = (int64_t)r.M * ((p->desc.N + 3) / 4);
-    experts_join_kernel<TYPE><<<dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st>>>(r, (const float *)(ws + l.part), l.splits, l.pairs, l.columns, (uint16_t *)y, y_stride,
-                                                                                          p->desc.N);
+    const int stretches = (p->desc.N + 1023) / 1024;
+    experts_join_kernel<TYPE><<<dim3((unsigned)(r.M * stretches)), dim3(256), 0, st>>>(r, (const float *)(ws + l.part), l.splits, l.pairs, l.columns, (uint16_t *)y, y_stride, p->desc.N,
+                                                                                       stretches);
     return launch_status("experts_join_kernel");
 }
 
@@ -876,7 +896,8 @@ static int experts_fit(const hipq_w4_experts_plan *p, int M)
         const ExpertsLayout l = layout_of(p, M);
         const int tiles = p->tiles[0] > p->tiles[1] ? p->tiles[0] : p->tiles[1];
         HIPQ_REQUIRE(l.blocks * ((tiles + 7) / 8) <= (1 << 23) - 8, "experts: %d rows of %d outputs", M, p->desc.N);
-        HIPQ_REQUIRE((int64_t)M * ((p->desc.N + 3) / 4) < ((int64_t)1 << 32) - 256, "experts: %d rows of %d outputs", M, p->desc.N);
+        HIPQ_REQUIRE(l.kernel > FEW_16 || l.blocks * (p->tiles[0] / 2) < (1 << 24), "experts: %d rows of %d experts, %d hidden values each", M, p->desc.top, p->desc.inner);
+        HIPQ_REQUIRE((int64_t)M * ((p->desc.N + 1023) / 1024) < (1 << 24), "experts: %d rows of %d outputs", M, p->desc.N);
     }
     return 0;
 }
