@@ -2,7 +2,8 @@
 //
 // A pass over memory: a score is read once and written once.  What a row's history does to a score depends on how often its token has occurred, so a work-group has a
 // slice of the vocabulary with a counter for each of its tokens in LDS, reads the whole history, which is short and in the L2 for all but the first of a row's slices,
-// and counts what falls into its slice; integers, so that the order does not matter.  Its own scores are on their way meanwhile.
+// and counts what falls into its slice; integers, so that the order does not matter.  Its own scores are on their way meanwhile.  256 rows of 128000 in float32 with histories of up to
+// 4000: 270 MB in 60 us, 4.5 TB/s of the 5.1 of a copy; one row 6 us, a launch and three rounds of loads and barriers.
 #include "overlap.h"
 #include "real16.h"
 

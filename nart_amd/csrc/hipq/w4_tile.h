@@ -106,7 +106,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void w4_tile_kernel(const W4Args
         column = local / number;
         m0 = __builtin_amdgcn_readfirstlane(groups.block[base + block].first), end = __builtin_amdgcn_readfirstlane(groups.block[base + block].end);
         q += array * groups.q_bytes, scales += array * groups.s_bytes;
-        // in step: an array's columns side by side share their rows, and which rows a block has may change from call to call (us of 2048 tokens of two of 8 experts of 4096 x 14336,
+        // in step: an array's columns side by side share their rows, and which rows a block has may change from call to call (us of 2048 tokens of four of 32 experts of 4096 x 2048,
         // in step 606, from the column on 612, from the item on 618; 1024 tokens of six of 64 of 2048 x 1408 248, 248, 248)
         phase = 0;
     }
