@@ -434,7 +434,9 @@ struct FewArgs {
 // The hidden rows: a work-group has a tile of the gate and its one of the other projection, for a block of rows, and four waves take the blocks of k in turn, two
 // ahead each: little for one wave, but many are there.  us of the whole layer with 2 and 4 tiles, 4 and 8 waves, 2 and 3 or 4 blocks: one token through 2 of 8 experts of 4096 x 14336
 // 47.5; 48.1 with 4 tiles; 48.1 with 8 waves; 50.0 with 4 blocks; 54 with 4 tiles and 3 blocks; 16 tokens through 6 of 64 of 2048 x 1408 51.8, 52.5, 55.1, 53.2, 56.5.
-template <int TYPE, int GPB, bool ZEROS, int ROWS>
+// One token has a block for each of its experts, and every wave chooses them itself (EACH > 0) rather than wait for a launch that does: 4.8 us less 0.5; the first work-group
+// leaves the list for the second product.
+template <int TYPE, int GPB, bool ZEROS, int ROWS, int EACH>
 __global__ __launch_bounds__(256) void experts_few_up_kernel(const FewArgs f)
 {
     constexpr int WAVES = 4, NT = 2, DEPTH = 2;
@@ -443,12 +445,30 @@ __global__ __launch_bounds__(256) void experts_few_up_kernel(const FewArgs f)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, j = lane >> 4;
     const W4Args &a = f.a;
     const int block = blockIdx.x / f.groups, tile0 = (int)(blockIdx.x - block * f.groups) * NT;
-    const W4Block b = f.r.block[block]; // read before it is known whether it is there
-    if (block >= *f.r.count)
-        return;
-    const int first = b.first, rows = b.end - first, expert = b.array;
+    int first, rows, expert;
+    const uint16_t *row = a.x + S::k_of(c, j);
+    if constexpr (EACH > 0) {
+        uint32_t raw[EACH];
+        load_scores<EACH>(f.r, 0, lane, raw);
+        const Choice own = choose<EACH>(f.r, raw, lane);
+        if (blockIdx.x == 0 && wave == 0) {
+            if (lane < f.r.top)
+                f.r.block[lane] = W4Block{own.expert, lane, lane + 1, 0, 0}, f.r.row[lane] = 0, f.r.placed_share[lane] = own.share;
+            const int count = __builtin_popcountll(__ballot(own.expert >= 0));
+            if (lane == 0)
+                *f.r.count = count;
+        }
+        first = block, rows = 1, expert = __builtin_amdgcn_readlane(own.expert, block);
+        if (expert < 0)
+            return;
+    } else {
+        const W4Block b = f.r.block[block]; // read before it is known whether it is there
+        if (block >= *f.r.count)
+            return;
+        first = b.first, rows = b.end - first, expert = b.array;
+        row += (int64_t)f.r.row[first + min(S::row_of(c), rows - 1)] * a.x_stride;
+    }
     const uint8_t *const q = a.q + expert * f.q_bytes, *const scales = a.scales + expert * f.s_bytes;
-    const uint16_t *const row = a.x + (int64_t)f.r.row[first + min(S::row_of(c), rows - 1)] * a.x_stride + S::k_of(c, j);
     S stream;
     stream.clear();
 #pragma unroll
@@ -727,6 +747,9 @@ static int launch_few_down(const hipq_w4_experts_plan *p, const FewArgs &f, int 
     return launch_status("experts_few_down_kernel");
 }
 
+// one token, whose blocks have 4 rows, and as many scores as a wave keeps in few registers
+static bool chooses_itself(const RouteArgs &r) { return r.M == 1 && r.experts <= 256; }
+
 // 16 waves of a work-group where a CU has one, 8 where it has two: us, one token through one of 16 experts of 5120 x 8192 with 5120 outputs, 320 work-groups, 26 and 24; through 2 of 8
 // of 4096 x 14336, 256, 48 and 52
 template <int TYPE, int GPB, bool ZEROS, int ROWS>
@@ -734,7 +757,13 @@ static int launch_few(const hipq_w4_experts_plan *p, FewArgs f, const uint16_t *
 {
     f.a = p->args[0], f.q_bytes = p->groups[0].q_bytes, f.s_bytes = p->groups[0].s_bytes, f.groups = p->tiles[0] / 2;
     f.a.x = x, f.a.x_stride = x_stride, f.a.y = hidden, f.a.y_stride = p->desc.inner;
-    experts_few_up_kernel<TYPE, GPB, ZEROS, ROWS><<<dim3(f.r.most_blocks * f.groups), dim3(256), 0, st>>>(f);
+    const dim3 grid(f.r.most_blocks * f.groups);
+    if (ROWS == 4 && chooses_itself(f.r) && f.r.experts <= 64)
+        experts_few_up_kernel<TYPE, GPB, ZEROS, 4, 1><<<grid, dim3(256), 0, st>>>(f);
+    else if (ROWS == 4 && chooses_itself(f.r))
+        experts_few_up_kernel<TYPE, GPB, ZEROS, 4, 4><<<grid, dim3(256), 0, st>>>(f);
+    else
+        experts_few_up_kernel<TYPE, GPB, ZEROS, ROWS, 0><<<grid, dim3(256), 0, st>>>(f);
     if (launch_status("experts_few_up_kernel"))
         return 1;
     f.a = p->args[1], f.q_bytes = p->groups[1].q_bytes, f.s_bytes = p->groups[1].s_bytes;
@@ -793,7 +822,7 @@ static int run_experts(const hipq_w4_experts_plan *p, const ExpertsLayout &l, Ro
 {
     if (l.kernel <= FEW_16)
         r.placed_share = (float *)(ws + l.share_by_number), r.most_blocks = (int)l.blocks;
-    if (r.experts <= 64 ? route<1>(p, r, st) : r.experts <= 256 ? route<4>(p, r, st) : route<16>(p, r, st))
+    if (!chooses_itself(r) && (r.experts <= 64 ? route<1>(p, r, st) : r.experts <= 256 ? route<4>(p, r, st) : route<16>(p, r, st)))
         return 1;
     if (l.kernel <= FEW_16)
         return launch_few<TYPE>(p, r, (const uint16_t *)x, x_stride, (uint16_t *)(ws + l.hidden), (float *)(ws + l.part), l.splits, (uint16_t *)y, y_stride, st);

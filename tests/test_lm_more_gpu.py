@@ -133,6 +133,28 @@ def test_experts_many_pairs(m, experts, top):
     layer.check(randn(g, F16, m, 64), randn(g, F32, m, experts))
 
 
+@pytest.mark.parametrize("dtype, group, zeros", [(BF16, 128, False), (F16, 128, True), (BF16, 64, True), (F16, 64, False), (BF16, 32, True), (F16, 32, False)])
+@pytest.mark.parametrize("experts, top", [(4, 4), (64, 6), (70, 5), (256, 16), (257, 3)])
+def test_experts_of_one_token(experts, top, dtype, group, zeros):
+    """One token, which has kernels of its own: ordinary scores, equal ones, fewer experts than `top`, none, the last ones alone."""
+    g = gen(experts + group)
+    layer = Layer(g, dtype, experts, 288, 160, 100, top, group, zeros, scores="sigmoid" if top == 5 else "softmax", normalize=top != 6)
+    x = randn(g, dtype, 1, 288)
+    for kind in range(5):
+        s = randn(g, F32, 1, experts)
+        if kind == 1:
+            s[:] = 0.25
+        elif kind == 2:
+            s[:, 1:] = -math.inf
+        elif kind == 3:
+            s[:] = math.nan
+        elif kind == 4:
+            s[:, -top:] += 50
+        got = layer.check(x, s)
+        if kind == 3:
+            assert (got == 0).all()
+
+
 @pytest.mark.parametrize("m, experts", [(3, 4), (14, 4), (40, 30), (60, 3), (200, 4), (900, 4)])
 def test_experts_rows_that_are_not_finite(m, experts):
     """An infinity or NaN in a row of x stays in its token's result."""
