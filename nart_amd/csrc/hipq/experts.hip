@@ -8,8 +8,8 @@
 // rows then have an expert each.  The hidden rows between the products are rounded to 16 bits, as the matrix unit takes them.  The tiles' second product leaves float32 sums,
 // of which a last kernel adds a token's, each times its share.
 //
-// What bounds them, with the launches' own times in us: one token of two of 8 experts of 4096 x 14336 5 + 25 + 16, its 183 MB of weights at 4.5 TB/s of the 5.1 that a copy reaches;
-// of six of 64 of 2048 x 1408 5 + 7.6 + 6.8, three launches' beginnings and ends; 24 tokens of those, groups of 64 with zero points, 7 + 33 + 24 + 5, 209 MB at 3.7 TB/s.  2048 tokens of
+// What bounds them, with the launches' own times in us: one token of two of 8 experts of 4096 x 14336 26 + 16, its 183 MB of weights at 4.5 TB/s of the 5.1 that a copy reaches;
+// of six of 64 of 2048 x 1408 8.6 + 6.8, two launches' beginnings and ends; 24 tokens of those, groups of 64 with zero points, 7 + 33 + 24 + 5, 209 MB at 3.7 TB/s.  2048 tokens of
 // four of 32 of 4096 x 2048 5 + 8 + 8 + 304 + 6 + 188 + 24: 1.02 PFLOP/s of the products, with the rows that fill up the blocks (a fifth), as w4_tile_kernel reaches without experts.  333 tokens of three of 13 of 1056 x 1120 4 + 4 + 21 + 14 + 5:
 // vector instructions of groups of 32 with zero points, on a chip that is filled once.
 #include <cmath>
