@@ -71,7 +71,7 @@ def runs_of_experts():
         return lib.hipq_w4_experts_run(plan, x, x_stride, logits, logits_type, logits_stride, y, y_stride, M, workspace, size, None)
     r = Refusals(call, 3)
     r.takes(0, M=0, x=None, y=None, logits=None, workspace=None)
-    r.takes(3, M=1, x_stride=0, y_stride=0, logits_stride=0)
+    r.takes(2, M=1, x_stride=0, y_stride=0, logits_stride=0)
     r.takes(3, x_stride=520, y_stride=513, y=(P << 11) + 2, logits_stride=5, size=need[8])
     r.takes(3, logits_type=BF16, logits=(P << 10) + 2)
     assert lib.hipq_w4_experts_kernel(h, 1) == b"w4_experts_stream_4" and lib.hipq_w4_experts_kernel(None, 1) == b""
