@@ -162,6 +162,18 @@ __device__ static __forceinline__ int list_blocks(const RouteArgs &a, int pairs_
     return first;
 }
 
+// the lanes with the same expert
+__device__ static __forceinline__ uint64_t same_expert(int e, int experts)
+{
+    uint64_t lanes = __ballot(e >= 0);
+#pragma unroll 1
+    for (int bit = 0; experts > 1 << bit; bit++) {
+        const uint64_t set = __ballot((e >> bit) & 1);
+        lanes &= (e >> bit) & 1 ? set : ~set;
+    }
+    return lanes;
+}
+
 // Few tokens: chooses their experts and numbers the pairs, by expert and then by token: a row's block, and with it the order of its sums, is the same every time.  Each of 16
 // waves has a contiguous part of the pairs, and goes through it 64 at a time twice: to count each expert's, and to number them from where the waves before it end.
 constexpr int CHOOSE_TOKENS = 128;
@@ -194,15 +206,6 @@ __global__ __launch_bounds__(1024) void experts_route_kernel(const RouteArgs a)
         counts[i] = 0;
     __syncthreads();
     const int pairs = a.M * a.top, part = (pairs + 1023) / 1024 * 64, from = wave * part, to = min(pairs, from + part);
-    auto same = [&](int e) { // the lanes with the same expert
-        uint64_t lanes = __ballot(e >= 0);
-#pragma unroll 1
-        for (int bit = 0; a.experts > 1 << bit; bit++) {
-            const uint64_t set = __ballot((e >> bit) & 1);
-            lanes &= (e >> bit) & 1 ? set : ~set;
-        }
-        return lanes;
-    };
 #pragma unroll 1
     for (int p = from + lane; p - lane < to; p += 64)
         if (p < to && chosen[p] >= 0)
@@ -228,7 +231,7 @@ __global__ __launch_bounds__(1024) void experts_route_kernel(const RouteArgs a)
 #pragma unroll 1
     for (int p = from + lane; p - lane < to; p += 64) {
         const int e = p < to ? chosen[p] : -1;
-        const uint64_t lanes = same(e);
+        const uint64_t lanes = same_expert(e, a.experts);
         int place = -1;
         if (e >= 0) {
             place = counts[wave * a.experts + e] + __builtin_popcountll(lanes & ((1ull << lane) - 1));
@@ -434,8 +437,10 @@ struct FewArgs {
 // The hidden rows: a work-group has a tile of the gate and its one of the other projection, for a block of rows, and four waves take the blocks of k in turn, two
 // ahead each: little for one wave, but many are there.  us of the whole layer with 2 and 4 tiles, 4 and 8 waves, 2 and 3 or 4 blocks: one token through 2 of 8 experts of 4096 x 14336
 // 47.5; 48.1 with 4 tiles; 48.1 with 8 waves; 50.0 with 4 blocks; 54 with 4 tiles and 3 blocks; 16 tokens through 6 of 64 of 2048 x 1408 51.8, 52.5, 55.1, 53.2, 56.5.
-// One token has a block for each of its experts, and every wave chooses them itself (EACH > 0) rather than wait for a launch that does: 4.8 us less 0.5; the first work-group
-// leaves the list for the second product.
+// Of up to four tokens, whose experts have a block each, every work-group chooses them itself (EACH > 0) rather than wait for a launch that does: a wave a token, and blocks in the
+// order in which their experts come first.  One more work-group leaves the list for the second product.  us of the layer with and without, 1, 2 and 4 tokens through 2 of 8 experts of
+// 4096 x 14336 50 and 52, 51 and 53, 77 and 78, 6 of 64 of 2048 x 1408 15.3 and 19.2, 20.6 and 23.8, 29.2 and 30.9, 8 of 128 of 2048 x 768 14.1 and 17.7 (1), 26.2 and 28.3 (4), 16 of 256 of
+// 1024 x 256 22.8 and 22.7 (4).
 template <int TYPE, int GPB, bool ZEROS, int ROWS, int EACH>
 __global__ __launch_bounds__(256) void experts_few_up_kernel(const FewArgs f)
 {
@@ -444,23 +449,72 @@ __global__ __launch_bounds__(256) void experts_few_up_kernel(const FewArgs f)
     __shared__ f32x4 red[WAVES][NT][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, j = lane >> 4;
     const W4Args &a = f.a;
-    const int block = blockIdx.x / f.groups, tile0 = (int)(blockIdx.x - block * f.groups) * NT;
+    // the first work-group leaves the list
+    const int item = (int)blockIdx.x - (EACH > 0), block = item / f.groups, tile0 = (item - block * f.groups) * NT;
     int first, rows, expert;
     const uint16_t *row = a.x + S::k_of(c, j);
     if constexpr (EACH > 0) {
-        uint32_t raw[EACH];
-        load_scores<EACH>(f.r, 0, lane, raw);
-        const Choice own = choose<EACH>(f.r, raw, lane);
-        if (blockIdx.x == 0 && wave == 0) {
-            if (lane < f.r.top)
-                f.r.block[lane] = W4Block{own.expert, lane, lane + 1, 0, 0}, f.r.row[lane] = 0, f.r.placed_share[lane] = own.share;
-            const int count = __builtin_popcountll(__ballot(own.expert >= 0));
-            if (lane == 0)
-                *f.r.count = count;
+        static_assert(ROWS == 4 && WAVES == 4, "a block for an expert, a wave for a token");
+        __shared__ int32_t chosen[64];
+        __shared__ float share[64];
+        const int top = f.r.top;
+        int e = -1, leader = 64; // of the pair that a lane is: its expert, and that expert's first pair
+        float part = 0;
+        if (f.r.M == 1) {
+            uint32_t raw[EACH];
+            load_scores<EACH>(f.r, 0, lane, raw);
+            const Choice own = choose<EACH>(f.r, raw, lane);
+            e = own.expert, part = own.share, leader = e >= 0 ? lane : 64;
+        } else {
+            if (wave < f.r.M) {
+                uint32_t raw[EACH];
+                load_scores<EACH>(f.r, wave, lane, raw);
+                const Choice own = choose<EACH>(f.r, raw, lane);
+                if (lane < top)
+                    chosen[wave * top + lane] = own.expert, share[wave * top + lane] = own.share;
+            }
+            __syncthreads();
+            if (lane < f.r.M * top)
+                e = chosen[lane], part = share[lane];
+            const uint64_t same = same_expert(e, f.r.experts);
+            leader = e >= 0 ? __builtin_ctzll(same) : 64;
         }
-        first = block, rows = 1, expert = __builtin_amdgcn_readlane(own.expert, block);
-        if (expert < 0)
+        const uint64_t leaders = __ballot(leader == lane);
+        if (item < 0) { // block by block
+            if (wave > 0)
+                return;
+            int base = 0, number = 0;
+#pragma unroll 1
+            for (uint64_t left = leaders; left; left &= left - 1, number++) {
+                const int of = __builtin_ctzll(left);
+                const uint64_t pairs = __ballot(leader == of);
+                if (leader == of) {
+                    const int place = base + __builtin_popcountll(pairs & ((1ull << lane) - 1));
+                    f.r.row[place] = lane / top, f.r.placed_share[place] = part;
+                }
+                if (lane == of)
+                    f.r.block[number] = W4Block{e, base, base + __builtin_popcountll(pairs), 0, 0};
+                base += __builtin_popcountll(pairs);
+            }
+            if (lane == 0)
+                *f.r.count = number;
             return;
+        }
+        if (block >= __builtin_popcountll(leaders))
+            return;
+        if (f.r.M == 1)
+            first = block, rows = 1, expert = __builtin_amdgcn_readlane(e, block);
+        else {
+            const int of = __builtin_ctzll(__ballot(leader == lane && __builtin_popcountll(leaders & ((1ull << lane) - 1)) == block));
+            expert = __builtin_amdgcn_readlane(e, of);
+            uint64_t pairs = __ballot(leader == of);
+            first = __builtin_popcountll(__ballot(leader < of)), rows = __builtin_popcountll(pairs);
+#pragma unroll
+            for (int r = 0; r < ROWS - 1; r++) // a lane's row, the last one again behind it
+                if (r < min(S::row_of(c), rows - 1))
+                    pairs &= pairs - 1;
+            row += __builtin_ctzll(pairs) / top * a.x_stride;
+        }
     } else {
         const W4Block b = f.r.block[block]; // read before it is known whether it is there
         if (block >= *f.r.count)
@@ -747,8 +801,8 @@ static int launch_few_down(const hipq_w4_experts_plan *p, const FewArgs &f, int 
     return launch_status("experts_few_down_kernel");
 }
 
-// one token, whose blocks have 4 rows, and as many scores as a wave keeps in few registers
-static bool chooses_itself(const RouteArgs &r) { return r.M == 1 && r.experts <= 256; }
+// a wave for a token, a lane for a pair, blocks that hold all of an expert's rows, and as many scores as a wave keeps in few registers
+static bool chooses_itself(const RouteArgs &r) { return r.M <= 4 && r.M * r.top <= 64 && r.block_rows == 4 && r.experts <= 256; }
 
 // 16 waves of a work-group where a CU has one, 8 where it has two: us, one token through one of 16 experts of 5120 x 8192 with 5120 outputs, 320 work-groups, 26 and 24; through 2 of 8
 // of 4096 x 14336, 256, 48 and 52
@@ -759,9 +813,9 @@ static int launch_few(const hipq_w4_experts_plan *p, FewArgs f, const uint16_t *
     f.a.x = x, f.a.x_stride = x_stride, f.a.y = hidden, f.a.y_stride = p->desc.inner;
     const dim3 grid(f.r.most_blocks * f.groups);
     if (ROWS == 4 && chooses_itself(f.r) && f.r.experts <= 64)
-        experts_few_up_kernel<TYPE, GPB, ZEROS, 4, 1><<<grid, dim3(256), 0, st>>>(f);
+        experts_few_up_kernel<TYPE, GPB, ZEROS, 4, 1><<<dim3(grid.x + 1), dim3(256), 0, st>>>(f);
     else if (ROWS == 4 && chooses_itself(f.r))
-        experts_few_up_kernel<TYPE, GPB, ZEROS, 4, 4><<<grid, dim3(256), 0, st>>>(f);
+        experts_few_up_kernel<TYPE, GPB, ZEROS, 4, 4><<<dim3(grid.x + 1), dim3(256), 0, st>>>(f);
     else
         experts_few_up_kernel<TYPE, GPB, ZEROS, ROWS, 0><<<grid, dim3(256), 0, st>>>(f);
     if (launch_status("experts_few_up_kernel"))
@@ -932,7 +986,7 @@ static int experts_fit(const hipq_w4_experts_plan *p, int M)
         const ExpertsLayout l = layout_of(p, M);
         const int tiles = p->tiles[0] > p->tiles[1] ? p->tiles[0] : p->tiles[1];
         HIPQ_REQUIRE(l.blocks * ((tiles + 7) / 8) <= (1 << 23) - 8, "experts: %d rows of %d outputs", M, p->desc.N);
-        HIPQ_REQUIRE(l.kernel > FEW_16 || l.blocks * (p->tiles[0] / 2) < (1 << 24), "experts: %d rows of %d experts, %d hidden values each", M, p->desc.top, p->desc.inner);
+        HIPQ_REQUIRE(l.kernel > FEW_16 || l.blocks * (p->tiles[0] / 2) < (1 << 24) - 1, "experts: %d rows of %d experts, %d hidden values each", M, p->desc.top, p->desc.inner);
         HIPQ_REQUIRE((int64_t)M * ((p->desc.N + 1023) / 1024) < (1 << 24), "experts: %d rows of %d outputs", M, p->desc.N);
     }
     return 0;

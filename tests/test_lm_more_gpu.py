@@ -155,6 +155,28 @@ def test_experts_of_one_token(experts, top, dtype, group, zeros):
             assert (got == 0).all()
 
 
+@pytest.mark.parametrize("dtype, group, zeros", [(BF16, 128, False), (F16, 64, True), (BF16, 32, True)])
+@pytest.mark.parametrize("experts, top", [(3, 1), (8, 4), (64, 6), (70, 16), (256, 16), (257, 5)])
+@pytest.mark.parametrize("m", [2, 3, 4, 5])
+def test_experts_of_up_to_four_tokens(m, experts, top, dtype, group, zeros):
+    """They have kernels of their own: experts that they share, all, some and none of them, tokens without any, rows with gaps between them."""
+    g = gen(experts + group + m)
+    layer = Layer(g, dtype, experts, 288, 160, 100, top, group, zeros, scores="sigmoid" if top == 5 else "softmax", normalize=top != 6)
+    x = randn(g, dtype, m, 320)[:, :288]
+    for kind in range(4):
+        s = randn(g, F32, m, experts + 3)[:, 1:experts + 1]
+        if kind == 1:
+            s[:] = s[:1].clone()       # the same for all
+        elif kind == 2:
+            s[0] = -math.inf           # none
+            s[m - 1, 1:] = math.nan    # one
+        elif kind == 3:
+            s[:, -1] += 50             # one that all have
+        got = layer.check(x, s)
+        if kind == 2:
+            assert (got[0] == 0).all()
+
+
 @pytest.mark.parametrize("m, experts", [(3, 4), (14, 4), (40, 30), (60, 3), (200, 4), (900, 4)])
 def test_experts_rows_that_are_not_finite(m, experts):
     """An infinity or NaN in a row of x stays in its token's result."""
