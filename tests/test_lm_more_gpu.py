@@ -207,7 +207,7 @@ def test_experts_more_dimensions_and_no_rows():
     assert layer.plan(x[:0, 0], s[:0, 0]).shape == (0, 40)
 
 
-@pytest.mark.parametrize("m", [1, 9, 40, 200, 900])
+@pytest.mark.parametrize("m", [1, 3, 9, 40, 200, 900])
 def test_experts_same_result_every_time(m):
     """Also in a captured graph, with other calls and other inputs between its replays, and on another stream."""
     g = gen(m)
@@ -234,6 +234,37 @@ def test_experts_same_result_every_time(m):
         again = layer.plan(x, s)
     stream.synchronize()
     assert torch.equal(again, first)
+
+
+@pytest.mark.parametrize("sizes", [(1, 3), (2, 30), (4, 200), (60, 900)])
+def test_experts_two_calls_at_once(sizes):
+    """One layer on two streams, and in two graphs that are replayed side by side."""
+    g = gen(sum(sizes))
+    layer = Layer(g, BF16, 12, 512, 256, 300, 3)
+    inputs = [(randn(g, BF16, m, 512), randn(g, F32, m, 12)) for m in sizes]
+    want = [layer.plan(x, s) for x, s in inputs]
+    outputs, streams, graphs = [torch.zeros_like(w) for w in want], [torch.cuda.Stream() for _ in sizes], [torch.cuda.CUDAGraph() for _ in sizes]
+    for (x, s), y, graph in zip(inputs, outputs, graphs):
+        with torch.cuda.graph(graph):
+            for _ in range(3):
+                layer.plan(x, s, y)
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(8):
+        for (x, s), stream in zip(inputs, streams):
+            with torch.cuda.stream(stream):
+                got.append(layer.plan(x, s))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(got))
+    for _ in range(4):
+        for y in outputs:
+            y.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, w) for y, w in zip(outputs, want))
 
 
 # ---- penalties --------------------------------------------------------------------------------------------------------
