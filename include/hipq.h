@@ -658,6 +658,7 @@ int hipq_kv_weigh(const hipq_kv_cache *cache, const hipq_kv_weigh_desc *desc, vo
  * heaviest (the first of equal ones; NaN below every number) until there are `budget`; one of no more keeps all.  The kept tokens, in their order, become
  * tokens 0, 1, ... of the blocks to[b]: keys, values, scales and weights move there.  left[b] = min(lens[b], budget), the sequence's new length, may be lens[b]
  * itself.  kept[b][h][j]: the place that token j had, -1 behind the last.
+ * kept, left (but for lens itself) and weights lie over none of each other, of lens, of the blocks or of the cache, which is not looked at.
  * to may be blocks (same stride): in place.  Otherwise none of its pages is one of any sequence's in blocks.  No page stands twice in either, so that a page that several
  * sequences share is not to be evicted from.  A token whose block, or whose new one, lies outside the cache is not moved, and counts as one whose weight is NaN.
  * Keys keep the rotation of the positions that they had.  Sequences' lengths count up to `longest`.  `to` holds at least min(budget, longest) tokens of a sequence.

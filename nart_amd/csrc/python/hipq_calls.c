@@ -807,6 +807,18 @@ static PyObject *py_kv_weigh(ARGS)
     return PyLong_FromLong(rc);
 }
 
+/* `n` entries of a whole tensor have none in common with `rows` rows of another, `entries` each: 4 bytes an entry */
+static int apart(const view_t *v, const char *name, int64_t n, const view_t *u, const char *other, int64_t rows, int64_t entries)
+{
+    const int64_t lo = (int64_t)(uintptr_t)v->p, at = (int64_t)(uintptr_t)u->p, step = 4 * u->stride[0], behind = lo - (at + 4 * entries);
+    const int64_t r = behind < 0 ? 0 : step > 0 ? behind / step + 1 : rows; /* the first row that ends behind lo */
+    if (n > 0 && entries > 0 && r < rows && at + r * step < lo + 4 * n) {
+        PyErr_Format(PyExc_ValueError, "%s lies over %s", name, other);
+        return 0;
+    }
+    return 1;
+}
+
 /* cache, its device, weights, lens, blocks, to, left, kept, budget, recent, first, longest or None, allocate: (bytes) -> uint8 tensor */
 static PyObject *py_kv_evict(ARGS)
 {
@@ -841,8 +853,21 @@ static PyObject *py_kv_evict(ARGS)
         any.type = BF16; /* codes are moved as they are */
     d.weights = weights.p, d.lens = lens.p, d.blocks = blocks.p, d.to = to.p, d.left = left.p, d.kept = kept.p;
     d.blocks_stride = blocks.stride[0], d.to_stride = to.stride[0], d.sequences = (int)b, d.blocks_per_sequence = (int)blocks.shape[1], d.to_per_sequence = (int)to.shape[1];
+    const size_t need = hipq_kv_evict_workspace(&any, &d);
+    /* what is written lies apart from what the launches read, but for left in the place of lens; a call that is refused for something else says that */
+    const int64_t many = b * c->heads * d.budget, pool = (int64_t)c->pages * c->heads * c->page;
+    const struct {
+        const view_t *v;
+        const char *name;
+        int64_t rows, entries;
+    } read[5] = {{&lens, "lens", 1, b}, {&blocks, "blocks", b, blocks.shape[1]}, {&to, "to", b, to.shape[1]}, {&left, "left", 1, b}, {&kept, "kept", 1, many}};
+    for (int i = 0; i < 5 && hipq_last_error()[0] == 0; i++)
+        if (!apart(&weights, "weights", pool, read[i].v, read[i].name, read[i].rows, read[i].entries)
+            || (i < 4 && !apart(&kept, "kept", many, read[i].v, read[i].name, read[i].rows, read[i].entries))
+            || (i < 3 && (i > 0 || left.p != lens.p) && !apart(&left, "left", b, read[i].v, read[i].name, read[i].rows, read[i].entries)))
+            return NULL;
     PyObject *workspace;
-    if (!allocated(a[12], hipq_kv_evict_workspace(&any, &d), device, &workspace, &w))
+    if (!allocated(a[12], need, device, &workspace, &w))
         return NULL;
     int rc;
     Py_BEGIN_ALLOW_THREADS;
