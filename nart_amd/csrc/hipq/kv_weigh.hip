@@ -134,12 +134,15 @@ __global__ __launch_bounds__(256, 2) void kv_scores_kernel(const WeighArgs w)
             // scores to the base 2; of 16-bit keys, where nothing needs them, as they are
             constexpr bool RAW = !QUANT && !SCORES;
             const uint32_t sees = masked ? seen_by(a, seq, new_token(w, row_of(rt)), t, j, now) : 255u;
-            float x[8], p[8];
+            float x[8], p[8], left[8]; // left: for the next launch, where NONE is what the row does not see, and nothing else
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 x[e] = RAW ? s[e / 4][e % 4] : s[e / 4][e % 4] * (QUANT ? ksc[e / 4][e % 4] : a.scale2);
-                if (masked)
+                left[e] = fmaxf(x[e], LOWEST);
+                if (masked) {
+                    left[e] = (sees >> e) & 1 ? left[e] : NONE;
                     x[e] = (sees >> e) & 1 ? x[e] : NONE;
+                }
             }
             // no branch for a reference that stays: blocks of rows would wait for each other's
             float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
@@ -152,7 +155,7 @@ __global__ __launch_bounds__(256, 2) void kv_scores_kernel(const WeighArgs w)
             if (SCORES && to[rt])
 #pragma unroll
                 for (int half = 0; half < 2; half++)
-                    *(f32x4 *)(to[rt] + t + 16 * half) = f32x4{x[4 * half], x[4 * half + 1], x[4 * half + 2], x[4 * half + 3]};
+                    *(f32x4 *)(to[rt] + t + 16 * half) = f32x4{left[4 * half], left[4 * half + 1], left[4 * half + 2], left[4 * half + 3]};
         }
     };
     int t = t0 + wave * 32;
