@@ -636,7 +636,8 @@ int hipq_kv_attend(const hipq_kv_cache *cache, const hipq_kv_attend_desc *desc, 
  * quantized cache do, float32 at ((p * heads + h) * page + t); out may be weights, otherwise it lies over none of it.  A page belongs to one sequence: of one that
  * several have, the content afterwards means nothing.  A sequence without new tokens is left alone, as is what belongs to no sequence or lies behind its end.  A row
  * that sees nothing adds nothing; one with a score of +infinity or NaN makes the weights of what it sees NaN.  Sums are over rows in a fixed order.
- * workspace: as for hipq_kv_attend, hipq_kv_weigh_workspace bytes.
+ * workspace: as for hipq_kv_attend, hipq_kv_weigh_workspace bytes.  Where rows are few their scores are left there, 4 bytes for a row, head and token of `sequences` times
+ * `longest` or of the cache, whichever are fewer: half of what the cache's keys take at most.
  */
 typedef struct hipq_kv_weigh_desc {
     const void *q;

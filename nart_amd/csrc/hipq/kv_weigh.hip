@@ -24,9 +24,10 @@ struct WeighArgs {
     AttendArgs a; // of the attention whose weights they are; a.splits, a.row_blocks and a.rows are the first launch's
     const float *old;
     float *out;
-    float *scores;          // [sequence][head][row][stride], or nullptr
+    float *scores;          // [sequence][head][row][stride], or by_page [page][head][row][stride], or nullptr
     float *lse;             // [sequence][head][row]; nullptr: the second launch joins the parts itself
     int64_t stride;
+    bool by_page;
     uint32_t group_magic;   // of a.group
     int group_shift;
     int splits, chunk;      // the second launch's work-groups for a sequence and head, and their tokens
@@ -40,6 +41,12 @@ __device__ static __forceinline__ const uint16_t *query(const WeighArgs &w, cons
 {
     const int own = new_token(w, row);
     return (const uint16_t *)w.a.d.q + (int64_t)(seq.row0 + own) * w.a.d.q_token + (int64_t)(h * w.a.group + row - own * w.a.group) * w.a.d.q_head;
+}
+
+// where a row's scores of 16 tokens begin, behind those of the row's number times stride: of the tokens from t on, which lie in a cache row and its place of a page
+__device__ static __forceinline__ int64_t scores_at(const WeighArgs &w, int bh, int t, int64_t row, int place)
+{
+    return w.by_page ? (row - place) * w.a.rows + place : (int64_t)bh * w.a.rows * w.stride + t;
 }
 
 constexpr float LOWEST = -0x1.fffffep127f; // a reference where nothing has been seen: finite, so that differences are numbers
@@ -106,7 +113,7 @@ __global__ __launch_bounds__(256, 2) void kv_scores_kernel(const WeighArgs w)
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         m[rt] = LOWEST, l[rt] = 0;
-        to[rt] = SCORES && r0 + 16 * rt + c < rows ? w.scores + (((int64_t)b * a.cache.heads + h) * a.rows + row_of(rt)) * w.stride + j * 4 : nullptr;
+        to[rt] = SCORES && r0 + 16 * rt + c < rows ? w.scores + row_of(rt) * w.stride + j * 4 : nullptr;
 #pragma unroll
         for (int ks = 0; ks < KS; ks++)
             q[rt][ks] = *K::query(query(w, seq, h, row_of(rt)), ks, j);
@@ -155,7 +162,8 @@ __global__ __launch_bounds__(256, 2) void kv_scores_kernel(const WeighArgs w)
             if (SCORES && to[rt])
 #pragma unroll
                 for (int half = 0; half < 2; half++)
-                    *(f32x4 *)(to[rt] + t + 16 * half) = f32x4{left[4 * half], left[4 * half + 1], left[4 * half + 2], left[4 * half + 3]};
+                    if (!w.by_page || now.page[half] >= 0)
+                        *(f32x4 *)(to[rt] + scores_at(w, rest, t + 16 * half, paging.row(now, half, h), now.place[half])) = f32x4{left[4 * half], left[4 * half + 1], left[4 * half + 2], left[4 * half + 3]};
         }
     };
     int t = t0 + wave * 32;
@@ -352,12 +360,13 @@ __device__ static __forceinline__ float joined(const AttendArgs &a, int bh, int 
     return sum == 0 ? __builtin_inff() : top + log2f(sum);
 }
 
-// where a token's weight lies, its four neighbours behind it; -1: in no page
-__device__ static __forceinline__ int64_t weight_at(const AttendArgs &a, int b, int h, int t)
+// where a token's weight lies, its four neighbours behind it, and its place in its page; -1: in no page
+__device__ static __forceinline__ int64_t weight_at(const AttendArgs &a, int b, int h, int t, int &place)
 {
     const int t16 = t / 16, page16 = a.cache.page / 16, block = a.page_magic ? (int)(((uint64_t)(uint32_t)t16 * a.page_magic) >> 32) >> a.page_shift : t16;
     const int page = a.d.blocks[(int64_t)b * a.d.blocks_stride + block];
-    return page < 0 || page >= a.cache.pages ? -1 : ((int64_t)page * a.cache.heads + h) * a.cache.page + t - block * (page16 * 16);
+    place = t - block * (page16 * 16);
+    return page < 0 || page >= a.cache.pages ? -1 : ((int64_t)page * a.cache.heads + h) * a.cache.page + place;
 }
 
 // the sum over 16 neighbouring lanes, in all of them
@@ -397,7 +406,8 @@ __global__ __launch_bounds__(256) void kv_sum_scores_kernel(const WeighArgs w)
     const int rows = seq.count * a.group, t = (chunk * 256 + (int)threadIdx.x) * 4;
     if (chunk * 1024 >= seq.len || rows == 0)
         return;
-    const int64_t at = t < seq.len ? weight_at(a, b, h, t) : -1;
+    int place = 0;
+    const int64_t at = t < seq.len ? weight_at(a, b, h, t, place) : -1;
     f32x4 old = {0, 0, 0, 0}, sum = {0, 0, 0, 0};
     if (at >= 0 && t < seq.old)
         old = *(const f32x4 *)(w.old + at);
@@ -408,7 +418,7 @@ __global__ __launch_bounds__(256) void kv_sum_scores_kernel(const WeighArgs w)
     __syncthreads();
     if (at < 0)
         return;
-    const float *from = w.scores + (int64_t)bh * a.rows * w.stride + t;
+    const float *from = w.scores + scores_at(w, bh, t, at, place);
 #pragma unroll 4
     for (int r = 0; r < rows; r++) {
         const f32x4 s = *(const f32x4 *)(from + r * w.stride);
@@ -533,7 +543,7 @@ __global__ __launch_bounds__(256, 2) void kv_sum_keys_kernel(const WeighArgs w)
 // ---- host ----------------------------------------------------------------------------------------------------------------------
 struct WeighShape {
     int rt, row_blocks, rows, splits, chunks, chunk;
-    bool scores, lse;
+    bool scores, lse, by_page;
     int64_t stride;
     size_t part, workspace; // bytes: of the parts; of all
 };
@@ -561,8 +571,12 @@ static WeighShape shape_of(const hipq_kv_cache *c, const hipq_kv_attend_desc *d)
     s.chunks = (int)((longest + s.chunk - 1) / s.chunk);
     const size_t heads = (size_t)d->sequences * c->heads;
     s.stride = (longest + 31) / 32 * 32;
+    // a table may be far wider than the sequences are long: where it has more tokens than the cache, scores lie as the cache's tokens do, in at most half of what the keys take
+    s.by_page = s.scores && d->sequences * s.stride > (int64_t)c->pages * c->page;
+    if (s.by_page)
+        s.stride = c->page;
     s.part = (heads * s.splits * s.rows * 8 + 255) / 256 * 256;
-    s.workspace = s.part + (s.scores ? heads * s.rows * s.stride * 4 : s.lse ? heads * s.rows * 4 : 0);
+    s.workspace = s.part + (s.scores ? (s.by_page ? (size_t)c->pages * c->heads : heads) * s.rows * s.stride * 4 : s.lse ? heads * s.rows * 4 : 0);
     return s;
 }
 
@@ -668,7 +682,7 @@ extern "C" int hipq_kv_weigh(const hipq_kv_cache *cache, const hipq_kv_weigh_des
         return fail("weigh: pages of %d tokens", cache->page);
     if (hipq_div_magic((uint32_t)w.a.group, &w.group_magic, &w.group_shift))
         return fail("weigh: %d query heads on %d heads of the cache", d.q_heads, cache->heads);
-    w.old = desc->weights, w.out = desc->out, w.stride = s.stride, w.splits = s.chunks, w.chunk = s.chunk;
+    w.old = desc->weights, w.out = desc->out, w.stride = s.stride, w.by_page = s.by_page, w.splits = s.chunks, w.chunk = s.chunk;
     w.a.part_ml = (float *)workspace;
     if (s.scores)
         w.scores = (float *)((uint8_t *)workspace + s.part);

@@ -834,7 +834,8 @@ class KvCache:
 
     def weigh(self, q, starts, lens, blocks, most_new, weights, mask=None, scale=None, out=None, longest=None):
         """The attention that every token of the cache receives from the new tokens q, added to `weights` float32 [pages, heads, page] (those of the new tokens begin
-        with it), in place or to `out`; the other arguments are attend()'s (include/hipq.h: hipq_kv_weigh)."""
+        with it), in place or to `out`; the other arguments are attend()'s (include/hipq.h: hipq_kv_weigh).  longest: no sequence is longer (None: what its blocks hold), by
+        which work and workspace are sized."""
         calls = _CALLS or _calls()
         if out is None:
             out = weights
