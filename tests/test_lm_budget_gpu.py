@@ -1,12 +1,14 @@
-"""The cache held to a budget on the GPU: weights where scores are not finite, scores kept by pages."""
+"""The cache held to a budget on the GPU: weights where scores are not finite, scores kept by pages, long sequences whose tokens several work-groups choose from,
+blocks that are not there."""
 import math
 
 import numpy as np
 import pytest
 import torch
 
+import lm_more_reference as more
 from nart_amd import hipq
-from test_lm_more_gpu import BF16, Sequences, gen, randn, whole
+from test_lm_more_gpu import BF16, F16, F32, Sequences, check_evicted, check_weighed, gen, randn, same, whole
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +58,89 @@ def test_weigh_with_wide_tables(lens, counts, heads, group, dim, page, int8, tre
     assert torch.isfinite(got).all() and (got != 7).sum() >= sum(n for n, c in zip(lens, counts) if c) * heads - heads * page
     rows = max(counts) * group
     assert len(asked) == 1 and rows * s.pages * heads * page * 4 <= asked[0] <= rows * heads * (s.pages * page * 4 + len(lens) * 256 * 8) + 256
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("lens, counts, heads, group, dim", [([1500, 700], [700, 513], 2, 4, 128), ([2100], [300], 1, 3, 256), ([900, 40], [260, 40], 1, 8, 64)])
+def test_weigh_a_prompt(lens, counts, heads, group, dim, int8):
+    """Some hundred new tokens, which pass through LDS in several rounds."""
+    g = gen(sum(counts))
+    check_weighed(g, Sequences(g, BF16, lens, heads, dim, 48, int8), BF16, counts, group)
+
+
+# ---- eviction: long sequences, whose tokens several work-groups choose from ------------------------------------------------------
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("what", ["equal", "few values", "zeros", "not finite", "either sign", "close", "one heavy part"])
+def test_evict_ties_of_several_parts(what, in_place):
+    """Equal weights at the border on both sides of the parts' ends, beside a sequence within the budget."""
+    g = gen(10)
+    s = Sequences(g, F16, [40000, 16400, 77], 2, 64, 32, False, spare=3 * 282)
+    w = s.weights
+    if what == "equal":
+        w.fill_(0.25)
+    elif what == "few values":
+        w.copy_(whole(g, 0, 3, torch.int32, *w.shape).float())
+    elif what == "zeros":
+        w.copy_(torch.where(torch.rand(w.shape, device="cuda", generator=g) < 0.97, 0.0, w))
+        w[::2] *= -1
+    elif what == "not finite":
+        u = torch.rand(w.shape, device="cuda", generator=g)
+        w.copy_(torch.where(u < 0.5, math.nan, torch.where(u < 0.9, -math.inf, torch.where(u < 0.95, math.inf, w))))
+    elif what == "either sign":
+        w.copy_(randn(g, F32, *w.shape))
+    elif what == "close":
+        w.copy_(1 + whole(g, 0, 3000, torch.int32, *w.shape).float() * 2.0 ** -23)
+    else:
+        w.zero_()
+        w[torch.from_numpy(s.blocks[0, 2 * 256 + 3:3 * 256 + 3]).cuda()] = 1.0  # the third part's, nearly
+    check_evicted(s, 9000, 20, 5, in_place)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("lens, budget, recent, first", [([40000, 300, 17000], 9000, 8600, 400), ([40000], 9000, 0, 9000), ([20000, 16385], 16384, 0, 0), ([40000, 8192, 8193], 20000, 8500, 9000),
+                                                         ([33000, 24576], 24575, 1, 0), ([17000], 1, 0, 0)])
+def test_evict_forced_tokens_of_several_parts(lens, budget, recent, first, in_place):
+    """First and last tokens that fill the budget, or whole parts."""
+    g = gen(sum(lens))
+    s = Sequences(g, BF16, lens, 2, 64, 32, True, spare=len(lens) * (-(-budget // 32) + 1))
+    check_evicted(s, budget, recent, first, in_place)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("lens, budget", [([300, 200, 33], 64), ([17000, 90], 5000)])
+def test_evict_blocks_outside(lens, budget, int8, in_place):
+    """Tokens whose block or whose new one is not there are not moved, all others are, and nothing else changes."""
+    g = gen(budget)
+    page, heads, need = 16, 2, -(-budget // 16)
+    s = Sequences(g, BF16, lens, heads, 64, page, int8, spare=len(lens) * need)
+    blocks = s.blocks.copy()
+    to = blocks if in_place else np.random.default_rng(2).permutation(s.rest)[:len(lens) * need].reshape(len(lens), need)
+    blocks[0, 2], blocks[0, lens[0] // page - 1], blocks[1, 1], blocks[1, lens[1] // page] = -1, s.pages, -2 ** 31, 2 ** 31 - 1
+    if not in_place:
+        to[0, 1], to[1, 3] = s.pages + 5, -1
+    before = {name: p.clone() for name, p in (("k", s.cache.k), ("v", s.cache.v), ("ks", s.cache.k_scale), ("vs", s.cache.v_scale), ("w", s.weights)) if p is not None}
+    ranked = []
+    for b, n in enumerate(lens):
+        t = np.arange(n)
+        there = (blocks[b, t // page] >= 0) & (blocks[b, t // page] < s.pages)
+        at = torch.from_numpy(np.where(there, blocks[b, t // page], 0)).cuda()
+        w = before["w"][at, :, torch.from_numpy(t % page).cuda()].t()
+        ranked.append(torch.where(torch.from_numpy(there).cuda(), w, math.nan))
+    want = more.evict(ranked, lens, budget, 7, 3)
+    expected = {name: p.clone() for name, p in before.items()}
+    for b, n in enumerate(lens):
+        for h in range(heads):
+            t, j = want[b][h], np.arange(min(n, budget))
+            source, target = blocks[b, t // page], to[b, j // page]
+            ok = (source >= 0) & (source < s.pages) & (target >= 0) & (target < s.pages)
+            index = lambda x: torch.from_numpy(np.ascontiguousarray(x[ok])).long().cuda()  # noqa: E731
+            for name, p in before.items():
+                expected[name][index(target), h, index(j % page)] = p[index(source), h, index(t % page)]
+    table = s.ints(blocks)
+    left, kept = s.cache.evict(s.weights, s.ints(lens), table, budget, recent=7, first=3, to=None if in_place else s.ints(to))
+    assert left.tolist() == [min(n, budget) for n in lens]
+    for b, n in enumerate(lens):
+        assert np.array_equal(kept[b, :, :min(n, budget)].cpu().numpy(), want[b]) and (kept[b, :, min(n, budget):] == -1).all()
+    for name, p in (("k", s.cache.k), ("v", s.cache.v), ("ks", s.cache.k_scale), ("vs", s.cache.v_scale), ("w", s.weights)):
+        assert p is None or same(p, expected[name]), name
