@@ -533,7 +533,9 @@ int hipq_w4_run(const hipq_w4_plan *plan, const void *x, int64_t x_stride, void 
  *   HIPQ_SCORES_SOFTMAX: share[e] = exp(logit_e) / sum of exp(logit) over all experts, or with normalize over the token's (of +infinities each counts as much, and
  *                        nothing else does),
  *   HIPQ_SCORES_SIGMOID: share[e] = 1 / (1 + exp(-logit_e)), with normalize divided by the sum of the token's.
- * The hidden rows are rounded to 16 bits between the products; in float16 one beyond 65504 is an infinity there. */
+ * The hidden rows are rounded to 16 bits between the products; in float16 one beyond 65504 is an infinity there.
+ * Equal calls give equal results.  The order of a token's float32 sums depends on M, and for M up to 64 on which experts the other tokens choose as well, so that its result
+ * may differ by their rounding. */
 #define HIPQ_SCORES_SOFTMAX 0
 #define HIPQ_SCORES_SIGMOID 1
 

@@ -19,7 +19,7 @@ INC = os.path.join(ROOT, "include")
 
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.environ.get("HIPCC", os.path.join(ROCM, "bin", "hipcc"))
-# packed-fp32 instructions are switched off on purpose (they have produced wrong results on this pool)
+# packed-fp32 instructions are switched off on purpose (some of their forms have given wrong results now and then)
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wall", "-Wno-unused-function",
              # MFMA accumulators live in ordinary VGPRs: the epilogue reads them without v_accvgpr_read round trips

@@ -8,7 +8,7 @@
 // rows then have an expert each.  The hidden rows between the products are rounded to 16 bits, as the matrix unit takes them.  The tiles' second product leaves float32 sums,
 // of which a last kernel adds a token's, each times its share.
 //
-// What bounds them, with the launches' own times in us: one token of two of 8 experts of 4096 x 14336 26 + 16, its 183 MB of weights at 4.5 TB/s of the 5.1 that a copy reaches;
+// What bounds them, with the launches' own times in us: one token of two of 8 experts of 4096 x 14336 26 + 16, its 183 MB of weights at 4.4 TB/s of the 5.1 that a copy reaches;
 // of six of 64 of 2048 x 1408 8.6 + 6.8, two launches' beginnings and ends; 24 tokens of those, groups of 64 with zero points, 7 + 33 + 24 + 5, 209 MB at 3.7 TB/s.  2048 tokens of
 // four of 32 of 4096 x 2048 5 + 8 + 8 + 304 + 6 + 188 + 24: 1.02 PFLOP/s of the products, with the rows that fill up the blocks (a fifth), as w4_tile_kernel reaches without experts.  333 tokens of three of 13 of 1056 x 1120 4 + 4 + 21 + 14 + 5:
 // vector instructions of groups of 32 with zero points, on a chip that is filled once.
@@ -688,6 +688,8 @@ static const struct {
 //     first, 16 rows each, 280 against 253; with blocks of 4 rows up to 2 each: 4 of the first 77 against 84, but 32 of the second, 3 each, 83 against 78;
 //   * tiles of 16, 32, 64 and 128 x 256: 12 rows each 147, 146, 176, 217; 32 each 370, 327, 378, 486; 48 each 282, 239, 233, 253; 96 each 494, 374, 346, 312; but where the
 //     widest would have too few work-groups 71, 60, 53, 67 (333 tokens of the fourth, 77 each).
+// The rows of an expert are a mean.  One that many tokens choose has several blocks of rows, each of which reads its weights: 64 tokens of two of 64 experts of 2048 x 1408,
+// blocks of 4 rows, 64 us with scores at random, 59 where half of them choose one expert, 56 where all do (16 blocks of its rows, but other experts' weights stay unread).
 static ExpertsLayout layout_of(const hipq_w4_experts_plan *p, int M)
 {
     const hipq_w4_experts_desc &d = p->desc;

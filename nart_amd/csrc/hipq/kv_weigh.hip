@@ -8,7 +8,7 @@
 // belongs to one lane.  Where rows are few the first leaves its scores as well, 4 bytes a row and token, less than the keys that the second would have to read again;
 // where they are many the second multiplies anew, with a tile's keys in registers and the rows going by.
 //
-// us of both launches and what bounds them: one token of 2 sequences of up to 131072 (64 query heads on 8) 105 to 122 + 18, 4.7 TB/s of keys and scores, of the 5.1 of a copy; of 8 of up to 2000
+// us of both launches and what bounds them: one token of 2 sequences of up to 131072 (64 query heads on 8) 105 to 124 + 18, 4.7 TB/s of keys and scores, of the 5.1 of a copy; of 8 of up to 2000
 // 10.6 + 5.5, latency: two tiles a wave; 32 tokens of one of up to 30000 in 8 bits 21 + 23, vector instructions (a score's scaling, maximum and power, twice: 2700 a wave with
 // 460 of the matrix unit).
 #include <type_traits>

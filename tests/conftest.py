@@ -11,7 +11,7 @@ REF_SO = os.path.join(ROOT, "oracle", "_ref", "libnart_ref.so")
 
 
 def pytest_configure(config):
-    config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu on the GPU box)")
+    config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu)")
 
 
 @pytest.fixture(scope="session")
